@@ -84,6 +84,19 @@ class Conv3dArgs(ctypes.Structure):
                 ("status", c_vp)]
 
 
+SRDIT_BF16, SRDIT_FP16, SRDIT_FP32 = 0, 1, 2
+SRDIT_Q_INT8, SRDIT_Q_E4M3 = 0, 1
+
+
+class CrossAttnArgs(ctypes.Structure):
+    _fields_ = [("q", c_vp), ("k", c_vp), ("v", c_vp), ("out", c_vp), ("dtype", c_int),
+                ("B", c_int), ("Lq", c_int), ("Lk", c_int), ("H", c_int), ("Hkv", c_int),
+                ("D", c_int), ("q_stride", c_ll * 3), ("k_stride", c_ll * 3),
+                ("v_stride", c_ll * 3), ("o_stride", c_ll * 3), ("kv_lens", c_vp),
+                ("key_mask", c_vp), ("mask_stride", c_ll), ("scale", c_float),
+                ("workspace", c_vp), ("workspace_bytes", c_ll), ("status", c_vp)]
+
+
 # name -> argtypes (every function returns int)
 SIGNATURES = {
     "srdit_version": [],
@@ -124,6 +137,13 @@ SIGNATURES = {
     "srdit_ipc_open": [c_vp, ctypes.POINTER(c_vp)],
     "srdit_ipc_close": [c_vp],
     "srdit_residual": [c_vp, c_ll, c_int, c_int, c_vp, c_int, c_ll, c_ll, c_vp, c_vp, c_vp],
+    "srdit_add_rms_quant": [c_vp, c_ll, c_int, c_int, c_int, c_vp, c_ll, c_vp, c_float, c_vp,
+                            c_ll, c_vp, c_ll, c_int, c_vp, c_vp],
+    "srdit_quant_rows": [c_vp, c_ll, c_int, c_int, c_int, c_vp, c_ll, c_int, c_vp, c_vp],
+    "srdit_int8_gemm": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_ll,
+                        c_ll, c_ll, c_vp, c_vp],
+    "srdit_cross_attn": [ctypes.POINTER(CrossAttnArgs), c_vp],
+    "srdit_cross_attn_splits": [ctypes.POINTER(CrossAttnArgs)],
     "srdit_winattn_plan": [c_vp, c_int, c_int, c_int, ctypes.POINTER(WinattnTiling)],
     "srdit_winattn_fwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int,
                           ctypes.POINTER(WinattnGeom), ctypes.POINTER(WinattnTiling), c_vp,

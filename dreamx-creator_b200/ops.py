@@ -47,6 +47,10 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _stream(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
@@ -173,6 +177,196 @@ def rms_rope(src, weight, eps, dst, *, frame_tokens, slot0=0, n_slots=1 << 30, c
             _stream(src.device), kind="rms_rope",
             work=M * K * 2 * (4 if v_src is not None else 2))
     return dst
+
+
+DTYPES = {torch.bfloat16: _lib.SRDIT_BF16, torch.float16: _lib.SRDIT_FP16,
+          torch.float32: _lib.SRDIT_FP32}
+HALF_TYPES = {torch.bfloat16: _lib.SRDIT_BF16, torch.float16: _lib.SRDIT_FP16}
+CODES = {torch.int8: _lib.SRDIT_Q_INT8, torch.float8_e4m3fn: _lib.SRDIT_Q_E4M3}
+
+
+def _code(table, dtype, what):
+    code = table.get(dtype)
+    if code is None:
+        raise _lib.SrditError(f"{what} takes {', '.join(map(str, table))}, got {dtype}")
+    return code
+
+
+def _same_device(x, *ts):
+    """Every given tensor on x's device, and that the current one (kernels are
+    launched on the current device)."""
+    dev = x.device
+    if not x.is_cuda:
+        _need_cuda(x)
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise _lib.SrditError(f"tensors on {dev} and {t.device}")
+    if dev.index != torch.cuda.current_device():
+        raise _lib.SrditError(f"tensors on {dev}, the current device is "
+                              f"cuda:{torch.cuda.current_device()}")
+
+
+def _scales(t, n, what):
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise _lib.SrditError(f"{what} must be contiguous float32 [{n}]")
+
+
+def code_rows(M, K, dtype, device):
+    """An empty [M, K] of 8-bit codes whose rows start 16 bytes apart at least, as the
+    products' operands have to."""
+    return torch.empty(M, (K + 15) // 16 * 16, dtype=dtype, device=device)[:, :K]
+
+
+def _codes_out(x, qdtype, q, qscale):
+    """The output tensors of a row quantiser of x [M, K], checked or made."""
+    M, K = x.shape
+    if q is None:
+        q = code_rows(M, K, qdtype or torch.int8, x.device)
+    elif q.shape != x.shape or (qdtype is not None and q.dtype != qdtype):
+        raise _lib.SrditError(f"q {tuple(q.shape)} {q.dtype} for rows {tuple(x.shape)} to "
+                              f"{qdtype or q.dtype}")
+    if qscale is None:
+        qscale = torch.empty(M, dtype=torch.float32, device=x.device)
+    else:
+        _scales(qscale, M, "qscale")
+    return q, qscale
+
+
+def add_rms_quant(x, weight, eps=1e-6, *, residual=None, sum_out=None, qdtype=None, q=None,
+                  qscale=None):
+    """RMS norm of x [+ residual], quantised per row to 8 bits in the same pass.
+
+    x, residual [M, K] and weight [K] in one type (bf16, fp16 or fp32), K at most 32768.
+    Returns (q, qscale, sum): codes [M, K] of ``qdtype`` (int8, the default, or
+    float8_e4m3fn; or ``q``'s own), fp32 scales [M], and x + residual in x's type (None
+    without a residual). ``sum_out`` may be x or residual, which is then updated in place.
+    Without ``q`` the codes' rows are laid out as ``int8_gemm`` takes them."""
+    _same_device(x, weight, residual, sum_out, q, qscale)
+    ldx = _rows(x)
+    M, K = x.shape
+    dt = _code(DTYPES, x.dtype, "add_rms_quant")
+    if weight.dtype != x.dtype or weight.shape != (K,) or not weight.is_contiguous():
+        raise _lib.SrditError(f"weight must be contiguous {x.dtype} [{K}]")
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise _lib.SrditError(f"residual must be {x.dtype} {tuple(x.shape)}")
+        if sum_out is None:
+            sum_out = torch.empty(M, K, dtype=x.dtype, device=x.device)
+        elif sum_out.shape != x.shape or sum_out.dtype != x.dtype:
+            raise _lib.SrditError(f"sum_out must be {x.dtype} {tuple(x.shape)}")
+        ldr, lds = _rows(residual), _rows(sum_out)
+    elif sum_out is not None:
+        raise _lib.SrditError("sum_out without a residual")
+    else:
+        ldr = lds = 0
+    q, qscale = _codes_out(x, qdtype, q, qscale)
+    e = x.element_size()
+    _launch("srdit_add_rms_quant", x.data_ptr(), ldx, M, K, dt, _addr(residual), ldr,
+            weight.data_ptr(), float(eps), _addr(sum_out), lds, q.data_ptr(), _rows(q),
+            _code(CODES, q.dtype, "qdtype"), qscale.data_ptr(), _stream(x.device),
+            kind="add_rms_quant", work=M * K * ((3 if residual is not None else 1) * e + 1))
+    return q, qscale, sum_out
+
+
+def quant_rows(x, *, qdtype=None, q=None, qscale=None):
+    """(codes [M, K], fp32 scales [M]) of rows of bf16, fp16 or fp32, K at most 32768: the
+    row-wise quantiser for int8 codes and for the widths and types ``quant_rowwise`` does
+    not take. Arguments as ``add_rms_quant``."""
+    _same_device(x, q, qscale)
+    ldx = _rows(x)
+    M, K = x.shape
+    dt = _code(DTYPES, x.dtype, "quant_rows")
+    q, qscale = _codes_out(x, qdtype, q, qscale)
+    _launch("srdit_quant_rows", x.data_ptr(), ldx, M, K, dt, q.data_ptr(), _rows(q),
+            _code(CODES, q.dtype, "qdtype"), qscale.data_ptr(), _stream(x.device),
+            kind="quant_rows", work=M * K * (x.element_size() + 1))
+    return q, qscale
+
+
+def int8_gemm(a_q, a_scale, w_q, w_scale, bias=None, out=None, *, out_dtype=None, status=None):
+    """out[M,N] = a_q @ w_q^T * a_scale[:,None] * w_scale[None,:] + bias, the sum exact in int32.
+
+    a_q [M, K], w_q [N, K] int8 with row pitches that are multiples of 16 (``code_rows``
+    makes such), fp32 scales [M] and [N]; bias [N] in out's type: ``out_dtype`` bf16 (the
+    default), fp16 or fp32, or ``out``'s own. Any M, N and K up to 131072."""
+    _same_device(a_q, a_scale, w_q, w_scale, bias, out, status)
+    if a_q.dtype != torch.int8 or w_q.dtype != torch.int8:
+        raise _lib.SrditError("int8_gemm operands must be int8")
+    lda, ldw = _rows(a_q), _rows(w_q)
+    M, K = a_q.shape
+    N, K2 = w_q.shape
+    if K != K2:
+        raise _lib.SrditError(f"K mismatch {K} vs {K2}")
+    _scales(a_scale, M, "a_scale")
+    _scales(w_scale, N, "w_scale")
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype or torch.bfloat16, device=a_q.device)
+    elif out.shape != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
+        raise _lib.SrditError(f"out {tuple(out.shape)} {out.dtype} for a product {(M, N)} in "
+                              f"{out_dtype or out.dtype}")
+    if bias is not None and (bias.dtype != out.dtype or bias.shape != (N,)
+                             or not bias.is_contiguous()):
+        raise _lib.SrditError(f"bias must be contiguous {out.dtype} [{N}]")
+    _launch("srdit_int8_gemm", a_q.data_ptr(), a_scale.data_ptr(), w_q.data_ptr(),
+            w_scale.data_ptr(), _addr(bias), out.data_ptr(), _code(DTYPES, out.dtype, "int8_gemm"),
+            M, N, K, lda, ldw, _rows(out), _addr(status), _stream(a_q.device), kind="int8_gemm",
+            work=2 * M * N * K)
+    return out
+
+
+def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, status=None):
+    """Attention of q [B, Lq, H, D] over an encoder's k, v [B, Lk, Hkv, D] (bf16 or fp16, unit
+    stride over D, D a multiple of 8 up to 128, H a multiple of Hkv; views with other strides
+    that are multiples of 8 elements are read in place). Returns out [B, Lq, H, D].
+
+    ``kv_lens`` (int32 [B] on the device): sample b sees its first kv_lens[b] keys.
+    ``key_mask`` (bool or uint8 [B, Lk]): keys that are seen. A query that sees no key gets
+    zeros; what lies in the rows of unseen keys does not matter. ``scale``: D ** -0.5."""
+    _same_device(q, k, v, out, kv_lens, key_mask, status)
+    dt = _code(HALF_TYPES, q.dtype, "cross_attn")
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise _lib.SrditError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: "
+                              "[B, L, heads, D] each")
+    B, Lq, H, D = q.shape
+    Bk, Lk, Hkv, Dk = k.shape
+    if Bk != B or Dk != D or Hkv == 0 or H % Hkv or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise _lib.SrditError(f"q {tuple(q.shape)} {q.dtype} does not go with k "
+                              f"{tuple(k.shape)} {k.dtype}, v {v.dtype}")
+    if out is None:
+        out = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise _lib.SrditError(f"out must be {q.dtype} {tuple(q.shape)}")
+    a = _lib.CrossAttnArgs()
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.dtype, a.B, a.Lq, a.Lk, a.H, a.Hkv, a.D = dt, B, Lq, Lk, H, Hkv, D
+    for t, nm, st in ((q, "q", a.q_stride), (k, "k", a.k_stride), (v, "v", a.v_stride),
+                      (out, "out", a.o_stride)):
+        s0, s1, s2, s3 = t.stride()
+        if s3 != 1 and D > 1:
+            raise _lib.SrditError(f"{nm} needs unit stride over D, has {t.stride()}")
+        st[0], st[1], st[2] = s0, s1, s2
+    if kv_lens is not None:
+        if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
+            raise _lib.SrditError(f"kv_lens must be contiguous int32 [{B}]")
+        a.kv_lens = kv_lens.data_ptr()
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Lk):
+            raise _lib.SrditError(f"key_mask must be bool or uint8 {(B, Lk)}")
+        if Lk > 1 and key_mask.stride(1) != 1:
+            raise _lib.SrditError("key_mask needs unit stride over the keys")
+        a.key_mask, a.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+    a.scale = D ** -0.5 if scale is None else float(scale)
+    if status is not None:
+        a.status = status.data_ptr()
+    ref = ctypes.byref(a)
+    n = _lib.count("srdit_cross_attn_splits", ref)
+    ws = None
+    if n > 1:
+        ws = torch.empty(n * B * Lq * H * (D + 2), dtype=torch.float32, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel() * 4
+    _launch("srdit_cross_attn", ref, _stream(q.device), kind="cross_attn",
+            work=4 * B * Lq * H * D * Lk)
+    return out
 
 
 def row_reduce(x, op, out=None):

@@ -538,6 +538,90 @@ int srdit_winattn_fwd(const void* q, const void* k_hr, const void* v_hr, const v
                       const srdit_winattn_tiling* tiling, uint32_t* status,
                       cudaStream_t stream);
 
+/* element types of the entry points below */
+#define SRDIT_BF16 0
+#define SRDIT_FP16 1
+#define SRDIT_FP32 2
+/* 8-bit code types */
+#define SRDIT_Q_INT8 0
+#define SRDIT_Q_E4M3 1
+
+/*
+ * RMS norm with the residual's addition, quantised to 8 bits per row:
+ *   s = x + residual (fp32);  sum = s in x's type
+ *   y[m,k] = s[m,k] / sqrt(mean_k(s[m,:]^2) + eps) * weight[k]
+ *   scale[m] = max(max_k |y[m,k]| / Q, 1e-12), Q = 127 (SRDIT_Q_INT8) or 448 (SRDIT_Q_E4M3)
+ *   q[m,k] = round(y[m,k] / scale[m]), ties to even
+ * x, residual, sum [M, K] and weight [K] of type dtype (SRDIT_BF16 / FP16 / FP32), q [M, K]
+ * bytes; row pitches ld* in elements, any alignment of the element type (rows of 16-byte
+ * aligned base, pitch and width are the fast ones). K at most 32768. residual and
+ * sum are given together or both NULL (then s = x); sum may be x or residual itself.
+ * A row holding a NaN or an infinity gets the scale NaN.
+ * Replaces: WanRMSNorm.forward (video_refiner/wan/modules/sr_dit/models.py:424-440) after a
+ *   residual addition (models.py:1257) and before Fp8Linear's row-wise quantiser
+ *   (fp8_linear.py:93-103); the integer codes have no counterpart there.
+ */
+int srdit_add_rms_quant(const void* x, long long ldx, int M, int K, int dtype,
+                        const void* residual, long long ldr, const void* weight, float eps,
+                        void* sum, long long ld_sum, void* q, long long ldq, int q_type,
+                        float* scale, cudaStream_t stream);
+
+/*
+ * The same row-wise quantiser without the norm (y = x), for any width up to 32768, type and
+ * code type: scale[m] = max(max|x| / Q, 1e-12), q = round(x / scale).
+ * Replaces: quantize_rowwise (fp8_linear.py:93-103, :146-171) where srdit_quant_rowwise's
+ *   types or alignments do not fit.
+ */
+int srdit_quant_rows(const void* x, long long ldx, int M, int K, int dtype, void* q,
+                     long long ldq, int q_type, float* scale, cudaStream_t stream);
+
+/*
+ * Row-wise scaled int8 GEMM:
+ *   out[m,n] = a_scale[m] * w_scale[n] * sum_k A[m,k] W[n,k] + bias[n]
+ * A [M, lda] and W [N, ldw] int8 (W is the nn.Linear [out, in] weight), lda and ldw multiples
+ * of 16 and both bases 16-byte aligned; the sum is exact in int32 (K at most 131072); scales
+ * fp32; bias [N] (optional) and out [M, ldo] of type dtype. Any M, N, K, ldo.
+ * Replaces: Fp8Linear.forward's scaled product (fp8_linear.py:282-297) for weights held as
+ *   integers.
+ */
+int srdit_int8_gemm(const void* a, const float* a_scale, const void* w, const float* w_scale,
+                    const void* bias, void* out, int dtype, int M, int N, int K, long long lda,
+                    long long ldw, long long ldo, uint32_t* status, cudaStream_t stream);
+
+/*
+ * Attention of queries over an encoder's keys and values of another length:
+ *   o[b,i,h] = sum_j p_j v[b,j,g] / sum_j p_j,  p_j = exp(scale * q[b,i,h].k[b,j,g] - max)
+ * over the keys j < kv_lens[b] (optional int32 [B] on the device, clamped to [0, Lk]; NULL: Lk)
+ * with key_mask[b * mask_stride + j] != 0 (optional bytes), g = h / (H / Hkv). A row that sees
+ * no key is 0, and keys that are not seen may hold anything, NaN included. q, out
+ * [B, Lq, H, D], k, v [B, Lk, Hkv, D] of type dtype (SRDIT_BF16 / FP16), each with its strides
+ * {batch, token, head} in elements (multiples of 8; 0 repeats one entry) and unit stride over D;
+ * bases 16-byte aligned. D a multiple of 8, at most 128. scale > 0. workspace: where
+ * srdit_cross_attn_splits (which reads the sizes and the type only) returns n > 1, n partial
+ * results per row are joined through it: n * B * Lq * H * (D + 2) floats, 16-byte aligned; else
+ * it may be NULL.
+ * Replaces: flash_attention with k_lens (video_refiner/wan/modules/attention.py:61-168, called
+ *   at wan/modules/sr_dit/models.py:1057).
+ */
+typedef struct srdit_cross_attn_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int dtype;
+  int B, Lq, Lk, H, Hkv, D;
+  long long q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+  const int32_t* kv_lens;
+  const uint8_t* key_mask;
+  long long mask_stride;
+  float scale;
+  void* workspace;
+  long long workspace_bytes;
+  uint32_t* status;
+} srdit_cross_attn_args;
+int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t stream);
+int srdit_cross_attn_splits(const srdit_cross_attn_args* args);
+
 #ifdef __cplusplus
 }
 #endif
