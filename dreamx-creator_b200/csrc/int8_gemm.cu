@@ -1,8 +1,24 @@
-// int8_gemm.cu -- row-wise scaled int8 GEMM.
+// int8_gemm.cu -- row-wise scaled int8 GEMM on the tensor cores (sm_100a).
 //
 //   out[m, n] = a_scale[m] * w_scale[n] * sum_k A[m, k] W[n, k] + bias[n]
 //
-// The sum is exact in int32 (|A|, |W| <= 128 and K <= 131072 keep it below 2^31).
+// The sum is exact in int32 (|A|, |W| <= 128 and K < 131072 keep it below 2^31), so
+// neither the order of the products nor a split of K changes a bit of the result.
+//
+// Two kernels, one for each thing that bounds the product:
+//
+//   pair_kernel    many tokens, bounded by the tensor cores. A CTA pair computes a
+//                  256 x BN tile with one tcgen05.mma.cta_group::2.kind::i8 per
+//                  32-deep step; two accumulators in tensor memory let a tile's
+//                  epilogue run under the next tile's products; persistent.
+//   split_kernel   few tokens, bounded by the weights' bytes, and token counts that
+//                  give the pairs too few tiles. The weights take the MMA's 128
+//                  rows and the tokens its columns (16 to 128), so a token count of
+//                  1 wastes 15 columns and not 255 rows. K is split over a cluster
+//                  of up to 8 CTAs, whose int32 partial sums meet in shared memory
+//                  of the cluster: no workspace, no atomics, no second launch.
+#include <atomic>
+
 #include "sm100.cuh"
 #include "srdit_internal.h"
 
@@ -12,47 +28,561 @@
 namespace srdit {
 namespace i8 {
 
+constexpr int BK = 128;  // bytes of K per stage: one 128-byte swizzled row
+constexpr int NUM_THREADS = 192;
+
 struct Params {
-  const int8_t* a;
-  const int8_t* w;
   const float* a_scale;
   const float* w_scale;
   const void* bias;
   void* out;
-  long long lda, ldw, ldo;
+  long long ldo;
   int M, N, K;
+  int splits;  // split_kernel: CTAs of a cluster along K
+  int o_tma;   // pair_kernel: tmO is valid (out and its pitch are 16-byte aligned)
+  uint32_t* status;
 };
 
 template <typename T>
 SRDIT_DEV float to_f(T v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else return static_cast<float>(v);
+  return static_cast<float>(v);
+}
+template <typename T>
+SRDIT_DEV float bias_at(const Params& p, int n) {
+  return p.bias ? to_f(static_cast<const T*>(p.bias)[n]) : 0.f;
+}
+// acc * sa * sw + bias: the conversion, one product and one fma, a rounding each
+SRDIT_DEV float scaled(uint32_t acc, float sa, float sw, float b) {
+  return fmaf(static_cast<float>(static_cast<int>(acc)) * sa, sw, b);
+}
+SRDIT_DEV uint32_t pack2(float x, float y, __nv_bfloat16) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(y), "f"(x));
+  return d;
+}
+SRDIT_DEV uint32_t pack2(float x, float y, __half) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(y), "f"(x));
+  return d;
 }
 
-// One output per thread, four products per dp4a.
-template <typename T>
-__global__ void __launch_bounds__(256) simple_kernel(const Params p) {
+// ---------------------------------------------------------------- few tokens
+template <int BT>
+struct SplitCfg {
+  static constexpr int W_BYTES = 128 * BK;
+  static constexpr int STAGE_BYTES = W_BYTES + BT * BK;
+  // up to 32 tokens two CTAs share an SM's shared memory; above, one has it
+  static constexpr int STAGES = BT == 32 ? 4 : 5;
+  static constexpr int OFF_PART = STAGES * STAGE_BYTES;  // int32 [splits][BT / splits][128]
+  static constexpr int OFF_BAR = OFF_PART + BT * 128 * 4;
+  static constexpr int SMEM = OFF_BAR + 128 + 1024;
+  static constexpr uint32_t TMEM_COLS = BT < 32 ? 32 : BT;
+  static_assert(SMEM <= (BT <= 32 ? 115712 : 232448), "shared memory budget");
+};
+
+template <typename T, int BT>
+__global__ void __launch_bounds__(NUM_THREADS)
+    split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                 const Params p) {
   pdl_begin();
-  const int n = blockIdx.x * 16 + (threadIdx.x & 15);
-  const int m = blockIdx.y * 16 + (threadIdx.x >> 4);
-  if (m >= p.M || n >= p.N) return;
-  const int8_t* a = p.a + m * p.lda;
-  const int8_t* w = p.w + n * p.ldw;
-  int acc = 0;
-  int k = 0;
-  for (; k + 4 <= p.K; k += 4)
-    acc = __dp4a(*reinterpret_cast<const int*>(a + k), *reinterpret_cast<const int*>(w + k), acc);
-  for (; k < p.K; ++k) acc += static_cast<int>(a[k]) * static_cast<int>(w[k]);
-  float y = static_cast<float>(acc) * p.a_scale[m] * p.w_scale[n];
-  if (p.bias) y += to_f<T>(static_cast<const T*>(p.bias)[n]);
-  static_cast<T*>(p.out)[m * p.ldo + n] = static_cast<T>(y);
+  using C = SplitCfg<BT>;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* empty = full + STAGES;
+  uint64_t* done = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int n0 = (static_cast<int>(blockIdx.x) / p.splits) * 128;
+  const int m0 = static_cast<int>(blockIdx.y) * BT;
+  const int num_kb = (p.K + BK - 1) / BK;
+  const int kb0 = static_cast<int>(static_cast<long long>(num_kb) * split / p.splits);
+  const int kb1 = static_cast<int>(static_cast<long long>(num_kb) * (split + 1) / p.splits);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0u;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (p.splits > 1) cluster_arrive();  // waited for before the first remote store
+  const uint32_t tmem_base = *tmem_slot;
+
+  bool ok = true;
+  if (warp == 0) {
+    if (elect_one()) {
+      for (int i = 0, kb = kb0; kb < kb1; ++i, ++kb) {
+        const int s = i % STAGES;
+        if (!mbar_wait(&empty[s], (static_cast<uint32_t>(i / STAGES) & 1u) ^ 1u, p.status,
+                       abort_flag)) {
+          ok = false;
+          break;
+        }
+        uint8_t* st = smem + s * C::STAGE_BYTES;
+        mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
+        tma_load_2d(st, &tmW, &full[s], kb * BK, n0);
+        tma_load_2d(st + C::W_BYTES, &tmA, &full[s], kb * BK, m0);
+      }
+      // having given up, let the loads in flight land before the CTA exits
+      if (!ok)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = idesc_i8(128, BT);
+      for (int i = 0, kb = kb0; kb < kb1; ++i, ++kb) {
+        const int s = i % STAGES;
+        if (!mbar_wait(&full[s], static_cast<uint32_t>(i / STAGES) & 1u, p.status, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t w_addr = smem_u32(smem + s * C::STAGE_BYTES);
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k)
+          mma_i8_ss(tmem_base, sdesc_sw128(w_addr + k * 32, 16, 1024),
+                    sdesc_sw128(w_addr + C::W_BYTES + k * 32, 16, 1024), idesc,
+                    (i > 0 || k > 0) ? 1u : 0u);
+        tc_commit(&empty[s]);
+      }
+      if (ok) tc_commit(done);
+    }
+    __syncwarp();
+  }
+
+  // the accumulator: lane = weight row, column = token
+  const int sub = warp & 3;
+  const uint32_t t_row = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
+  const int n = n0 + sub * 32 + lane;
+  T* out = static_cast<T*>(p.out) + n;
+  if (p.splits == 1) {
+    if (warp >= 2 && mbar_wait(done, 0u, p.status, abort_flag)) {
+      tc_fence_after();
+      const float sw = n < p.N ? p.w_scale[n] : 0.f;
+      const float b = n < p.N ? bias_at<T>(p, n) : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < BT && m0 + c < p.M; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(t_row + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int m = m0 + c + e;
+          if (m < p.M && n < p.N)
+            out[m * p.ldo] = static_cast<T>(scaled(r[e], __ldg(p.a_scale + m), sw, b));
+        }
+      }
+    }
+  } else {
+    // token column c belongs to CTA c / per of the cluster, which gets every CTA's
+    // partial sums of it at part[source][c % per][row]
+    const int per = BT / p.splits;
+    const uint32_t part = smem_u32(smem + C::OFF_PART);
+    bool got = true;
+    if (warp >= 2) got = mbar_wait(done, 0u, p.status, abort_flag);
+    __syncwarp();
+    cluster_wait();
+    if (warp >= 2 && got) {
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < BT && m0 + c < p.M; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(t_row + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int owner = (c + e) / per, at = (c + e) - owner * per;
+          const uint32_t addr =
+              part + static_cast<uint32_t>(((split * per + at) * 128 + sub * 32 + lane) * 4);
+          st_cluster_u32(mapa_shared(addr, static_cast<uint32_t>(owner)), r[e]);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 2 && got && n < p.N) {
+      const float sw = p.w_scale[n];
+      const float b = bias_at<T>(p, n);
+      const int* mine = reinterpret_cast<const int*>(smem + C::OFF_PART) + sub * 32 + lane;
+      for (int at = 0; at < per; ++at) {
+        const int m = m0 + split * per + at;
+        if (m >= p.M) break;
+        int acc = 0;
+        for (int s = 0; s < p.splits; ++s) acc += mine[(s * per + at) * 128];
+        out[m * p.ldo] = static_cast<T>(
+            scaled(static_cast<uint32_t>(acc), __ldg(p.a_scale + m), sw, b));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- many tokens
+constexpr int EPI_WARPS = 4;
+constexpr int STG_BYTES = 32 * 128;  // a warp's staging box: 32 rows x 128 bytes
+
+template <int BN>
+struct PairCfg {
+  static constexpr int A_BYTES = 128 * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + (BN / 2) * BK;
+  static constexpr int STAGES = BN == 192 ? 6 : 5;
+  static constexpr int OFF_STG = STAGES * STAGE_BYTES;
+  static constexpr int OFF_COL = OFF_STG + EPI_WARPS * 2 * STG_BYTES;
+  static constexpr int OFF_BAR = OFF_COL + 2 * 2 * 256 * 4;  // w_scale, bias
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static_assert(STAGE_BYTES % 1024 == 0, "stages stay 1024-byte aligned");
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+template <typename T, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                const __grid_constant__ CUtensorMap tmO, const Params p) {
+  pdl_begin();
+  using C = PairCfg<BN>;
+  constexpr int STAGES = C::STAGES;
+  constexpr int CHUNK = 128 / sizeof(T);  // output columns of a staging box
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // completed in the even CTA
+  uint64_t* empty = full + STAGES;   // one per CTA
+  uint64_t* tfull = empty + STAGES;  // [2]
+  uint64_t* tempty = tfull + 2;      // [2], in the even CTA, one arrival per epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  float* col_s = reinterpret_cast<float*>(smem + C::OFF_COL);  // [2][256] w_scale
+  float* col_b = col_s + 512;                                  // [2][256] bias
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int num_m = (p.M + 255) / 256;
+  const int num_n = (p.N + BN - 1) / BN;
+  const int num_tiles = num_m * num_n;
+  const int num_kb = (p.K + BK - 1) / BK;
+  const int cid = static_cast<int>(cluster_id_x());
+  const int ncl = static_cast<int>(num_clusters_x());
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * EPI_WARPS);
+    }
+    *abort_flag = 0u;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+    if (p.o_tma) tma_prefetch_desc(&tmO);
+  }
+  if (warp == 1) {
+    tmem_alloc_2sm(tmem_slot, 512);
+    tmem_relinquish_2sm();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint32_t full_even = mapa_shared(smem_u32(&full[0]), 0);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = cid; tile < num_tiles && ok; tile += ncl) {
+        const int mt = tile / num_n, nt = tile % num_n;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[s], ph ^ 1u, p.status, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * C::STAGE_BYTES);
+          uint8_t* st = smem + s * C::STAGE_BYTES;
+          tma_load_2d_2sm(st, &tmA, full_even + 8u * s, kb * BK, mt * 256 + rank * 128);
+          tma_load_2d_2sm(st + C::A_BYTES, &tmW, full_even + 8u * s, kb * BK,
+                          nt * BN + rank * (BN / 2));
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // having given up, let the loads in flight land before the CTA exits (their
+      // completions are counted on the even CTA's barriers)
+      if (!ok)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = idesc_i8(256, BN);
+      const uint32_t empty_own = mapa_shared(smem_u32(&empty[0]), 0);
+      const uint32_t empty_peer = mapa_shared(smem_u32(&empty[0]), 1);
+      const uint32_t tfull_own = mapa_shared(smem_u32(&tfull[0]), 0);
+      const uint32_t tfull_peer = mapa_shared(smem_u32(&tfull[0]), 1);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      int local = 0;
+      for (int tile = cid; tile < num_tiles && ok; tile += ncl, ++local) {
+        const int acc = local & 1;
+        if (!mbar_wait(&tempty[acc], (static_cast<uint32_t>(local >> 1) & 1u) ^ 1u, p.status,
+                       abort_flag))
+          break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[s], ph, p.status, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma_i8_ss_2sm(d_tmem, sdesc_sw128(a_addr + k * 32, 16, 1024),
+                          sdesc_sw128(a_addr + C::A_BYTES + k * 32, 16, 1024), idesc,
+                          (kb > 0 || k > 0) ? 1u : 0u);
+          tc_commit_2sm(empty_own + 8u * s);
+          tc_commit_2sm(empty_peer + 8u * s);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) {
+          tc_commit_2sm(tfull_own + 8u * acc);
+          tc_commit_2sm(tfull_peer + 8u * acc);
+        }
+      }
+    }
+  } else {
+    const int sub = warp & 3;
+    const int ep_tid = threadIdx.x - 64;
+    uint8_t* stg = smem + C::OFF_STG + sub * 2 * STG_BYTES;
+    const uint32_t tempty_even = mapa_shared(smem_u32(&tempty[0]), 0);
+    int stores = 0;
+    int local = 0;
+    for (int tile = cid; tile < num_tiles; tile += ncl, ++local) {
+      const int acc = local & 1;
+      const int mt = tile / num_n, nt = tile % num_n;
+      const int n0 = nt * BN;
+      // this tile's column scales and bias (double-buffered; 0 past N)
+      for (int c = ep_tid; c < BN; c += 128) {
+        const int col = n0 + c;
+        col_s[acc * 256 + c] = col < p.N ? __ldg(p.w_scale + col) : 0.f;
+        col_b[acc * 256 + c] = col < p.N ? bias_at<T>(p, col) : 0.f;
+      }
+      named_barrier_sync(1, 128);
+      if (!mbar_wait(&tfull[acc], static_cast<uint32_t>(local >> 1) & 1u, p.status, abort_flag))
+        break;
+      tc_fence_after();
+      const int row0 = mt * 256 + static_cast<int>(rank) * 128 + sub * 32;
+      const float sa = row0 + lane < p.M ? p.a_scale[row0 + lane] : 0.f;
+      const float* cs = col_s + acc * 256;
+      const float* cb = col_b + acc * 256;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) +
+                             static_cast<uint32_t>(acc * BN);
+      const bool rows_on = row0 < p.M;
+#pragma unroll 1
+      for (int ch = 0; ch < BN / CHUNK; ++ch) {
+        const int col0 = n0 + ch * CHUNK;
+        if (!rows_on || col0 >= p.N) break;  // warp-uniform: nothing of the box is stored
+        uint8_t* buf = stg + (stores & 1) * STG_BYTES;
+        if (p.o_tma && stores >= 2) {
+          if (lane == 0) bulk_wait_group_read1();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < CHUNK / 32; ++h) {
+          const int c0 = ch * CHUNK + h * 32;
+          uint32_t r[32];
+          tmem_ld32(t_row + c0, r);
+          tmem_ld_wait();
+          uint32_t pw[sizeof(T) == 4 ? 32 : 16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float y0 = scaled(r[j], sa, cs[c0 + j], cb[c0 + j]);
+            const float y1 = scaled(r[j + 1], sa, cs[c0 + j + 1], cb[c0 + j + 1]);
+            if constexpr (sizeof(T) == 4) {
+              pw[j] = __float_as_uint(y0);
+              pw[j + 1] = __float_as_uint(y1);
+            } else {
+              pw[j >> 1] = pack2(y0, y1, T{});
+            }
+          }
+          // 16-byte piece q of the box row at q ^ (row & 7): the 128-byte TMA swizzle
+#pragma unroll
+          for (int q = 0; q < static_cast<int>(sizeof(pw) / 16); ++q)
+            *reinterpret_cast<uint4*>(buf + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4)) =
+                make_uint4(pw[4 * q], pw[4 * q + 1], pw[4 * q + 2], pw[4 * q + 3]);
+        }
+        if (p.o_tma) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmO, buf, col0, row0);
+            bulk_commit_group();
+          }
+        } else {
+          // an output that TMA cannot address: the box row by row, lanes along N
+          __syncwarp();
+          const int rows = min(32, p.M - row0);
+          for (int r = 0; r < rows; ++r) {
+            T* o = static_cast<T*>(p.out) + (row0 + r) * p.ldo + col0;
+#pragma unroll
+            for (int c = lane; c < CHUNK; c += 32) {
+              const int byte = c * static_cast<int>(sizeof(T));
+              if (col0 + c < p.N)
+                o[c] = *reinterpret_cast<const T*>(buf + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) +
+                                                   (byte & 15));
+            }
+          }
+          __syncwarp();
+        }
+        ++stores;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty_even + 8u * acc);
+    }
+    if (lane == 0) bulk_wait_group_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_2sm(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------- launch
+template <typename Kern>
+static int set_smem(Kern kern, int bytes, std::atomic<bool>* done, int dev) {
+  if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return 0;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
+  return 0;
+}
+
+struct Operands {
+  const void* a;
+  const void* w;
+  long long lda, ldw;
+};
+
+template <typename T, int BT>
+static int launch_split(const Operands& o, Params& p, int dev, cudaStream_t stream) {
+  using C = SplitCfg<BT>;
+  auto kern = split_kernel<T, BT>;
+  static std::atomic<bool> attr_done[kMaxDevices] = {};
+  int rc = set_smem(kern, C::SMEM, attr_done, dev);
+  if (rc) return rc;
+  CUtensorMap ta, tw;
+  rc = make_tmap_2d(&ta, o.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, o.lda, BK, BT);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tw, o.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, o.ldw, BK, 128);
+  if (rc) return rc;
+  const int n_tiles = (p.N + 127) / 128, m_tiles = (p.M + BT - 1) / BT;
+  const int slots = num_sms(dev) * (BT <= 32 ? 2 : 1);
+  const int num_kb = (p.K + BK - 1) / BK;
+  // the most splits that still run at once, each with two stages of K at least
+  int splits = 1;
+  while (splits < 8 && 2 * splits * n_tiles * m_tiles <= slots && num_kb >= 4 * splits) splits *= 2;
+  p.splits = splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles));
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tw, p));
+}
+
+template <typename T, int BN>
+static int launch_pair(const Operands& o, Params& p, int dev, cudaStream_t stream) {
+  using C = PairCfg<BN>;
+  auto kern = pair_kernel<T, BN>;
+  static std::atomic<bool> attr_done[kMaxDevices] = {};
+  int rc = set_smem(kern, C::SMEM, attr_done, dev);
+  if (rc) return rc;
+  CUtensorMap ta, tw, to;
+  rc = make_tmap_2d(&ta, o.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, o.lda, BK, 128);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tw, o.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, o.ldw, BK, BN / 2);
+  if (rc) return rc;
+  p.o_tma = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && (p.ldo * sizeof(T)) % 16 == 0;
+  to = ta;
+  if (p.o_tma) {
+    const CUtensorMapDataType dt = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    rc = make_tmap_2d(&to, p.out, dt, sizeof(T), p.N, p.M, p.ldo, 128 / sizeof(T), 32);
+    if (rc) return rc;
+  }
+  const int tiles = ((p.M + 255) / 256) * ((p.N + BN - 1) / BN);
+  const int pairs = num_sms(dev) / 2;
+  SRDIT_LAUNCH((kern), 2 * (tiles < pairs ? tiles : pairs), NUM_THREADS, C::SMEM, stream, ta, tw,
+               to, p);
+  return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T>
-static int launch(const Params& p, cudaStream_t stream) {
-  const dim3 grid((p.N + 15) / 16, (p.M + 15) / 16);
-  SRDIT_LAUNCH((simple_kernel<T>), grid, 256, 0, stream, p);
-  return static_cast<int>(cudaGetLastError());
+static int launch(const Operands& o, Params& p, cudaStream_t stream) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (p.M <= 16) return launch_split<T, 16>(o, p, dev, stream);
+  if (p.M <= 32) return launch_split<T, 32>(o, p, dev, stream);
+  if (p.M <= 64) return launch_split<T, 64>(o, p, dev, stream);
+  const int pairs = num_sms(dev) / 2;
+  const long long m256 = (p.M + 255) / 256;
+  const long long t256 = m256 * ((p.N + 255) / 256), t192 = m256 * ((p.N + 191) / 192);
+  if (p.M <= 128 || t256 <= pairs / 2) return launch_split<T, 128>(o, p, dev, stream);
+  const long long c256 = (t256 + pairs - 1) / pairs * 256, c192 = (t192 + pairs - 1) / pairs * 192;
+  return c192 < c256 ? launch_pair<T, 192>(o, p, dev, stream)
+                     : launch_pair<T, 256>(o, p, dev, stream);
 }
 
 }  // namespace i8
@@ -64,21 +594,24 @@ extern "C" int srdit_int8_gemm(const void* a, const float* a_scale, const void* 
                                const float* w_scale, const void* bias, void* out, int dtype, int M,
                                int N, int K, long long lda, long long ldw, long long ldo,
                                uint32_t* status, cudaStream_t stream) {
-  (void)status;
   if (M < 0 || N < 0 || K <= 0) return SRDIT_EINVAL;
   if (M == 0 || N == 0) return 0;
   if (!a || !a_scale || !w || !w_scale || !out) return SRDIT_EINVAL;
   if (lda < K || ldw < K || ldo < N) return SRDIT_EINVAL;
-  if (K > 131072) return SRDIT_EUNSUPPORTED;
+  if (K >= 131072) return SRDIT_EUNSUPPORTED;
   if ((lda % 16) || (ldw % 16) || (reinterpret_cast<uintptr_t>(a) & 15u) ||
       (reinterpret_cast<uintptr_t>(w) & 15u))
     return SRDIT_EALIGN;
-  i8::Params p = {static_cast<const int8_t*>(a), static_cast<const int8_t*>(w), a_scale, w_scale,
-                  bias, out, lda, ldw, ldo, M, N, K};
+  const uintptr_t e = dtype == SRDIT_FP32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(out) % e || reinterpret_cast<uintptr_t>(bias) % e ||
+      reinterpret_cast<uintptr_t>(a_scale) % 4 || reinterpret_cast<uintptr_t>(w_scale) % 4)
+    return SRDIT_EALIGN;
+  const i8::Operands o = {a, w, lda, ldw};
+  i8::Params p = {a_scale, w_scale, bias, out, ldo, M, N, K, 1, 0, status};
   switch (dtype) {
-    case SRDIT_BF16: return i8::launch<__nv_bfloat16>(p, stream);
-    case SRDIT_FP16: return i8::launch<__half>(p, stream);
-    case SRDIT_FP32: return i8::launch<float>(p, stream);
+    case SRDIT_BF16: return i8::launch<__nv_bfloat16>(o, p, stream);
+    case SRDIT_FP16: return i8::launch<__half>(o, p, stream);
+    case SRDIT_FP32: return i8::launch<float>(o, p, stream);
     default: return SRDIT_EINVAL;
   }
 }

@@ -203,6 +203,16 @@ SRDIT_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
                ::: "memory");
 }
+// the two halves of cluster_sync
+SRDIT_DEV void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+SRDIT_DEV void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+SRDIT_DEV void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
 // arrive on an mbarrier given by its shared::cluster address (any CTA of the cluster)
 SRDIT_DEV void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
@@ -351,6 +361,26 @@ SRDIT_DEV void mma_bf16_ss_2sm(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc
       : "memory");
 }
 
+// D(tmem, s32) (+)= A(smem) * B(smem)^T, 8-bit integers, exact; one CTA's tile or a pair's.
+SRDIT_DEV void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+SRDIT_DEV void mma_i8_ss_2sm(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // 32 lanes x 32 consecutive 32-bit columns: thread t of the warp receives lane
 // (warp's sub-partition base + t), columns [col, col+32).
 SRDIT_DEV void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -377,6 +407,16 @@ SRDIT_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
       "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+// 32 lanes x 16 consecutive 32-bit columns (the x16 form of tmem_ld32).
+SRDIT_DEV void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 // 32 lanes x 16 consecutive 32-bit columns (the x16 form of tmem_st32).
 SRDIT_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -430,6 +470,12 @@ SRDIT_DEV uint32_t idesc_make(uint32_t a_fmt, uint32_t b_fmt, uint32_t a_mn_majo
   d |= ((N >> 3) & 0x3Fu) << 17;
   d |= ((M >> 4) & 0x1Fu) << 24;
   return d;
+}
+
+// The same for kind::i8: s32 accumulators (D format 2), signed 8-bit operands (format 1),
+// both K-major.
+SRDIT_DEV uint32_t idesc_i8(uint32_t M, uint32_t N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) & 0x3Fu) << 17 | ((M >> 4) & 0x1Fu) << 24;
 }
 
 // ---------------------------------------------------------------- packed pairs

@@ -288,7 +288,7 @@ def int8_gemm(a_q, a_scale, w_q, w_scale, bias=None, out=None, *, out_dtype=None
 
     a_q [M, K], w_q [N, K] int8 with row pitches that are multiples of 16 (``code_rows``
     makes such), fp32 scales [M] and [N]; bias [N] in out's type: ``out_dtype`` bf16 (the
-    default), fp16 or fp32, or ``out``'s own. Any M, N and K up to 131072."""
+    default), fp16 or fp32, or ``out``'s own. Any M and N; K below 131072."""
     _same_device(a_q, a_scale, w_q, w_scale, bias, out, status)
     if a_q.dtype != torch.int8 or w_q.dtype != torch.int8:
         raise _lib.SrditError("int8_gemm operands must be int8")

@@ -579,7 +579,7 @@ int srdit_quant_rows(const void* x, long long ldx, int M, int K, int dtype, void
  * Row-wise scaled int8 GEMM:
  *   out[m,n] = a_scale[m] * w_scale[n] * sum_k A[m,k] W[n,k] + bias[n]
  * A [M, lda] and W [N, ldw] int8 (W is the nn.Linear [out, in] weight), lda and ldw multiples
- * of 16 and both bases 16-byte aligned; the sum is exact in int32 (K at most 131072); scales
+ * of 16 and both bases 16-byte aligned; the sum is exact in int32 (K below 131072); scales
  * fp32; bias [N] (optional) and out [M, ldo] of type dtype. Any M, N, K, ldo.
  * Replaces: Fp8Linear.forward's scaled product (fp8_linear.py:282-297) for weights held as
  *   integers.
