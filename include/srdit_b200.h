@@ -595,7 +595,8 @@ int srdit_int8_gemm(const void* a, const float* a_scale, const void* w, const fl
  * with key_mask[b * mask_stride + j] != 0 (optional bytes), g = h / (H / Hkv). A row that sees
  * no key is 0, and keys that are not seen may hold anything, NaN included. q, out
  * [B, Lq, H, D], k, v [B, Lk, Hkv, D] of type dtype (SRDIT_BF16 / FP16), each with its strides
- * {batch, token, head} in elements (multiples of 8; 0 repeats one entry) and unit stride over D;
+ * {batch, token, head} in elements (multiples of 8; a batch stride of 0 repeats one sample, a
+ * head stride of 0 of k or v one head) and unit stride over D;
  * bases 16-byte aligned. D a multiple of 8, at most 128. scale > 0. workspace: where
  * srdit_cross_attn_splits (which reads the sizes and the type only) returns n > 1, n partial
  * results per row are joined through it: n * B * Lq * H * (D + 2) floats, 16-byte aligned; else
