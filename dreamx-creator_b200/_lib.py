@@ -143,7 +143,7 @@ SIGNATURES = {
     "srdit_int8_gemm": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_ll,
                         c_ll, c_ll, c_vp, c_vp],
     "srdit_cross_attn": [ctypes.POINTER(CrossAttnArgs), c_vp],
-    "srdit_cross_attn_splits": [ctypes.POINTER(CrossAttnArgs)],
+    "srdit_cross_attn_workspace": [ctypes.POINTER(CrossAttnArgs)],
     "srdit_winattn_plan": [c_vp, c_int, c_int, c_int, ctypes.POINTER(WinattnTiling)],
     "srdit_winattn_fwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int,
                           ctypes.POINTER(WinattnGeom), ctypes.POINTER(WinattnTiling), c_vp,

@@ -20,7 +20,8 @@
 //                 layout of the mma operands, without shared memory.
 //
 // Long contexts with few rows are split over the keys; the parts' (m, l, O) meet in
-// shared memory of a cluster (token_kernel) or in the workspace (combine_kernel).
+// shared memory of a cluster (token_kernel) or in the workspace (join_parts_kernel,
+// join_ranges_kernel).
 #include <atomic>
 
 #include "sm100.cuh"
@@ -48,13 +49,13 @@ struct Args {
   int nq, nhp;     // tile_kernel: query-tile pairs per head pack, head packs
   int q_one, k_one, v_one;         // one sample's tensor for all (batch stride 0)
   int k_one_head, v_one_head;      // one key head for all (head stride 0)
-  int splits;      // parts of the key range
-  int items;       // tile_kernel: work items
+  int ranged;      // tile_kernel: every CTA has an equal range of key-tile steps
+  int splits;      // token_kernel: parts of the key range
   const int32_t* kv_lens;
   const uint8_t* mask;
   long long mask_stride;
   float c;         // scale * log2(e)
-  float* ws;       // [parts][rows][D] O, then [parts][rows] {m, l}
+  float* ws;       // parts of rows: O, then {m, l}
   uint32_t* status;
 };
 
@@ -83,44 +84,166 @@ SRDIT_DEV int key_count(const Args& a, int b) {
   return a.kv_lens ? min(max(__ldg(a.kv_lens + b), 0), a.Lk) : a.Lk;
 }
 
+// One row of the output from n parts of it in the workspace, by one warp: part p's O at
+// row at(p), its {m, l} at ml[at(p)]. Four parts' loads are in flight at a time.
+template <typename T, typename At>
+SRDIT_DEV void join_rows(const Args& a, int n, At at, const float2* ml, T* out, int lane) {
+  float m = neg_inf(), l = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool on = lane * 4 < a.D;
+  for (int p0 = 0; p0 < n; p0 += 4) {
+    float2 pm[4];
+    float4 v[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      pm[x] = make_float2(neg_inf(), 0.f);
+      v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p0 + x < n) {
+        const long long row = at(p0 + x);
+        pm[x] = ml[row];
+        if (on) v[x] = *reinterpret_cast<const float4*>(a.ws + row * a.D + lane * 4);
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) mn = fmaxf(mn, pm[x].x);
+    if (mn == neg_inf()) continue;  // no key seen yet
+    const float f = ex2(m - mn);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (pm[x].x == neg_inf()) continue;  // a part that saw no key
+      const float g = ex2(pm[x].x - m);
+      l = fmaf(pm[x].y, g, l);
+      acc[0] = fmaf(v[x].x, g, acc[0]);
+      acc[1] = fmaf(v[x].y, g, acc[1]);
+      acc[2] = fmaf(v[x].z, g, acc[2]);
+      acc[3] = fmaf(v[x].w, g, acc[3]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (on)
+    *reinterpret_cast<uint2*>(out + lane * 4) =
+        make_uint2(pack2(acc[0] * inv, acc[1] * inv, T{}), pack2(acc[2] * inv, acc[3] * inv, T{}));
+}
+
 // ---------------------------------------------------------------- tile_kernel
-constexpr int TILE_THREADS = 320;  // producer, MMA issuer, 2 x 4 softmax warps
+constexpr int TILE_THREADS = 384;  // producer and MMA issuer, 2 x 4 softmax warps
+constexpr int SLOT_ROWS = 2 * TILE;
+constexpr int MAX_RANGES = 256;  // CTAs of a ranged launch
 
 template <int DP>
 struct TileCfg {
   static constexpr int SLAB = TILE * 128;  // 128 rows x 64 values
   static constexpr int BYTES = SLAB * (DP / 64);
-  static constexpr int STAGES = DP == 128 ? 5 : 10;
+  static constexpr int STAGES = DP == 128 ? 4 : 10;
   static constexpr int OFF_KV = 2 * BYTES;
-  static constexpr int OFF_BAR = OFF_KV + STAGES * BYTES;
+  static constexpr int OFF_STG = OFF_KV + STAGES * BYTES;  // 32 rows x 128 bytes per warp
+  static constexpr int OFF_BAR = OFF_STG + 8 * 4096;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
-// One work item: a pair of query tiles of one head pack against one part of a
-// sample's keys.
+// A work item is a pair of query tiles of one head pack against a sample's key tiles
+// [t0, t1). Items are ordered by sample, head pack and query tiles, so that items
+// which run at the same time share keys.
 struct Item {
-  int b, h0, tok0, part;
-  int len;
-  int t0, t1;  // key tiles
-  bool act1;   // the second query tile has tokens
+  int b, h0, tok0, len;
+  int t0, t1;
+  int slot;   // -1: all of the sample's keys; else where in the workspace the part goes
+  bool act1;  // the second query tile has tokens
 };
-SRDIT_DEV Item item_of(const Args& a, int i) {
-  Item o;
-  const int qt = i % a.nq;
-  i /= a.nq;
-  o.h0 = (i % a.nhp) * a.pack;
-  i /= a.nhp;
-  o.b = i % a.B;
-  o.part = i / a.B;
-  o.tok0 = qt * 2 * a.rt;
-  o.act1 = o.tok0 + a.rt < a.Lq;
-  o.len = key_count(a, o.b);
-  const int nt = (o.len + TILE - 1) / TILE;
-  o.t0 = static_cast<int>(static_cast<long long>(nt) * o.part / a.splits);
-  o.t1 = static_cast<int>(static_cast<long long>(nt) * (o.part + 1) / a.splits);
-  return o;
-}
+
+// The items of one CTA. Either whole items, every gridDim-th one; or (ranged) an equal
+// share of all key-tile steps, whose first and last items may be parts of items. Parts
+// cost a trip through the workspace and a second launch, whole items cost the CTAs'
+// idle time in the last round: make_plan compares them.
+struct Walk {
+  const Args& a;
+  int b, rest;          // sample, item within it
+  int nt, per;          // the sample's key tiles; items per sample
+  long long s, s1;      // ranged: next step, end
+  int t0;               // ranged: first key tile of the next item
+  SRDIT_DEV int tiles(int x) const { return (key_count(a, x) + TILE - 1) / TILE; }
+  SRDIT_DEV long long total() const {
+    if (!a.kv_lens) return static_cast<long long>((a.Lk + TILE - 1) / TILE) * per * a.B;
+    long long t = 0;
+    for (int x = 0; x < a.B; ++x) t += static_cast<long long>(tiles(x)) * per;
+    return t;
+  }
+  SRDIT_DEV static long long bound(long long total, int cta, int ctas) { return total * cta / ctas; }
+  // the item that holds step `at` (which is below total())
+  SRDIT_DEV void locate(long long at) {
+    b = 0;
+    for (;; ++b) {
+      nt = tiles(b);
+      const long long n = static_cast<long long>(nt) * per;
+      if (at < n) break;
+      at -= n;
+    }
+    rest = static_cast<int>(at / nt);
+    t0 = static_cast<int>(at - static_cast<long long>(rest) * nt);
+  }
+  SRDIT_DEV Walk(const Args& args, int cta, int ctas)
+      : a(args), b(0), rest(0), nt(0), per(args.nq * args.nhp), s(0), s1(0), t0(0) {
+    if (a.ranged) {
+      const long long all = total();
+      s = bound(all, cta, ctas);
+      s1 = bound(all, cta + 1, ctas);
+      if (s < s1) locate(s);
+    } else {
+      b = cta / per;
+      rest = cta % per;
+      if (b < a.B) nt = tiles(b);
+    }
+  }
+  SRDIT_DEV void item(Item& o) const {
+    o.b = b;
+    o.h0 = rest / a.nq * a.pack;
+    o.tok0 = rest % a.nq * 2 * a.rt;
+    o.act1 = o.tok0 + a.rt < a.Lq;
+    o.len = key_count(a, b);
+  }
+  // the next item with keys, or false
+  SRDIT_DEV bool next(Item& o) {
+    if (a.ranged) {
+      if (s >= s1) return false;
+      while (rest >= per) {
+        rest = 0;
+        nt = tiles(++b);
+        if (nt == 0) rest = per;
+      }
+      item(o);
+      o.t0 = t0;
+      o.t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + (s1 - s)));
+      const int slot = 2 * static_cast<int>(blockIdx.x);
+      o.slot = o.t0 > 0 ? slot : o.t1 < nt ? slot + 1 : -1;
+      s += o.t1 - o.t0;
+      t0 = 0;
+      ++rest;
+      return true;
+    }
+    while (b < a.B && nt == 0) step();
+    if (b >= a.B) return false;
+    item(o);
+    o.t0 = 0;
+    o.t1 = nt;
+    o.slot = -1;
+    step();
+    return true;
+  }
+  SRDIT_DEV void step() {
+    rest += gridDim.x;
+    if (rest >= per) {
+      b += rest / per;
+      rest %= per;
+      if (b < a.B) nt = tiles(b);
+    }
+  }
+};
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
@@ -173,8 +296,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   tc_fence_after();
   // tensor memory: S0 @0, S1 @128 (weights over the first 64 columns), O0 @256, O1 @384
   const uint32_t tmem_base = *tmem_slot;
-  const int step = static_cast<int>(gridDim.x);
-
+  // registers: 104 for the producer's and the issuer's warps, 200 for the softmax's (3 x
+  // 128 threads were launched with 168 each)
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
@@ -205,9 +330,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         ++nq[t];
         return true;
       };
-      for (int i = blockIdx.x; i < a.items && ok; i += step) {
-        const Item it = item_of(a, i);
-        if (it.t0 == it.t1) continue;
+      Walk walk(a, blockIdx.x, gridDim.x);
+      Item it;
+      while (ok && walk.next(it)) {
         const int g = it.h0 / a.group;
         const int kh = a.k_one_head ? 0 : g, kb = a.k_one ? 0 : it.b;
         const int vh = a.v_one_head ? 0 : g, vb = a.v_one ? 0 : it.b;
@@ -254,19 +379,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                       sdesc_sw128(v_addr + k * 16 * 128, C::SLAB, 1024), idesc_o,
                       (!first || k > 0) ? 1u : 0u);
       };
-      // first item with keys
-      int i = blockIdx.x;
+      Walk walk(a, blockIdx.x, gridDim.x);
       Item it = {};
-      auto seek = [&](int from, Item& o) {
-        int x = from;
-        for (; x < a.items; x += step) {
-          o = item_of(a, x);
-          if (o.t0 < o.t1) break;
-        }
-        return x;
-      };
-      i = seek(i, it);
-      bool ok = i < a.items;
+      bool on = walk.next(it), ok = on;
       if (ok) {
         ok = mbar_wait(&q_full[0], 0u, a.status, abort_flag) && kv_wait(0);
         if (ok) {
@@ -287,16 +402,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         }
       }
       int j = it.t0;
-      while (ok && i < a.items) {
+      while (ok && on) {
         // the step after (it, j): the item's next key tile, or another item's first
         Item nx = it;
-        int ni = i, nj = j + 1;
+        int nj = j + 1;
         const bool last = nj == it.t1;
+        bool more = true;
         if (last) {
-          ni = seek(i + step, nx);
+          more = walk.next(nx);
           nj = nx.t0;
         }
-        const bool more = ni < a.items;
         const int uv = idx + 1, uk = idx + 2;
         ok = kv_wait(uv);
         bool k_ready = false;
@@ -327,30 +442,30 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         if (more) tc_commit(&empty[uk % STAGES]);
         idx += 2;
         it = nx;
-        i = ni;
+        on = more;
         j = nj;
       }
     }
     __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------ softmax
-    const int t = (warp - 2) >> 2;  // query tile
+    const int t = (warp - 4) >> 2;  // query tile
     const int sub = warp & 3;       // tensor-memory lane quarter
     const int row = sub * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>(sub * 32) << 16;
     const uint32_t s_tmem = tmem_base + t_lane + t * 128u;
     const uint32_t o_tmem = tmem_base + t_lane + 256u + t * 128u;
     const uint64_t c2 = f2_pack(a.c, a.c);
-    const int row_tok = row / a.pack, row_head = row % a.pack;
-    const bool row_in = row < a.pack * a.rt;
+    uint8_t* stg = smem + C::OFF_STG + (warp - 4) * 4096;
     int ns = 0, no = 0, idx = 0;
     bool ok = true;
-    for (int i = blockIdx.x; i < a.items && ok; i += step) {
-      const Item it = item_of(a, i);
+    Walk walk(a, blockIdx.x, gridDim.x);
+    Item it;
+    while (walk.next(it)) {
       const int n_tiles = it.t1 - it.t0;
       const bool act = t == 0 || it.act1;
-      const int tok = it.tok0 + t * a.rt + row_tok;
-      const bool row_ok = act && row_in && tok < a.Lq;
       float m = neg_inf(), l = 0.f;
       if (act) {
         for (int j = 0; j < n_tiles; ++j) {
@@ -452,64 +567,91 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
           if (lane == 0) mbar_arrive(&p_full[t]);
         }
         if (!ok) break;
-        if (n_tiles > 0) {
-          if (!mbar_wait(&o_full[t], static_cast<uint32_t>(no) & 1u, a.status, abort_flag)) {
-            ok = false;
-            break;
-          }
-          ++no;
-          tc_fence_after();
+        if (!mbar_wait(&o_full[t], static_cast<uint32_t>(no) & 1u, a.status, abort_flag)) {
+          ok = false;
+          break;
         }
-        // O / l (or, of a part, O, m and l) of this row
-        const int head = it.h0 + row_head;
-        if (a.splits == 1) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          T* out = static_cast<T*>(a.out) + it.b * a.os[0] + tok * a.os[1] + head * a.os[2];
+        ++no;
+        tc_fence_after();
+        // O / l (or, of a part, O, m and l): the warp's 32 rows go through its staging
+        // buffer 128 bytes of each at a time, so that a store covers four whole rows
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int r0 = lane >> 3, piece = lane & 7;
+        if (it.slot < 0) {
+          T* out = static_cast<T*>(a.out) + it.b * a.os[0] + it.h0 * a.os[2];
 #pragma unroll 1
-          for (int w = 0; w < DP / 16; ++w) {
-            uint32_t o[16];
-            if (n_tiles > 0) {
-              tmem_ld16(o_tmem + w * 16, o);
+          for (int d = 0; d < DP; d += 64) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              uint32_t o[32];
+              tmem_ld32(o_tmem + d + w * 32, o);
               tmem_ld_wait();
-            } else {
+              uint32_t r[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = 0u;
-            }
-            uint32_t r[8];
+              for (int e = 0; e < 16; ++e)
+                r[e] = pack2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv, T{});
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              r[e] = pack2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv, T{});
-            if (row_ok) {
-              if (w * 16 < a.D)
-                *reinterpret_cast<uint4*>(out + w * 16) = make_uint4(r[0], r[1], r[2], r[3]);
-              if (w * 16 + 8 < a.D)
-                *reinterpret_cast<uint4*>(out + w * 16 + 8) = make_uint4(r[4], r[5], r[6], r[7]);
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint4*>(stg + lane * 128 + (((w * 4 + e) ^ (lane & 7)) << 4)) =
+                    make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
             }
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int r = x * 4 + r0;
+              const int at = sub * 32 + r;
+              const int rt = at / a.pack;
+              const int tok = it.tok0 + t * a.rt + rt;
+              if (rt < a.rt && tok < a.Lq && d + piece * 8 < a.D)
+                *reinterpret_cast<uint4*>(out + tok * a.os[1] + (at - rt * a.pack) * a.os[2] + d +
+                                          piece * 8) =
+                    *reinterpret_cast<const uint4*>(stg + r * 128 + ((piece ^ (r & 7)) << 4));
+            }
+            __syncwarp();
           }
         } else {
-          const long long rows = static_cast<long long>(a.B) * a.Lq * a.H;
-          const long long at = it.part * rows + (static_cast<long long>(it.b) * a.Lq + tok) * a.H + head;
-          float* ml = a.ws + a.splits * rows * a.D + at * 2;
-          if (row_ok) *reinterpret_cast<float2*>(ml) = make_float2(m, l);
-          if (n_tiles > 0) {
-            float* po = a.ws + at * a.D;
+          const long long at = static_cast<long long>(it.slot) * SLOT_ROWS + t * TILE + row;
+          float* po = a.ws + (at - lane) * a.D;
+          float* ml = a.ws + 2ll * gridDim.x * SLOT_ROWS * a.D + at * 2;
+          *reinterpret_cast<float2*>(ml) = make_float2(m, l);
 #pragma unroll 1
-            for (int w = 0; w < DP / 16; ++w) {
-              uint32_t o[16];
-              tmem_ld16(o_tmem + w * 16, o);
-              tmem_ld_wait();
+          for (int d = 0; d < DP; d += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_tmem + d, o);
+            tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 16; e += 4)
-                if (row_ok && w * 16 + e < a.D)
-                  *reinterpret_cast<uint4*>(po + w * 16 + e) =
-                      make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int r = x * 4 + r0;
+              if (d + piece * 4 < a.D)
+                *reinterpret_cast<uint4*>(po + static_cast<long long>(r) * a.D + d + piece * 4) =
+                    *reinterpret_cast<const uint4*>(stg + r * 128 + ((piece ^ (r & 7)) << 4));
             }
+            __syncwarp();
           }
         }
         // the next item's first weights, published after this, free O
         tc_fence_before();
       }
       idx += 2 * n_tiles;
+    }
+    // samples without keys
+    if (a.kv_lens || a.Lk == 0) {
+      const int pieces = a.D / 8;
+      const int n = a.Lq * a.H * pieces;  // below 2^31: checked at the call
+      for (int b = 0; b < a.B; ++b) {
+        if (key_count(a, b) > 0) continue;
+        for (int x = blockIdx.x * 256 + threadIdx.x - 128; x < n; x += gridDim.x * 256) {
+          const int th = x / pieces;
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + b * a.os[0] + (th / a.H) * a.os[1] +
+                                    (th % a.H) * a.os[2] + (x - th * pieces) * 8) =
+              make_uint4(0, 0, 0, 0);
+        }
+      }
     }
   }
   tc_fence_before();
@@ -520,158 +662,291 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   }
 }
 
-// ---------------------------------------------------------------- token_kernel
-// mma.sync m16n8k16: rows = the query rows of one key head (tokens x grouped
-// heads, up to 16). A warp takes blocks of 16 keys. The contraction over the head's
-// dims may run in any order, so thread c of a quad holds dims 8c..8c+7 of each 32 (one
-// 16-byte load) for both operands; the output's columns may be numbered in any order,
-// so lane group g holds value columns 8g..8g+7 of each 64.
-constexpr int TOKEN_WARPS = 4;
-
+// One block per 32 rows of the slot at each bound between two CTAs' ranges: joins the
+// parts of the item that the bound cuts, at the first bound inside it. The parts'
+// slots are found once per block.
 template <typename T>
-SRDIT_DEV void mma16816(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+__global__ void __launch_bounds__(256)
+    join_ranges_kernel(const __grid_constant__ Args a, int ctas) {
+  pdl_begin();
+  __shared__ int slots[MAX_RANGES];
+  __shared__ int n_slots;
+  __shared__ Item it;
+  if (threadIdx.x == 0) {
+    n_slots = 0;
+    Walk w(a, 0, 1);
+    const long long all = w.total();
+    const int c = blockIdx.x + 1;
+    const long long at = Walk::bound(all, c, ctas);
+    if (at < all) {
+      w.locate(at);
+      const long long start = at - w.t0, end = start + w.nt;
+      // (not between two items, and not a later bound of an item cut before)
+      if (w.t0 > 0 && Walk::bound(all, c - 1, ctas) <= start) {
+        w.item(it);
+        int n = 0;
+        long long from = Walk::bound(all, c - 1, ctas);
+        for (int p = c - 1; p < ctas && from < end; ++p) {
+          const long long to = Walk::bound(all, p + 1, ctas);
+          if (from < to) slots[n++] = from > start ? 2 * p : 2 * p + 1;
+          from = to;
+        }
+        n_slots = n;
+      }
+    }
+  }
+  __syncthreads();
+  const int n = n_slots;
+  if (n == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + 2ll * ctas * SLOT_ROWS * a.D);
+#pragma unroll 1
+  for (int x = warp; x < 32; x += 8) {
+    const int r = blockIdx.y * 32 + x;
+    const int tr = r % TILE, rt = tr / a.pack;
+    const int tok = it.tok0 + (r / TILE) * a.rt + rt;
+    if (rt >= a.rt || tok >= a.Lq) continue;
+    join_rows<T>(a, n, [&](int p) { return static_cast<long long>(slots[p]) * SLOT_ROWS + r; }, ml,
+                 static_cast<T*>(a.out) + it.b * a.os[0] + tok * a.os[1] +
+                     (it.h0 + tr - rt * a.pack) * a.os[2],
+                 lane);
+  }
+}
+
+// ---------------------------------------------------------------- token_kernel
+// mma.sync m16n8k16 with the keys as its rows, S^T = K Q^T and O^T = V^T P^T: the query
+// rows of one key head (tokens x grouped heads) are the columns, NT times 8 of them. A warp
+// takes blocks of 16 keys. The contraction over the head's dims may run in any order, so
+// thread c of a quad holds dims 16c..16c+15 of each 64 (16-byte loads) for both operands;
+// O's rows may be numbered in any order, so lane group g holds value columns 8g..8g+7 of
+// each 64. The weights change from accumulator to operand layout by movmatrix.
+template <typename T>
+SRDIT_DEV void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                        uint32_t b0, uint32_t b1) {
   if constexpr (__is_same(T, __nv_bfloat16))
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-SRDIT_DEV uint4 ld16(const void* p) {
+SRDIT_DEV uint32_t transpose8x8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+SRDIT_DEV uint4 lds16(uint32_t src) {
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-      : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(src));
   return v;
 }
 
+// PER_SM: CTAs that share an SM's shared memory, which leaves a warp's ring 6, 3 or 2 blocks
+// of 128-wide heads, twice that of 64-wide ones. A warp alone on its scheduler takes 1300
+// cycles for a block's 230 instructions, nearly all of it their latency, so a full grid has
+// three CTAs an SM (168 registers) and is bounded by memory; a small grid is bounded by
+// that latency and wants its next blocks there already.
+constexpr int TOKEN_WARPS = 4;
+
+template <int DP, int NT, int PER_SM>
+struct TokenCfg {
+  static constexpr int NC = DP / 32;  // 32-dim pieces of q and k
+  static constexpr int NV = DP / 64;  // 64-column pieces of v
+  static constexpr int SLAB = 16 * 128;         // 16 rows x 64 values, 128-byte swizzle
+  static constexpr int BLK = 2 * NV * SLAB;     // a block: k, then v
+  static constexpr int STAGES = 6 / PER_SM * (DP == 128 ? 1 : 2);
+  static constexpr int RING = TOKEN_WARPS * STAGES * BLK;
+  // after the keys: each warp's O [8 NT][DP + 4], then the CTA's, over the ring
+  static constexpr int SMEM = RING + 1024;
+  static_assert(RING >= (TOKEN_WARPS + 1) * 8 * NT * (DP + 4) * 4, "O fits the ring");
+};
+
 // blockIdx.x: part of the keys, blockIdx.y: (sample, key head). The parts of a row
 // that run as one cluster are joined in its shared memory.
-template <typename T, int DP>
-__global__ void __launch_bounds__(TOKEN_WARPS * 32)
-    token_kernel(const __grid_constant__ Args a, int cluster) {
+//
+// A warp's ring in shared memory is its own. A block goes to registers whole, and its slot
+// is refilled before the block is computed. (Of the ways to fill it, TMA boxes of 16 rows
+// keep up with the memory; 16 bytes a lane by cp.async held an SM to 45 GB/s, and a bulk
+// copy per row to one row in 8 to 20 cycles.)
+template <typename T, int DP, int NT, int PER_SM>
+__global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
+    token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ Args a, int cluster) {
   pdl_begin();
-  constexpr int NC = DP / 32;  // 32-dim pieces of q and k
-  constexpr int NV = DP / 64;  // 64-column pieces of v
-  __shared__ float so[TOKEN_WARPS][16][DP + 4];
-  __shared__ float2 sml[TOKEN_WARPS][16];  // {m, l} of each warp
-  __shared__ float co[16][DP + 4];         // the CTA's own part
-  __shared__ float2 cml[16];
+  using C = TokenCfg<DP, NT, PER_SM>;
+  constexpr int NC = C::NC, NV = C::NV, STAGES = C::STAGES, R = 8 * NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float(*so)[R][DP + 4] = reinterpret_cast<float(*)[R][DP + 4]>(ring);
+  float(*co)[DP + 4] = so[TOKEN_WARPS];   // the CTA's own part
+  __shared__ float2 sml[TOKEN_WARPS][R];  // {m, l} of each warp
+  __shared__ float2 cml[R];
+  __shared__ uint64_t bars[TOKEN_WARPS][STAGES];
   if (cluster > 1) cluster_arrive();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int part = blockIdx.x;
-  const int b = blockIdx.y / a.Hkv, kvh = blockIdx.y % a.Hkv;
+  // samples of different lengths side by side, so that an SM gets some of each
+  const int b = blockIdx.y % a.B, kvh = blockIdx.y / a.B;
   const int rows = a.Lq * a.group;
   const int len = key_count(a, b);
   const int nblk = (len + 15) / 16;
   const int blk0 = static_cast<int>(static_cast<long long>(nblk) * part / a.splits);
   const int blk1 = static_cast<int>(static_cast<long long>(nblk) * (part + 1) / a.splits);
-  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
-  const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const uint8_t* mrow = a.mask ? a.mask + b * a.mask_stride : nullptr;
 
-  // row r: token r / group, head kvh * group + r % group
-  uint4 qf[2][NC];
+  uint64_t* full = bars[warp];
+  if (lane == 0) {
+    if (warp == 0) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
+    for (int x = 0; x < STAGES; ++x) mbar_init(&full[x], 1);
+    fence_barrier_init();
+  }
+  uint8_t* mine = ring + warp * STAGES * C::BLK;
+  auto fetch = [&](int blk, int slot) {  // by lane 0
+    if (blk < blk1) {
+      uint8_t* dst = mine + slot * C::BLK;
+      mbar_arrive_expect_tx(&full[slot], C::BLK);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = g + 8 * h;
+      for (int x = 0; x < NV; ++x) {
+        tma_load_4d(dst + x * C::SLAB, &tmK, &full[slot], x * 64, a.k_one_head ? 0 : kvh, blk * 16,
+                    a.k_one ? 0 : b);
+        tma_load_4d(dst + (NV + x) * C::SLAB, &tmV, &full[slot], x * 64, a.v_one_head ? 0 : kvh,
+                    blk * 16, a.v_one ? 0 : b);
+      }
+    }
+  };
+  if (lane == 0) {
+#pragma unroll
+    for (int x = 0; x < STAGES; ++x) fetch(blk0 + warp + x * TOKEN_WARPS, x);
+  }
+  __syncwarp();
+  // column r: token r / group, head kvh * group + r % group
+  uint4 qf[NT][NC];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = g + 8 * n;
     const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + (r / a.group) * a.qs[1] +
                   (static_cast<long long>(kvh) * a.group + r % a.group) * a.qs[2];
 #pragma unroll
-    for (int x = 0; x < NC; ++x)
-      qf[h][x] = r < rows && x * 32 + c * 8 < a.D ? ld16(qp + x * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+    for (int x = 0; x < NC; ++x) {
+      const int d = (x >> 1) * 64 + c * 16 + (x & 1) * 8;
+      qf[n][x] = r < rows && d < a.D ? *reinterpret_cast<const uint4*>(qp + d)
+                                     : make_uint4(0, 0, 0, 0);
+    }
   }
-  float o[NV * 8][4];
+  float o[NT][NV * 4][4];
+  // of columns 2c and 2c + 1, in every lane group; l: this lane's keys only
+  float m[NT][2], l[NT][2];
 #pragma unroll
-  for (int x = 0; x < NV * 8; ++x)
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[x][e] = 0.f;
-  float m[2] = {neg_inf(), neg_inf()}, l[2] = {0.f, 0.f};
+    for (int x = 0; x < NV * 4; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][x][e] = 0.f;
+    m[n][0] = m[n][1] = neg_inf();
+    l[n][0] = l[n][1] = 0.f;
+  }
 
+  // a lane's pieces of a swizzled slab: k row g (piece 2c, 2c + 1), v rows 2c and 2c + 1
+  // (piece g); every read of 8 lanes meets all banks once
+  const uint32_t k_at = static_cast<uint32_t>(g * 128 + (((2 * c) ^ g) << 4));
+  const uint32_t v_at = static_cast<uint32_t>(2 * c * 128 + ((g ^ (2 * c)) << 4));
+  const uint32_t v_at1 = static_cast<uint32_t>((2 * c + 1) * 128 + ((g ^ (2 * c + 1)) << 4));
+  int slot = 0;
+  uint32_t phase = 0;
 #pragma unroll 1
   for (int blk = blk0 + warp; blk < blk1; blk += TOKEN_WARPS) {
     const int key0 = blk * 16;
-    // k rows g and g + 8 of the block; v rows 2c, 2c + 1, 2c + 8, 2c + 9
-    uint4 kf[2][NC], vf[4][NV];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long long key = min(key0 + g + 8 * h, len - 1);
-#pragma unroll
-      for (int x = 0; x < NC; ++x)
-        kf[h][x] = x * 32 + c * 8 < a.D ? ld16(kp + key * a.ks[1] + x * 32 + c * 8)
-                                        : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const long long key = min(key0 + 2 * c + (r & 1) + (r >> 1) * 8, len - 1);
-#pragma unroll
-      for (int x = 0; x < NV; ++x)
-        vf[r][x] = x * 64 + g * 8 < a.D ? ld16(vp + key * a.vs[1] + x * 64 + g * 8)
-                                        : make_uint4(0, 0, 0, 0);
-    }
     uint32_t vis = 0xffffu;
     if (mrow || key0 + 16 > len) {
       const int key = key0 + (lane & 15);
       vis = __ballot_sync(0xffffffffu, key < len && (!mrow || __ldg(mrow + key) != 0)) & 0xffffu;
-      if (vis == 0u) continue;  // warp-uniform
     }
-    float s[2][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[h][e] = 0.f;
-#pragma unroll
-      for (int x = 0; x < NC; ++x) {
-        const uint32_t a0[4] = {qf[0][x].x, qf[1][x].x, qf[0][x].y, qf[1][x].y};
-        const uint32_t a1[4] = {qf[0][x].z, qf[1][x].z, qf[0][x].w, qf[1][x].w};
-        mma16816<T>(s[h], a0, kf[h][x].x, kf[h][x].y);
-        mma16816<T>(s[h], a1, kf[h][x].z, kf[h][x].w);
-      }
+    if (!mbar_wait(&full[slot], phase, a.status)) {
+      // having given up, let the loads in flight land before the ring is used again
+      for (int i = 0; i < 200; ++i) __nanosleep(1000);
+      break;
     }
-    if (vis != 0xffffu) {
+    // k rows g and g + 8; v rows 2c, 2c + 1, 2c + 8, 2c + 9
+    const uint32_t src = smem_u32(mine) + static_cast<uint32_t>(slot * C::BLK);
+    uint4 kf[2][NC], vf[4][NV];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!((vis >> (h * 8 + 2 * c + (e & 1))) & 1u)) s[h][e] = neg_inf();
+      for (int x = 0; x < NC; ++x)
+        kf[h][x] = lds16(src + (x >> 1) * C::SLAB + h * 1024 + ((x & 1) ? k_at ^ 16u : k_at));
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int x = 0; x < NV; ++x)
+        vf[r][x] = lds16(src + (NV + x) * C::SLAB + (r >> 1) * 1024 + ((r & 1) ? v_at1 : v_at));
+    __syncwarp();  // every lane has read the slot
+    if (lane == 0) fetch(blk + STAGES * TOKEN_WARPS, slot);
+    __syncwarp();
+    if (++slot == STAGES) {
+      slot = 0;
+      phase ^= 1u;
+    }
+    if (vis != 0xffffu) {  // values of unseen keys: zeros
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (!((vis >> (2 * c + (r & 1) + (r >> 1) * 8)) & 1u))
 #pragma unroll
           for (int x = 0; x < NV; ++x) vf[r][x] = make_uint4(0, 0, 0, 0);
     }
-    // rows g (e = 0, 1) and g + 8 (e = 2, 3), keys 2c, 2c + 1 of both halves
-    uint32_t pf[4];
-    float alpha[2];
+    uint32_t pf[NT][2];
+    bool moved = false;
+    float alpha[NT][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float top = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * a.c;
-      const float mn = fmaxf(m[r], top);
-      const float neg = mn == neg_inf() ? 0.f : -mn;
-      alpha[r] = ex2(m[r] + neg);
-      m[r] = mn;
-      float p[4];
+    for (int n = 0; n < NT; ++n) {
+      // two chains of products, joined at the end
+      float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = ex2(fmaf(s[e >> 1][2 * r + (e & 1)], a.c, neg));
-      l[r] = l[r] * alpha[r] + ((p[0] + p[1]) + (p[2] + p[3]));
-      pf[r] = pack2(p[0], p[1], T{});
-      pf[r + 2] = pack2(p[2], p[3], T{});
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-      for (int x = 0; x < NV * 8; ++x) {
-        o[x][0] *= alpha[0];
-        o[x][1] *= alpha[0];
-        o[x][2] *= alpha[1];
-        o[x][3] *= alpha[1];
+      for (int x = 0; x < NC; ++x) {
+        mma16816<T>(s, kf[0][x].x, kf[1][x].x, kf[0][x].y, kf[1][x].y, qf[n][x].x, qf[n][x].y);
+        mma16816<T>(s2, kf[0][x].z, kf[1][x].z, kf[0][x].w, kf[1][x].w, qf[n][x].z, qf[n][x].w);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += s2[e];
+      if (vis != 0xffffu) {
+        if (!((vis >> g) & 1u)) s[0] = s[1] = neg_inf();
+        if (!((vis >> (g + 8)) & 1u)) s[2] = s[3] = neg_inf();
+      }
+      // s[0], s[2]: column 2c, keys g and g + 8; s[1], s[3]: column 2c + 1
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = fmaxf(s[e], s[2 + e]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float mn = fmaxf(m[n][e], top * a.c);
+        const float neg = mn == neg_inf() ? 0.f : -mn;
+        alpha[n][e] = ex2(m[n][e] + neg);
+        moved |= mn != m[n][e];
+        m[n][e] = mn;
+        s[e] = ex2(fmaf(s[e], a.c, neg));
+        s[2 + e] = ex2(fmaf(s[2 + e], a.c, neg));
+        l[n][e] = fmaf(l[n][e], alpha[n][e], s[e] + s[2 + e]);
+      }
+      pf[n][0] = transpose8x8(pack2(s[0], s[1], T{}));
+      pf[n][1] = transpose8x8(pack2(s[2], s[3], T{}));
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < NV * 4; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][x][e] *= alpha[n][e & 1];
     }
 #pragma unroll
     for (int x = 0; x < NV; ++x) {
@@ -681,48 +956,59 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32)
       const uint32_t r3[4] = {vf[3][x].x, vf[3][x].y, vf[3][x].z, vf[3][x].w};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        // columns 2w (low halves) and 2w + 1 (high halves) of the lane group's eight
-        mma16816<T>(o[x * 8 + 2 * w], pf, __byte_perm(r0[w], r1[w], 0x5410),
-                    __byte_perm(r2[w], r3[w], 0x5410));
-        mma16816<T>(o[x * 8 + 2 * w + 1], pf, __byte_perm(r0[w], r1[w], 0x7632),
-                    __byte_perm(r2[w], r3[w], 0x7632));
+        // the lane group's columns 2w (operand row g) and 2w + 1 (row g + 8)
+        const uint32_t a0 = __byte_perm(r0[w], r1[w], 0x5410), a1 = __byte_perm(r0[w], r1[w], 0x7632);
+        const uint32_t a2 = __byte_perm(r2[w], r3[w], 0x5410), a3 = __byte_perm(r2[w], r3[w], 0x7632);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          mma16816<T>(o[n][x * 4 + w], a0, a1, a2, a3, pf[n][0], pf[n][1]);
       }
     }
   }
-  // this warp's part to shared memory. Output column n = 2c + (e & 1) of mma x is lane
-  // group n's: value column (x / 8) * 64 + n * 8 + x % 8
+  // every warp is done with its ring; O takes its place
+  __syncthreads();
+  // this warp's part: o[n][x * 4 + w][e] is query column 8n + 2c + (e & 1), value
+  // column 64x + 8g + 2w + (e >> 1)
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int row = g + 8 * r;
-    if (c == 0) sml[warp][row] = make_float2(m[r], l[r]);
-    if (row < rows) {
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int x = 0; x < NV * 8; ++x)
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          so[warp][row][(x >> 3) * 64 + (2 * c + e) * 8 + (x & 7)] = o[x][2 * r + e];
+      for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+      const int row = 8 * n + 2 * c + e;
+      if (g == 0) sml[warp][row] = make_float2(m[n][e], l[n][e]);
+      if (row < rows) {
+#pragma unroll
+        for (int x = 0; x < NV * 4; ++x)
+          *reinterpret_cast<float2*>(&so[warp][row][(x >> 2) * 64 + g * 8 + (x & 3) * 2]) =
+              make_float2(o[n][x][e], o[n][x][2 + e]);
+      }
     }
   }
   __syncthreads();
-  // the CTA's part
-  for (int x = threadIdx.x; x < rows * DP; x += TOKEN_WARPS * 32) {
-    const int row = x / DP, d = x % DP;
+  // the CTA's part, four columns a thread
+  constexpr int DQ = DP / 4;
+  for (int x = threadIdx.x; x < rows * DQ; x += TOKEN_WARPS * 32) {
+    const int row = x / DQ, d = x % DQ * 4;
     float top = neg_inf();
 #pragma unroll
     for (int w = 0; w < TOKEN_WARPS; ++w) top = fmaxf(top, sml[w][row].x);
-    float acc = 0.f, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
     if (top != neg_inf()) {
 #pragma unroll
       for (int w = 0; w < TOKEN_WARPS; ++w) {
         const float2 ml = sml[w][row];
         const float f = ex2(ml.x - top);
-        acc = fmaf(so[w][row][d], f, acc);
+        const float4 v = *reinterpret_cast<const float4*>(&so[w][row][d]);
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
         sum = fmaf(ml.y, f, sum);
       }
     }
-    co[row][d] = acc;
+    *reinterpret_cast<float4*>(&co[row][d]) = acc;
     if (d == 0) cml[row] = make_float2(top, sum);
   }
   int share = 0, shares = 1;
@@ -735,23 +1021,30 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32)
   } else {
     __syncthreads();
   }
-  // CTA `share` of the cluster joins every shares-th value of the parts
+  // CTA `share` of the cluster joins every shares-th four columns of the parts
   const long long all_rows = static_cast<long long>(a.B) * a.Lq * a.H;
   const int wparts = a.splits / cluster;
-  for (int x = threadIdx.x * shares + share; x < rows * a.D; x += TOKEN_WARPS * 32 * shares) {
-    const int row = x / a.D, d = x % a.D;
-    float top = neg_inf(), acc = 0.f, sum = 0.f;
+  const int dq = a.D / 4;
+  for (int x = threadIdx.x * shares + share; x < rows * dq; x += TOKEN_WARPS * 32 * shares) {
+    const int row = x / dq, d = (x - row * dq) * 4;
+    float top = neg_inf(), sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (cluster > 1) {
       const uint32_t ml0 = smem_u32(&cml[row]), o0 = smem_u32(&co[row][d]);
-      float pm[8], pl[8], po[8];
+      float pm[8], pl[8];
+      float4 po[8];
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
         pm[s] = neg_inf();
-        pl[s] = po[s] = 0.f;
+        pl[s] = 0.f;
+        po[s] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (s < cluster) {
-          const uint32_t ra = mapa_shared(ml0, s);
-          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(pm[s]), "=f"(pl[s]) : "r"(ra));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(po[s]) : "r"(mapa_shared(o0, s)));
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                       : "=f"(pm[s]), "=f"(pl[s])
+                       : "r"(mapa_shared(ml0, s)));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(po[s].x), "=f"(po[s].y), "=f"(po[s].z), "=f"(po[s].w)
+                       : "r"(mapa_shared(o0, s)));
         }
         top = fmaxf(top, pm[s]);
       }
@@ -759,22 +1052,28 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32)
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
           const float f = ex2(pm[s] - top);
-          acc = fmaf(po[s], f, acc);
+          acc.x = fmaf(po[s].x, f, acc.x);
+          acc.y = fmaf(po[s].y, f, acc.y);
+          acc.z = fmaf(po[s].z, f, acc.z);
+          acc.w = fmaf(po[s].w, f, acc.w);
           sum = fmaf(pl[s], f, sum);
         }
       }
     } else {
       top = cml[row].x;
       sum = cml[row].y;
-      acc = co[row][d];
+      acc = *reinterpret_cast<const float4*>(&co[row][d]);
     }
     const int tok = row / a.group, head = kvh * a.group + row % a.group;
     if (wparts == 1) {
-      static_cast<T*>(a.out)[b * a.os[0] + tok * a.os[1] + head * a.os[2] + d] =
-          static_cast<T>(sum == 0.f ? 0.f : acc / sum);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.os[0] + tok * a.os[1] +
+                                head * a.os[2] + d) =
+          make_uint2(pack2(acc.x * inv, acc.y * inv, T{}), pack2(acc.z * inv, acc.w * inv, T{}));
     } else {
-      const long long at = (part / cluster) * all_rows + (static_cast<long long>(b) * a.Lq + tok) * a.H + head;
-      a.ws[at * a.D + d] = acc;
+      const long long at =
+          (part / cluster) * all_rows + (static_cast<long long>(b) * a.Lq + tok) * a.H + head;
+      *reinterpret_cast<float4*>(a.ws + at * a.D + d) = acc;
       if (d == 0)
         *reinterpret_cast<float2*>(a.ws + wparts * all_rows * a.D + at * 2) = make_float2(top, sum);
     }
@@ -785,41 +1084,19 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32)
   }
 }
 
-// ---------------------------------------------------------------- combine_kernel
 // One warp per (sample, token, head): joins the parts that went through the workspace.
 template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Args a, int parts) {
+__global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__ Args a, int parts) {
   pdl_begin();
   const long long rows = static_cast<long long>(a.B) * a.Lq * a.H;
-  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const float* ml = a.ws + parts * rows * a.D;
-  float top = neg_inf();
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, ml[(s * rows + row) * 2]);
-#pragma unroll
-  for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int s = 0; s < parts; ++s) {
-    const float2 p = *reinterpret_cast<const float2*>(ml + (s * rows + row) * 2);
-    if (p.x == neg_inf()) continue;  // a part that saw no key wrote no O
-    const float f = ex2(p.x - top);
-    sum = fmaf(p.y, f, sum);
-    if (lane * 4 < a.D) {
-      const float4 v = *reinterpret_cast<const float4*>(a.ws + (s * rows + row) * a.D + lane * 4);
-      acc[0] = fmaf(v.x, f, acc[0]);
-      acc[1] = fmaf(v.y, f, acc[1]);
-      acc[2] = fmaf(v.z, f, acc[2]);
-      acc[3] = fmaf(v.w, f, acc[3]);
-    }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int h = static_cast<int>(row % a.H);
   const long long bi = row / a.H;
-  T* out = static_cast<T*>(a.out) + (bi / a.Lq) * a.os[0] + (bi % a.Lq) * a.os[1] + h * a.os[2];
-  if (lane * 4 < a.D)
-    *reinterpret_cast<uint2*>(out + lane * 4) =
-        make_uint2(pack2(acc[0] * inv, acc[1] * inv, T{}), pack2(acc[2] * inv, acc[3] * inv, T{}));
+  join_rows<T>(a, parts, [&](int p) { return p * rows + row; },
+               reinterpret_cast<const float2*>(a.ws + parts * rows * a.D),
+               static_cast<T*>(a.out) + (bi / a.Lq) * a.os[0] + (bi % a.Lq) * a.os[1] + h * a.os[2],
+               threadIdx.x & 31);
 }
 
 // ---------------------------------------------------------------- launch
@@ -827,8 +1104,14 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Ar
 struct Plan {
   bool token;
   int pack, rt, nq, nhp;
-  int splits, cluster, parts;  // parts: partial results per row in the workspace (1: none)
-  int items;
+  int per_sm;                  // token_kernel: CTAs that share an SM
+  int splits, cluster, parts;  // token_kernel; parts in the workspace per row (1: none)
+  bool ranged;
+  int ctas;                    // tile_kernel
+  long long ws_floats(const srdit_cross_attn_args& a) const {
+    if (token) return parts > 1 ? static_cast<long long>(parts) * a.B * a.Lq * a.H * (a.D + 2) : 0;
+    return ranged ? 2ll * ctas * SLOT_ROWS * (a.D + 2) : 0;
+  }
 };
 
 static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
@@ -837,17 +1120,26 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   p.token = static_cast<long long>(a.Lq) * group <= 16;
   p.splits = p.cluster = p.parts = 1;
   if (p.token) {
-    // about two CTAs an SM, each with a block of 16 keys per warp at least
     const int pairs = a.B * a.Hkv;
-    int want = (2 * sms + pairs - 1) / pairs;
-    const int most = (a.Lk + 63) / 64;
+    const int most_per_sm = a.Lq * group <= 8 ? 3 : 2;
+    const int blocks = (a.Lk + 15) / 16;
+    // CTAs that run at once, each with a block per warp at least
+    int want = sms * most_per_sm / pairs;
+    const int most = (blocks + TOKEN_WARPS - 1) / TOKEN_WARPS;
     if (want > most) want = most;
     while (p.cluster < 8 && 2 * p.cluster <= want) p.cluster *= 2;
     p.splits = p.cluster;
-    if (p.cluster == 8) {
-      p.parts = want / 8;
+    // more than a cluster's 8 parts cost a second launch: from 8 blocks a warp, and no more
+    // parts than leave it 4
+    const int warps = 8 * TOKEN_WARPS;
+    if (p.cluster == 8 && blocks >= 8 * warps) {
+      p.parts = want / 8 < blocks / (4 * warps) ? want / 8 : blocks / (4 * warps);
+      if (p.parts < 1) p.parts = 1;
       p.splits = 8 * p.parts;
     }
+    // (CTAs of one SM's whole shared memory and in clusters need room to be placed)
+    const int grid = pairs * p.splits;
+    p.per_sm = grid <= sms / 2 ? 1 : grid <= 2 * sms ? 2 : 3;
     return p;
   }
   // as many heads of a group in a tile as fill its rows (94% of them at least)
@@ -861,13 +1153,18 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   p.nq = (a.Lq + 2 * p.rt - 1) / (2 * p.rt);
   p.nhp = a.H / p.pack;
   const long long items = static_cast<long long>(p.nq) * p.nhp * a.B;
-  const int tiles = (a.Lk + TILE - 1) / TILE;
-  if (items * 2 <= sms) {
-    long long s = sms / items;
-    if (s > tiles / 2) s = tiles / 2;
-    if (s > 1) p.splits = p.parts = static_cast<int>(s);
-  }
-  p.items = static_cast<int>(items * p.splits);
+  const long long tiles = (a.Lk + TILE - 1) / TILE;
+  // Whole items leave a last round partly filled (and samples of different lengths,
+  // which only the device knows, more than that); ranges of equal steps do not, but
+  // joining their parts costs about what four steps do.
+  const long long whole = (items + sms - 1) / sms * tiles;
+  const long long steps = items * tiles;
+  if (sms > MAX_RANGES) sms = MAX_RANGES;
+  long long ctas = steps / 2 < sms ? steps / 2 : sms;
+  if (ctas < items && ctas < sms) ctas = items < sms ? items : sms;
+  p.ranged = a.B <= 64 && ctas > 1 && whole > (steps + ctas - 1) / ctas + 4;
+  if (!p.ranged) ctas = items < sms ? items : sms;
+  p.ctas = static_cast<int>(ctas);
   return p;
 }
 
@@ -889,36 +1186,58 @@ static int map_of(CUtensorMap* m, const void* p, const long long st[3], int B, i
   return make_tmap_4d(m, p, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, dims, strides, box);
 }
 
-template <typename T, int DP>
-static int launch_tile(const srdit_cross_attn_args& u, Args& a, const Plan& p, int sms,
-                       cudaStream_t stream) {
-  using C = TileCfg<DP>;
-  auto kern = tile_kernel<T, DP>;
+// k and v in boxes of `rows` keys (without keys nothing is loaded: the maps only have to be
+// valid)
+static int kv_maps(CUtensorMap* tk, CUtensorMap* tv, const srdit_cross_attn_args& u, int rows) {
+  const bool kv = u.Lk > 0;
+  const int B = kv ? u.B : 1;
+  const int rc = map_of(tk, kv ? u.k : u.q, u.k_stride, B, u.Lk, u.Hkv, u.D, 1, rows);
+  return rc ? rc : map_of(tv, kv ? u.v : u.q, u.v_stride, B, u.Lk, u.Hkv, u.D, 1, rows);
+}
+
+// the kernel's shared memory, set once per device
+template <typename Kern>
+static int set_smem(Kern kern, int bytes, std::atomic<bool>* done) {
   int dev = 0;
   cudaGetDevice(&dev);
-  static std::atomic<bool> attr_done[kMaxDevices] = {};
-  if (dev >= kMaxDevices || !attr_done[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    if (dev < kMaxDevices) attr_done[dev].store(true, std::memory_order_release);
-  }
-  CUtensorMap tq, tk, tv;
-  int rc = map_of(&tq, u.q, u.q_stride, u.B, u.Lq, u.H, u.D, p.pack, p.rt);
-  // (without keys nothing is loaded: the maps only have to be valid)
-  const bool kv = u.Lk > 0;
-  if (!rc) rc = map_of(&tk, kv ? u.k : u.q, u.k_stride, kv ? u.B : 1, u.Lk, u.Hkv, u.D, 1, TILE);
-  if (!rc) rc = map_of(&tv, kv ? u.v : u.q, u.v_stride, kv ? u.B : 1, u.Lk, u.Hkv, u.D, 1, TILE);
-  if (rc) return rc;
-  SRDIT_LAUNCH((kern), p.items < sms ? p.items : sms, TILE_THREADS, C::SMEM, stream, tq, tk, tv, a);
-  return static_cast<int>(cudaGetLastError());
+  if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return 0;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
+  return 0;
 }
 
 template <typename T, int DP>
-static int launch_token(const Args& a, const Plan& p, cudaStream_t stream) {
+static int launch_tile(const srdit_cross_attn_args& u, Args& a, const Plan& p,
+                       cudaStream_t stream) {
+  using C = TileCfg<DP>;
+  auto kern = tile_kernel<T, DP>;
+  static std::atomic<bool> attr_done[kMaxDevices] = {};
+  int rc = set_smem(kern, C::SMEM, attr_done);
+  if (rc) return rc;
+  CUtensorMap tq, tk, tv;
+  rc = map_of(&tq, u.q, u.q_stride, u.B, u.Lq, u.H, u.D, p.pack, p.rt);
+  if (!rc) rc = kv_maps(&tk, &tv, u, TILE);
+  if (rc) return rc;
+  SRDIT_LAUNCH((kern), p.ctas, TILE_THREADS, C::SMEM, stream, tq, tk, tv, a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int DP, int NT, int PER_SM>
+static int launch_token(const srdit_cross_attn_args& u, const Args& a, const Plan& p,
+                        cudaStream_t stream) {
+  using C = TokenCfg<DP, NT, PER_SM>;
+  static std::atomic<bool> attr_done[kMaxDevices] = {};
+  int rc = set_smem(token_kernel<T, DP, NT, PER_SM>, C::SMEM, attr_done);
+  if (rc) return rc;
+  CUtensorMap tk, tv;
+  rc = kv_maps(&tk, &tv, u, 16);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.B * a.Hkv));
   cfg.blockDim = dim3(TOKEN_WARPS * 32);
+  cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -929,21 +1248,39 @@ static int launch_token(const Args& a, const Plan& p, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, token_kernel<T, DP>, a, p.cluster));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, token_kernel<T, DP, NT, PER_SM>, tk, tv, a, p.cluster));
+}
+
+template <typename T, int DP>
+static int launch_token_n(const srdit_cross_attn_args& u, const Args& a, const Plan& p,
+                          cudaStream_t stream) {
+  if (a.Lq * a.group <= 8)
+    switch (p.per_sm) {
+      case 1: return launch_token<T, DP, 1, 1>(u, a, p, stream);
+      case 2: return launch_token<T, DP, 1, 2>(u, a, p, stream);
+      default: return launch_token<T, DP, 1, 3>(u, a, p, stream);
+    }
+  return p.per_sm == 1 ? launch_token<T, DP, 2, 1>(u, a, p, stream)
+                       : launch_token<T, DP, 2, 2>(u, a, p, stream);
 }
 
 template <typename T>
-static int run(const srdit_cross_attn_args& u, Args& a, const Plan& p, int sms,
-               cudaStream_t stream) {
+static int run(const srdit_cross_attn_args& u, Args& a, const Plan& p, cudaStream_t stream) {
   int rc;
   if (p.token)
-    rc = u.D <= 64 ? launch_token<T, 64>(a, p, stream) : launch_token<T, 128>(a, p, stream);
+    rc = u.D <= 64 ? launch_token_n<T, 64>(u, a, p, stream)
+                   : launch_token_n<T, 128>(u, a, p, stream);
   else
-    rc = u.D <= 64 ? launch_tile<T, 64>(u, a, p, sms, stream)
-                   : launch_tile<T, 128>(u, a, p, sms, stream);
-  if (rc || p.parts == 1) return rc;
+    rc = u.D <= 64 ? launch_tile<T, 64>(u, a, p, stream) : launch_tile<T, 128>(u, a, p, stream);
+  if (rc) return rc;
+  if (p.ranged) {
+    const dim3 grid(static_cast<unsigned>(p.ctas - 1), SLOT_ROWS / 32);
+    SRDIT_LAUNCH((join_ranges_kernel<T>), grid, 256, 0, stream, a, p.ctas);
+    return static_cast<int>(cudaGetLastError());
+  }
+  if (p.parts == 1) return 0;
   const long long rows = static_cast<long long>(u.B) * u.Lq * u.H;
-  SRDIT_LAUNCH((combine_kernel<T>), static_cast<unsigned>((rows + 7) / 8), 256, 0, stream, a, p.parts);
+  SRDIT_LAUNCH((join_parts_kernel<T>), static_cast<unsigned>((rows + 3) / 4), 128, 0, stream, a, p.parts);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -966,7 +1303,7 @@ static int check(const srdit_cross_attn_args& a) {
     return SRDIT_EINVAL;
   if (a.D <= 0 || a.D > 128 || a.D % 8) return SRDIT_EUNSUPPORTED;
   if (static_cast<long long>(a.B) * a.Hkv > 65535 ||
-      static_cast<long long>(a.B) * a.Lq * a.H > (1ll << 30))
+      static_cast<long long>(a.B) * a.Lq * a.H > (1ll << 26))
     return SRDIT_EUNSUPPORTED;
   if (!check_view(a.q, a.q_stride, a.B, a.Lq, a.H) || !check_view(a.k, a.k_stride, a.B, a.Lk, a.Hkv) ||
       !check_view(a.v, a.v_stride, a.B, a.Lk, a.Hkv) || !check_view(a.out, a.o_stride, a.B, a.Lq, a.H))
@@ -985,9 +1322,9 @@ static int check(const srdit_cross_attn_args& a) {
 
 using namespace srdit;
 
-extern "C" int srdit_cross_attn_splits(const srdit_cross_attn_args* args) {
-  if (!args || xattn::check(*args) != 0) return 1;
-  return xattn::make_plan(*args, xattn::sms_here()).parts;
+extern "C" int srdit_cross_attn_workspace(const srdit_cross_attn_args* args) {
+  if (!args || xattn::check(*args) != 0) return 0;
+  return static_cast<int>((xattn::make_plan(*args, xattn::sms_here()).ws_floats(*args) + 255) / 256);
 }
 
 extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t stream) {
@@ -995,10 +1332,9 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   const srdit_cross_attn_args& u = *args;
   const int rc = xattn::check(u);
   if (rc) return rc < 0 ? rc : 0;
-  const int sms = xattn::sms_here();
-  const xattn::Plan p = xattn::make_plan(u, sms);
-  if (p.parts > 1) {
-    const long long need = static_cast<long long>(p.parts) * u.B * u.Lq * u.H * (u.D + 2) * 4;
+  const xattn::Plan p = xattn::make_plan(u, xattn::sms_here());
+  const long long need = 4 * p.ws_floats(u);
+  if (need > 0) {
     if (!u.workspace || u.workspace_bytes < need) return SRDIT_EINVAL;
     if (reinterpret_cast<uintptr_t>(u.workspace) & 15u) return SRDIT_EALIGN;
   }
@@ -1025,7 +1361,7 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.nq = p.nq;
   a.nhp = p.nhp;
   a.splits = p.splits;
-  a.items = p.items;
+  a.ranged = p.ranged;
   a.q_one = u.q_stride[0] == 0;
   a.k_one = u.k_stride[0] == 0;
   a.v_one = u.v_stride[0] == 0;
@@ -1037,6 +1373,6 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.c = u.scale * xattn::kLog2e;
   a.ws = static_cast<float*>(u.workspace);
   a.status = u.status;
-  return u.dtype == SRDIT_BF16 ? xattn::run<__nv_bfloat16>(u, a, p, sms, stream)
-                               : xattn::run<__half>(u, a, p, sms, stream);
+  return u.dtype == SRDIT_BF16 ? xattn::run<__nv_bfloat16>(u, a, p, stream)
+                               : xattn::run<__half>(u, a, p, stream);
 }

@@ -359,11 +359,10 @@ def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, st
     if status is not None:
         a.status = status.data_ptr()
     ref = ctypes.byref(a)
-    n = _lib.count("srdit_cross_attn_splits", ref)
-    ws = None
-    if n > 1:
-        ws = torch.empty(n * B * Lq * H * (D + 2), dtype=torch.float32, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel() * 4
+    kib = _lib.count("srdit_cross_attn_workspace", ref)
+    if kib:
+        ws = torch.empty(kib << 10, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), kib << 10
     _launch("srdit_cross_attn", ref, _stream(q.device), kind="cross_attn",
             work=4 * B * Lq * H * D * Lk)
     return out

@@ -598,9 +598,9 @@ int srdit_int8_gemm(const void* a, const float* a_scale, const void* w, const fl
  * {batch, token, head} in elements (multiples of 8; a batch stride of 0 repeats one sample, a
  * head stride of 0 of k or v one head) and unit stride over D;
  * bases 16-byte aligned. D a multiple of 8, at most 128. scale > 0. workspace: where
- * srdit_cross_attn_splits (which reads the sizes and the type only) returns n > 1, n partial
- * results per row are joined through it: n * B * Lq * H * (D + 2) floats, 16-byte aligned; else
- * it may be NULL.
+ * srdit_cross_attn_workspace (which reads the sizes and the type only) returns n > 0, partial
+ * results of rows split over their keys are joined through it: n KiB, 16-byte aligned. B * Lq * H
+ * at most 2^26, B * Hkv at most 65535.
  * Replaces: flash_attention with k_lens (video_refiner/wan/modules/attention.py:61-168, called
  *   at wan/modules/sr_dit/models.py:1057).
  */
@@ -621,7 +621,7 @@ typedef struct srdit_cross_attn_args {
   uint32_t* status;
 } srdit_cross_attn_args;
 int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t stream);
-int srdit_cross_attn_splits(const srdit_cross_attn_args* args);
+int srdit_cross_attn_workspace(const srdit_cross_attn_args* args);
 
 #ifdef __cplusplus
 }
