@@ -46,6 +46,7 @@ struct Args {
   int group;       // H / Hkv
   int pack;        // tile_kernel: heads of a group side by side in a query tile
   int rt;          // tile_kernel: tokens of a query tile (pack * rt rows)
+  uint32_t pack_inv;  // ceil(2^16 / pack): x / pack = x * pack_inv >> 16 for x < 128
   int nq, nhp;     // tile_kernel: query-tile pairs per head pack, head packs
   int q_one, k_one, v_one;         // one sample's tensor for all (batch stride 0)
   int k_one_head, v_one_head;      // one key head for all (head stride 0)
@@ -65,10 +66,40 @@ SRDIT_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// the largest of three; NaN if one is
 SRDIT_DEV float max3(float x, float y, float z) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
+}
+// 2^x of a pair on the FMA and ALU pipes, for x <= 2^8: x = n + f with n the nearest
+// integer, 2^f by a polynomial that is off by 7.5e-5 (degree 3) or 2.7e-6 (degree 4) of it
+// at most (fitted for the smallest largest relative error on [-1/2, 1/2]; bf16 weights are
+// rounded by 3.9e-3, fp16 ones by 4.9e-4), n added to the exponent's bits. x below -126
+// counts as -126, whose weight is nothing beside the maximum's.
+template <int DEG>
+SRDIT_DEV uint64_t ex2_poly(uint64_t x2) {
+  const float2 x = f2_split(x2);
+  const uint64_t c = f2_pack(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const uint64_t magic = f2_pack(12582912.f, 12582912.f);  // 1.5 2^23: the sum's low bits are n
+  const uint64_t t = f2_add(c, magic);
+  const uint64_t f = f2_sub(c, f2_sub(t, magic));
+  uint64_t p;
+  if constexpr (DEG == 3) {
+    p = f2_fma(f, f2_pack(0.05517166852951050f, 0.05517166852951050f),
+               f2_pack(0.24261112511157990f, 0.24261112511157990f));
+    p = f2_fma(f, p, f2_pack(0.69326096773147583f, 0.69326096773147583f));
+    p = f2_fma(f, p, f2_pack(0.99992805719375610f, 0.99992805719375610f));
+  } else {
+    p = f2_fma(f, f2_pack(0.00957010220736265f, 0.00957010220736265f),
+               f2_pack(0.05591785907745361f, 0.05591785907745361f));
+    p = f2_fma(f, p, f2_pack(0.24024744331836700f, 0.24024744331836700f));
+    p = f2_fma(f, p, f2_pack(0.69312179088592529f, 0.69312179088592529f));
+    p = f2_fma(f, p, f2_pack(0.99999928474426270f, 0.99999928474426270f));
+  }
+  const float2 tf = f2_split(t), pf = f2_split(p);
+  return u64_of((__float_as_uint(tf.x) << 23) + __float_as_uint(pf.x),
+                (__float_as_uint(tf.y) << 23) + __float_as_uint(pf.y));
 }
 SRDIT_DEV uint32_t pack2(float x, float y, __nv_bfloat16) {
   uint32_t d;
@@ -133,7 +164,14 @@ SRDIT_DEV void join_rows(const Args& a, int n, At at, const float2* ml, T* out, 
 // ---------------------------------------------------------------- tile_kernel
 constexpr int TILE_THREADS = 384;  // producer and MMA issuer, 2 x 4 softmax warps
 constexpr int SLOT_ROWS = 2 * TILE;
-constexpr int MAX_RANGES = 256;  // CTAs of a ranged launch
+#ifndef POLY_OF_4
+#define POLY_OF_4 0
+#endif
+#ifndef HALVES
+#define HALVES 1
+#endif
+constexpr int MAX_RANGES = 256;  // CTAs of a launch that may be ranged
+constexpr int RANGE_STEPS = 4;
 
 template <int DP>
 struct TileCfg {
@@ -143,7 +181,7 @@ struct TileCfg {
   static constexpr int OFF_KV = 2 * BYTES;
   static constexpr int OFF_STG = OFF_KV + STAGES * BYTES;  // 32 rows x 128 bytes per warp
   static constexpr int OFF_BAR = OFF_STG + 8 * 4096;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
@@ -157,48 +195,80 @@ struct Item {
   bool act1;  // the second query tile has tokens
 };
 
-// The items of one CTA. Either whole items, every gridDim-th one; or (ranged) an equal
-// share of all key-tile steps, whose first and last items may be parts of items. Parts
-// cost a trip through the workspace and a second launch, whole items cost the CTAs'
-// idle time in the last round: make_plan compares them.
+// The items of one CTA: whole items, every gridDim-th one; and (ranged) in place of a last
+// round that would leave CTAs idle, an equal share of its items' key-tile steps, whose
+// first and last items may be parts of items. Whole rounds come first: their CTAs go through
+// a head's keys side by side, out of the same lines of the cache; ranges do not. Parts cost
+// a trip through the workspace and a second launch; make_plan compares.
 struct Walk {
   const Args& a;
-  int b, rest;          // sample, item within it
-  int nt, per;          // the sample's key tiles; items per sample
-  long long s, s1;      // ranged: next step, end
+  int cta, ctas;
+  int per;              // items per sample
+  int b, rest, nt;      // sample, item within it, the sample's key tiles
+  long long whole;      // items that are taken whole, in rounds of ctas
+  long long at;         // the next of this CTA's whole items
+  long long s, s1;      // ranged: next step, end; steps count from the first ranged item
   int t0;               // ranged: first key tile of the next item
+  bool in_range;
+
   SRDIT_DEV int tiles(int x) const { return (key_count(a, x) + TILE - 1) / TILE; }
-  SRDIT_DEV long long total() const {
-    if (!a.kv_lens) return static_cast<long long>((a.Lk + TILE - 1) / TILE) * per * a.B;
-    long long t = 0;
-    for (int x = 0; x < a.B; ++x) t += static_cast<long long>(tiles(x)) * per;
-    return t;
-  }
   SRDIT_DEV static long long bound(long long total, int cta, int ctas) { return total * cta / ctas; }
-  // the item that holds step `at` (which is below total())
-  SRDIT_DEV void locate(long long at) {
-    b = 0;
-    for (;; ++b) {
+  // items and steps of the samples that have keys
+  SRDIT_DEV void totals(long long& items, long long& steps) const {
+    items = steps = 0;
+    if (!a.kv_lens) {
+      items = a.Lk > 0 ? static_cast<long long>(per) * a.B : 0;
+      steps = items * ((a.Lk + TILE - 1) / TILE);
+      return;
+    }
+    for (int x = 0; x < a.B; ++x) {
+      const int n = tiles(x);
+      if (n > 0) items += per;
+      steps += static_cast<long long>(n) * per;
+    }
+  }
+  // the n-th item of samples with keys; returns the steps before it
+  SRDIT_DEV long long find_item(long long n) {
+    long long before = 0;
+    for (b = 0;; ++b) {
+      nt = tiles(b);
+      if (nt == 0) continue;
+      if (n < per) break;
+      n -= per;
+      before += static_cast<long long>(nt) * per;
+    }
+    rest = static_cast<int>(n);
+    return before + n * nt;
+  }
+  // the item that holds step x, counted from the first step of all
+  SRDIT_DEV void find_step(long long x) {
+    for (b = 0;; ++b) {
       nt = tiles(b);
       const long long n = static_cast<long long>(nt) * per;
-      if (at < n) break;
-      at -= n;
+      if (x < n) break;
+      x -= n;
     }
-    rest = static_cast<int>(at / nt);
-    t0 = static_cast<int>(at - static_cast<long long>(rest) * nt);
+    rest = static_cast<int>(x / nt);
+    t0 = static_cast<int>(x - static_cast<long long>(rest) * nt);
   }
-  SRDIT_DEV Walk(const Args& args, int cta, int ctas)
-      : a(args), b(0), rest(0), nt(0), per(args.nq * args.nhp), s(0), s1(0), t0(0) {
+  // the ranged steps [first, first + count), from the first step of all
+  SRDIT_DEV void ranged_steps(long long& first, long long& count) {
+    long long items, steps;
+    totals(items, steps);
+    whole = a.ranged ? items / ctas * ctas : items;
+    first = whole < items ? find_item(whole) : steps;
+    count = steps - first;
+  }
+  SRDIT_DEV Walk(const Args& args, int cta_, int ctas_)
+      : a(args), cta(cta_), ctas(ctas_), per(args.nq * args.nhp), b(0), rest(0), nt(0), at(cta_), s(0),
+        s1(0), t0(0), in_range(false) {
+    long long first, count;
+    ranged_steps(first, count);
     if (a.ranged) {
-      const long long all = total();
-      s = bound(all, cta, ctas);
-      s1 = bound(all, cta + 1, ctas);
-      if (s < s1) locate(s);
-    } else {
-      b = cta / per;
-      rest = cta % per;
-      if (b < a.B) nt = tiles(b);
+      s = first + bound(count, cta, ctas);
+      s1 = first + bound(count, cta + 1, ctas);
     }
+    if (at < whole) find_item(at);
   }
   SRDIT_DEV void item(Item& o) const {
     o.b = b;
@@ -207,41 +277,40 @@ struct Walk {
     o.act1 = o.tok0 + a.rt < a.Lq;
     o.len = key_count(a, b);
   }
-  // the next item with keys, or false
+  // the next item, or false
   SRDIT_DEV bool next(Item& o) {
-    if (a.ranged) {
-      if (s >= s1) return false;
-      while (rest >= per) {
-        rest = 0;
-        nt = tiles(++b);
-        if (nt == 0) rest = per;
-      }
+    if (at < whole) {
       item(o);
-      o.t0 = t0;
-      o.t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + (s1 - s)));
-      const int slot = 2 * static_cast<int>(blockIdx.x);
-      o.slot = o.t0 > 0 ? slot : o.t1 < nt ? slot + 1 : -1;
-      s += o.t1 - o.t0;
-      t0 = 0;
-      ++rest;
+      o.t0 = 0;
+      o.t1 = nt;
+      o.slot = -1;
+      at += ctas;
+      if (at < whole) {
+        rest += ctas;
+        while (rest >= per || nt == 0) {
+          if (nt > 0) rest -= per;
+          nt = tiles(++b);
+        }
+      }
       return true;
     }
-    while (b < a.B && nt == 0) step();
-    if (b >= a.B) return false;
-    item(o);
-    o.t0 = 0;
-    o.t1 = nt;
-    o.slot = -1;
-    step();
-    return true;
-  }
-  SRDIT_DEV void step() {
-    rest += gridDim.x;
-    if (rest >= per) {
-      b += rest / per;
-      rest %= per;
-      if (b < a.B) nt = tiles(b);
+    if (s >= s1) return false;
+    if (!in_range) {
+      find_step(s);
+      in_range = true;
     }
+    while (rest >= per || nt == 0) {
+      rest = 0;
+      nt = tiles(++b);
+    }
+    item(o);
+    o.t0 = t0;
+    o.t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + (s1 - s)));
+    o.slot = o.t0 > 0 ? 2 * cta : o.t1 < nt ? 2 * cta + 1 : -1;
+    s += o.t1 - o.t0;
+    t0 = 0;
+    ++rest;
+    return true;
   }
 };
 
@@ -261,10 +330,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   uint64_t* q_empty = q_full + 2;
   uint64_t* s_full = q_empty + 2;     // scores of a tile ready
   uint64_t* p_full = s_full + 2;      // its weights written (one arrival per warp)
-  uint64_t* o_full = p_full + 2;      // its last product done
+  uint64_t* p_half = p_full + 2;      // the first half of them
+  uint64_t* o_full = p_half + 2;      // its last product done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  static_assert((2 * STAGES + 10) * 8 + 8 <= 256, "barrier area");
+  static_assert((2 * STAGES + 12) * 8 + 8 <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -277,6 +347,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
+      mbar_init(&p_half[t], 4);
       mbar_init(&o_full[t], 1);
     }
     *abort_flag = 0u;
@@ -371,10 +442,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         }
         tc_commit(&s_full[t]);
       };
-      auto product = [&](int t, int u, bool first) {  // O_t (+)= P_t V, V in ring use u
+      auto product = [&](int t, int u, bool first, int k0, int k1) {  // O_t (+)= P_t V, V in use u
         const uint32_t v_addr = smem_u32(smem + C::OFF_KV + (u % STAGES) * C::BYTES);
 #pragma unroll
-        for (int k = 0; k < TILE / 16; ++k)
+        for (int k = k0; k < k1; ++k)
           mma_bf16_ts(tmem_base + 256u + t * 128u, tmem_base + t * 128u + k * 8u,
                       sdesc_sw128(v_addr + k * 16 * 128, C::SLAB, 1024), idesc_o,
                       (!first || k > 0) ? 1u : 0u);
@@ -417,11 +488,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         bool k_ready = false;
         for (int t = 0; t < 2 && ok; ++t) {
           if (t == 0 || it.act1) {
+            if (HALVES) {
+              ok = mbar_wait(&p_half[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              product(t, uv, j == it.t0, 0, 4);
+            }
             ok = mbar_wait(&p_full[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
             if (!ok) break;
             tc_fence_after();
             ++np[t];
-            product(t, uv, j == it.t0);
+            product(t, uv, j == it.t0, HALVES ? 4 : 0, 8);
             if (last) tc_commit(&o_full[t]);
           }
           if (more && (t == 0 || nx.act1)) {
@@ -467,19 +544,30 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       const int n_tiles = it.t1 - it.t0;
       const bool act = t == 0 || it.act1;
       float m = neg_inf(), l = 0.f;
+      const uint8_t* mrow = a.mask ? a.mask + it.b * a.mask_stride : nullptr;
+      // the mask's bytes of this lane's four keys of a tile, read a tile ahead
+      uint32_t seen = 0xfu;
+      auto read_mask = [&](int key0) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int key = key0 + w * 32 + lane;
+          r |= (key < it.len && __ldg(mrow + key) != 0 ? 1u : 0u) << w;
+        }
+        return r;
+      };
       if (act) {
+        if (mrow) seen = read_mask(it.t0 * TILE);
         for (int j = 0; j < n_tiles; ++j) {
           const int key0 = (it.t0 + j) * TILE;
           const bool masked = a.mask != nullptr || key0 + TILE > it.len;
           uint32_t vis[4];
           if (masked) {
-            const uint8_t* mrow = a.mask ? a.mask + it.b * a.mask_stride : nullptr;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const int key = key0 + w * 32 + lane;
+            for (int w = 0; w < 4; ++w)
               vis[w] = __ballot_sync(0xffffffffu,
-                                     key < it.len && (!mrow || __ldg(mrow + key) != 0));
-            }
+                                     key0 + w * 32 + lane < it.len && ((seen >> w) & 1u));
+            if (mrow && j + 1 < n_tiles) seen = read_mask(key0 + TILE);
             // the values of unseen keys are zeroed: thread r of tile 0 has key r
             if (t == 0) {
               const int u = idx + 2 * j + 1;
@@ -523,12 +611,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll
             for (int e = 1; e < 31; e += 2)
               mx[w] = max3(mx[w], __uint_as_float(s[w][e]), __uint_as_float(s[w][e + 1]));
-            mx[w] = fmaxf(mx[w], __uint_as_float(s[w][31]));
+            mx[w] = max3(mx[w], mx[w], __uint_as_float(s[w][31]));
           }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.c;
+          const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.c;
           // the maximum moves (and O is rescaled) only when a tile's is 8 above it:
           // weights stay below 2^8 and the quotient is the same
-          const bool raise = top > m + 8.f || (m == neg_inf() && top != neg_inf());
+          // (written so that a NaN raises it too, and stays in l and O)
+          const bool raise = !(top <= m + 8.f) && top != neg_inf();
           const float m_new = raise ? top : m;
           const float alpha = raise ? ex2(m - m_new) : 1.f;
           m = m_new;
@@ -552,12 +641,25 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             uint32_t pw[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const float2 x = f2_split(f2_fma(u64_of(s[w][e], s[w][e + 1]), c2, neg_m2));
-              const float p0 = ex2(x.x), p1 = ex2(x.y);
-              sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], f2_pack(p0, p1));
-              pw[e >> 1] = pack2(p0, p1, T{});
+              const uint64_t x2 = f2_fma(u64_of(s[w][e], s[w][e + 1]), c2, neg_m2);
+              uint64_t p2;
+              if (((e >> 1) & 3) < POLY_OF_4) {
+                p2 = ex2_poly<__is_same(T, __nv_bfloat16) ? 3 : 4>(x2);
+              } else {
+                const float2 x = f2_split(x2);
+                p2 = f2_pack(ex2(x.x), ex2(x.y));
+              }
+              sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], p2);
+              const float2 p = f2_split(p2);
+              pw[e >> 1] = pack2(p.x, p.y, T{});
             }
             tmem_st16(s_tmem + w * 16, pw);
+            if (HALVES && w == 1) {  // the first 64 keys' weights: their product can begin
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[t]);
+            }
           }
           const float2 sp = f2_split(f2_add(sum[0], sum[1]));
           l = l * alpha + (sp.x + sp.y);
@@ -578,34 +680,42 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int r0 = lane >> 3, piece = lane & 7;
         if (it.slot < 0) {
-          T* out = static_cast<T*>(a.out) + it.b * a.os[0] + it.h0 * a.os[2];
-#pragma unroll 1
+          T* out = static_cast<T*>(a.out) + it.b * a.os[0] + it.h0 * a.os[2] + piece * 8;
+          T* rows[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int at = sub * 32 + x * 4 + r0;
+            const int rt = static_cast<int>(at * a.pack_inv >> 16);
+            const int tok = it.tok0 + t * a.rt + rt;
+            rows[x] = rt < a.rt && tok < a.Lq
+                          ? out + tok * a.os[1] + (at - rt * a.pack) * a.os[2]
+                          : nullptr;
+          }
+#pragma unroll
           for (int d = 0; d < DP; d += 64) {
+            uint32_t o[2][32];
+            tmem_ld32(o_tmem + d, o[0]);
+            tmem_ld32(o_tmem + d + 32, o[1]);
+            tmem_ld_wait();
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              uint32_t o[32];
-              tmem_ld32(o_tmem + d + w * 32, o);
-              tmem_ld_wait();
-              uint32_t r[16];
+            for (int e = 0; e < 8; ++e) {
+              uint32_t r[4];
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                r[e] = pack2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv, T{});
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<uint4*>(stg + lane * 128 + (((w * 4 + e) ^ (lane & 7)) << 4)) =
-                    make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+              for (int y = 0; y < 4; ++y) {
+                const int at = (e & 3) * 8 + y * 2;
+                r[y] = pack2(__uint_as_float(o[e >> 2][at]) * inv,
+                             __uint_as_float(o[e >> 2][at + 1]) * inv, T{});
+              }
+              *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                  make_uint4(r[0], r[1], r[2], r[3]);
             }
             __syncwarp();
+            if (d + piece * 8 < a.D) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const int r = x * 4 + r0;
-              const int at = sub * 32 + r;
-              const int rt = at / a.pack;
-              const int tok = it.tok0 + t * a.rt + rt;
-              if (rt < a.rt && tok < a.Lq && d + piece * 8 < a.D)
-                *reinterpret_cast<uint4*>(out + tok * a.os[1] + (at - rt * a.pack) * a.os[2] + d +
-                                          piece * 8) =
-                    *reinterpret_cast<const uint4*>(stg + r * 128 + ((piece ^ (r & 7)) << 4));
+              for (int x = 0; x < 8; ++x)
+                if (rows[x])
+                  *reinterpret_cast<uint4*>(rows[x] + d) = *reinterpret_cast<const uint4*>(
+                      stg + (x * 4 + r0) * 128 + ((piece ^ ((x * 4 + r0) & 7)) << 4));
             }
             __syncwarp();
           }
@@ -674,20 +784,21 @@ __global__ void __launch_bounds__(256)
   __shared__ Item it;
   if (threadIdx.x == 0) {
     n_slots = 0;
-    Walk w(a, 0, 1);
-    const long long all = w.total();
+    Walk w(a, 0, ctas);
+    long long first, count;
+    w.ranged_steps(first, count);
     const int c = blockIdx.x + 1;
-    const long long at = Walk::bound(all, c, ctas);
-    if (at < all) {
-      w.locate(at);
+    const long long at = Walk::bound(count, c, ctas);
+    if (at < count) {
+      w.find_step(first + at);
       const long long start = at - w.t0, end = start + w.nt;
       // (not between two items, and not a later bound of an item cut before)
-      if (w.t0 > 0 && Walk::bound(all, c - 1, ctas) <= start) {
+      if (w.t0 > 0 && Walk::bound(count, c - 1, ctas) <= start) {
         w.item(it);
         int n = 0;
-        long long from = Walk::bound(all, c - 1, ctas);
+        long long from = Walk::bound(count, c - 1, ctas);
         for (int p = c - 1; p < ctas && from < end; ++p) {
-          const long long to = Walk::bound(all, p + 1, ctas);
+          const long long to = Walk::bound(count, p + 1, ctas);
           if (from < to) slots[n++] = from > start ? 2 * p : 2 * p + 1;
           from = to;
         }
@@ -700,16 +811,50 @@ __global__ void __launch_bounds__(256)
   if (n == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float2* ml = reinterpret_cast<const float2*>(a.ws + 2ll * ctas * SLOT_ROWS * a.D);
-#pragma unroll 1
-  for (int x = warp; x < 32; x += 8) {
-    const int r = blockIdx.y * 32 + x;
-    const int tr = r % TILE, rt = tr / a.pack;
-    const int tok = it.tok0 + (r / TILE) * a.rt + rt;
-    if (rt >= a.rt || tok >= a.Lq) continue;
-    join_rows<T>(a, n, [&](int p) { return static_cast<long long>(slots[p]) * SLOT_ROWS + r; }, ml,
-                 static_cast<T*>(a.out) + it.b * a.os[0] + tok * a.os[1] +
-                     (it.h0 + tr - rt * a.pack) * a.os[2],
-                 lane);
+  // four rows of a warp together
+  float m[4], l[4];
+  float4 acc[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    m[x] = neg_inf();
+    l[x] = 0.f;
+    acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const int r0 = blockIdx.y * 32 + warp * 4;
+  const bool on = lane * 4 < a.D;
+  for (int p = 0; p < n; ++p) {
+    const long long row = static_cast<long long>(slots[p]) * SLOT_ROWS + r0;
+    float2 pm[4];
+    float4 v[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      pm[x] = ml[row + x];
+      v[x] = on ? *reinterpret_cast<const float4*>(a.ws + (row + x) * a.D + lane * 4)
+                : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (pm[x].x == neg_inf()) continue;  // it saw no key (or the row is none)
+      const float mn = max3(m[x], m[x], pm[x].x);
+      const float f0 = ex2(m[x] - mn), f1 = ex2(pm[x].x - mn);
+      m[x] = mn;
+      l[x] = l[x] * f0 + pm[x].y * f1;
+      acc[x].x = acc[x].x * f0 + v[x].x * f1;
+      acc[x].y = acc[x].y * f0 + v[x].y * f1;
+      acc[x].z = acc[x].z * f0 + v[x].z * f1;
+      acc[x].w = acc[x].w * f0 + v[x].w * f1;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int tr = (r0 + x) % TILE, rt = tr / a.pack;
+    const int tok = it.tok0 + (r0 + x) / TILE * a.rt + rt;
+    if (rt >= a.rt || tok >= a.Lq || !on) continue;
+    const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + it.b * a.os[0] + tok * a.os[1] +
+                              (it.h0 + tr - rt * a.pack) * a.os[2] + lane * 4) =
+        make_uint2(pack2(acc[x].x * inv, acc[x].y * inv, T{}),
+                   pack2(acc[x].z * inv, acc[x].w * inv, T{}));
   }
 }
 
@@ -1154,16 +1299,19 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   p.nhp = a.H / p.pack;
   const long long items = static_cast<long long>(p.nq) * p.nhp * a.B;
   const long long tiles = (a.Lk + TILE - 1) / TILE;
-  // Whole items leave a last round partly filled (and samples of different lengths,
-  // which only the device knows, more than that); ranges of equal steps do not, but
-  // joining their parts costs about what four steps do.
-  const long long whole = (items + sms - 1) / sms * tiles;
-  const long long steps = items * tiles;
+  // A last round of whole items is partly empty (and samples of different lengths, which
+  // only the device knows, leave more idle than that); ranges of equal steps are not, but
+  // joining their parts costs about what RANGE_STEPS steps do.
   if (sms > MAX_RANGES) sms = MAX_RANGES;
-  long long ctas = steps / 2 < sms ? steps / 2 : sms;
-  if (ctas < items && ctas < sms) ctas = items < sms ? items : sms;
-  p.ranged = a.B <= 64 && ctas > 1 && whole > (steps + ctas - 1) / ctas + 4;
-  if (!p.ranged) ctas = items < sms ? items : sms;
+  const long long last = items % sms;
+  long long ctas = sms;
+  if (items < sms) {  // one round
+    ctas = last * tiles / 2 < sms ? last * tiles / 2 : sms;
+    if (ctas < items) ctas = items;
+  }
+  const long long idle = last ? tiles - (last * tiles + ctas - 1) / ctas : 0;
+  p.ranged = a.B <= 64 && idle > RANGE_STEPS;
+  if (!p.ranged && items < sms) ctas = items;
   p.ctas = static_cast<int>(ctas);
   return p;
 }
@@ -1358,6 +1506,7 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.group = u.H / u.Hkv;
   a.pack = p.pack;
   a.rt = p.rt;
+  a.pack_inv = p.pack > 0 ? (65536u + p.pack - 1) / p.pack : 0;
   a.nq = p.nq;
   a.nhp = p.nhp;
   a.splits = p.splits;
