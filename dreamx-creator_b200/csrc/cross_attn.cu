@@ -46,7 +46,6 @@ struct Args {
   int group;       // H / Hkv
   int pack;        // tile_kernel: heads of a group side by side in a query tile
   int rt;          // tile_kernel: tokens of a query tile (pack * rt rows)
-  uint32_t pack_inv;  // ceil(2^16 / pack): x / pack = x * pack_inv >> 16 for x < 128
   int nq, nhp;     // tile_kernel: query-tile pairs per head pack, head packs
   int q_one, k_one, v_one;         // one sample's tensor for all (batch stride 0)
   int k_one_head, v_one_head;      // one key head for all (head stride 0)
@@ -71,35 +70,6 @@ SRDIT_DEV float max3(float x, float y, float z) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
-}
-// 2^x of a pair on the FMA and ALU pipes, for x <= 2^8: x = n + f with n the nearest
-// integer, 2^f by a polynomial that is off by 7.5e-5 (degree 3) or 2.7e-6 (degree 4) of it
-// at most (fitted for the smallest largest relative error on [-1/2, 1/2]; bf16 weights are
-// rounded by 3.9e-3, fp16 ones by 4.9e-4), n added to the exponent's bits. x below -126
-// counts as -126, whose weight is nothing beside the maximum's.
-template <int DEG>
-SRDIT_DEV uint64_t ex2_poly(uint64_t x2) {
-  const float2 x = f2_split(x2);
-  const uint64_t c = f2_pack(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const uint64_t magic = f2_pack(12582912.f, 12582912.f);  // 1.5 2^23: the sum's low bits are n
-  const uint64_t t = f2_add(c, magic);
-  const uint64_t f = f2_sub(c, f2_sub(t, magic));
-  uint64_t p;
-  if constexpr (DEG == 3) {
-    p = f2_fma(f, f2_pack(0.05517166852951050f, 0.05517166852951050f),
-               f2_pack(0.24261112511157990f, 0.24261112511157990f));
-    p = f2_fma(f, p, f2_pack(0.69326096773147583f, 0.69326096773147583f));
-    p = f2_fma(f, p, f2_pack(0.99992805719375610f, 0.99992805719375610f));
-  } else {
-    p = f2_fma(f, f2_pack(0.00957010220736265f, 0.00957010220736265f),
-               f2_pack(0.05591785907745361f, 0.05591785907745361f));
-    p = f2_fma(f, p, f2_pack(0.24024744331836700f, 0.24024744331836700f));
-    p = f2_fma(f, p, f2_pack(0.69312179088592529f, 0.69312179088592529f));
-    p = f2_fma(f, p, f2_pack(0.99999928474426270f, 0.99999928474426270f));
-  }
-  const float2 tf = f2_split(t), pf = f2_split(p);
-  return u64_of((__float_as_uint(tf.x) << 23) + __float_as_uint(pf.x),
-                (__float_as_uint(tf.y) << 23) + __float_as_uint(pf.y));
 }
 SRDIT_DEV uint32_t pack2(float x, float y, __nv_bfloat16) {
   uint32_t d;
@@ -164,12 +134,6 @@ SRDIT_DEV void join_rows(const Args& a, int n, At at, const float2* ml, T* out, 
 // ---------------------------------------------------------------- tile_kernel
 constexpr int TILE_THREADS = 384;  // producer and MMA issuer, 2 x 4 softmax warps
 constexpr int SLOT_ROWS = 2 * TILE;
-#ifndef POLY_OF_4
-#define POLY_OF_4 0
-#endif
-#ifndef HALVES
-#define HALVES 1
-#endif
 constexpr int MAX_RANGES = 256;  // CTAs of a launch that may be ranged
 constexpr int RANGE_STEPS = 4;
 
@@ -317,7 +281,8 @@ struct Walk {
 template <typename T, int DP>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Args a) {
+                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                const __grid_constant__ Args a) {
   pdl_begin();
   using C = TileCfg<DP>;
   constexpr int STAGES = C::STAGES;
@@ -488,17 +453,15 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         bool k_ready = false;
         for (int t = 0; t < 2 && ok; ++t) {
           if (t == 0 || it.act1) {
-            if (HALVES) {
-              ok = mbar_wait(&p_half[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-              product(t, uv, j == it.t0, 0, 4);
-            }
+            ok = mbar_wait(&p_half[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            product(t, uv, j == it.t0, 0, 4);
             ok = mbar_wait(&p_full[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
             if (!ok) break;
             tc_fence_after();
             ++np[t];
-            product(t, uv, j == it.t0, HALVES ? 4 : 0, 8);
+            product(t, uv, j == it.t0, 4, 8);
             if (last) tc_commit(&o_full[t]);
           }
           if (more && (t == 0 || nx.act1)) {
@@ -642,19 +605,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               const uint64_t x2 = f2_fma(u64_of(s[w][e], s[w][e + 1]), c2, neg_m2);
-              uint64_t p2;
-              if (((e >> 1) & 3) < POLY_OF_4) {
-                p2 = ex2_poly<__is_same(T, __nv_bfloat16) ? 3 : 4>(x2);
-              } else {
-                const float2 x = f2_split(x2);
-                p2 = f2_pack(ex2(x.x), ex2(x.y));
-              }
+              const float2 x = f2_split(x2);
+              const uint64_t p2 = f2_pack(ex2(x.x), ex2(x.y));
               sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], p2);
               const float2 p = f2_split(p2);
               pw[e >> 1] = pack2(p.x, p.y, T{});
             }
             tmem_st16(s_tmem + w * 16, pw);
-            if (HALVES && w == 1) {  // the first 64 keys' weights: their product can begin
+            if (w == 1) {  // the first 64 keys' weights: their product can begin
               tmem_st_wait();
               tc_fence_before();
               __syncwarp();
@@ -680,23 +638,18 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int r0 = lane >> 3, piece = lane & 7;
         if (it.slot < 0) {
-          T* out = static_cast<T*>(a.out) + it.b * a.os[0] + it.h0 * a.os[2] + piece * 8;
-          T* rows[8];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int at = sub * 32 + x * 4 + r0;
-            const int rt = static_cast<int>(at * a.pack_inv >> 16);
-            const int tok = it.tok0 + t * a.rt + rt;
-            rows[x] = rt < a.rt && tok < a.Lq
-                          ? out + tok * a.os[1] + (at - rt * a.pack) * a.os[2]
-                          : nullptr;
-          }
-#pragma unroll
+          // the warp's rows are a box of the output: heads x tokens
+          const int tok = it.tok0 + t * a.rt + sub * 32 / a.pack;
+          const int head = it.h0 + sub * 32 % a.pack;
+#pragma unroll 1
           for (int d = 0; d < DP; d += 64) {
             uint32_t o[2][32];
             tmem_ld32(o_tmem + d, o[0]);
             tmem_ld32(o_tmem + d + 32, o[1]);
+            // the box before this one has left the buffer
+            if (lane == 0) bulk_wait_group_read0();
             tmem_ld_wait();
+            __syncwarp();
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               uint32_t r[4];
@@ -709,18 +662,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
               *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
                   make_uint4(r[0], r[1], r[2], r[3]);
             }
+            fence_proxy_async_smem();
             __syncwarp();
-            if (d + piece * 8 < a.D) {
-#pragma unroll
-              for (int x = 0; x < 8; ++x)
-                if (rows[x])
-                  *reinterpret_cast<uint4*>(rows[x] + d) = *reinterpret_cast<const uint4*>(
-                      stg + (x * 4 + r0) * 128 + ((piece ^ ((x * 4 + r0) & 7)) << 4));
+            if (lane == 0 && tok < a.Lq && d < a.D) {  // boxes start inside the output
+              tma_store_4d(&tmO, stg, d, head, tok, it.b);
+              bulk_commit_group();
             }
-            __syncwarp();
           }
         } else {
           const long long at = static_cast<long long>(it.slot) * SLOT_ROWS + t * TILE + row;
+          if (lane == 0) bulk_wait_group_read0();  // (the last box has left the buffer)
+          __syncwarp();
           float* po = a.ws + (at - lane) * a.D;
           float* ml = a.ws + 2ll * gridDim.x * SLOT_ROWS * a.D + at * 2;
           *reinterpret_cast<float2*>(ml) = make_float2(m, l);
@@ -749,6 +701,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       }
       idx += 2 * n_tiles;
     }
+    if (lane == 0) bulk_wait_group_all();
     // samples without keys
     if (a.kv_lens || a.Lk == 0) {
       const int pieces = a.D / 8;
@@ -1287,13 +1240,9 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
     p.per_sm = grid <= sms / 2 ? 1 : grid <= 2 * sms ? 2 : 3;
     return p;
   }
-  // as many heads of a group in a tile as fill its rows (94% of them at least)
+  // heads of a group side by side in a query tile, a power of two of them
   p.pack = 1;
-  for (int x = group < 128 ? group : 128; x > 1; --x)
-    if (group % x == 0 && x * (128 / x) >= 120) {
-      p.pack = x;
-      break;
-    }
+  while (p.pack < 128 && group % (2 * p.pack) == 0) p.pack *= 2;
   p.rt = 128 / p.pack;
   p.nq = (a.Lq + 2 * p.rt - 1) / (2 * p.rt);
   p.nhp = a.H / p.pack;
@@ -1364,11 +1313,13 @@ static int launch_tile(const srdit_cross_attn_args& u, Args& a, const Plan& p,
   static std::atomic<bool> attr_done[kMaxDevices] = {};
   int rc = set_smem(kern, C::SMEM, attr_done);
   if (rc) return rc;
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   rc = map_of(&tq, u.q, u.q_stride, u.B, u.Lq, u.H, u.D, p.pack, p.rt);
   if (!rc) rc = kv_maps(&tk, &tv, u, TILE);
+  const int box_h = p.pack < 32 ? p.pack : 32;
+  if (!rc) rc = map_of(&to, u.out, u.o_stride, u.B, u.Lq, u.H, u.D, box_h, 32 / box_h);
   if (rc) return rc;
-  SRDIT_LAUNCH((kern), p.ctas, TILE_THREADS, C::SMEM, stream, tq, tk, tv, a);
+  SRDIT_LAUNCH((kern), p.ctas, TILE_THREADS, C::SMEM, stream, tq, tk, tv, to, a);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1506,7 +1457,6 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.group = u.H / u.Hkv;
   a.pack = p.pack;
   a.rt = p.rt;
-  a.pack_inv = p.pack > 0 ? (65536u + p.pack - 1) / p.pack : 0;
   a.nq = p.nq;
   a.nhp = p.nhp;
   a.splits = p.splits;
