@@ -55,7 +55,9 @@ struct Args {
   const uint8_t* mask;
   long long mask_stride;
   float c;         // scale * log2(e)
-  float* ws;       // parts of rows: O, then {m, l}
+  float* ws;       // parts of rows: O
+  float* ml;       // ... their {m, l}
+  void* cuts;      // tile_kernel: a Cut per CTA
   uint32_t* status;
 };
 
@@ -134,6 +136,7 @@ SRDIT_DEV void join_rows(const Args& a, int n, At at, const float2* ml, T* out, 
 // ---------------------------------------------------------------- tile_kernel
 constexpr int TILE_THREADS = 384;  // producer and MMA issuer, 2 x 4 softmax warps
 constexpr int SLOT_ROWS = 2 * TILE;
+constexpr int MASK_SLOTS = 8;
 constexpr int MAX_RANGES = 256;  // CTAs of a launch that may be ranged
 constexpr int RANGE_STEPS = 4;
 
@@ -145,7 +148,7 @@ struct TileCfg {
   static constexpr int OFF_KV = 2 * BYTES;
   static constexpr int OFF_STG = OFF_KV + STAGES * BYTES;  // 32 rows x 128 bytes per warp
   static constexpr int OFF_BAR = OFF_STG + 8 * 4096;
-  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static constexpr int SMEM = OFF_BAR + 384 + MASK_SLOTS * 16 + 1024;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
@@ -156,6 +159,7 @@ struct Item {
   int b, h0, tok0, len;
   int t0, t1;
   int slot;   // -1: all of the sample's keys; else where in the workspace the part goes
+  int parts;  // of an item that this CTA begins and others end: in how many it is
   bool act1;  // the second query tile has tokens
 };
 
@@ -169,68 +173,62 @@ struct Walk {
   int cta, ctas;
   int per;              // items per sample
   int b, rest, nt;      // sample, item within it, the sample's key tiles
-  long long whole;      // items that are taken whole, in rounds of ctas
-  long long at;         // the next of this CTA's whole items
-  long long s, s1;      // ranged: next step, end; steps count from the first ranged item
+  int whole;            // items that are taken whole, in rounds of ctas
+  int at;               // the next of this CTA's whole items
+  int b0, rest0;        // ranged: the first item that is not
+  int count;            // ranged: key-tile steps of the ranged items
+  int s, s1;            // ranged: this CTA's next step and its end, from the first item's first
   int t0;               // ranged: first key tile of the next item
   bool in_range;
 
   SRDIT_DEV int tiles(int x) const { return (key_count(a, x) + TILE - 1) / TILE; }
-  SRDIT_DEV static long long bound(long long total, int cta, int ctas) { return total * cta / ctas; }
-  // items and steps of the samples that have keys
-  SRDIT_DEV void totals(long long& items, long long& steps) const {
-    items = steps = 0;
-    if (!a.kv_lens) {
-      items = a.Lk > 0 ? static_cast<long long>(per) * a.B : 0;
-      steps = items * ((a.Lk + TILE - 1) / TILE);
-      return;
-    }
-    for (int x = 0; x < a.B; ++x) {
-      const int n = tiles(x);
-      if (n > 0) items += per;
-      steps += static_cast<long long>(n) * per;
-    }
-  }
-  // the n-th item of samples with keys; returns the steps before it
-  SRDIT_DEV long long find_item(long long n) {
-    long long before = 0;
+  // where the ranged steps of a CTA begin (make_plan keeps the product below 2^31)
+  SRDIT_DEV int bound(int c) const { return count * c / ctas; }
+  // to the n-th item of samples with keys
+  SRDIT_DEV void find_item(int n) {
     for (b = 0;; ++b) {
       nt = tiles(b);
       if (nt == 0) continue;
       if (n < per) break;
       n -= per;
-      before += static_cast<long long>(nt) * per;
     }
-    rest = static_cast<int>(n);
-    return before + n * nt;
+    rest = n;
   }
-  // the item that holds step x, counted from the first step of all
-  SRDIT_DEV void find_step(long long x) {
-    for (b = 0;; ++b) {
+  // to the item and key tile of ranged step x
+  SRDIT_DEV void find_step(int x) {
+    int r = rest0;
+    for (b = b0;; ++b) {
       nt = tiles(b);
-      const long long n = static_cast<long long>(nt) * per;
+      const int n = nt * (per - r);
       if (x < n) break;
       x -= n;
+      r = 0;
     }
-    rest = static_cast<int>(x / nt);
-    t0 = static_cast<int>(x - static_cast<long long>(rest) * nt);
-  }
-  // the ranged steps [first, first + count), from the first step of all
-  SRDIT_DEV void ranged_steps(long long& first, long long& count) {
-    long long items, steps;
-    totals(items, steps);
-    whole = a.ranged ? items / ctas * ctas : items;
-    first = whole < items ? find_item(whole) : steps;
-    count = steps - first;
+    rest = r + x / nt;
+    t0 = x % nt;
   }
   SRDIT_DEV Walk(const Args& args, int cta_, int ctas_)
-      : a(args), cta(cta_), ctas(ctas_), per(args.nq * args.nhp), b(0), rest(0), nt(0), at(cta_), s(0),
-        s1(0), t0(0), in_range(false) {
-    long long first, count;
-    ranged_steps(first, count);
+      : a(args), cta(cta_), ctas(ctas_), per(args.nq * args.nhp), b(0), rest(0), nt(0), at(cta_),
+        b0(0), rest0(0), count(0), s(0), s1(0), t0(0), in_range(false) {
+    int items = 0;
+    if (a.kv_lens) {
+      for (int x = 0; x < a.B; ++x)
+        if (key_count(a, x) > 0) items += per;
+    } else if (a.Lk > 0) {
+      items = per * a.B;
+    }
+    whole = items;
     if (a.ranged) {
-      s = first + bound(count, cta, ctas);
-      s1 = first + bound(count, cta + 1, ctas);
+      whole = items / ctas * ctas;
+      if (whole < items) {
+        find_item(whole);
+        b0 = b;
+        rest0 = rest;
+        count = nt * (per - rest);
+        for (int x = b + 1; x < a.B; ++x) count += tiles(x) * per;
+      }
+      s = bound(cta);
+      s1 = bound(cta + 1);
     }
     if (at < whole) find_item(at);
   }
@@ -240,6 +238,7 @@ struct Walk {
     o.tok0 = rest % a.nq * 2 * a.rt;
     o.act1 = o.tok0 + a.rt < a.Lq;
     o.len = key_count(a, b);
+    o.parts = 0;
   }
   // the next item, or false
   SRDIT_DEV bool next(Item& o) {
@@ -269,13 +268,26 @@ struct Walk {
     }
     item(o);
     o.t0 = t0;
-    o.t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + (s1 - s)));
+    o.t1 = min(nt, t0 + (s1 - s));
     o.slot = o.t0 > 0 ? 2 * cta : o.t1 < nt ? 2 * cta + 1 : -1;
+    if (o.t0 == 0 && o.t1 < nt) {  // this CTA's part and those of the CTAs up to the item's end
+      const int end = s + nt;
+      o.parts = 2;
+      while (bound(cta + o.parts) < end) ++o.parts;
+    }
     s += o.t1 - o.t0;
     t0 = 0;
     ++rest;
     return true;
   }
+};
+
+// What a CTA leaves for join_ranges_kernel: the item that it begins and does not end, whose
+// parts are in its second slot and the first slots of the CTAs after it.
+struct Cut {
+  int parts, b, h0, tok0;
+  int count;  // Walk's, from which the CTAs' ranges follow
+  int pad[3];
 };
 
 template <typename T, int DP>
@@ -297,9 +309,12 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   uint64_t* p_full = s_full + 2;      // its weights written (one arrival per warp)
   uint64_t* p_half = p_full + 2;      // the first half of them
   uint64_t* o_full = p_half + 2;      // its last product done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* m_full = o_full + 2;      // [8] a key tile's mask ready and its values clean
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_full + MASK_SLOTS);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  static_assert((2 * STAGES + 12) * 8 + 8 <= 512, "barrier area");
+  uint4* masks = reinterpret_cast<uint4*>(smem + C::OFF_BAR + 384);  // [MASK_SLOTS] 128 bits
+  static_assert((2 * STAGES + 12 + MASK_SLOTS) * 8 + 8 <= 384, "barrier area");
+  static_assert(STAGES / 2 < MASK_SLOTS, "a mask is not overwritten while it is read");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -315,6 +330,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       mbar_init(&p_half[t], 4);
       mbar_init(&o_full[t], 1);
     }
+    for (int x = 0; x < MASK_SLOTS; ++x) mbar_init(&m_full[x], 1);
     *abort_flag = 0u;
     fence_barrier_init();
   }
@@ -390,7 +406,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       constexpr uint32_t fmt = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
       const uint32_t idesc_s = idesc_make(fmt, fmt, 0u, 0u, 128u, 128u);
       const uint32_t idesc_o = idesc_make(fmt, fmt, 0u, 1u, 128u, static_cast<uint32_t>(DP));
-      int idx = 0;
+      int idx = 0;            // ring use of the current key tile; its number is idx / 2
       int nq[2] = {0, 0}, np[2] = {0, 0};
       auto kv_wait = [&](int u) {
         return mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
@@ -450,6 +466,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         }
         const int uv = idx + 1, uk = idx + 2;
         ok = kv_wait(uv);
+        if (ok && (a.mask || (j + 1) * TILE > it.len)) {
+          const int u = idx >> 1;
+          ok = mbar_wait(&m_full[u % MASK_SLOTS], static_cast<uint32_t>(u / MASK_SLOTS) & 1u, a.status,
+                         abort_flag);
+        }
         bool k_ready = false;
         for (int t = 0; t < 2 && ok; ++t) {
           if (t == 0 || it.act1) {
@@ -487,6 +508,58 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       }
     }
     __syncwarp();
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ mask
+    // Of every key tile with unseen keys: the 128 bits that the softmax hides scores by,
+    // and zeros in the rows of their values. A tile's values are here only after the
+    // products of the tiles STAGES / 2 before it, so the masks of those have been read.
+    Walk walk(a, blockIdx.x, gridDim.x);
+    Item it;
+    bool ok = true;
+    int u = 0;  // key tiles so far
+    while (ok && walk.next(it)) {
+      const uint8_t* mrow = a.mask ? a.mask + it.b * a.mask_stride : nullptr;
+      for (int j = it.t0; j < it.t1; ++j, ++u) {
+        const int key0 = j * TILE;
+        const bool masked = mrow || key0 + TILE > it.len;
+        uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (masked) {
+          bool seen[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int key = key0 + w * 32 + lane;
+            seen[w] = key < it.len && (!mrow || __ldg(mrow + key) != 0);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) vis[w] = __ballot_sync(0xffffffffu, seen[w]);
+        }
+        const int v = 2 * u + 1;
+        ok = mbar_wait(&full[v % STAGES], static_cast<uint32_t>(v / STAGES) & 1u, a.status, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (masked) {
+          if (lane == 0) masks[u % MASK_SLOTS] = make_uint4(vis[0], vis[1], vis[2], vis[3]);
+          uint8_t* tile = smem + C::OFF_KV + (v % STAGES) * C::BYTES;
+          // eight lanes to a row
+          const int row0 = lane >> 3;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (vis[w] == 0xffffffffu) continue;
+#pragma unroll
+            for (int r = 0; r < 32; r += 4)
+              if (!((vis[w] >> (r + row0)) & 1u))
+                for (int d = 0; d < DP / 64; ++d)
+                  *reinterpret_cast<uint4*>(tile + d * C::SLAB + (w * 32 + r + row0) * 128 +
+                                            (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m_full[u % MASK_SLOTS]);
+      }
+    }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -499,56 +572,31 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     const uint32_t o_tmem = tmem_base + t_lane + 256u + t * 128u;
     const uint64_t c2 = f2_pack(a.c, a.c);
     uint8_t* stg = smem + C::OFF_STG + (warp - 4) * 4096;
-    int ns = 0, no = 0, idx = 0;
+    int ns = 0, no = 0, tile0 = 0;
     bool ok = true;
     Walk walk(a, blockIdx.x, gridDim.x);
     Item it;
+    if (a.ranged && threadIdx.x == 128) reinterpret_cast<Cut*>(a.cuts)[blockIdx.x].parts = 0;
     while (walk.next(it)) {
       const int n_tiles = it.t1 - it.t0;
       const bool act = t == 0 || it.act1;
       float m = neg_inf(), l = 0.f;
-      const uint8_t* mrow = a.mask ? a.mask + it.b * a.mask_stride : nullptr;
-      // the mask's bytes of this lane's four keys of a tile, read a tile ahead
-      uint32_t seen = 0xfu;
-      auto read_mask = [&](int key0) {
-        uint32_t r = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int key = key0 + w * 32 + lane;
-          r |= (key < it.len && __ldg(mrow + key) != 0 ? 1u : 0u) << w;
-        }
-        return r;
-      };
       if (act) {
-        if (mrow) seen = read_mask(it.t0 * TILE);
         for (int j = 0; j < n_tiles; ++j) {
-          const int key0 = (it.t0 + j) * TILE;
-          const bool masked = a.mask != nullptr || key0 + TILE > it.len;
+          const bool masked = a.mask != nullptr || (it.t0 + j + 1) * TILE > it.len;
           uint32_t vis[4];
           if (masked) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-              vis[w] = __ballot_sync(0xffffffffu,
-                                     key0 + w * 32 + lane < it.len && ((seen >> w) & 1u));
-            if (mrow && j + 1 < n_tiles) seen = read_mask(key0 + TILE);
-            // the values of unseen keys are zeroed: thread r of tile 0 has key r
-            if (t == 0) {
-              const int u = idx + 2 * j + 1;
-              if (!mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
-                             abort_flag)) {
-                ok = false;
-                break;
-              }
-              const uint32_t mine = sub == 0 ? vis[0] : sub == 1 ? vis[1] : sub == 2 ? vis[2] : vis[3];
-              if (!((mine >> lane) & 1u)) {
-                uint8_t* vrow = smem + C::OFF_KV + (u % STAGES) * C::BYTES + row * 128;
-                for (int d = 0; d < DP / 64; ++d)
-#pragma unroll
-                  for (int x = 0; x < 8; ++x)
-                    *reinterpret_cast<uint4*>(vrow + d * C::SLAB + x * 16) = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async_smem();
+            const int u = tile0 + j;
+            if (!mbar_wait(&m_full[u % MASK_SLOTS], static_cast<uint32_t>(u / MASK_SLOTS) & 1u,
+                           a.status, abort_flag)) {
+              ok = false;
+              break;
             }
+            const uint4 v = masks[u % MASK_SLOTS];
+            vis[0] = v.x;
+            vis[1] = v.y;
+            vis[2] = v.z;
+            vis[3] = v.w;
           }
           if (!mbar_wait(&s_full[t], static_cast<uint32_t>(ns) & 1u, a.status, abort_flag)) {
             ok = false;
@@ -563,9 +611,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
           if (masked) {
 #pragma unroll
             for (int w = 0; w < 4; ++w)
+              if (vis[w] != 0xffffffffu) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((vis[w] >> e) & 1u)) s[w][e] = __float_as_uint(neg_inf());
+                for (int e = 0; e < 32; ++e)
+                  if (!((vis[w] >> e) & 1u)) s[w][e] = __float_as_uint(neg_inf());
+              }
           }
           float mx[4];
 #pragma unroll
@@ -634,9 +684,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         ++no;
         tc_fence_after();
         // O / l (or, of a part, O, m and l): the warp's 32 rows go through its staging
-        // buffer 128 bytes of each at a time, so that a store covers four whole rows
+        // buffer 128 bytes of each at a time
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int r0 = lane >> 3, piece = lane & 7;
         if (it.slot < 0) {
           // the warp's rows are a box of the output: heads x tokens
           const int tok = it.tok0 + t * a.rt + sub * 32 / a.pack;
@@ -670,36 +719,40 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             }
           }
         } else {
-          const long long at = static_cast<long long>(it.slot) * SLOT_ROWS + t * TILE + row;
-          if (lane == 0) bulk_wait_group_read0();  // (the last box has left the buffer)
-          __syncwarp();
-          float* po = a.ws + (at - lane) * a.D;
-          float* ml = a.ws + 2ll * gridDim.x * SLOT_ROWS * a.D + at * 2;
-          *reinterpret_cast<float2*>(ml) = make_float2(m, l);
+          // a part: the slot holds each warp's rows as [D / 32][32 rows][32 values] in the
+          // staging buffer's own order, one bulk store per 4 KiB
+          const long long box = (static_cast<long long>(it.slot) * 8 + t * 4 + sub) * (DP / 32);
+          reinterpret_cast<float2*>(a.ml)[it.slot * SLOT_ROWS + t * TILE + row] = make_float2(m, l);
+          if (t == 0 && row == 0 && it.parts) {
+            Cut cut = {it.parts, it.b, it.h0, it.tok0, walk.count};
+            reinterpret_cast<Cut*>(a.cuts)[blockIdx.x] = cut;
+          }
 #pragma unroll 1
-          for (int d = 0; d < DP; d += 32) {
+          for (int d = 0; d < DP / 32; ++d) {
             uint32_t o[32];
-            tmem_ld32(o_tmem + d, o);
+            tmem_ld32(o_tmem + d * 32, o);
+            if (lane == 0) bulk_wait_group_read0();  // the box before has left the buffer
             tmem_ld_wait();
+            __syncwarp();
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
                   make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            fence_proxy_async_smem();
             __syncwarp();
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const int r = x * 4 + r0;
-              if (d + piece * 4 < a.D)
-                *reinterpret_cast<uint4*>(po + static_cast<long long>(r) * a.D + d + piece * 4) =
-                    *reinterpret_cast<const uint4*>(stg + r * 128 + ((piece ^ (r & 7)) << 4));
+            if (lane == 0) {
+              asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                               a.ws + (box + d) * 1024),
+                           "r"(smem_u32(stg)), "r"(4096)
+                           : "memory");
+              bulk_commit_group();
             }
-            __syncwarp();
           }
         }
         // the next item's first weights, published after this, free O
         tc_fence_before();
       }
-      idx += 2 * n_tiles;
+      tile0 += n_tiles;
     }
     if (lane == 0) bulk_wait_group_all();
     // samples without keys
@@ -725,46 +778,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   }
 }
 
-// One block per 32 rows of the slot at each bound between two CTAs' ranges: joins the
-// parts of the item that the bound cuts, at the first bound inside it. The parts'
-// slots are found once per block.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    join_ranges_kernel(const __grid_constant__ Args a, int ctas) {
+// One block per 32 rows of the items that the CTAs' ranges cut: joins their parts.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) join_ranges_kernel(const __grid_constant__ Args a) {
   pdl_begin();
-  __shared__ int slots[MAX_RANGES];
-  __shared__ int n_slots;
-  __shared__ Item it;
-  if (threadIdx.x == 0) {
-    n_slots = 0;
-    Walk w(a, 0, ctas);
-    long long first, count;
-    w.ranged_steps(first, count);
-    const int c = blockIdx.x + 1;
-    const long long at = Walk::bound(count, c, ctas);
-    if (at < count) {
-      w.find_step(first + at);
-      const long long start = at - w.t0, end = start + w.nt;
-      // (not between two items, and not a later bound of an item cut before)
-      if (w.t0 > 0 && Walk::bound(count, c - 1, ctas) <= start) {
-        w.item(it);
-        int n = 0;
-        long long from = Walk::bound(count, c - 1, ctas);
-        for (int p = c - 1; p < ctas && from < end; ++p) {
-          const long long to = Walk::bound(count, p + 1, ctas);
-          if (from < to) slots[n++] = from > start ? 2 * p : 2 * p + 1;
-          from = to;
-        }
-        n_slots = n;
-      }
-    }
-  }
-  __syncthreads();
-  const int n = n_slots;
-  if (n == 0) return;
+  const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[blockIdx.x];
+  if (cut.parts == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float2* ml = reinterpret_cast<const float2*>(a.ws + 2ll * ctas * SLOT_ROWS * a.D);
-  // four rows of a warp together
+  const int group = blockIdx.y;  // query tile x lane quarter
+  const int r0 = warp * 4;       // four rows of the 32 a warp
+  const int quad = lane & 7, d = lane >> 3;
   float m[4], l[4];
   float4 acc[4];
 #pragma unroll
@@ -773,17 +796,21 @@ __global__ void __launch_bounds__(256)
     l[x] = 0.f;
     acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const int r0 = blockIdx.y * 32 + warp * 4;
-  const bool on = lane * 4 < a.D;
-  for (int p = 0; p < n; ++p) {
-    const long long row = static_cast<long long>(slots[p]) * SLOT_ROWS + r0;
+  for (int p = 0; p < cut.parts; ++p) {
+    const int cta = static_cast<int>(blockIdx.x) + p, ctas = static_cast<int>(gridDim.x) + 1;
+    if (cut.count * cta / ctas == cut.count * (cta + 1) / ctas) continue;  // an empty range
+    const int slot = p == 0 ? 2 * cta + 1 : 2 * cta;
+    const float2* ml = reinterpret_cast<const float2*>(a.ml) + slot * SLOT_ROWS + group * 32 + r0;
+    const float* box = a.ws + (static_cast<long long>(slot) * 8 + group) * (DP / 32) * 1024;
     float2 pm[4];
     float4 v[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      pm[x] = ml[row + x];
-      v[x] = on ? *reinterpret_cast<const float4*>(a.ws + (row + x) * a.D + lane * 4)
-                : make_float4(0.f, 0.f, 0.f, 0.f);
+      const int r = r0 + x;
+      pm[x] = ml[x];
+      v[x] = d < DP / 32 ? *reinterpret_cast<const float4*>(box + (d * 32 + r) * 32 +
+                                                            ((quad ^ (r & 7)) << 2))
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -798,14 +825,15 @@ __global__ void __launch_bounds__(256)
       acc[x].w = acc[x].w * f0 + v[x].w * f1;
     }
   }
+  const int col = d * 32 + quad * 4;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const int tr = (r0 + x) % TILE, rt = tr / a.pack;
-    const int tok = it.tok0 + (r0 + x) / TILE * a.rt + rt;
-    if (rt >= a.rt || tok >= a.Lq || !on) continue;
+    const int r = (group & 3) * 32 + r0 + x, rt = r / a.pack;
+    const int tok = cut.tok0 + (group >> 2) * a.rt + rt;
+    if (tok >= a.Lq || col >= a.D) continue;
     const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + it.b * a.os[0] + tok * a.os[1] +
-                              (it.h0 + tr - rt * a.pack) * a.os[2] + lane * 4) =
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + cut.b * a.os[0] + tok * a.os[1] +
+                              (cut.h0 + r % a.pack) * a.os[2] + col) =
         make_uint2(pack2(acc[x].x * inv, acc[x].y * inv, T{}),
                    pack2(acc[x].z * inv, acc[x].w * inv, T{}));
   }
@@ -1173,7 +1201,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
           (part / cluster) * all_rows + (static_cast<long long>(b) * a.Lq + tok) * a.H + head;
       *reinterpret_cast<float4*>(a.ws + at * a.D + d) = acc;
       if (d == 0)
-        *reinterpret_cast<float2*>(a.ws + wparts * all_rows * a.D + at * 2) = make_float2(top, sum);
+        *reinterpret_cast<float2*>(a.ml + at * 2) = make_float2(top, sum);
     }
   }
   if (cluster > 1) {  // no CTA leaves while another reads its shared memory
@@ -1192,7 +1220,7 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
   const int h = static_cast<int>(row % a.H);
   const long long bi = row / a.H;
   join_rows<T>(a, parts, [&](int p) { return p * rows + row; },
-               reinterpret_cast<const float2*>(a.ws + parts * rows * a.D),
+               reinterpret_cast<const float2*>(a.ml),
                static_cast<T*>(a.out) + (bi / a.Lq) * a.os[0] + (bi % a.Lq) * a.os[1] + h * a.os[2],
                threadIdx.x & 31);
 }
@@ -1208,7 +1236,7 @@ struct Plan {
   int ctas;                    // tile_kernel
   long long ws_floats(const srdit_cross_attn_args& a) const {
     if (token) return parts > 1 ? static_cast<long long>(parts) * a.B * a.Lq * a.H * (a.D + 2) : 0;
-    return ranged ? 2ll * ctas * SLOT_ROWS * (a.D + 2) : 0;
+    return ranged ? 2ll * ctas * SLOT_ROWS * ((a.D <= 64 ? 64 : 128) + 2) + 8 * ctas : 0;
   }
 };
 
@@ -1259,7 +1287,7 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
     if (ctas < items) ctas = items;
   }
   const long long idle = last ? tiles - (last * tiles + ctas - 1) / ctas : 0;
-  p.ranged = a.B <= 64 && idle > RANGE_STEPS;
+  p.ranged = a.B <= 64 && idle > RANGE_STEPS && tiles < (1 << 14);  // (steps x CTAs in 32 bits)
   if (!p.ranged && items < sms) ctas = items;
   p.ctas = static_cast<int>(ctas);
   return p;
@@ -1374,7 +1402,10 @@ static int run(const srdit_cross_attn_args& u, Args& a, const Plan& p, cudaStrea
   if (rc) return rc;
   if (p.ranged) {
     const dim3 grid(static_cast<unsigned>(p.ctas - 1), SLOT_ROWS / 32);
-    SRDIT_LAUNCH((join_ranges_kernel<T>), grid, 256, 0, stream, a, p.ctas);
+    if (u.D <= 64)
+      SRDIT_LAUNCH((join_ranges_kernel<T, 64>), grid, 256, 0, stream, a);
+    else
+      SRDIT_LAUNCH((join_ranges_kernel<T, 128>), grid, 256, 0, stream, a);
     return static_cast<int>(cudaGetLastError());
   }
   if (p.parts == 1) return 0;
@@ -1471,6 +1502,13 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.mask_stride = u.mask_stride;
   a.c = u.scale * xattn::kLog2e;
   a.ws = static_cast<float*>(u.workspace);
+  if (p.token) {
+    a.ml = a.ws + static_cast<long long>(p.parts) * u.B * u.Lq * u.H * u.D;
+  } else {
+    const long long slots = 2ll * p.ctas * xattn::SLOT_ROWS;
+    a.ml = a.ws + slots * (u.D <= 64 ? 64 : 128);
+    a.cuts = a.ml + 2 * slots;
+  }
   a.status = u.status;
   return u.dtype == SRDIT_BF16 ? xattn::run<__nv_bfloat16>(u, a, p, stream)
                                : xattn::run<__half>(u, a, p, stream);
