@@ -136,9 +136,9 @@ SRDIT_DEV void join_rows(const Args& a, int n, At at, const float2* ml, T* out, 
 // ---------------------------------------------------------------- tile_kernel
 constexpr int TILE_THREADS = 384;  // producer and MMA issuer, 2 x 4 softmax warps
 constexpr int SLOT_ROWS = 2 * TILE;
-constexpr int MASK_SLOTS = 8;
 constexpr int MAX_RANGES = 256;  // CTAs of a launch that may be ranged
 constexpr int RANGE_STEPS = 4;
+constexpr int MAX_LENS = 32;     // samples whose key counts are kept in shared memory
 
 template <int DP>
 struct TileCfg {
@@ -147,8 +147,9 @@ struct TileCfg {
   static constexpr int STAGES = DP == 128 ? 4 : 10;
   static constexpr int OFF_KV = 2 * BYTES;
   static constexpr int OFF_STG = OFF_KV + STAGES * BYTES;  // 32 rows x 128 bytes per warp
-  static constexpr int OFF_BAR = OFF_STG + 8 * 4096;
-  static constexpr int SMEM = OFF_BAR + 384 + MASK_SLOTS * 16 + 1024;
+  static constexpr int OFF_LENS = OFF_STG + 8 * 4096;
+  static constexpr int OFF_BAR = OFF_LENS + MAX_LENS * 4;
+  static constexpr int SMEM = OFF_BAR + 384 + 1024;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
@@ -181,7 +182,10 @@ struct Walk {
   int t0;               // ranged: first key tile of the next item
   bool in_range;
 
-  SRDIT_DEV int tiles(int x) const { return (key_count(a, x) + TILE - 1) / TILE; }
+  const int* lens;      // the samples' key counts in shared memory (null: read where needed)
+
+  SRDIT_DEV int keys(int x) const { return lens ? lens[x] : key_count(a, x); }
+  SRDIT_DEV int tiles(int x) const { return (keys(x) + TILE - 1) / TILE; }
   // where the ranged steps of a CTA begin (make_plan keeps the product below 2^31)
   SRDIT_DEV int bound(int c) const { return count * c / ctas; }
   // to the n-th item of samples with keys
@@ -207,18 +211,14 @@ struct Walk {
     rest = r + x / nt;
     t0 = x % nt;
   }
-  SRDIT_DEV Walk(const Args& args, int cta_, int ctas_)
+  SRDIT_DEV Walk(const Args& args, int cta_, int ctas_, const int* lens_)
       : a(args), cta(cta_), ctas(ctas_), per(args.nq * args.nhp), b(0), rest(0), nt(0), at(cta_),
-        b0(0), rest0(0), count(0), s(0), s1(0), t0(0), in_range(false) {
-    int items = 0;
-    if (a.kv_lens) {
+        b0(0), rest0(0), count(0), s(0), s1(0), t0(0), in_range(false), lens(lens_) {
+    whole = per * a.B;
+    if (a.ranged) {  // (make_plan: lens is there)
+      int items = 0;
       for (int x = 0; x < a.B; ++x)
-        if (key_count(a, x) > 0) items += per;
-    } else if (a.Lk > 0) {
-      items = per * a.B;
-    }
-    whole = items;
-    if (a.ranged) {
+        if (keys(x) > 0) items += per;
       whole = items / ctas * ctas;
       if (whole < items) {
         find_item(whole);
@@ -230,32 +230,49 @@ struct Walk {
       s = bound(cta);
       s1 = bound(cta + 1);
     }
-    if (at < whole) find_item(at);
+    if (at < whole) {
+      if (a.ranged) {
+        find_item(at);
+      } else {  // of all samples: those without keys are passed over in next()
+        b = at / per;
+        rest = at % per;
+        nt = tiles(b);
+      }
+    }
   }
   SRDIT_DEV void item(Item& o) const {
     o.b = b;
     o.h0 = rest / a.nq * a.pack;
     o.tok0 = rest % a.nq * 2 * a.rt;
     o.act1 = o.tok0 + a.rt < a.Lq;
-    o.len = key_count(a, b);
+    o.len = keys(b);
     o.parts = 0;
   }
   // the next item, or false
   SRDIT_DEV bool next(Item& o) {
-    if (at < whole) {
-      item(o);
-      o.t0 = 0;
-      o.t1 = nt;
-      o.slot = -1;
+    while (at < whole) {
+      const bool found = nt > 0;
+      if (found) {
+        item(o);
+        o.t0 = 0;
+        o.t1 = nt;
+        o.slot = -1;
+      }
       at += ctas;
       if (at < whole) {
         rest += ctas;
-        while (rest >= per || nt == 0) {
-          if (nt > 0) rest -= per;
-          nt = tiles(++b);
+        if (a.ranged) {
+          while (rest >= per || nt == 0) {
+            if (nt > 0) rest -= per;
+            nt = tiles(++b);
+          }
+        } else if (rest >= per) {
+          b += rest / per;
+          rest %= per;
+          nt = tiles(b);
         }
       }
-      return true;
+      if (found) return true;
     }
     if (s >= s1) return false;
     if (!in_range) {
@@ -309,12 +326,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   uint64_t* p_full = s_full + 2;      // its weights written (one arrival per warp)
   uint64_t* p_half = p_full + 2;      // the first half of them
   uint64_t* o_full = p_half + 2;      // its last product done
-  uint64_t* m_full = o_full + 2;      // [8] a key tile's mask ready and its values clean
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_full + MASK_SLOTS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  uint4* masks = reinterpret_cast<uint4*>(smem + C::OFF_BAR + 384);  // [MASK_SLOTS] 128 bits
-  static_assert((2 * STAGES + 12 + MASK_SLOTS) * 8 + 8 <= 384, "barrier area");
-  static_assert(STAGES / 2 < MASK_SLOTS, "a mask is not overwritten while it is read");
+  int* lens = reinterpret_cast<int*>(smem + C::OFF_LENS);
+  static_assert((2 * STAGES + 12) * 8 + 8 <= 384, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -330,7 +345,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       mbar_init(&p_half[t], 4);
       mbar_init(&o_full[t], 1);
     }
-    for (int x = 0; x < MASK_SLOTS; ++x) mbar_init(&m_full[x], 1);
     *abort_flag = 0u;
     fence_barrier_init();
   }
@@ -339,6 +353,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
+  if (threadIdx.x >= 128 && static_cast<int>(threadIdx.x) - 128 < min(a.B, MAX_LENS))
+    lens[threadIdx.x - 128] = key_count(a, threadIdx.x - 128);
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -382,7 +398,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         ++nq[t];
         return true;
       };
-      Walk walk(a, blockIdx.x, gridDim.x);
+      Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
       Item it;
       while (ok && walk.next(it)) {
         const int g = it.h0 / a.group;
@@ -406,7 +422,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       constexpr uint32_t fmt = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
       const uint32_t idesc_s = idesc_make(fmt, fmt, 0u, 0u, 128u, 128u);
       const uint32_t idesc_o = idesc_make(fmt, fmt, 0u, 1u, 128u, static_cast<uint32_t>(DP));
-      int idx = 0;            // ring use of the current key tile; its number is idx / 2
+      int idx = 0;
       int nq[2] = {0, 0}, np[2] = {0, 0};
       auto kv_wait = [&](int u) {
         return mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
@@ -431,7 +447,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                       sdesc_sw128(v_addr + k * 16 * 128, C::SLAB, 1024), idesc_o,
                       (!first || k > 0) ? 1u : 0u);
       };
-      Walk walk(a, blockIdx.x, gridDim.x);
+      Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
       Item it = {};
       bool on = walk.next(it), ok = on;
       if (ok) {
@@ -466,11 +482,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         }
         const int uv = idx + 1, uk = idx + 2;
         ok = kv_wait(uv);
-        if (ok && (a.mask || (j + 1) * TILE > it.len)) {
-          const int u = idx >> 1;
-          ok = mbar_wait(&m_full[u % MASK_SLOTS], static_cast<uint32_t>(u / MASK_SLOTS) & 1u, a.status,
-                         abort_flag);
-        }
         bool k_ready = false;
         for (int t = 0; t < 2 && ok; ++t) {
           if (t == 0 || it.act1) {
@@ -508,58 +519,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 2) {
-    // ------------------------------------------------------------ mask
-    // Of every key tile with unseen keys: the 128 bits that the softmax hides scores by,
-    // and zeros in the rows of their values. A tile's values are here only after the
-    // products of the tiles STAGES / 2 before it, so the masks of those have been read.
-    Walk walk(a, blockIdx.x, gridDim.x);
-    Item it;
-    bool ok = true;
-    int u = 0;  // key tiles so far
-    while (ok && walk.next(it)) {
-      const uint8_t* mrow = a.mask ? a.mask + it.b * a.mask_stride : nullptr;
-      for (int j = it.t0; j < it.t1; ++j, ++u) {
-        const int key0 = j * TILE;
-        const bool masked = mrow || key0 + TILE > it.len;
-        uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        if (masked) {
-          bool seen[4];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int key = key0 + w * 32 + lane;
-            seen[w] = key < it.len && (!mrow || __ldg(mrow + key) != 0);
-          }
-#pragma unroll
-          for (int w = 0; w < 4; ++w) vis[w] = __ballot_sync(0xffffffffu, seen[w]);
-        }
-        const int v = 2 * u + 1;
-        ok = mbar_wait(&full[v % STAGES], static_cast<uint32_t>(v / STAGES) & 1u, a.status, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (masked) {
-          if (lane == 0) masks[u % MASK_SLOTS] = make_uint4(vis[0], vis[1], vis[2], vis[3]);
-          uint8_t* tile = smem + C::OFF_KV + (v % STAGES) * C::BYTES;
-          // eight lanes to a row
-          const int row0 = lane >> 3;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if (vis[w] == 0xffffffffu) continue;
-#pragma unroll
-            for (int r = 0; r < 32; r += 4)
-              if (!((vis[w] >> (r + row0)) & 1u))
-                for (int d = 0; d < DP / 64; ++d)
-                  *reinterpret_cast<uint4*>(tile + d * C::SLAB + (w * 32 + r + row0) * 128 +
-                                            (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m_full[u % MASK_SLOTS]);
-      }
-    }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -572,31 +531,57 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     const uint32_t o_tmem = tmem_base + t_lane + 256u + t * 128u;
     const uint64_t c2 = f2_pack(a.c, a.c);
     uint8_t* stg = smem + C::OFF_STG + (warp - 4) * 4096;
-    int ns = 0, no = 0, tile0 = 0;
+    int ns = 0, no = 0, idx = 0;
     bool ok = true;
-    Walk walk(a, blockIdx.x, gridDim.x);
+    Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
     Item it;
     if (a.ranged && threadIdx.x == 128) reinterpret_cast<Cut*>(a.cuts)[blockIdx.x].parts = 0;
     while (walk.next(it)) {
       const int n_tiles = it.t1 - it.t0;
       const bool act = t == 0 || it.act1;
       float m = neg_inf(), l = 0.f;
+      const uint8_t* mrow = a.mask ? a.mask + it.b * a.mask_stride : nullptr;
+      // the mask's bytes of this lane's four keys of a tile, read a tile ahead
+      uint32_t seen = 0xfu;
+      auto read_mask = [&](int key0) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int key = key0 + w * 32 + lane;
+          r |= (key < it.len && __ldg(mrow + key) != 0 ? 1u : 0u) << w;
+        }
+        return r;
+      };
       if (act) {
+        if (mrow) seen = read_mask(it.t0 * TILE);
         for (int j = 0; j < n_tiles; ++j) {
-          const bool masked = a.mask != nullptr || (it.t0 + j + 1) * TILE > it.len;
+          const int key0 = (it.t0 + j) * TILE;
+          const bool masked = a.mask != nullptr || key0 + TILE > it.len;
           uint32_t vis[4];
           if (masked) {
-            const int u = tile0 + j;
-            if (!mbar_wait(&m_full[u % MASK_SLOTS], static_cast<uint32_t>(u / MASK_SLOTS) & 1u,
-                           a.status, abort_flag)) {
-              ok = false;
-              break;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              vis[w] = __ballot_sync(0xffffffffu,
+                                     key0 + w * 32 + lane < it.len && ((seen >> w) & 1u));
+            if (mrow && j + 1 < n_tiles) seen = read_mask(key0 + TILE);
+            // the values of unseen keys are zeroed: thread r of tile 0 has key r
+            if (t == 0) {
+              const int u = idx + 2 * j + 1;
+              if (!mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
+                             abort_flag)) {
+                ok = false;
+                break;
+              }
+              const uint32_t mine = sub == 0 ? vis[0] : sub == 1 ? vis[1] : sub == 2 ? vis[2] : vis[3];
+              if (!((mine >> lane) & 1u)) {
+                uint8_t* vrow = smem + C::OFF_KV + (u % STAGES) * C::BYTES + row * 128;
+                for (int d = 0; d < DP / 64; ++d)
+#pragma unroll
+                  for (int x = 0; x < 8; ++x)
+                    *reinterpret_cast<uint4*>(vrow + d * C::SLAB + x * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
             }
-            const uint4 v = masks[u % MASK_SLOTS];
-            vis[0] = v.x;
-            vis[1] = v.y;
-            vis[2] = v.z;
-            vis[3] = v.w;
           }
           if (!mbar_wait(&s_full[t], static_cast<uint32_t>(ns) & 1u, a.status, abort_flag)) {
             ok = false;
@@ -611,11 +596,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
           if (masked) {
 #pragma unroll
             for (int w = 0; w < 4; ++w)
-              if (vis[w] != 0xffffffffu) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!((vis[w] >> e) & 1u)) s[w][e] = __float_as_uint(neg_inf());
-              }
+              for (int e = 0; e < 32; ++e)
+                if (!((vis[w] >> e) & 1u)) s[w][e] = __float_as_uint(neg_inf());
           }
           float mx[4];
 #pragma unroll
@@ -752,7 +735,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         // the next item's first weights, published after this, free O
         tc_fence_before();
       }
-      tile0 += n_tiles;
+      idx += 2 * n_tiles;
     }
     if (lane == 0) bulk_wait_group_all();
     // samples without keys
@@ -1287,7 +1270,7 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
     if (ctas < items) ctas = items;
   }
   const long long idle = last ? tiles - (last * tiles + ctas - 1) / ctas : 0;
-  p.ranged = a.B <= 64 && idle > RANGE_STEPS && tiles < (1 << 14);  // (steps x CTAs in 32 bits)
+  p.ranged = a.B <= MAX_LENS && idle > RANGE_STEPS && tiles < (1 << 14);  // (steps x CTAs in 32 bits)
   if (!p.ranged && items < sms) ctas = items;
   p.ctas = static_cast<int>(ctas);
   return p;
