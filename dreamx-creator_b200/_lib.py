@@ -200,5 +200,13 @@ def check(rc: int, what: str) -> None:
         raise SrditError(f"{what} failed with code {rc}: {msg}")
 
 
+_fns = {}
+
+
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
+    rc = fn(*args)
+    if rc:
+        check(rc, name)

@@ -63,10 +63,11 @@ def _need_cuda(*ts):
 
 def _rows(t: torch.Tensor):
     """(row stride in elements) of a 2-D row-major view with unit inner stride."""
-    if t.dim() != 2 or t.stride(1) != 1:
+    st = t.stride()
+    if len(st) != 2 or st[1] != 1:
         raise _lib.SrditError(f"expected a 2-D row-major tensor, got shape {tuple(t.shape)} "
-                              f"strides {t.stride()}")
-    return t.stride(0)
+                              f"strides {st}")
+    return st[0]
 
 
 def fp8_gemm(a_fp8, a_scale, w_fp8, w_scale, bias=None, out=None, *, epilogue="store",
@@ -193,21 +194,22 @@ def _code(table, dtype, what):
 
 
 def _same_device(x, *ts):
-    """Every given tensor on x's device, and that the current one (kernels are
-    launched on the current device)."""
-    dev = x.device
-    if not x.is_cuda:
+    """Every given tensor on x's device, and that the current one (kernels are launched
+    on the current device). Returns the current stream's handle there."""
+    dev = x.get_device()
+    if dev < 0:
         _need_cuda(x)
     for t in ts:
-        if t is not None and t.device != dev:
-            raise _lib.SrditError(f"tensors on {dev} and {t.device}")
-    if dev.index != torch.cuda.current_device():
-        raise _lib.SrditError(f"tensors on {dev}, the current device is "
+        if t is not None and t.get_device() != dev:
+            raise _lib.SrditError(f"tensors on {x.device} and {t.device}")
+    if dev != torch._C._cuda_getDevice():
+        raise _lib.SrditError(f"tensors on {x.device}, the current device is "
                               f"cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _scales(t, n, what):
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise _lib.SrditError(f"{what} must be contiguous float32 [{n}]")
 
 
@@ -217,19 +219,19 @@ def code_rows(M, K, dtype, device):
     return torch.empty(M, (K + 15) // 16 * 16, dtype=dtype, device=device)[:, :K]
 
 
-def _codes_out(x, qdtype, q, qscale):
-    """The output tensors of a row quantiser of x [M, K], checked or made."""
-    M, K = x.shape
+def _codes_out(x, M, K, qdtype, q, qscale):
+    """The output tensors of a row quantiser of x [M, K], checked or made, and the code
+    type's number."""
     if q is None:
         q = code_rows(M, K, qdtype or torch.int8, x.device)
-    elif q.shape != x.shape or (qdtype is not None and q.dtype != qdtype):
-        raise _lib.SrditError(f"q {tuple(q.shape)} {q.dtype} for rows {tuple(x.shape)} to "
+    elif q.shape != (M, K) or (qdtype is not None and q.dtype != qdtype):
+        raise _lib.SrditError(f"q {tuple(q.shape)} {q.dtype} for rows {(M, K)} to "
                               f"{qdtype or q.dtype}")
     if qscale is None:
         qscale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
         _scales(qscale, M, "qscale")
-    return q, qscale
+    return q, qscale, _code(CODES, q.dtype, "qdtype")
 
 
 def add_rms_quant(x, weight, eps=1e-6, *, residual=None, sum_out=None, qdtype=None, q=None,
@@ -241,7 +243,7 @@ def add_rms_quant(x, weight, eps=1e-6, *, residual=None, sum_out=None, qdtype=No
     float8_e4m3fn; or ``q``'s own), fp32 scales [M], and x + residual in x's type (None
     without a residual). ``sum_out`` may be x or residual, which is then updated in place.
     Without ``q`` the codes' rows are laid out as ``int8_gemm`` takes them."""
-    _same_device(x, weight, residual, sum_out, q, qscale)
+    stream = _same_device(x, weight, residual, sum_out, q, qscale)
     ldx = _rows(x)
     M, K = x.shape
     dt = _code(DTYPES, x.dtype, "add_rms_quant")
@@ -259,12 +261,11 @@ def add_rms_quant(x, weight, eps=1e-6, *, residual=None, sum_out=None, qdtype=No
         raise _lib.SrditError("sum_out without a residual")
     else:
         ldr = lds = 0
-    q, qscale = _codes_out(x, qdtype, q, qscale)
-    e = x.element_size()
+    q, qscale, code = _codes_out(x, M, K, qdtype, q, qscale)
     _launch("srdit_add_rms_quant", x.data_ptr(), ldx, M, K, dt, _addr(residual), ldr,
-            weight.data_ptr(), float(eps), _addr(sum_out), lds, q.data_ptr(), _rows(q),
-            _code(CODES, q.dtype, "qdtype"), qscale.data_ptr(), _stream(x.device),
-            kind="add_rms_quant", work=M * K * ((3 if residual is not None else 1) * e + 1))
+            weight.data_ptr(), eps, _addr(sum_out), lds, q.data_ptr(), _rows(q), code,
+            qscale.data_ptr(), stream, kind="add_rms_quant",
+            work=M * K * ((3 if residual is not None else 1) * x.element_size() + 1))
     return q, qscale, sum_out
 
 
@@ -272,14 +273,13 @@ def quant_rows(x, *, qdtype=None, q=None, qscale=None):
     """(codes [M, K], fp32 scales [M]) of rows of bf16, fp16 or fp32, K at most 32768: the
     row-wise quantiser for int8 codes and for the widths and types ``quant_rowwise`` does
     not take. Arguments as ``add_rms_quant``."""
-    _same_device(x, q, qscale)
+    stream = _same_device(x, q, qscale)
     ldx = _rows(x)
     M, K = x.shape
     dt = _code(DTYPES, x.dtype, "quant_rows")
-    q, qscale = _codes_out(x, qdtype, q, qscale)
-    _launch("srdit_quant_rows", x.data_ptr(), ldx, M, K, dt, q.data_ptr(), _rows(q),
-            _code(CODES, q.dtype, "qdtype"), qscale.data_ptr(), _stream(x.device),
-            kind="quant_rows", work=M * K * (x.element_size() + 1))
+    q, qscale, code = _codes_out(x, M, K, qdtype, q, qscale)
+    _launch("srdit_quant_rows", x.data_ptr(), ldx, M, K, dt, q.data_ptr(), _rows(q), code,
+            qscale.data_ptr(), stream, kind="quant_rows", work=M * K * (x.element_size() + 1))
     return q, qscale
 
 
@@ -289,7 +289,7 @@ def int8_gemm(a_q, a_scale, w_q, w_scale, bias=None, out=None, *, out_dtype=None
     a_q [M, K], w_q [N, K] int8 with row pitches that are multiples of 16 (``code_rows``
     makes such), fp32 scales [M] and [N]; bias [N] in out's type: ``out_dtype`` bf16 (the
     default), fp16 or fp32, or ``out``'s own. Any M and N; K below 131072."""
-    _same_device(a_q, a_scale, w_q, w_scale, bias, out, status)
+    stream = _same_device(a_q, a_scale, w_q, w_scale, bias, out, status)
     if a_q.dtype != torch.int8 or w_q.dtype != torch.int8:
         raise _lib.SrditError("int8_gemm operands must be int8")
     lda, ldw = _rows(a_q), _rows(w_q)
@@ -309,7 +309,7 @@ def int8_gemm(a_q, a_scale, w_q, w_scale, bias=None, out=None, *, out_dtype=None
         raise _lib.SrditError(f"bias must be contiguous {out.dtype} [{N}]")
     _launch("srdit_int8_gemm", a_q.data_ptr(), a_scale.data_ptr(), w_q.data_ptr(),
             w_scale.data_ptr(), _addr(bias), out.data_ptr(), _code(DTYPES, out.dtype, "int8_gemm"),
-            M, N, K, lda, ldw, _rows(out), _addr(status), _stream(a_q.device), kind="int8_gemm",
+            M, N, K, lda, ldw, _rows(out), _addr(status), stream, kind="int8_gemm",
             work=2 * M * N * K)
     return out
 
@@ -322,7 +322,7 @@ def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, st
     ``kv_lens`` (int32 [B] on the device): sample b sees its first kv_lens[b] keys.
     ``key_mask`` (bool or uint8 [B, Lk]): keys that are seen. A query that sees no key gets
     zeros; what lies in the rows of unseen keys does not matter. ``scale``: D ** -0.5."""
-    _same_device(q, k, v, out, kv_lens, key_mask, status)
+    stream = _same_device(q, k, v, out, kv_lens, key_mask, status)
     dt = _code(HALF_TYPES, q.dtype, "cross_attn")
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise _lib.SrditError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: "
@@ -363,7 +363,7 @@ def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, st
     if kib:
         ws = torch.empty(kib << 10, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), kib << 10
-    _launch("srdit_cross_attn", ref, _stream(q.device), kind="cross_attn",
+    _launch("srdit_cross_attn", ref, stream, kind="cross_attn",
             work=4 * B * Lq * H * D * Lk)
     return out
 
