@@ -39,6 +39,8 @@ struct Params {
   long long ldo;
   int M, N, K;
   int splits;  // split_kernel: CTAs of a cluster along K
+  int tile_n;  // split_kernel: weight rows of a tile, up to 128
+  int stages;  // split_kernel: blocks of K in flight
   int o_tma;   // pair_kernel: tmO is valid (out and its pitch are 16-byte aligned)
   uint32_t* status;
 };
@@ -67,17 +69,19 @@ SRDIT_DEV uint32_t pack2(float x, float y, __half) {
 }
 
 // ---------------------------------------------------------------- few tokens
+// Shared memory: a ring of p.stages stages (weight rows, then tokens), the other CTAs'
+// partial sums, barriers. An MMA reads 128 weight rows of a stage whatever tile_n is; past
+// the last stage that is still inside this CTA's memory.
+constexpr int MAX_STAGES = 16;
 template <int BT>
 struct SplitCfg {
-  static constexpr int W_BYTES = 128 * BK;
-  static constexpr int STAGE_BYTES = W_BYTES + BT * BK;
-  // up to 32 tokens two CTAs share an SM's shared memory; above, one has it
-  static constexpr int STAGES = BT == 32 ? 4 : 5;
-  static constexpr int OFF_PART = STAGES * STAGE_BYTES;  // int32 [splits][BT / splits][128]
-  static constexpr int OFF_BAR = OFF_PART + BT * 128 * 4;
-  static constexpr int SMEM = OFF_BAR + 128 + 1024;
+  static constexpr int PART = BT * 512;  // int32 [splits][4 warps][BT / splits][32]
+  static constexpr int BARS = (2 * MAX_STAGES + 5) * 8 + 8;
+  static constexpr int MOST = 232448 - 1024 - PART - BARS;  // for the ring
   static constexpr uint32_t TMEM_COLS = BT < 32 ? 32 : BT;
-  static_assert(SMEM <= (BT <= 32 ? 115712 : 232448), "shared memory budget");
+  static int smem(int stages, int tile_n) {
+    return stages * (tile_n + BT) * BK + PART + BARS + 1024;
+  }
 };
 
 template <typename T, int BT>
@@ -86,37 +90,55 @@ __global__ void __launch_bounds__(NUM_THREADS)
                  const Params p) {
   pdl_begin();
   using C = SplitCfg<BT>;
-  constexpr int STAGES = C::STAGES;
+  const int STAGES = p.stages;
+  const int w_bytes = p.tile_n * BK, stage_bytes = w_bytes + BT * BK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* empty = full + STAGES;
-  uint64_t* done = empty + STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint8_t* part_smem = smem + STAGES * stage_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(part_smem + C::PART);
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* done = empty + MAX_STAGES;
+  uint64_t* recv = done + 1;  // [4] the other CTAs' partial sums, for each epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(recv + 4);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int n0 = (static_cast<int>(blockIdx.x) / p.splits) * 128;
+  const int n0 = (static_cast<int>(blockIdx.x) / p.splits) * p.tile_n;
   const int m0 = static_cast<int>(blockIdx.y) * BT;
   const int num_kb = (p.K + BK - 1) / BK;
   const int kb0 = static_cast<int>(static_cast<long long>(num_kb) * split / p.splits);
   const int kb1 = static_cast<int>(static_cast<long long>(num_kb) * (split + 1) / p.splits);
 
+  auto load = [&](int i, int s) {  // block i of this CTA's K range into stage s
+    uint8_t* st = smem + s * stage_bytes;
+    mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(stage_bytes));
+    tma_load_2d(st, &tmW, &full[s], (kb0 + i) * BK, n0);
+    tma_load_2d(st + w_bytes, &tmA, &full[s], (kb0 + i) * BK, m0);
+  };
+  const int n_kb = kb1 - kb0;
+  // token columns of this CTA in its cluster: [split * per, split * per + mine)
+  const int per = BT / p.splits;
+  const int mine = min(max(p.M - m0 - split * per, 0), per);
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmA);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
+    for (int x = 0; x < 4; ++x) mbar_init(&recv[x], 1);
     *abort_flag = 0u;
     fence_barrier_init();
+    fence_proxy_async_smem();
+    for (int x = 0; x < 4 && p.splits > 1; ++x)
+      mbar_arrive_expect_tx(&recv[x], static_cast<uint32_t>((p.splits - 1) * mine * 128));
+    // the first loads need none of what the other warps still set up
+    for (int i = 0; i < STAGES && i < n_kb; ++i) load(i, i);
   }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmW);
-  }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
@@ -129,18 +151,19 @@ __global__ void __launch_bounds__(NUM_THREADS)
 
   bool ok = true;
   if (warp == 0) {
-    if (elect_one()) {
-      for (int i = 0, kb = kb0; kb < kb1; ++i, ++kb) {
-        const int s = i % STAGES;
-        if (!mbar_wait(&empty[s], (static_cast<uint32_t>(i / STAGES) & 1u) ^ 1u, p.status,
-                       abort_flag)) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int i = STAGES; i < n_kb; ++i) {
+        if (!mbar_wait(&empty[s], ph, p.status, abort_flag)) {
           ok = false;
           break;
         }
-        uint8_t* st = smem + s * C::STAGE_BYTES;
-        mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
-        tma_load_2d(st, &tmW, &full[s], kb * BK, n0);
-        tma_load_2d(st + C::W_BYTES, &tmA, &full[s], kb * BK, m0);
+        load(i, s);
+        if (++s == STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
       }
       // having given up, let the loads in flight land before the CTA exits
       if (!ok)
@@ -150,90 +173,126 @@ __global__ void __launch_bounds__(NUM_THREADS)
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = idesc_i8(128, BT);
-      for (int i = 0, kb = kb0; kb < kb1; ++i, ++kb) {
-        const int s = i % STAGES;
-        if (!mbar_wait(&full[s], static_cast<uint32_t>(i / STAGES) & 1u, p.status, abort_flag)) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int i = 0; i < n_kb; ++i) {
+        if (!mbar_wait(&full[s], ph, p.status, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t w_addr = smem_u32(smem + s * C::STAGE_BYTES);
+        const uint32_t w_addr = smem_u32(smem + s * stage_bytes);
 #pragma unroll
         for (int k = 0; k < BK / 32; ++k)
           mma_i8_ss(tmem_base, sdesc_sw128(w_addr + k * 32, 16, 1024),
-                    sdesc_sw128(w_addr + C::W_BYTES + k * 32, 16, 1024), idesc,
+                    sdesc_sw128(w_addr + w_bytes + k * 32, 16, 1024), idesc,
                     (i > 0 || k > 0) ? 1u : 0u);
         tc_commit(&empty[s]);
+        if (++s == STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
       }
       if (ok) tc_commit(done);
     }
     __syncwarp();
   }
 
-  // the accumulator: lane = weight row, column = token
+  // the accumulator: lane = weight row, column = token (rows past tile_n: whatever the
+  // buffer held)
   const int sub = warp & 3;
   const uint32_t t_row = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
   const int n = n0 + sub * 32 + lane;
+  const bool n_on = sub * 32 + lane < p.tile_n && n < p.N;
   T* out = static_cast<T*>(p.out) + n;
   if (p.splits == 1) {
     if (warp >= 2 && mbar_wait(done, 0u, p.status, abort_flag)) {
       tc_fence_after();
-      const float sw = n < p.N ? p.w_scale[n] : 0.f;
-      const float b = n < p.N ? bias_at<T>(p, n) : 0.f;
+      const float sw = n_on ? p.w_scale[n] : 0.f;
+      const float b = n_on ? bias_at<T>(p, n) : 0.f;
 #pragma unroll 1
       for (int c = 0; c < BT && m0 + c < p.M; c += 16) {
         uint32_t r[16];
         tmem_ld16(t_row + c, r);
+        float sa[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sa[e] = m0 + c + e < p.M ? __ldg(p.a_scale + m0 + c + e) : 0.f;
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int m = m0 + c + e;
-          if (m < p.M && n < p.N)
-            out[m * p.ldo] = static_cast<T>(scaled(r[e], __ldg(p.a_scale + m), sw, b));
+          if (m < p.M && n_on) out[m * p.ldo] = static_cast<T>(scaled(r[e], sa[e], sw, b));
         }
       }
     }
   } else {
-    // token column c belongs to CTA c / per of the cluster, which gets every CTA's
-    // partial sums of it at part[source][c % per][row]
-    const int per = BT / p.splits;
-    const uint32_t part = smem_u32(smem + C::OFF_PART);
+    // Token column c belongs to CTA c / per of the cluster. Each epilogue warp lays its 32
+    // rows' partial sums out as [c][32] over the ring, which is done with, and copies each
+    // CTA's columns to it; the copies are counted on that CTA's barrier for the warp. (Stores
+    // into the other CTAs' memory, 4 bytes a lane, took 40 ns each.)
     bool got = true;
     if (warp >= 2) got = mbar_wait(done, 0u, p.status, abort_flag);
     __syncwarp();
     cluster_wait();
     if (warp >= 2 && got) {
       tc_fence_after();
+      int* send = reinterpret_cast<int*>(smem) + sub * BT * 32;
 #pragma unroll 1
       for (int c = 0; c < BT && m0 + c < p.M; c += 16) {
         uint32_t r[16];
         tmem_ld16(t_row + c, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int owner = (c + e) / per, at = (c + e) - owner * per;
-          const uint32_t addr =
-              part + static_cast<uint32_t>(((split * per + at) * 128 + sub * 32 + lane) * 4);
-          st_cluster_u32(mapa_shared(addr, static_cast<uint32_t>(owner)), r[e]);
+        for (int e = 0; e < 16; ++e) send[(c + e) * 32 + lane] = static_cast<int>(r[e]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      const int theirs = min(max(p.M - m0 - lane * per, 0), per);  // of CTA `lane`
+      if (lane < p.splits && lane != split && theirs > 0) {
+        const uint32_t dst = smem_u32(part_smem) +
+                             static_cast<uint32_t>((split * 4 + sub) * per * 128);
+        asm volatile(
+            "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, "
+            "[%3];" ::"r"(mapa_shared(dst, static_cast<uint32_t>(lane))),
+            "r"(smem_u32(send + lane * per * 32)), "r"(theirs * 128),
+            "r"(mapa_shared(smem_u32(&recv[sub]), static_cast<uint32_t>(lane)))
+            : "memory");
+      }
+      __syncwarp();
+      if (mine > 0 && mbar_wait(&recv[sub], 0u, p.status, abort_flag)) {
+        const float sw = n_on ? p.w_scale[n] : 0.f;
+        const float b = n_on ? bias_at<T>(p, n) : 0.f;
+        const int* part = reinterpret_cast<const int*>(part_smem) + sub * per * 32 + lane;
+        const int* own = send + split * per * 32 + lane;
+        const int m1 = m0 + split * per;
+        for (int a0 = 0; a0 < mine; a0 += 8) {
+          // eight tokens together: their scales, and their sums over the splits
+          float sa[8];
+          int acc[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool on = a0 + e < mine;
+            sa[e] = on ? __ldg(p.a_scale + m1 + a0 + e) : 0.f;
+            acc[e] = on ? own[(a0 + e) * 32] : 0;
+          }
+          for (int s = 0; s < p.splits; ++s) {
+            if (s == split) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (a0 + e < mine) acc[e] += part[(s * 4 * per + a0 + e) * 32];
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (a0 + e < mine && n_on)
+              out[(m1 + a0 + e) * p.ldo] =
+                  static_cast<T>(scaled(static_cast<uint32_t>(acc[e]), sa[e], sw, b));
         }
       }
     }
     __syncwarp();
+    // no CTA leaves while another copies from or to its memory
     cluster_arrive();
     cluster_wait();
-    if (warp >= 2 && got && n < p.N) {
-      const float sw = p.w_scale[n];
-      const float b = bias_at<T>(p, n);
-      const int* mine = reinterpret_cast<const int*>(smem + C::OFF_PART) + sub * 32 + lane;
-      for (int at = 0; at < per; ++at) {
-        const int m = m0 + split * per + at;
-        if (m >= p.M) break;
-        int acc = 0;
-        for (int s = 0; s < p.splits; ++s) acc += mine[(s * per + at) * 128];
-        out[m * p.ldo] = static_cast<T>(
-            scaled(static_cast<uint32_t>(acc), __ldg(p.a_scale + m), sw, b));
-      }
-    }
   }
   tc_fence_before();
   __syncthreads();
@@ -511,30 +570,58 @@ static int launch_split(const Operands& o, Params& p, int dev, cudaStream_t stre
   using C = SplitCfg<BT>;
   auto kern = split_kernel<T, BT>;
   static std::atomic<bool> attr_done[kMaxDevices] = {};
-  int rc = set_smem(kern, C::SMEM, attr_done, dev);
+  int rc = set_smem(kern, 232448, attr_done, dev);
   if (rc) return rc;
+  // The tile's weight rows and the splits of K with the least time, in cycles: what an SM's
+  // CTAs read at 38 bytes a cycle (an SM's share of the memory is 23; the latency of 2000
+  // cycles wants 76 KB in flight), each wave's start and end, the cluster's exchange.
+  // Clusters of large CTAs do not fill every SM.
+  const int sms = num_sms(dev);
+  const int m_tiles = (p.M + BT - 1) / BT, num_kb = (p.K + BK - 1) / BK;
+  long long best = -1;
+  for (int tile = 128; tile >= 64; tile -= 16) {
+    for (int splits = 1; splits <= 8 && (splits == 1 || splits * 2 <= num_kb); splits *= 2) {
+      const long long ctas = static_cast<long long>((p.N + tile - 1) / tile) * m_tiles * splits;
+      const int n_kb = (num_kb + splits - 1) / splits, stage = (tile + BT) * BK;
+      int stages = C::MOST / stage < MAX_STAGES ? C::MOST / stage : MAX_STAGES;
+      if (stages > n_kb) stages = n_kb;
+      int per_sm = C::smem(stages, tile) <= 115712 ? 2 : 1;
+      if (ctas > sms && per_sm == 1) {  // two smaller rings on an SM rather than a second wave
+        const int half = (115712 - (232448 - C::MOST)) / stage;
+        if (half >= 3) {
+          stages = half < stages ? half : stages;
+          per_sm = 2;
+        }
+      }
+      const long long room = splits > 1 ? sms * per_sm * 7 / 8 : sms * per_sm;
+      const long long waves = (ctas + room - 1) / room;
+      const long long rounds = (ctas + sms - 1) / sms;
+      const long long cost = (rounds > waves ? rounds : waves) * n_kb * stage / 38 + waves * 3000 +
+                             (splits > 1 ? 1500 + BT / splits * 20 : 0);
+      if (best < 0 || cost < best) {
+        best = cost;
+        p.tile_n = tile;
+        p.splits = splits;
+        p.stages = stages;
+      }
+    }
+  }
+  const int n_tiles = (p.N + p.tile_n - 1) / p.tile_n;
   CUtensorMap ta, tw;
   rc = make_tmap_2d(&ta, o.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, o.lda, BK, BT);
   if (rc) return rc;
-  rc = make_tmap_2d(&tw, o.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, o.ldw, BK, 128);
+  rc = make_tmap_2d(&tw, o.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, o.ldw, BK, p.tile_n);
   if (rc) return rc;
-  const int n_tiles = (p.N + 127) / 128, m_tiles = (p.M + BT - 1) / BT;
-  const int slots = num_sms(dev) * (BT <= 32 ? 2 : 1);
-  const int num_kb = (p.K + BK - 1) / BK;
-  // the most splits that still run at once, each with two stages of K at least
-  int splits = 1;
-  while (splits < 8 && 2 * splits * n_tiles * m_tiles <= slots && num_kb >= 4 * splits) splits *= 2;
-  p.splits = splits;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles));
+  cfg.gridDim = dim3(static_cast<unsigned>(n_tiles * p.splits), static_cast<unsigned>(m_tiles));
   cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.dynamicSmemBytes = static_cast<size_t>(C::smem(p.stages, p.tile_n));
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.splits);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -607,7 +694,7 @@ extern "C" int srdit_int8_gemm(const void* a, const float* a_scale, const void* 
       reinterpret_cast<uintptr_t>(a_scale) % 4 || reinterpret_cast<uintptr_t>(w_scale) % 4)
     return SRDIT_EALIGN;
   const i8::Operands o = {a, w, lda, ldw};
-  i8::Params p = {a_scale, w_scale, bias, out, ldo, M, N, K, 1, 0, status};
+  i8::Params p = {a_scale, w_scale, bias, out, ldo, M, N, K, 1, 128, 1, 0, status};
   switch (dtype) {
     case SRDIT_BF16: return i8::launch<__nv_bfloat16>(o, p, stream);
     case SRDIT_FP16: return i8::launch<__half>(o, p, stream);
