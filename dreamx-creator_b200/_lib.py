@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 import threading
 
 PKG = pathlib.Path(__file__).resolve().parent
@@ -97,6 +98,11 @@ class CrossAttnArgs(ctypes.Structure):
                 ("workspace", c_vp), ("workspace_bytes", c_ll), ("status", c_vp)]
 
 
+# the same fields for one pack_into (a third of the time of setting them one by one)
+CROSS_ATTN_LAYOUT = struct.Struct("@4P7i12q2PqfPqP")
+assert CROSS_ATTN_LAYOUT.size == ctypes.sizeof(CrossAttnArgs)
+
+
 # name -> argtypes (every function returns int)
 SIGNATURES = {
     "srdit_version": [],
@@ -157,6 +163,7 @@ class SrditError(RuntimeError):
 
 _lock = threading.Lock()
 _lib = None
+_fns = {}   # entry points by name
 
 
 def header_symbols() -> list[str]:
@@ -191,16 +198,16 @@ def lib() -> ctypes.CDLL:
 
 def count(name: str, *args) -> int:
     """Call an entry point that returns a count (not a status)."""
-    return int(getattr(lib(), name)(*args))
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
+    return int(fn(*args))
 
 
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().srdit_strerror(rc).decode()
         raise SrditError(f"{what} failed with code {rc}: {msg}")
-
-
-_fns = {}
 
 
 def call(name: str, *args) -> None:

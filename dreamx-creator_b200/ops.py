@@ -329,40 +329,40 @@ def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, st
                               "[B, L, heads, D] each")
     B, Lq, H, D = q.shape
     Bk, Lk, Hkv, Dk = k.shape
-    if Bk != B or Dk != D or Hkv == 0 or H % Hkv or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise _lib.SrditError(f"q {tuple(q.shape)} {q.dtype} does not go with k "
+    dtype = q.dtype
+    if Bk != B or Dk != D or Hkv == 0 or H % Hkv or k.dtype != dtype or v.dtype != dtype:
+        raise _lib.SrditError(f"q {tuple(q.shape)} {dtype} does not go with k "
                               f"{tuple(k.shape)} {k.dtype}, v {v.dtype}")
     if out is None:
-        out = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise _lib.SrditError(f"out must be {q.dtype} {tuple(q.shape)}")
-    a = _lib.CrossAttnArgs()
-    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.dtype, a.B, a.Lq, a.Lk, a.H, a.Hkv, a.D = dt, B, Lq, Lk, H, Hkv, D
-    for t, nm, st in ((q, "q", a.q_stride), (k, "k", a.k_stride), (v, "v", a.v_stride),
-                      (out, "out", a.o_stride)):
-        s0, s1, s2, s3 = t.stride()
-        if s3 != 1 and D > 1:
-            raise _lib.SrditError(f"{nm} needs unit stride over D, has {t.stride()}")
-        st[0], st[1], st[2] = s0, s1, s2
+        out = torch.empty(B, Lq, H, D, dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype:
+        raise _lib.SrditError(f"out must be {dtype} {tuple(q.shape)}")
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (qs[3] == ks[3] == vs[3] == os[3] == 1):
+        raise _lib.SrditError(f"q, k, v, out need unit stride over D, have {qs}, {ks}, {vs}, {os}")
+    lens = mask = mask_stride = 0
     if kv_lens is not None:
         if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
             raise _lib.SrditError(f"kv_lens must be contiguous int32 [{B}]")
-        a.kv_lens = kv_lens.data_ptr()
+        lens = kv_lens.data_ptr()
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Lk):
             raise _lib.SrditError(f"key_mask must be bool or uint8 {(B, Lk)}")
         if Lk > 1 and key_mask.stride(1) != 1:
             raise _lib.SrditError("key_mask needs unit stride over the keys")
-        a.key_mask, a.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-    a.scale = D ** -0.5 if scale is None else float(scale)
-    if status is not None:
-        a.status = status.data_ptr()
+        mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+    a = _lib.CrossAttnArgs()
+    fill = _lib.CROSS_ATTN_LAYOUT.pack_into
+    fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dt, B, Lq, Lk, H, Hkv, D,
+              *qs[:3], *ks[:3], *vs[:3], *os[:3], lens, mask, mask_stride,
+              D ** -0.5 if scale is None else scale)
+    st = 0 if status is None else status.data_ptr()
+    fill(a, 0, *fields, 0, 0, st)
     ref = ctypes.byref(a)
     kib = _lib.count("srdit_cross_attn_workspace", ref)
     if kib:
         ws = torch.empty(kib << 10, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), kib << 10
+        fill(a, 0, *fields, ws.data_ptr(), kib << 10, st)
     _launch("srdit_cross_attn", ref, stream, kind="cross_attn",
             work=4 * B * Lq * H * D * Lk)
     return out
