@@ -131,8 +131,13 @@ def convert_linears_to_fp8(model: nn.Module, targets=TARGETS_ALL, skip_first=0, 
     Fp8Linear from an earlier call), is left alone, so the call is idempotent.
     Returns the qualified names converted, e.g. ``"blocks.3.ffn.0"``.
     """
+    return convert_linears(model, Fp8Linear, targets, skip_first, skip_last, blocks_attr)
+
+
+def convert_linears(model, layer, targets, skip_first=0, skip_last=0, blocks_attr="blocks"):
+    """``convert_linears_to_fp8`` with any ``layer`` class that has ``from_linear``."""
     if not torch.cuda.is_available():
-        raise _lib.SrditError("Fp8Linear needs a CUDA device (there is no CPU path)")
+        raise _lib.SrditError(f"{layer.__name__} needs a CUDA device (there is no CPU path)")
     blocks = getattr(model, blocks_attr, None)
     if blocks is None:
         return []
@@ -149,6 +154,6 @@ def convert_linears_to_fp8(model: nn.Module, targets=TARGETS_ALL, skip_first=0, 
                 continue
             owner_path, _, leaf = path.rpartition(".")
             owner = block.get_submodule(owner_path) if owner_path else block
-            owner.add_module(leaf, Fp8Linear.from_linear(lin))
+            owner.add_module(leaf, layer.from_linear(lin))
             converted.append(f"{blocks_attr}.{idx}.{path}")
     return converted

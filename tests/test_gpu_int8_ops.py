@@ -408,3 +408,70 @@ def test_refusals(srdit, cuda_device):
             c()
             pytest.fail(f"case {i} was taken")
     torch.cuda.synchronize()   # nothing was launched that faults
+
+
+# ------------------------------------------------------------------ modules
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,N", [((5, 96), 40), ((2, 3, 50), 33), ((1, 256), 128)])
+def test_int8_linear(srdit, cuda_device, dtype, shape, N):
+    """The module against its own codes: the activation's codes are those of quant_rows
+    (checked above), the product that of int8_gemm."""
+    g = _gen(N)
+    lin = torch.nn.Linear(shape[-1], N, device="cuda", dtype=dtype)
+    m = srdit.int8_linear.Int8Linear.from_linear(lin)
+    x = _randn(g, *shape).to(dtype)
+    y = m(x)
+    assert y.shape == (*shape[:-1], N) and y.dtype == dtype
+    q, s = srdit.ops.quant_rows(x.reshape(-1, shape[-1]))
+    wq, ws = srdit.int8_linear.quantize_weight_int8(lin.weight)
+    prod = (q.double() @ wq.double().t()) * s.double()[:, None] * ws.double()
+    ref = (prod + lin.bias.double()).view(y.shape)
+    size = prod.abs().view(y.shape) + lin.bias.double().abs()
+    assert ((y.double() - ref).abs() <= 4 * U32 * size + U[dtype] * ref.abs() * (1 + 2.0 ** -7)
+            + 2.0 ** -24).all()
+    # and against the Linear itself: an int8 step is 1/127 of the largest value, half of it off
+    # per value at most, in both operands
+    full = x.double() @ lin.weight.double().t() + lin.bias.double()
+    xs, w_abs = x.double().abs(), lin.weight.double().abs()
+    half_x, half_w = xs.amax(-1, keepdim=True) / 254, w_abs.amax(1) / 254
+    off = half_x * w_abs.sum(1) + xs.sum(-1, keepdim=True) * half_w + half_x * half_w * shape[-1]
+    assert ((y.double() - full).abs() <= 1.01 * off + 2 * U[dtype] * full.abs() + 1e-4).all()
+
+
+@pytest.mark.parametrize("B,L,heads,kv_heads", [(1, 1, 2, 2), (3, 1, 4, 2), (2, 70, 4, 1),
+                                                (1, 300, 2, 2)])
+def test_cross_stack(srdit, cuda_device, B, L, heads, kv_heads):
+    """The blocks on the operators against the same blocks with the dequantised weights in 64
+    bits. Each of a block's three quantisations is off by half a step of 1/127 of a row's
+    largest value (4 to 5 sigma), 1% of a row's norm; with two blocks of a norm, an attention
+    and products that keep such relative errors, 5% of the added part bounds their sum."""
+    import importlib
+    tb = importlib.import_module("dreamx-creator_b200.text_block")
+    dim, text_dim, hd = heads * 64, 96, 64
+    stack = tb.CrossStack.random_init(dim=dim, text_dim=text_dim, heads=heads, kv_heads=kv_heads,
+                                      layers=2, seed=3)
+    g = _gen(B + L)
+    x = _randn(g, B, L, dim).to(torch.bfloat16)
+    states = _randn(g, B, 77, text_dim).to(torch.bfloat16)
+    lens = torch.tensor([77, 5, 0][:B], dtype=torch.int32, device="cuda")
+    x0 = x.clone()
+    out = stack(x, stack.text_kv(states), kv_lens=lens)
+    assert torch.equal(x, x0)
+
+    def lin(m, v):
+        w = m.weight_int8[:, :m.in_features].double() * m.weight_scale.double()[:, None]
+        return v @ w.t() + m.bias.double()
+
+    ref = x.double()
+    for b in stack.blocks:
+        n = ref / (ref.pow(2).mean(-1, keepdim=True) + b.eps).sqrt() * b.norm.double()
+        q = lin(b.q, n).view(B, L, heads, hd)
+        kv = lin(b.kv, states.double()).view(B, 77, 2, kv_heads, hd).repeat_interleave(
+            heads // kv_heads, 3)
+        s = torch.einsum("bihd,bjhd->bhij", q, kv[:, :, 0]) * hd ** -0.5
+        keep = torch.arange(77, device="cuda")[None] < lens[:, None]
+        p = torch.softmax(s.masked_fill(~keep[:, None, None], -1e300), -1)
+        p = p * keep[:, None, None]
+        ref = ref + lin(b.o, torch.einsum("bhij,bjhd->bihd", p, kv[:, :, 1]).reshape(B, L, dim))
+    added = ref - x.double()
+    assert (out.double() - ref).norm() <= 0.05 * added.norm() + 2 * U[torch.bfloat16] * ref.norm()
