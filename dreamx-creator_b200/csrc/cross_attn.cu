@@ -36,6 +36,22 @@ namespace xattn {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int TILE = 128;
 
+// n / d and n % d for 0 <= n < 2^31 by a product: mul = ceil(2^(31 + l) / d), 2^l >= d
+struct Divisor {
+  uint32_t mul, shift;
+  int d;
+  static Divisor of(int d) {
+    uint32_t l = 0;
+    while ((1ll << l) < d) ++l;
+    const uint64_t two = 1ull << (31 + l);
+    return {static_cast<uint32_t>((two + d - 1) / d), 31 + l, d};
+  }
+  SRDIT_DEV int div(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
+  }
+  SRDIT_DEV int mod(int n) const { return n - div(n) * d; }
+};
+
 struct Args {
   const void* q;
   const void* k;
@@ -47,6 +63,7 @@ struct Args {
   int pack;        // tile_kernel: heads of a group side by side in a query tile
   int rt;          // tile_kernel: tokens of a query tile (pack * rt rows)
   int nq, nhp;     // tile_kernel: query-tile pairs per head pack, head packs
+  Divisor by_ctas, by_per, by_nq;  // ... by the CTAs, by nq * nhp, by nq
   int q_one, k_one, v_one;         // one sample's tensor for all (batch stride 0)
   int k_one_head, v_one_head;      // one key head for all (head stride 0)
   int ranged;      // tile_kernel: every CTA has an equal range of key-tile steps
@@ -67,7 +84,12 @@ SRDIT_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// the largest of three; NaN if one is
+// the larger of two, the largest of three; NaN if one is
+SRDIT_DEV float max2(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
 SRDIT_DEV float max3(float x, float y, float z) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -109,7 +131,7 @@ SRDIT_DEV void join_rows(const Args& a, int n, At at, const float2* ml, T* out, 
     }
     float mn = m;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) mn = fmaxf(mn, pm[x].x);
+    for (int x = 0; x < 4; ++x) mn = max2(mn, pm[x].x);
     if (mn == neg_inf()) continue;  // no key seen yet
     const float f = ex2(m - mn);
     m = mn;
@@ -187,7 +209,7 @@ struct Walk {
   SRDIT_DEV int keys(int x) const { return lens ? lens[x] : key_count(a, x); }
   SRDIT_DEV int tiles(int x) const { return (keys(x) + TILE - 1) / TILE; }
   // where the ranged steps of a CTA begin (make_plan keeps the product below 2^31)
-  SRDIT_DEV int bound(int c) const { return count * c / ctas; }
+  SRDIT_DEV int bound(int c) const { return a.by_ctas.div(count * c); }
   // to the n-th item of samples with keys
   SRDIT_DEV void find_item(int n) {
     for (b = 0;; ++b) {
@@ -219,7 +241,7 @@ struct Walk {
       int items = 0;
       for (int x = 0; x < a.B; ++x)
         if (keys(x) > 0) items += per;
-      whole = items / ctas * ctas;
+      whole = items - a.by_ctas.mod(items);
       if (whole < items) {
         find_item(whole);
         b0 = b;
@@ -234,16 +256,17 @@ struct Walk {
       if (a.ranged) {
         find_item(at);
       } else {  // of all samples: those without keys are passed over in next()
-        b = at / per;
-        rest = at % per;
+        b = a.by_per.div(at);
+        rest = at - b * per;
         nt = tiles(b);
       }
     }
   }
   SRDIT_DEV void item(Item& o) const {
     o.b = b;
-    o.h0 = rest / a.nq * a.pack;
-    o.tok0 = rest % a.nq * 2 * a.rt;
+    const int pack = a.by_nq.div(rest);
+    o.h0 = pack * a.pack;
+    o.tok0 = (rest - pack * a.nq) * 2 * a.rt;
     o.act1 = o.tok0 + a.rt < a.Lq;
     o.len = keys(b);
     o.parts = 0;
@@ -267,8 +290,9 @@ struct Walk {
             nt = tiles(++b);
           }
         } else if (rest >= per) {
-          b += rest / per;
-          rest %= per;
+          const int n = a.by_per.div(rest);
+          b += n;
+          rest -= n * per;
           nt = tiles(b);
         }
       }
@@ -607,9 +631,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll
             for (int e = 1; e < 31; e += 2)
               mx[w] = max3(mx[w], __uint_as_float(s[w][e]), __uint_as_float(s[w][e + 1]));
-            mx[w] = max3(mx[w], mx[w], __uint_as_float(s[w][31]));
+            mx[w] = max2(mx[w], __uint_as_float(s[w][31]));
           }
-          const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.c;
+          const float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]) * a.c;
           // the maximum moves (and O is rescaled) only when a tile's is 8 above it:
           // weights stay below 2^8 and the quotient is the same
           // (written so that a NaN raises it too, and stays in l and O)
@@ -780,8 +804,9 @@ __global__ void __launch_bounds__(256) join_ranges_kernel(const __grid_constant_
     acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   for (int p = 0; p < cut.parts; ++p) {
-    const int cta = static_cast<int>(blockIdx.x) + p, ctas = static_cast<int>(gridDim.x) + 1;
-    if (cut.count * cta / ctas == cut.count * (cta + 1) / ctas) continue;  // an empty range
+    const int cta = static_cast<int>(blockIdx.x) + p;
+    if (a.by_ctas.div(cut.count * cta) == a.by_ctas.div(cut.count * (cta + 1)))
+      continue;  // an empty range
     const int slot = p == 0 ? 2 * cta + 1 : 2 * cta;
     const float2* ml = reinterpret_cast<const float2*>(a.ml) + slot * SLOT_ROWS + group * 32 + r0;
     const float* box = a.ws + (static_cast<long long>(slot) * 8 + group) * (DP / 32) * 1024;
@@ -798,7 +823,7 @@ __global__ void __launch_bounds__(256) join_ranges_kernel(const __grid_constant_
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if (pm[x].x == neg_inf()) continue;  // it saw no key (or the row is none)
-      const float mn = max3(m[x], m[x], pm[x].x);
+      const float mn = max2(m[x], pm[x].x);
       const float f0 = ex2(m[x] - mn), f1 = ex2(pm[x].x - mn);
       m[x] = mn;
       l[x] = l[x] * f0 + pm[x].y * f1;
@@ -1034,10 +1059,10 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
       // s[0], s[2]: column 2c, keys g and g + 8; s[1], s[3]: column 2c + 1
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float top = fmaxf(s[e], s[2 + e]);
+        float top = max2(s[e], s[2 + e]);
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float mn = fmaxf(m[n][e], top * a.c);
+        for (int x = 4; x < 32; x <<= 1) top = max2(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float mn = max2(m[n][e], top * a.c);
         const float neg = mn == neg_inf() ? 0.f : -mn;
         alpha[n][e] = ex2(m[n][e] + neg);
         moved |= mn != m[n][e];
@@ -1101,7 +1126,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
     const int row = x / DQ, d = x % DQ * 4;
     float top = neg_inf();
 #pragma unroll
-    for (int w = 0; w < TOKEN_WARPS; ++w) top = fmaxf(top, sml[w][row].x);
+    for (int w = 0; w < TOKEN_WARPS; ++w) top = max2(top, sml[w][row].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
     if (top != neg_inf()) {
@@ -1155,7 +1180,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
                        : "=f"(po[s].x), "=f"(po[s].y), "=f"(po[s].z), "=f"(po[s].w)
                        : "r"(mapa_shared(o0, s)));
         }
-        top = fmaxf(top, pm[s]);
+        top = max2(top, pm[s]);
       }
       if (top != neg_inf()) {
 #pragma unroll
@@ -1473,6 +1498,11 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.rt = p.rt;
   a.nq = p.nq;
   a.nhp = p.nhp;
+  if (!p.token) {
+    a.by_ctas = xattn::Divisor::of(p.ctas);
+    a.by_per = xattn::Divisor::of(p.nq * p.nhp);
+    a.by_nq = xattn::Divisor::of(p.nq);
+  }
   a.splits = p.splits;
   a.ranged = p.ranged;
   a.q_one = u.q_stride[0] == 0;

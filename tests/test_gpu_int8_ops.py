@@ -300,6 +300,26 @@ def test_cross_attn_large_scores(srdit, cuda_device, Lq):
     assert ((y.double() - o).abs() <= 2.0 ** -10 * a + 2.0 ** -10 * o.abs() + 1e-4).all()
 
 
+@pytest.mark.parametrize("Lq", (1, 5, 200))
+@pytest.mark.parametrize("Lk", (1, 300, 9000))
+def test_cross_attn_seen_nan_stays_nan(srdit, cuda_device, Lq, Lk):
+    """A NaN in a seen key reaches every row of its sample, one in a query its own row, one in
+    a seen value its column; nothing else."""
+    g = _gen(Lk)
+    q, k, v = _qkv(g, 4, Lq, Lk, 2, 1, 64, torch.bfloat16)
+    clean = srdit.ops.cross_attn(q, k, v)
+    k[0, Lk // 2, 0, 3] = float("nan")
+    q[1, Lq - 1, 1, 7] = float("nan")
+    v[2, Lk - 1, 0, 9] = float("nan")
+    y = srdit.ops.cross_attn(q, k, v)
+    assert y[0].isnan().all()
+    assert y[1, Lq - 1, 1].isnan().all() and y[2, :, :, 9].isnan().all()
+    y[0] = clean[0]
+    y[1, Lq - 1, 1] = clean[1, Lq - 1, 1]
+    y[2, :, :, 9] = clean[2, :, :, 9]
+    assert torch.equal(y, clean)
+
+
 def test_cross_attn_empty(srdit, cuda_device):
     q = torch.randn(2, 3, 4, 64, device="cuda", dtype=torch.bfloat16)
     kv = torch.empty(2, 0, 4, 64, device="cuda", dtype=torch.bfloat16)
