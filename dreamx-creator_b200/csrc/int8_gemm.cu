@@ -7,16 +7,16 @@
 //
 // Two kernels, one for each thing that bounds the product:
 //
-//   pair_kernel    many tokens, bounded by the tensor cores. A CTA pair computes a
-//                  256 x BN tile with one tcgen05.mma.cta_group::2.kind::i8 per
-//                  32-deep step; two accumulators in tensor memory let a tile's
-//                  epilogue run under the next tile's products; persistent.
-//   split_kernel   few tokens, bounded by the weights' bytes, and token counts that
-//                  give the pairs too few tiles. The weights take the MMA's 128
-//                  rows and the tokens its columns (16 to 128), so a token count of
-//                  1 wastes 15 columns and not 255 rows. K is split over a cluster
-//                  of up to 8 CTAs, whose int32 partial sums meet in shared memory
-//                  of the cluster: no workspace, no atomics, no second launch.
+//   pair_kernel    more than 64 tokens: bounded by the tensor cores, or by what an SM can
+//                  load for them. A CTA pair computes a 256 x BN tile with one
+//                  tcgen05.mma.cta_group::2.kind::i8 per 32-deep step; two accumulators in
+//                  tensor memory let a tile's epilogue run under the next tile's products;
+//                  persistent. BN is chosen by the rounds of tiles it leaves (launch).
+//   split_kernel   up to 64 tokens: bounded by the weights' bytes. The weights take the
+//                  MMA's 128 rows and the tokens its columns (16, 32 or 64), so one token
+//                  wastes 15 columns and not 255 rows. K is split over a cluster of up to 8
+//                  CTAs, whose int32 partial sums meet in shared memory of the cluster: no
+//                  workspace, no atomics, no second launch.
 #include <atomic>
 
 #include "sm100.cuh"
@@ -310,7 +310,7 @@ template <int BN>
 struct PairCfg {
   static constexpr int A_BYTES = 128 * BK;
   static constexpr int STAGE_BYTES = A_BYTES + (BN / 2) * BK;
-  static constexpr int STAGES = BN == 192 ? 6 : 5;
+  static constexpr int STAGES = BN == 256 ? 5 : BN == 192 ? 6 : 7;
   static constexpr int OFF_STG = STAGES * STAGE_BYTES;
   static constexpr int OFF_COL = OFF_STG + EPI_WARPS * 2 * STG_BYTES;
   static constexpr int OFF_BAR = OFF_COL + 2 * 2 * 256 * 4;  // w_scale, bias
@@ -663,13 +663,28 @@ static int launch(const Operands& o, Params& p, cudaStream_t stream) {
   if (p.M <= 16) return launch_split<T, 16>(o, p, dev, stream);
   if (p.M <= 32) return launch_split<T, 32>(o, p, dev, stream);
   if (p.M <= 64) return launch_split<T, 64>(o, p, dev, stream);
+  // The tile width with the least time: rounds of tiles over the pairs, times the cycles of
+  // a block of K, which are the products' (two per column) or the loads' (60 bytes a cycle
+  // and SM), whichever is more.
   const int pairs = num_sms(dev) / 2;
-  const long long m256 = (p.M + 255) / 256;
-  const long long t256 = m256 * ((p.N + 255) / 256), t192 = m256 * ((p.N + 191) / 192);
-  if (p.M <= 128 || t256 <= pairs / 2) return launch_split<T, 128>(o, p, dev, stream);
-  const long long c256 = (t256 + pairs - 1) / pairs * 256, c192 = (t192 + pairs - 1) / pairs * 192;
-  return c192 < c256 ? launch_pair<T, 192>(o, p, dev, stream)
-                     : launch_pair<T, 256>(o, p, dev, stream);
+  const long long m_tiles = (p.M + 255) / 256;
+  int best = 0;
+  long long best_cost = 0;
+  for (int bn : {256, 192, 128, 64}) {
+    const long long rounds = (m_tiles * ((p.N + bn - 1) / bn) + pairs - 1) / pairs;
+    const int mma = 2 * bn, load = (128 + bn / 2) * BK / 60;
+    const long long cost = rounds * (mma > load ? mma : load);
+    if (!best || cost < best_cost) {
+      best = bn;
+      best_cost = cost;
+    }
+  }
+  switch (best) {
+    case 256: return launch_pair<T, 256>(o, p, dev, stream);
+    case 192: return launch_pair<T, 192>(o, p, dev, stream);
+    case 128: return launch_pair<T, 128>(o, p, dev, stream);
+    default: return launch_pair<T, 64>(o, p, dev, stream);
+  }
 }
 
 }  // namespace i8
