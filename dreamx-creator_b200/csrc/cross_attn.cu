@@ -66,7 +66,7 @@ struct Args {
   Divisor by_ctas, by_per, by_nq;  // ... by the CTAs, by nq * nhp, by nq
   int q_one, k_one, v_one;         // one sample's tensor for all (batch stride 0)
   int k_one_head, v_one_head;      // one key head for all (head stride 0)
-  int ranged;      // tile_kernel: every CTA has an equal range of key-tile steps
+  int ranged;      // tile_kernel: the last round's items are shared out by key tiles
   int splits;      // token_kernel: parts of the key range
   const int32_t* kv_lens;
   const uint8_t* mask;
@@ -391,159 +391,161 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   // registers: 104 for the producer's and the issuer's warps, 200 for the softmax's (3 x
   // 128 threads were launched with 168 each)
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (elect_one()) {
-      bool ok = true;
-      int idx = 0;              // ring slot uses
-      int nq[2] = {0, 0};       // query tiles loaded
-      auto load_kv = [&](const CUtensorMap* tm, int tile, int h, int b) {
-        const int s = idx % STAGES;
-        if (!mbar_wait(&empty[s], (static_cast<uint32_t>(idx / STAGES) & 1u) ^ 1u, a.status,
-                       abort_flag))
-          return false;
-        uint8_t* dst = smem + C::OFF_KV + s * C::BYTES;
-        mbar_arrive_expect_tx(&full[s], C::BYTES);
-        for (int d = 0; d < DP / 64; ++d)
-          tma_load_4d(dst + d * C::SLAB, tm, &full[s], d * 64, h, tile * TILE, b);
-        ++idx;
-        return true;
-      };
-      auto load_q = [&](const Item& it, int t) {
-        if (!mbar_wait(&q_empty[t], (static_cast<uint32_t>(nq[t]) & 1u) ^ 1u, a.status, abort_flag))
-          return false;
-        uint8_t* dst = smem + t * C::BYTES;
-        mbar_arrive_expect_tx(&q_full[t],
-                              static_cast<uint32_t>(a.pack * a.rt * 128 * (DP / 64)));
-        for (int d = 0; d < DP / 64; ++d)
-          tma_load_4d(dst + d * C::SLAB, &tmQ, &q_full[t], d * 64, it.h0, it.tok0 + t * a.rt,
-                      a.q_one ? 0 : it.b);
-        ++nq[t];
-        return true;
-      };
-      Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
-      Item it;
-      while (ok && walk.next(it)) {
-        const int g = it.h0 / a.group;
-        const int kh = a.k_one_head ? 0 : g, kb = a.k_one ? 0 : it.b;
-        const int vh = a.v_one_head ? 0 : g, vb = a.v_one ? 0 : it.b;
-        ok = load_q(it, 0) && load_kv(&tmK, it.t0, kh, kb);
-        if (ok && it.act1) ok = load_q(it, 1);
-        for (int j = it.t0; j < it.t1 && ok; ++j)
-          ok = load_kv(&tmV, j, vh, vb) && (j + 1 == it.t1 || load_kv(&tmK, j + 1, kh, kb));
-      }
-      // having given up, let the loads in flight land before the CTA exits
-      if (!ok)
-        for (int i = 0; i < 200; ++i) __nanosleep(1000);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    // S0 S1 | PV0 S0' PV1 S1' | ...: a tile's next scores follow its product, so the
-    // weights that share their columns have been read (the tensor core runs in order)
-    if (elect_one()) {
-      constexpr uint32_t fmt = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
-      const uint32_t idesc_s = idesc_make(fmt, fmt, 0u, 0u, 128u, 128u);
-      const uint32_t idesc_o = idesc_make(fmt, fmt, 0u, 1u, 128u, static_cast<uint32_t>(DP));
-      int idx = 0;
-      int nq[2] = {0, 0}, np[2] = {0, 0};
-      auto kv_wait = [&](int u) {
-        return mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
-                         abort_flag);
-      };
-      auto scores = [&](int t, int u) {  // S_t = Q_t K^T, K in ring use u
-        const uint32_t q_addr = smem_u32(smem + t * C::BYTES);
-        const uint32_t k_addr = smem_u32(smem + C::OFF_KV + (u % STAGES) * C::BYTES);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t off = static_cast<uint32_t>((k >> 2) * C::SLAB + (k & 3) * 32);
-          mma_bf16_ss(tmem_base + t * 128u, sdesc_sw128(q_addr + off, 16, 1024),
-                      sdesc_sw128(k_addr + off, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      if (elect_one()) {
+        bool ok = true;
+        int idx = 0;              // ring slot uses
+        int nq[2] = {0, 0};       // query tiles loaded
+        auto load_kv = [&](const CUtensorMap* tm, int tile, int h, int b) {
+          const int s = idx % STAGES;
+          if (!mbar_wait(&empty[s], (static_cast<uint32_t>(idx / STAGES) & 1u) ^ 1u, a.status,
+                         abort_flag))
+            return false;
+          uint8_t* dst = smem + C::OFF_KV + s * C::BYTES;
+          mbar_arrive_expect_tx(&full[s], C::BYTES);
+          for (int d = 0; d < DP / 64; ++d)
+            tma_load_4d(dst + d * C::SLAB, tm, &full[s], d * 64, h, tile * TILE, b);
+          ++idx;
+          return true;
+        };
+        auto load_q = [&](const Item& it, int t) {
+          if (!mbar_wait(&q_empty[t], (static_cast<uint32_t>(nq[t]) & 1u) ^ 1u, a.status,
+                         abort_flag))
+            return false;
+          uint8_t* dst = smem + t * C::BYTES;
+          mbar_arrive_expect_tx(&q_full[t],
+                                static_cast<uint32_t>(a.pack * a.rt * 128 * (DP / 64)));
+          for (int d = 0; d < DP / 64; ++d)
+            tma_load_4d(dst + d * C::SLAB, &tmQ, &q_full[t], d * 64, it.h0, it.tok0 + t * a.rt,
+                        a.q_one ? 0 : it.b);
+          ++nq[t];
+          return true;
+        };
+        Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
+        Item it;
+        while (ok && walk.next(it)) {
+          const int g = it.h0 / a.group;
+          const int kh = a.k_one_head ? 0 : g, kb = a.k_one ? 0 : it.b;
+          const int vh = a.v_one_head ? 0 : g, vb = a.v_one ? 0 : it.b;
+          ok = load_q(it, 0) && load_kv(&tmK, it.t0, kh, kb);
+          if (ok && it.act1) ok = load_q(it, 1);
+          for (int j = it.t0; j < it.t1 && ok; ++j)
+            ok = load_kv(&tmV, j, vh, vb) && (j + 1 == it.t1 || load_kv(&tmK, j + 1, kh, kb));
         }
-        tc_commit(&s_full[t]);
-      };
-      auto product = [&](int t, int u, bool first, int k0, int k1) {  // O_t (+)= P_t V, V in use u
-        const uint32_t v_addr = smem_u32(smem + C::OFF_KV + (u % STAGES) * C::BYTES);
+        // having given up, let the loads in flight land before the CTA exits
+        if (!ok)
+          for (int i = 0; i < 200; ++i) __nanosleep(1000);
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      // S0 S1 | PV0 S0' PV1 S1' | ...: a tile's next scores follow its product, so the
+      // weights that share their columns have been read (the tensor core runs in order)
+      if (elect_one()) {
+        constexpr uint32_t fmt = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
+        const uint32_t idesc_s = idesc_make(fmt, fmt, 0u, 0u, 128u, 128u);
+        const uint32_t idesc_o = idesc_make(fmt, fmt, 0u, 1u, 128u, static_cast<uint32_t>(DP));
+        int idx = 0;
+        int nq[2] = {0, 0}, np[2] = {0, 0};
+        auto kv_wait = [&](int u) {
+          return mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
+                           abort_flag);
+        };
+        auto scores = [&](int t, int u) {  // S_t = Q_t K^T, K in ring use u
+          const uint32_t q_addr = smem_u32(smem + t * C::BYTES);
+          const uint32_t k_addr = smem_u32(smem + C::OFF_KV + (u % STAGES) * C::BYTES);
 #pragma unroll
-        for (int k = k0; k < k1; ++k)
-          mma_bf16_ts(tmem_base + 256u + t * 128u, tmem_base + t * 128u + k * 8u,
-                      sdesc_sw128(v_addr + k * 16 * 128, C::SLAB, 1024), idesc_o,
-                      (!first || k > 0) ? 1u : 0u);
-      };
-      Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
-      Item it = {};
-      bool on = walk.next(it), ok = on;
-      if (ok) {
-        ok = mbar_wait(&q_full[0], 0u, a.status, abort_flag) && kv_wait(0);
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = static_cast<uint32_t>((k >> 2) * C::SLAB + (k & 3) * 32);
+            mma_bf16_ss(tmem_base + t * 128u, sdesc_sw128(q_addr + off, 16, 1024),
+                        sdesc_sw128(k_addr + off, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[t]);
+        };
+        // O_t (+)= P_t V over the keys 16 k0 to 16 k1, V in ring use u
+        auto product = [&](int t, int u, bool first, int k0, int k1) {
+          const uint32_t v_addr = smem_u32(smem + C::OFF_KV + (u % STAGES) * C::BYTES);
+#pragma unroll
+          for (int k = k0; k < k1; ++k)
+            mma_bf16_ts(tmem_base + 256u + t * 128u, tmem_base + t * 128u + k * 8u,
+                        sdesc_sw128(v_addr + k * 16 * 128, C::SLAB, 1024), idesc_o,
+                        (!first || k > 0) ? 1u : 0u);
+        };
+        Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
+        Item it = {};
+        bool on = walk.next(it), ok = on;
         if (ok) {
-          tc_fence_after();
-          scores(0, 0);
-          ++nq[0];
-          if (it.t1 - it.t0 == 1) tc_commit(&q_empty[0]);
-          if (it.act1) {
-            ok = mbar_wait(&q_full[1], 0u, a.status, abort_flag);
-            if (ok) {
+          ok = mbar_wait(&q_full[0], 0u, a.status, abort_flag) && kv_wait(0);
+          if (ok) {
+            tc_fence_after();
+            scores(0, 0);
+            ++nq[0];
+            if (it.t1 - it.t0 == 1) tc_commit(&q_empty[0]);
+            if (it.act1) {
+              ok = mbar_wait(&q_full[1], 0u, a.status, abort_flag);
+              if (ok) {
+                tc_fence_after();
+                scores(1, 0);
+                ++nq[1];
+                if (it.t1 - it.t0 == 1) tc_commit(&q_empty[1]);
+              }
+            }
+            tc_commit(&empty[0]);
+          }
+        }
+        int j = it.t0;
+        while (ok && on) {
+          // the step after (it, j): the item's next key tile, or another item's first
+          Item nx = it;
+          int nj = j + 1;
+          const bool last = nj == it.t1;
+          bool more = true;
+          if (last) {
+            more = walk.next(nx);
+            nj = nx.t0;
+          }
+          const int uv = idx + 1, uk = idx + 2;
+          ok = kv_wait(uv);
+          bool k_ready = false;
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (t == 0 || it.act1) {
+              ok = mbar_wait(&p_half[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
+              if (!ok) break;
               tc_fence_after();
-              scores(1, 0);
-              ++nq[1];
-              if (it.t1 - it.t0 == 1) tc_commit(&q_empty[1]);
+              product(t, uv, j == it.t0, 0, 4);
+              ok = mbar_wait(&p_full[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              ++np[t];
+              product(t, uv, j == it.t0, 4, 8);
+              if (last) tc_commit(&o_full[t]);
+            }
+            if (more && (t == 0 || nx.act1)) {
+              if (!k_ready) ok = kv_wait(uk);
+              k_ready = true;
+              if (ok && last) {
+                ok = mbar_wait(&q_full[t], static_cast<uint32_t>(nq[t]) & 1u, a.status, abort_flag);
+                ++nq[t];
+              }
+              if (!ok) break;
+              tc_fence_after();
+              scores(t, uk);
+              if (nj + 1 == nx.t1) tc_commit(&q_empty[t]);
             }
           }
-          tc_commit(&empty[0]);
+          if (!ok) break;
+          tc_commit(&empty[uv % STAGES]);
+          if (more) tc_commit(&empty[uk % STAGES]);
+          idx += 2;
+          it = nx;
+          on = more;
+          j = nj;
         }
       }
-      int j = it.t0;
-      while (ok && on) {
-        // the step after (it, j): the item's next key tile, or another item's first
-        Item nx = it;
-        int nj = j + 1;
-        const bool last = nj == it.t1;
-        bool more = true;
-        if (last) {
-          more = walk.next(nx);
-          nj = nx.t0;
-        }
-        const int uv = idx + 1, uk = idx + 2;
-        ok = kv_wait(uv);
-        bool k_ready = false;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (t == 0 || it.act1) {
-            ok = mbar_wait(&p_half[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            product(t, uv, j == it.t0, 0, 4);
-            ok = mbar_wait(&p_full[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            ++np[t];
-            product(t, uv, j == it.t0, 4, 8);
-            if (last) tc_commit(&o_full[t]);
-          }
-          if (more && (t == 0 || nx.act1)) {
-            if (!k_ready) ok = kv_wait(uk);
-            k_ready = true;
-            if (ok && last) {
-              ok = mbar_wait(&q_full[t], static_cast<uint32_t>(nq[t]) & 1u, a.status, abort_flag);
-              ++nq[t];
-            }
-            if (!ok) break;
-            tc_fence_after();
-            scores(t, uk);
-            if (nj + 1 == nx.t1) tc_commit(&q_empty[t]);
-          }
-        }
-        if (!ok) break;
-        tc_commit(&empty[uv % STAGES]);
-        if (more) tc_commit(&empty[uk % STAGES]);
-        idx += 2;
-        it = nx;
-        on = more;
-        j = nj;
-      }
+      __syncwarp();
     }
-    __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------ softmax
@@ -596,7 +598,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 ok = false;
                 break;
               }
-              const uint32_t mine = sub == 0 ? vis[0] : sub == 1 ? vis[1] : sub == 2 ? vis[2] : vis[3];
+              const uint32_t mine =
+                  sub == 0 ? vis[0] : sub == 1 ? vis[1] : sub == 2 ? vis[2] : vis[3];
               if (!((mine >> lane) & 1u)) {
                 uint8_t* vrow = smem + C::OFF_KV + (u % STAGES) * C::BYTES + row * 128;
                 for (int d = 0; d < DP / 64; ++d)
@@ -1091,8 +1094,10 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         // the lane group's columns 2w (operand row g) and 2w + 1 (row g + 8)
-        const uint32_t a0 = __byte_perm(r0[w], r1[w], 0x5410), a1 = __byte_perm(r0[w], r1[w], 0x7632);
-        const uint32_t a2 = __byte_perm(r2[w], r3[w], 0x5410), a3 = __byte_perm(r2[w], r3[w], 0x7632);
+        const uint32_t a0 = __byte_perm(r0[w], r1[w], 0x5410);
+        const uint32_t a1 = __byte_perm(r0[w], r1[w], 0x7632);
+        const uint32_t a2 = __byte_perm(r2[w], r3[w], 0x5410);
+        const uint32_t a3 = __byte_perm(r2[w], r3[w], 0x7632);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
           mma16816<T>(o[n][x * 4 + w], a0, a1, a2, a3, pf[n][0], pf[n][1]);
@@ -1220,7 +1225,8 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
 
 // One warp per (sample, token, head): joins the parts that went through the workspace.
 template <typename T>
-__global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__ Args a, int parts) {
+__global__ void __launch_bounds__(128)
+    join_parts_kernel(const __grid_constant__ Args a, int parts) {
   pdl_begin();
   const long long rows = static_cast<long long>(a.B) * a.Lq * a.H;
   const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
@@ -1295,7 +1301,8 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
     if (ctas < items) ctas = items;
   }
   const long long idle = last ? tiles - (last * tiles + ctas - 1) / ctas : 0;
-  p.ranged = a.B <= MAX_LENS && idle > RANGE_STEPS && tiles < (1 << 14);  // (steps x CTAs in 32 bits)
+  // (the last bound: steps x CTAs in 32 bits)
+  p.ranged = a.B <= MAX_LENS && idle > RANGE_STEPS && tiles < (1 << 14);
   if (!p.ranged && items < sms) ctas = items;
   p.ctas = static_cast<int>(ctas);
   return p;
@@ -1383,7 +1390,8 @@ static int launch_token(const srdit_cross_attn_args& u, const Args& a, const Pla
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, token_kernel<T, DP, NT, PER_SM>, tk, tv, a, p.cluster));
+  return static_cast<int>(
+      cudaLaunchKernelEx(&cfg, token_kernel<T, DP, NT, PER_SM>, tk, tv, a, p.cluster));
 }
 
 template <typename T, int DP>
@@ -1418,7 +1426,8 @@ static int run(const srdit_cross_attn_args& u, Args& a, const Plan& p, cudaStrea
   }
   if (p.parts == 1) return 0;
   const long long rows = static_cast<long long>(u.B) * u.Lq * u.H;
-  SRDIT_LAUNCH((join_parts_kernel<T>), static_cast<unsigned>((rows + 3) / 4), 128, 0, stream, a, p.parts);
+  SRDIT_LAUNCH((join_parts_kernel<T>), static_cast<unsigned>((rows + 3) / 4), 128, 0, stream, a,
+               p.parts);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1443,8 +1452,10 @@ static int check(const srdit_cross_attn_args& a) {
   if (static_cast<long long>(a.B) * a.Hkv > 65535 ||
       static_cast<long long>(a.B) * a.Lq * a.H > (1ll << 26))
     return SRDIT_EUNSUPPORTED;
-  if (!check_view(a.q, a.q_stride, a.B, a.Lq, a.H) || !check_view(a.k, a.k_stride, a.B, a.Lk, a.Hkv) ||
-      !check_view(a.v, a.v_stride, a.B, a.Lk, a.Hkv) || !check_view(a.out, a.o_stride, a.B, a.Lq, a.H))
+  if (!check_view(a.q, a.q_stride, a.B, a.Lq, a.H) ||
+      !check_view(a.k, a.k_stride, a.B, a.Lk, a.Hkv) ||
+      !check_view(a.v, a.v_stride, a.B, a.Lk, a.Hkv) ||
+      !check_view(a.out, a.o_stride, a.B, a.Lq, a.H))
     return SRDIT_EALIGN;
   if (reinterpret_cast<uintptr_t>(a.kv_lens) & 3u) return SRDIT_EALIGN;
   // an output entry is one place; of the inputs, samples and key heads may be repeated
@@ -1462,7 +1473,8 @@ using namespace srdit;
 
 extern "C" int srdit_cross_attn_workspace(const srdit_cross_attn_args* args) {
   if (!args || xattn::check(*args) != 0) return 0;
-  return static_cast<int>((xattn::make_plan(*args, xattn::sms_here()).ws_floats(*args) + 255) / 256);
+  const xattn::Plan p = xattn::make_plan(*args, xattn::sms_here());
+  return static_cast<int>((p.ws_floats(*args) + 255) / 256);
 }
 
 extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t stream) {
