@@ -33,6 +33,7 @@ struct Args {
   long long ldx, ldr, lds, ldq;
   int M, K;
   int warps;  // warps per row
+  int rows;   // rows per block
   float eps, inv_k;
 };
 
@@ -79,56 +80,127 @@ SRDIT_DEV float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-SRDIT_DEV uint32_t code_i8(float v) {
-  int d;
-  asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(d) : "f"(v));
-  return static_cast<uint32_t>(d) & 0xffu;
+// the largest magnitude of three
+SRDIT_DEV float amax3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
-SRDIT_DEV uint32_t code_e4m3x2(float lo, float hi) {
+SRDIT_DEV float warp_amax(float v) {
+  float d;
+  asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
+}
+SRDIT_DEV uint32_t code_e4m3x2(uint64_t v) {
+  const float2 f = f2_split(v);
   uint16_t h;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(f.y), "f"(f.x));
   return h;
 }
+// The integers nearest to s * inv, for |s * inv| < 2^22: one fma to 1.5 2^23, whose sum has
+// the integer in its low bits (to nearest, ties to even, from the exact product).
+SRDIT_DEV uint64_t near_ints(uint64_t s, uint64_t inv) {
+  return f2_fma(s, inv, f2_pack(12582912.f, 12582912.f));
+}
+SRDIT_DEV uint32_t low_bytes(uint64_t ab) {
+  const float2 f = f2_split(ab);
+  return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x0040);
+}
 
-// V codes as one aligned store
+// V codes of s * inv as one aligned store. `zero`: the row has no finite scale; its int8
+// codes are 0 (e4m3 codes become NaN by themselves)
 template <bool kInt8, int V>
-SRDIT_DEV void store_codes(uint8_t* p, const float (&y)[V]) {
-  if constexpr (V == 1) {
-    *p = static_cast<uint8_t>(kInt8 ? code_i8(y[0]) : code_e4m3x2(y[0], 0.f) & 0xffu);
-  } else {
-    uint32_t h[V / 2];
+SRDIT_DEV void store_codes(uint8_t* p, const float (&s)[V], uint64_t inv, bool zero) {
+  uint32_t h[(V + 1) / 2];
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i)
-      h[i] = kInt8 ? (code_i8(y[2 * i]) | code_i8(y[2 * i + 1]) << 8)
-                   : code_e4m3x2(y[2 * i], y[2 * i + 1]);
-    if constexpr (V == 2) {
-      *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(h[0]);
-    } else {
-      static_assert(V == 8, "1, 2 or 8 codes");
-      *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-    }
+  for (int i = 0; i < (V + 1) / 2; ++i) {
+    const uint64_t v = f2_pack(s[2 * i], V > 1 ? s[2 * i + 1] : 0.f);
+    h[i] = kInt8 ? low_bytes(near_ints(v, inv)) : code_e4m3x2(f2_mul(v, inv));
+    if (kInt8 && zero) h[i] = 0u;
+  }
+  if constexpr (V == 1) {
+    *p = static_cast<uint8_t>(h[0]);
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(h[0]);
+  } else {
+    static_assert(V == 8, "1, 2 or 8 codes");
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
   }
 }
 
-// One row per `warps` warps of the block; a thread holds 8 * NV values of its row as
-// vectors of V (V = 8: 16-byte loads of 16-bit values; 2 and 1 for rows whose width,
-// pitch or base is not so aligned), vector i of thread t at (i * threads + t) * V.
-template <typename T, bool kInt8, bool kNorm, bool kRes, int V, int NV>
+// What a row's values need: the sum of squares and the largest magnitude.
+template <bool kNorm, int V>
+SRDIT_DEV void accumulate(float (&s)[V], const float (&w)[V], uint64_t& ss2, float& mx) {
+#pragma unroll
+  for (int e = 0; e < V; e += 2) {
+    const bool two = e + 1 < V;
+    if constexpr (kNorm) {
+      const uint64_t v = f2_pack(s[e], two ? s[e + 1] : 0.f);
+      ss2 = f2_fma(v, v, ss2);
+      const float2 y = f2_split(f2_mul(v, f2_pack(w[e], two ? w[e + 1] : 0.f)));
+      s[e] = y.x;
+      if (two) s[e + 1] = y.y;
+    }
+    mx = amax3(mx, s[e], two ? s[e + 1] : 0.f);
+  }
+}
+
+// The row's sums over its `warps` warps, the first of them `warp0` of the block, in the same
+// order in every thread; then its scale and the factor from values to codes.
+template <bool kInt8, bool kNorm>
+SRDIT_DEV void row_scale(const Args& a, uint64_t ss2, float mx, int warps, int warp0, float2* part,
+                         float& scale, float& inv) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float2 sp = f2_split(ss2);
+  float ss = sp.x + sp.y;
+  mx = warp_amax(mx);
+  if constexpr (kNorm) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  }
+  if (warps > 1) {
+    if (lane == 0) part[warp] = make_float2(ss, mx);
+    __syncthreads();
+    const float2 p = lane < warps ? part[warp0 + lane] : make_float2(0.f, 0.f);
+    mx = warp_amax(p.y);
+    if constexpr (kNorm) {
+      ss = p.x;
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        if (o < warps) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      ss = __shfl_sync(0xffffffffu, ss, 0);
+    }
+  }
+  // Approximate root and quotient, 2 units in the last place: every thread computes these.
+  const float rstd = kNorm ? rsqrtf(fmaf(ss, a.inv_k, a.eps)) : 1.0f;
+  scale = max_nan(mx * rstd * (kInt8 ? 1.f / 127.f : 1.f / 448.f), 1e-12f);
+  inv = __fdividef(rstd, scale);
+}
+
+// Rows of up to 8192: one row per `warps` warps of the block, 8 values of it in a thread's
+// registers as vectors of V (V = 8: 16-byte loads of 16-bit values; 2 and 1 for rows whose
+// width, pitch or base is not so aligned), vector i of thread t at (i * threads + t) * V.
+// Bounded by memory: 6912 x 3072 bf16 with the residual takes 27.3 us, 5.45 TB/s, what a
+// copy of as many bytes reaches. (With scalar arithmetic, an exact root and quotients in every
+// thread it took 34 instructions a value, 70% of the issue slots, and 30.9 us. With 16, 24
+// and 32 values in a thread this one takes 29.3, 29.5 and 31.2 us, and a single row of 4096
+// 2.9, 3.3 and 3.8 us in place of 2.5.)
+template <typename T, bool kInt8, bool kNorm, bool kRes, int V>
 __global__ void __launch_bounds__(1024) rows_kernel(const Args a) {
   pdl_begin();
-  constexpr int N = 8 * NV / V;
+  constexpr int N = 8 / V;
   __shared__ float2 part[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int tpr = a.warps * 32;
-  const int sub = warp / a.warps;  // row of the block
+  const int sub = a.warps < 4 ? warp / a.warps : 0;  // row of the block
   const int t = threadIdx.x - sub * tpr;
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + sub;
+  const long long row = static_cast<long long>(blockIdx.x) * a.rows + sub;
   const bool on = row < a.M;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* r = kRes ? static_cast<const T*>(a.res) + row * a.ldr : nullptr;
   const T* w = static_cast<const T*>(a.w);
   float s[N][V];
-  float ss = 0.f, mx = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = (i * tpr + t) * V;
@@ -140,11 +212,10 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) s[i][e] += rr[e];
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[i][e] = 0.f;
     }
   }
+  uint64_t ss2 = f2_pack(0.f, 0.f);
+  float mx = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = (i * tpr + t) * V;
@@ -152,66 +223,81 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Args a) {
       if constexpr (kRes) store<T, V>(static_cast<T*>(a.sum) + row * a.lds + c, s[i]);
       float ww[V];
       if constexpr (kNorm) load<T, V>(w + c, ww);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if constexpr (kNorm) {
-          ss = fmaf(s[i][e], s[i][e], ss);
-          s[i][e] *= ww[e];
-        }
-        mx = max_nan(mx, fabsf(s[i][e]));
-      }
+      accumulate<kNorm, V>(s[i], ww, ss2, mx);
     }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    if constexpr (kNorm) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  }
-  if (a.warps > 1) {
-    if (lane == 0) part[warp] = make_float2(ss, mx);
-    __syncthreads();
-    // every warp reduces its row's partials itself, in the same order
-    const float2 p = lane < a.warps ? part[sub * a.warps + lane] : make_float2(0.f, 0.f);
-    ss = p.x;
-    mx = p.y;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      if constexpr (kNorm) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-  }
+  float scale, inv;
+  row_scale<kInt8, kNorm>(a, ss2, mx, a.warps, sub * a.warps, part, scale, inv);
   if (!on) return;
-  const float rstd = kNorm ? 1.0f / sqrtf(fmaf(ss, a.inv_k, a.eps)) : 1.0f;
-  const float scale = max_nan(mx * rstd / (kInt8 ? 127.f : 448.f), 1e-12f);
-  const float inv = rstd / scale;
+  const bool zero = !(scale < __int_as_float(0x7f800000));
   if (t == 0) a.scale[row] = scale;
   uint8_t* q = a.q + row * a.ldq;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = (i * tpr + t) * V;
-    if (c < a.K) {
-      float y[V];
+    if (c < a.K) store_codes<kInt8, V>(q + c, s[i], f2_pack(inv, inv), zero);
+  }
+}
+
+// Wider rows: one block of 512 threads a row, which it reads twice, the second time out of
+// the caches. The sum is stored in the second pass, since it may be x or the residual.
+template <typename T, bool kInt8, bool kNorm, bool kRes, int V>
+__global__ void __launch_bounds__(512) wide_rows_kernel(const Args a) {
+  pdl_begin();
+  __shared__ float2 part[16];
+  const long long row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* r = kRes ? static_cast<const T*>(a.res) + row * a.ldr : nullptr;
+  const T* w = static_cast<const T*>(a.w);
+  auto value = [&](int c, float(&s)[V]) {
+    load<T, V>(x + c, s);
+    if constexpr (kRes) {
+      float rr[V];
+      load<T, V>(r + c, rr);
 #pragma unroll
-      for (int e = 0; e < V; ++e) y[e] = s[i][e] * inv;
-      store_codes<kInt8, V>(q + c, y);
+      for (int e = 0; e < V; ++e) s[e] += rr[e];
     }
+  };
+  uint64_t ss2 = f2_pack(0.f, 0.f);
+  float mx = 0.f;
+#pragma unroll 4
+  for (int c = threadIdx.x * V; c < a.K; c += 512 * V) {
+    float s[V], ww[V];
+    value(c, s);
+    if constexpr (kNorm) load<T, V>(w + c, ww);
+    accumulate<kNorm, V>(s, ww, ss2, mx);
+  }
+  float scale, inv;
+  row_scale<kInt8, kNorm>(a, ss2, mx, 16, 0, part, scale, inv);
+  const bool zero = !(scale < __int_as_float(0x7f800000));
+  if (threadIdx.x == 0) a.scale[row] = scale;
+  uint8_t* q = a.q + row * a.ldq;
+#pragma unroll 4
+  for (int c = threadIdx.x * V; c < a.K; c += 512 * V) {
+    float s[V];
+    value(c, s);
+    if constexpr (kRes) store<T, V>(static_cast<T*>(a.sum) + row * a.lds + c, s);
+    if constexpr (kNorm) {
+      float ww[V];
+      load<T, V>(w + c, ww);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] *= ww[e];
+    }
+    store_codes<kInt8, V>(q + c, s, f2_pack(inv, inv), zero);
   }
 }
 
 template <typename T, bool kInt8, bool kNorm, bool kRes, int V>
 static int launch_v(Args& a, cudaStream_t stream) {
-  // 8 values per thread up to 8192 columns, 32 above (a row is one block's). With 16, 24
-  // and 32 a row of 4096 takes 2.9, 3.2 and 3.6 us in place of 2.6; 6912 rows of 3072 take
-  // 31.6, 30.5 and 32.2 in place of 30.9.
-  const int nv = a.K <= 8192 ? 1 : 4;
-  a.warps = (a.K + nv * 256 - 1) / (nv * 256);
-  const int rows = a.warps >= 4 ? 1 : 4 / a.warps;
-  const int threads = rows * a.warps * 32;
-  const unsigned grid = static_cast<unsigned>((a.M + rows - 1) / rows);
-  if (nv == 1)
-    SRDIT_LAUNCH((rows_kernel<T, kInt8, kNorm, kRes, V, 1>), grid, threads, 0, stream, a);
-  else
-    SRDIT_LAUNCH((rows_kernel<T, kInt8, kNorm, kRes, V, 4>), grid, threads, 0, stream, a);
+  if (a.K > 8192) {
+    SRDIT_LAUNCH((wide_rows_kernel<T, kInt8, kNorm, kRes, V>), static_cast<unsigned>(a.M), 512, 0,
+                 stream, a);
+    return static_cast<int>(cudaGetLastError());
+  }
+  a.warps = (a.K + 255) / 256;
+  a.rows = a.warps >= 4 ? 1 : 4 / a.warps;
+  const unsigned grid = static_cast<unsigned>((a.M + a.rows - 1) / a.rows);
+  SRDIT_LAUNCH((rows_kernel<T, kInt8, kNorm, kRes, V>), grid, a.rows * a.warps * 32, 0, stream, a);
   return static_cast<int>(cudaGetLastError());
 }
 
