@@ -16,8 +16,7 @@
 //                 and the exponentials. Two tiles of 128 query rows share every key
 //                 tile; while one is in its softmax the other has the tensor core.
 //   token_kernel  up to 16 query rows per key head (single tokens): bounded by the
-//                 bytes of k and v, which go from memory to registers once, in the
-//                 layout of the mma operands, without shared memory.
+//                 bytes of k and v, which each warp streams through a ring of its own.
 //
 // Long contexts with few rows are split over the keys; the parts' (m, l, O) meet in
 // shared memory of a cluster (token_kernel) or in the workspace (join_parts_kernel,
@@ -159,7 +158,6 @@ SRDIT_DEV void join_rows(const Args& a, int n, At at, const float2* ml, T* out, 
 constexpr int TILE_THREADS = 384;  // producer and MMA issuer, 2 x 4 softmax warps
 constexpr int SLOT_ROWS = 2 * TILE;
 constexpr int MAX_RANGES = 256;  // CTAs of a launch that may be ranged
-constexpr int RANGE_STEPS = 4;
 constexpr int MAX_LENS = 32;     // samples whose key counts are kept in shared memory
 
 template <int DP>
@@ -331,6 +329,19 @@ struct Cut {
   int pad[3];
 };
 
+// Warp 0 loads, warp 1 issues the products, warps 4 to 7 and 8 to 11 are the softmax of one
+// query tile each, a row a thread, so a row's maximum and sum need no exchange. A key tile of
+// a pair is four products of 128 x 128 x DP and 2 x 128 x 128 exponentials: at 128 columns
+// 2048 cycles of the tensor core (4096 multiply-adds a cycle) and as many of the unit that
+// takes exponentials (16 a cycle); both read 59% busy.
+// Measured: 24 heads of 128, 4096 queries on 8192 keys 326 us, 1.26 PFLOP/s; with the softmax
+// left out, the same loads and products take 294 (the clock falls under their power: cuBLAS
+// holds 1.39 PFLOP/s in such a loop). 6912 queries on 512 keys 51 us, 0.85 PFLOP/s: an item is
+// four key tiles there, between a load of q, the first scores and a store that nothing hides.
+// 3 x 777 queries on up to 1501 masked keys, 16 heads of 64 over 4: 34 us.
+// Slower: half of the exponentials as polynomials (no gain), the weights in two passes over
+// the scores (389 us), a warp that applies the mask, a ring of five K or V tiles, ranges
+// in place of whole rounds (365).
 template <typename T, int DP>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -911,6 +922,10 @@ struct TokenCfg {
 // is refilled before the block is computed. (Of the ways to fill it, TMA boxes of 16 rows
 // keep up with the memory; 16 bytes a lane by cp.async held an SM to 45 GB/s, and a bulk
 // copy per row to one row in 8 to 20 cycles.)
+// The scores are S^T = K Q^T, 16 keys by 8 rows an instruction, so a row's weights are the
+// operand of O^T = V^T P^T as they stand; v is turned in registers, 8 x 8 at a time.
+// Measured: 4 x 32768 keys, 32 heads over 8, one token 86 us, 6.25 TB/s (a sum over as many
+// bytes reads 5.65); 8 x up to 512 keys, 24 heads 8.2 us: start, one block's latency, join.
 template <typename T, int DP, int NT, int PER_SM>
 __global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
     token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -1257,6 +1272,8 @@ struct Plan {
 static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   Plan p = {};
   const int group = a.H / a.Hkv;
+  // 16 rows, token_kernel and tile_kernel: 8 x 512 keys, 24 heads 16.0 and 20.9 us (one row
+  // 12.3); 4 x 32768 keys, 8 heads 93.6 and 107.8 (four rows 87.4)
   p.token = static_cast<long long>(a.Lq) * group <= 16;
   p.splits = p.cluster = p.parts = 1;
   if (p.token) {
@@ -1292,7 +1309,10 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   const long long tiles = (a.Lk + TILE - 1) / TILE;
   // A last round of whole items is partly empty (and samples of different lengths, which
   // only the device knows, leave more idle than that); ranges of equal steps are not, but
-  // joining their parts costs about what RANGE_STEPS steps do.
+  // joining their parts costs what 4 steps of the only round do, and 7 of a last one (more
+  // CTAs with parts). Ranged and whole: 16 items of 5, 8, 16 key tiles 19.0 and 15.0, 18.3 and
+  // 20.5, 23.8 and 34.5 us; 192 items of 8, 12, 16 tiles 42.9 and 39.0, 51.7 and 53.4, 61.6
+  // and 67.8 us; 160 items of 8 tiles 39.5 and 38.4.
   if (sms > MAX_RANGES) sms = MAX_RANGES;
   const long long last = items % sms;
   long long ctas = sms;
@@ -1302,7 +1322,7 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   }
   const long long idle = last ? tiles - (last * tiles + ctas - 1) / ctas : 0;
   // (the last bound: steps x CTAs in 32 bits)
-  p.ranged = a.B <= MAX_LENS && idle > RANGE_STEPS && tiles < (1 << 14);
+  p.ranged = a.B <= MAX_LENS && idle > (items < sms ? 4 : 7) && tiles < (1 << 14);
   if (!p.ranged && items < sms) ctas = items;
   p.ctas = static_cast<int>(ctas);
   return p;
@@ -1376,22 +1396,9 @@ static int launch_token(const srdit_cross_attn_args& u, const Args& a, const Pla
   CUtensorMap tk, tv;
   rc = kv_maps(&tk, &tv, u, 16);
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.B * a.Hkv));
-  cfg.blockDim = dim3(TOKEN_WARPS * 32);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return static_cast<int>(
-      cudaLaunchKernelEx(&cfg, token_kernel<T, DP, NT, PER_SM>, tk, tv, a, p.cluster));
+  const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.B * a.Hkv));
+  return launch_clusters(p.cluster, token_kernel<T, DP, NT, PER_SM>, grid, TOKEN_WARPS * 32,
+                         C::SMEM, stream, tk, tv, a, p.cluster);
 }
 
 template <typename T, int DP>

@@ -62,6 +62,26 @@ int launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
 }
 
+// A launch as clusters of `cluster` CTAs along x. Never programmatic: one program that let
+// clusters of the next launch start early lost its context, and no cause was found.
+template <typename... KArgs, typename... Args>
+int launch_clusters(int cluster, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                    cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
+}
+
 }  // namespace srdit
 
 // Launch a kernel of the library (programmatic stream serialization when
