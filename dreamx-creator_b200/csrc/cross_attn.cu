@@ -799,57 +799,68 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   }
 }
 
-// One block per 32 rows of the items that the CTAs' ranges cut: joins their parts.
+// One block per JOIN_ROWS rows of the items that the CTAs' ranges cut: joins their parts, two
+// rows a warp and four parts' loads in flight. (With four rows a warp and one part at a time it
+// took MEASURED.)
+constexpr int JOIN_ROWS = 16;
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) join_ranges_kernel(const __grid_constant__ Args a) {
   pdl_begin();
   const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[blockIdx.x];
   if (cut.parts == 0) return;
+  constexpr int R = DP / 64;  // rows of a thread: a row of 64 takes half a warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = blockIdx.y;  // query tile x lane quarter
-  const int r0 = warp * 4;       // four rows of the 32 a warp
-  const int quad = lane & 7, d = lane >> 3;
-  float m[4], l[4];
-  float4 acc[4];
+  const int group = blockIdx.y >> 1;  // query tile x lane quarter
+  const int r0 = (blockIdx.y & 1) * JOIN_ROWS + warp * 2 + (DP == 64 ? lane >> 4 : 0);
+  const int quad = lane & 7, d = (lane >> 3) & (DP / 32 - 1);
+  float m[R], l[R];
+  float4 acc[R];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
+  for (int x = 0; x < R; ++x) {
     m[x] = neg_inf();
     l[x] = 0.f;
     acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  for (int p = 0; p < cut.parts; ++p) {
-    const int cta = static_cast<int>(blockIdx.x) + p;
-    if (a.by_ctas.div(cut.count * cta) == a.by_ctas.div(cut.count * (cta + 1)))
-      continue;  // an empty range
-    const int slot = p == 0 ? 2 * cta + 1 : 2 * cta;
-    const float2* ml = reinterpret_cast<const float2*>(a.ml) + slot * SLOT_ROWS + group * 32 + r0;
-    const float* box = a.ws + (static_cast<long long>(slot) * 8 + group) * (DP / 32) * 1024;
-    float2 pm[4];
-    float4 v[4];
+  for (int p0 = 0; p0 < cut.parts; p0 += 4) {
+    float2 pm[4][R];
+    float4 v[4][R];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int r = r0 + x;
-      pm[x] = ml[x];
-      v[x] = d < DP / 32 ? *reinterpret_cast<const float4*>(box + (d * 32 + r) * 32 +
-                                                            ((quad ^ (r & 7)) << 2))
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int y = 0; y < 4; ++y) {
+      const int cta = static_cast<int>(blockIdx.x) + p0 + y;
+      const bool on = p0 + y < cut.parts &&  // and its range is not empty
+                      a.by_ctas.div(cut.count * cta) < a.by_ctas.div(cut.count * (cta + 1));
+      const int slot = p0 + y == 0 ? 2 * cta + 1 : 2 * cta;
+      const float2* ml = reinterpret_cast<const float2*>(a.ml) + slot * SLOT_ROWS + group * 32;
+      const float* box = a.ws + (static_cast<long long>(slot) * 8 + group) * (DP / 32) * 1024;
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        const int r = r0 + x;
+        pm[y][x] = on ? ml[r] : make_float2(neg_inf(), 0.f);
+        v[y][x] = on ? *reinterpret_cast<const float4*>(box + (d * 32 + r) * 32 +
+                                                        ((quad ^ (r & 7)) << 2))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
     }
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if (pm[x].x == neg_inf()) continue;  // it saw no key (or the row is none)
-      const float mn = max2(m[x], pm[x].x);
-      const float f0 = ex2(m[x] - mn), f1 = ex2(pm[x].x - mn);
-      m[x] = mn;
-      l[x] = l[x] * f0 + pm[x].y * f1;
-      acc[x].x = acc[x].x * f0 + v[x].x * f1;
-      acc[x].y = acc[x].y * f0 + v[x].y * f1;
-      acc[x].z = acc[x].z * f0 + v[x].z * f1;
-      acc[x].w = acc[x].w * f0 + v[x].w * f1;
-    }
+    for (int y = 0; y < 4; ++y)
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        const float2 q = pm[y][x];
+        if (q.x == neg_inf()) continue;  // it saw no key (or the row is none)
+        const float mn = max2(m[x], q.x);
+        const float f0 = ex2(m[x] - mn), f1 = ex2(q.x - mn);
+        m[x] = mn;
+        l[x] = l[x] * f0 + q.y * f1;
+        acc[x].x = acc[x].x * f0 + v[y][x].x * f1;
+        acc[x].y = acc[x].y * f0 + v[y][x].y * f1;
+        acc[x].z = acc[x].z * f0 + v[y][x].z * f1;
+        acc[x].w = acc[x].w * f0 + v[y][x].w * f1;
+      }
   }
   const int col = d * 32 + quad * 4;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
+  for (int x = 0; x < R; ++x) {
     const int r = (group & 3) * 32 + r0 + x, rt = r / a.pack;
     const int tok = cut.tok0 + (group >> 2) * a.rt + rt;
     if (tok >= a.Lq || col >= a.D) continue;
@@ -1424,7 +1435,7 @@ static int run(const srdit_cross_attn_args& u, Args& a, const Plan& p, cudaStrea
     rc = u.D <= 64 ? launch_tile<T, 64>(u, a, p, stream) : launch_tile<T, 128>(u, a, p, stream);
   if (rc) return rc;
   if (p.ranged) {
-    const dim3 grid(static_cast<unsigned>(p.ctas - 1), SLOT_ROWS / 32);
+    const dim3 grid(static_cast<unsigned>(p.ctas - 1), SLOT_ROWS / JOIN_ROWS);
     if (u.D <= 64)
       SRDIT_LAUNCH((join_ranges_kernel<T, 64>), grid, 256, 0, stream, a);
     else
