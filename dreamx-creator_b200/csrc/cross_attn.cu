@@ -334,14 +334,19 @@ struct Cut {
 // a pair is four products of 128 x 128 x DP and 2 x 128 x 128 exponentials: at 128 columns
 // 2048 cycles of the tensor core (4096 multiply-adds a cycle) and as many of the unit that
 // takes exponentials (16 a cycle); both read 59% busy.
-// Measured: 24 heads of 128, 4096 queries on 8192 keys 326 us, 1.26 PFLOP/s; with the softmax
+// Measured: 24 heads of 128, 4096 queries on 8192 keys 324 us, 1.27 PFLOP/s; with the softmax
 // left out, the same loads and products take 294 (the clock falls under their power: cuBLAS
 // holds 1.39 PFLOP/s in such a loop). 6912 queries on 512 keys 51 us, 0.85 PFLOP/s: an item is
-// four key tiles there, between a load of q, the first scores and a store that nothing hides.
-// 3 x 777 queries on up to 1501 masked keys, 16 heads of 64 over 4: 34 us.
-// Slower: half of the exponentials as polynomials (no gain), the weights in two passes over
-// the scores (389 us), a warp that applies the mask, a ring of five K or V tiles, ranges
-// in place of whole rounds (365).
+// four key tiles there, and its end (the last product, 64 KB of output through the SM's port)
+// 3000 cycles beside their 3400 each; its five rounds are 88% full. 3 x 777 queries on up to
+// 1501 masked keys, 16 heads of 64 over 4: 32 us, a masked tile 4000 cycles.
+// Slower, or no faster: half of the exponentials as polynomials; two passes over the scores
+// (389 us); a warp that applies the mask; a ring of five K or V tiles; ranges in place of whole
+// rounds (365); the maximum's comparisons among the exponentials, or none at all, with the
+// sum as the test; the two warps of a scheduler taking turns at the exponentials; columns
+// of their own for the weights of 64-wide heads, so that scores never wait (336 for 286);
+// the mask as bounds from shared memory (77 for 70); rows stored by their threads, 32 bytes
+// at a time (53 for 51).
 template <typename T, int DP>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -579,28 +584,25 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       float m = neg_inf(), l = 0.f;
       const uint8_t* mrow = a.mask ? a.mask + it.b * a.mask_stride : nullptr;
       // the mask's bytes of this lane's four keys of a tile, read a tile ahead
-      uint32_t seen = 0xfu;
+      uint32_t seen[4];
       auto read_mask = [&](int key0) {
-        uint32_t r = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int key = key0 + w * 32 + lane;
-          r |= (key < it.len && __ldg(mrow + key) != 0 ? 1u : 0u) << w;
+          seen[w] = key < it.len ? (mrow ? __ldg(mrow + key) : 1u) : 0u;
         }
-        return r;
       };
       if (act) {
-        if (mrow) seen = read_mask(it.t0 * TILE);
+        if (mrow) read_mask(it.t0 * TILE);
         for (int j = 0; j < n_tiles; ++j) {
           const int key0 = (it.t0 + j) * TILE;
           const bool masked = a.mask != nullptr || key0 + TILE > it.len;
           uint32_t vis[4];
           if (masked) {
+            if (!mrow) read_mask(key0);
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              vis[w] = __ballot_sync(0xffffffffu,
-                                     key0 + w * 32 + lane < it.len && ((seen >> w) & 1u));
-            if (mrow && j + 1 < n_tiles) seen = read_mask(key0 + TILE);
+            for (int w = 0; w < 4; ++w) vis[w] = __ballot_sync(0xffffffffu, seen[w] != 0);
+            if (mrow && j + 1 < n_tiles) read_mask(key0 + TILE);
             // the values of unseen keys are zeroed: thread r of tile 0 has key r
             if (t == 0) {
               const int u = idx + 2 * j + 1;
@@ -669,26 +671,36 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
               tmem_st16(o_tmem + w * 16, o);
             }
           }
+          // (all exponents before the first exponential, and the first half published one
+          // group late, when its stores are done: 24 heads of 64, 4096 queries on 8192 keys 286
+          // us in place of 306; of 128 324 in place of 327)
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 x = f2_split(f2_fma(u64_of(s[w][e], s[w][e + 1]), c2, neg_m2));
+              s[w][e] = __float_as_uint(x.x);
+              s[w][e + 1] = __float_as_uint(x.y);
+            }
           uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             uint32_t pw[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const uint64_t x2 = f2_fma(u64_of(s[w][e], s[w][e + 1]), c2, neg_m2);
-              const float2 x = f2_split(x2);
-              const uint64_t p2 = f2_pack(ex2(x.x), ex2(x.y));
+              const uint64_t p2 =
+                  f2_pack(ex2(__uint_as_float(s[w][e])), ex2(__uint_as_float(s[w][e + 1])));
               sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], p2);
               const float2 p = f2_split(p2);
               pw[e >> 1] = pack2(p.x, p.y, T{});
             }
-            tmem_st16(s_tmem + w * 16, pw);
-            if (w == 1) {  // the first 64 keys' weights: their product can begin
+            if (w == 2) {  // the first 64 keys' weights, stored by now: their product can begin
               tmem_st_wait();
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&p_half[t]);
             }
+            tmem_st16(s_tmem + w * 16, pw);
           }
           const float2 sp = f2_split(f2_add(sum[0], sum[1]));
           l = l * alpha + (sp.x + sp.y);
@@ -800,8 +812,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 }
 
 // One block per JOIN_ROWS rows of the items that the CTAs' ranges cut: joins their parts, two
-// rows a warp and four parts' loads in flight. (With four rows a warp and one part at a time it
-// took MEASURED.)
+// rows a warp and four parts' loads in flight. Bounded by their latency: 512 queries on 8192
+// keys, 4 heads of 128 take 30.3 us with the join, 256 on 2048, 8 heads of 64 13.9. (Four rows a
+// warp, a part at a time: 38.0 and 17.2.)
 constexpr int JOIN_ROWS = 16;
 
 template <typename T, int DP>

@@ -265,6 +265,22 @@ def test_cross_attn_lengths_and_masks(srdit, cuda_device, dtype, Lq, H, Hkv, D, 
     assert ((y.float() - want.float()).abs() <= U[dtype] * want.float().abs()).all()
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 512, 4000, 4, 4, 128), (2, 300, 2100, 4, 1, 64),
+                                             (1, 130, 6000, 2, 2, 72), (7, 257, 900, 6, 3, 128)])
+def test_cross_attn_shared_items(srdit, cuda_device, dtype, B, Lq, Lk, H, Hkv, D):
+    """Few queries on many keys: query tiles whose keys are shared out over several CTAs and
+    joined, with and without a sample that has none."""
+    g = _gen(Lq + D)
+    q, k, v = _qkv(g, B, Lq, Lk, H, Hkv, D, dtype)
+    _check_attn(srdit, q, k, v)
+    lens = torch.tensor([Lk - 130 * b if b != 1 else 0 for b in range(B)], dtype=torch.int32,
+                        device="cuda")
+    mask = torch.rand(B, Lk, generator=g, device="cuda") < 0.5
+    mask[:, 128:384] = False   # whole key tiles without a seen key
+    _check_attn(srdit, q, k, v, lens, mask)
+
+
 @pytest.mark.parametrize("Lq", (1, 6, 200))
 def test_cross_attn_layouts(srdit, cuda_device, Lq):
     """Fused k|v buffers, heads before tokens, a shared prompt (batch stride 0), one key head
