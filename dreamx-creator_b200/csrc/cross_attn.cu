@@ -333,7 +333,11 @@ struct Cut {
 // query tile each, a row a thread, so a row's maximum and sum need no exchange. A key tile of
 // a pair is four products of 128 x 128 x DP and 2 x 128 x 128 exponentials: at 128 columns
 // 2048 cycles of the tensor core (4096 multiply-adds a cycle) and as many of the unit that
-// takes exponentials (16 a cycle); both read 59% busy.
+// takes exponentials (16 a cycle); both read 60% busy. What bounds it is the chain of one
+// query tile, 3200 cycles a key tile: its scores to registers and their maximum 500, the
+// weights 1500 (1160 of a warp that is alone and has no barriers), the second half of its
+// product and the next scores 770, and 300 for two barriers between the softmax and the
+// tensor core. The other query tile fills in for most of it, but is at the same point.
 // Measured: 24 heads of 128, 4096 queries on 8192 keys 324 us, 1.27 PFLOP/s; with the softmax
 // left out, the same loads and products take 294 (the clock falls under their power: cuBLAS
 // holds 1.39 PFLOP/s in such a loop). 6912 queries on 512 keys 51 us, 0.85 PFLOP/s: an item is
