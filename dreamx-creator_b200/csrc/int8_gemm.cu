@@ -7,8 +7,9 @@
 //
 // Two kernels, one for each thing that bounds the product:
 //
-//   pair_kernel    more than 64 tokens: bounded by the tensor cores, or by what an SM can
-//                  load for them. A CTA pair computes a 256 x BN tile with one
+//   pair_kernel    more than 64 tokens (32 where the weights are small): bounded by the
+//                  tensor cores, or by what an SM can load for them. A CTA pair computes a
+//                  256 x BN tile with one
 //                  tcgen05.mma.cta_group::2.kind::i8 per 32-deep step; two accumulators in
 //                  tensor memory let a tile's epilogue run under the next tile's products;
 //                  persistent. BN is chosen by the rounds of tiles it leaves (launch).
@@ -659,11 +660,16 @@ static int launch(const Operands& o, Params& p, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   // split_kernel and pair_kernel, K x N = 4096 x 4096: one token 9.0 and 16.0 us, 16 9.2 and
-  // 14.3, 48 10.5 and 10.6, 64 11.4 and 11.1, 72 11.4 and 11.1 (3072 x 14336: 64 14.2 and
-  // 15.7, 72 16.9 and 16.2; 16384 x 4096: 64 19.2 and 27.3)
+  // 14.3, 48 10.5 and 10.6, 64 11.4 and 11.1, 72 11.4 and 11.1.
+  // From 33 to 64 tokens what the clusters' exchange costs grows with the tokens, what a pair
+  // without a split of K loses with K, and large weights want split_kernel's deeper loads: 40
+  // tokens, 1024 x 1024 6.4 and 5.6, 1024 x 4096 8.2 and 7.6, 2048 x 2048 8.0 and 8.3; 64 tokens,
+  // 1024 x 1024 6.9 and 5.7, 2048 x 8192 10.3 and 9.6, 3072 x 3072 10.4 and 9.4, 4096 x 1024 8.8
+  // and 10.3, 3072 x 14336 14.2 and 15.7, 16384 x 4096 19.2 and 27.3.
   if (p.M <= 16) return launch_split<T, 16>(o, p, dev, stream);
   if (p.M <= 32) return launch_split<T, 32>(o, p, dev, stream);
-  if (p.M <= 64) return launch_split<T, 64>(o, p, dev, stream);
+  if (p.M <= 64 && (p.K > 48 * p.M || static_cast<long long>(p.K) * p.N > 24ll << 20))
+    return launch_split<T, 64>(o, p, dev, stream);
   // The tile width with the least time: rounds of tiles over the pairs, times the cycles of
   // a block of K, which are the products' (two per column) or the loads' (60 bytes a cycle
   // and SM), whichever is more.

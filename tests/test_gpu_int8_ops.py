@@ -158,6 +158,15 @@ def test_int8_gemm(srdit, cuda_device, dtype, M, N, K, bias):
     _check_gemm(srdit, _codes(srdit, g, M, K), _codes(srdit, g, N, K), dtype, bias, g)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(33, 200, 1584), (33, 200, 1600), (48, 70, 2500), (61, 513, 3000),
+                                   (64, 130, 4001), (64, 16400, 1540)])
+def test_int8_gemm_of_33_to_64_rows(srdit, cuda_device, dtype, M, N, K):
+    """Either side of where such products change kernels."""
+    g = _gen(M + N + K)
+    _check_gemm(srdit, _codes(srdit, g, M, K), _codes(srdit, g, N, K), dtype, True, g)
+
+
 @pytest.mark.parametrize("M", (1, 5, 40, 300))
 def test_int8_gemm_extremes(srdit, cuda_device, M):
     """-128 times -128 over the longest K: the int32 sum at its largest (2^31 - 2^14)."""
