@@ -924,15 +924,16 @@ SRDIT_DEV uint4 lds16(uint32_t src) {
   return v;
 }
 
-// PER_SM: CTAs that share an SM's shared memory, which leaves a warp's ring 6, 3 or 2 blocks
-// of 128-wide heads, twice that of 64-wide ones. A warp alone on its scheduler takes 1300
-// cycles for a block's 230 instructions, nearly all of it their latency, so a full grid has
-// three CTAs an SM (168 registers) and is bounded by memory; a small grid is bounded by
-// that latency and wants its next blocks there already.
+// A warp alone on its scheduler takes 1300 cycles for a block's 230 instructions, nearly all of
+// it their latency, so an SM gets three CTAs (168 registers; two of 16 rows), and a warp's
+// ring 2 or 3 blocks of 128-wide heads, twice that of 64-wide ones. (Two CTAs with 3 blocks: 4
+// x 32768 keys, 32 heads over 8, 87.6 us in place of 81.1, 8 x 512 keys, 24 heads 17.6 in place
+// of 12.7; one with 6: 136 and 22; of small grids none is better.)
 constexpr int TOKEN_WARPS = 4;
 
-template <int DP, int NT, int PER_SM>
+template <int DP, int NT>
 struct TokenCfg {
+  static constexpr int PER_SM = NT == 1 ? 3 : 2;
   static constexpr int NC = DP / 32;  // 32-dim pieces of q and k
   static constexpr int NV = DP / 64;  // 64-column pieces of v
   static constexpr int SLAB = 16 * 128;         // 16 rows x 64 values, 128-byte swizzle
@@ -953,14 +954,14 @@ struct TokenCfg {
 // copy per row to one row in 8 to 20 cycles.)
 // The scores are S^T = K Q^T, 16 keys by 8 rows an instruction, so a row's weights are the
 // operand of O^T = V^T P^T as they stand; v is turned in registers, 8 x 8 at a time.
-// Measured: 4 x 32768 keys, 32 heads over 8, one token 86 us, 6.25 TB/s (a sum over as many
+// Measured: 4 x 32768 keys, 32 heads over 8, one token 81 us, 6.63 TB/s (a sum over as many
 // bytes reads 5.65); 8 x up to 512 keys, 24 heads 8.2 us: start, one block's latency, join.
-template <typename T, int DP, int NT, int PER_SM>
-__global__ void __launch_bounds__(TOKEN_WARPS * 32, PER_SM)
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(TOKEN_WARPS * 32, TokenCfg<DP, NT>::PER_SM)
     token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ Args a, int cluster) {
   pdl_begin();
-  using C = TokenCfg<DP, NT, PER_SM>;
+  using C = TokenCfg<DP, NT>;
   constexpr int NC = C::NC, NV = C::NV, STAGES = C::STAGES, R = 8 * NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
@@ -1288,7 +1289,6 @@ __global__ void __launch_bounds__(128)
 struct Plan {
   bool token;
   int pack, rt, nq, nhp;
-  int per_sm;                  // token_kernel: CTAs that share an SM
   int splits, cluster, parts;  // token_kernel; parts in the workspace per row (1: none)
   bool ranged;
   int ctas;                    // tile_kernel
@@ -1301,16 +1301,16 @@ struct Plan {
 static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   Plan p = {};
   const int group = a.H / a.Hkv;
-  // 16 rows, token_kernel and tile_kernel: 8 x 512 keys, 24 heads 16.0 and 20.9 us (one row
-  // 12.3); 4 x 32768 keys, 8 heads 93.6 and 107.8 (four rows 87.4)
+  // 16 rows, token_kernel and tile_kernel: 8 x 512 keys, 24 heads 16.3 and 20.9 us (one row
+  // 12.7); 4 x 32768 keys, 8 heads 93.2 and 107.8 (four rows 81.0)
   p.token = static_cast<long long>(a.Lq) * group <= 16;
   p.splits = p.cluster = p.parts = 1;
   if (p.token) {
     const int pairs = a.B * a.Hkv;
-    const int most_per_sm = a.Lq * group <= 8 ? 3 : 2;
+    const int per_sm = a.Lq * group <= 8 ? TokenCfg<128, 1>::PER_SM : TokenCfg<128, 2>::PER_SM;
     const int blocks = (a.Lk + 15) / 16;
     // CTAs that run at once, each with a block per warp at least
-    int want = sms * most_per_sm / pairs;
+    int want = sms * per_sm / pairs;
     const int most = (blocks + TOKEN_WARPS - 1) / TOKEN_WARPS;
     if (want > most) want = most;
     while (p.cluster < 8 && 2 * p.cluster <= want) p.cluster *= 2;
@@ -1323,9 +1323,6 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
       if (p.parts < 1) p.parts = 1;
       p.splits = 8 * p.parts;
     }
-    // (CTAs of one SM's whole shared memory and in clusters need room to be placed)
-    const int grid = pairs * p.splits;
-    p.per_sm = grid <= sms / 2 ? 1 : grid <= 2 * sms ? 2 : 3;
     return p;
   }
   // heads of a group side by side in a query tile, a power of two of them
@@ -1415,32 +1412,26 @@ static int launch_tile(const srdit_cross_attn_args& u, Args& a, const Plan& p,
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T, int DP, int NT, int PER_SM>
+template <typename T, int DP, int NT>
 static int launch_token(const srdit_cross_attn_args& u, const Args& a, const Plan& p,
                         cudaStream_t stream) {
-  using C = TokenCfg<DP, NT, PER_SM>;
+  using C = TokenCfg<DP, NT>;
   static std::atomic<bool> attr_done[kMaxDevices] = {};
-  int rc = set_smem(token_kernel<T, DP, NT, PER_SM>, C::SMEM, attr_done);
+  int rc = set_smem(token_kernel<T, DP, NT>, C::SMEM, attr_done);
   if (rc) return rc;
   CUtensorMap tk, tv;
   rc = kv_maps(&tk, &tv, u, 16);
   if (rc) return rc;
   const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.B * a.Hkv));
-  return launch_clusters(p.cluster, token_kernel<T, DP, NT, PER_SM>, grid, TOKEN_WARPS * 32,
+  return launch_clusters(p.cluster, token_kernel<T, DP, NT>, grid, TOKEN_WARPS * 32,
                          C::SMEM, stream, tk, tv, a, p.cluster);
 }
 
 template <typename T, int DP>
 static int launch_token_n(const srdit_cross_attn_args& u, const Args& a, const Plan& p,
                           cudaStream_t stream) {
-  if (a.Lq * a.group <= 8)
-    switch (p.per_sm) {
-      case 1: return launch_token<T, DP, 1, 1>(u, a, p, stream);
-      case 2: return launch_token<T, DP, 1, 2>(u, a, p, stream);
-      default: return launch_token<T, DP, 1, 3>(u, a, p, stream);
-    }
-  return p.per_sm == 1 ? launch_token<T, DP, 2, 1>(u, a, p, stream)
-                       : launch_token<T, DP, 2, 2>(u, a, p, stream);
+  return a.Lq * a.group <= 8 ? launch_token<T, DP, 1>(u, a, p, stream)
+                             : launch_token<T, DP, 2>(u, a, p, stream);
 }
 
 template <typename T>
