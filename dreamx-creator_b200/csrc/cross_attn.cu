@@ -1309,17 +1309,24 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
     const int pairs = a.B * a.Hkv;
     const int per_sm = a.Lq * group <= 8 ? TokenCfg<128, 1>::PER_SM : TokenCfg<128, 2>::PER_SM;
     const int blocks = (a.Lk + 15) / 16;
-    // CTAs that run at once, each with a block per warp at least
-    int want = sms * per_sm / pairs;
+    // The keys are split until every SM has a CTA, each with a block per warp at least (until
+    // they have three: 8 x 512 keys, 24 heads 12.5 us in place of 11.7, 8 x 2048 34.4 and 32.7,
+    // 8 x 8192 122 and 117; until half of them have one: 4 x 32768, 8 heads 88 and 81), or with
+    // samples of different lengths three (8 x up to 2048 22.4 us in place of 27.2, 8 x up to 4096
+    // 39.5 and 49.8; six: 26.2 and 42.9).
     const int most = (blocks + TOKEN_WARPS - 1) / TOKEN_WARPS;
-    if (want > most) want = most;
-    while (p.cluster < 8 && 2 * p.cluster <= want) p.cluster *= 2;
+    while (p.cluster < 8 && 2 * p.cluster <= most &&
+           (pairs * p.cluster < sms || (a.kv_lens && 2 * pairs * p.cluster <= per_sm * sms)))
+      p.cluster *= 2;
     p.splits = p.cluster;
-    // more than a cluster's 8 parts cost a second launch: from 8 blocks a warp, and no more
-    // parts than leave it 4
+    // More than a cluster's 8 parts cost a second launch: from 8 blocks a warp, no more parts
+    // than leave it 4, and 1.6 CTAs an SM. (8 heads, 16384 keys: 6 parts 18.8 us, 4 17.4; 3 x
+    // 4096, whose clusters have a CTA for each SM: 2 parts 15.6, none 13.1; 1 x 8192: none 15.3,
+    // 4 12.9; 2 x 32768: none 52.8, 2 45.2.)
     const int warps = 8 * TOKEN_WARPS;
     if (p.cluster == 8 && blocks >= 8 * warps) {
-      p.parts = want / 8 < blocks / (4 * warps) ? want / 8 : blocks / (4 * warps);
+      p.parts = (sms + 5 * pairs / 2) / (5 * pairs);
+      if (p.parts > blocks / (4 * warps)) p.parts = blocks / (4 * warps);
       if (p.parts < 1) p.parts = 1;
       p.splits = 8 * p.parts;
     }

@@ -598,7 +598,7 @@ int srdit_int8_gemm(const void* a, const float* a_scale, const void* w, const fl
  * {batch, token, head} in elements (multiples of 8; a batch stride of 0 repeats one sample, a
  * head stride of 0 of k or v one head) and unit stride over D;
  * bases 16-byte aligned. D a multiple of 8, at most 128. scale > 0. workspace: where
- * srdit_cross_attn_workspace (which reads the sizes and the type only) returns n > 0, partial
+ * srdit_cross_attn_workspace (which reads the arguments, not the tensors) returns n > 0, partial
  * results of rows split over their keys are joined through it: n KiB, 16-byte aligned. B * Lq * H
  * at most 2^26, B * Hkv at most 65535.
  * Replaces: flash_attention with k_lens (video_refiner/wan/modules/sr_dit/attention.py:61-168, called
