@@ -601,8 +601,8 @@ int srdit_int8_gemm(const void* a, const float* a_scale, const void* w, const fl
  * srdit_cross_attn_workspace (which reads the arguments, not the tensors) returns n > 0, partial
  * results of rows split over their keys are joined through it: n KiB, 16-byte aligned. B * Lq * H
  * at most 2^26, B * Hkv at most 65535.
- * Replaces: flash_attention with k_lens (video_refiner/wan/modules/sr_dit/attention.py:61-168, called
- *   at wan/modules/sr_dit/models.py:1057).
+ * Replaces: flash_attention with k_lens (video_refiner/wan/modules/sr_dit/attention.py:61-168,
+ *   called at wan/modules/sr_dit/models.py:1057).
  */
 typedef struct srdit_cross_attn_args {
   const void* q;
