@@ -17,8 +17,8 @@ from __future__ import annotations
 import sys
 
 from . import _lib, blockgrid, ops  # noqa: F401
-from . import attention, fp8_linear, int8_linear  # noqa: F401
+from . import attention, fp8_linear, int8_linear, text_block  # noqa: F401
 
 sys.modules.setdefault("dreamx_creator_b200", sys.modules[__name__])
 
-__all__ = ["attention", "blockgrid", "fp8_linear", "int8_linear", "ops"]
+__all__ = ["attention", "blockgrid", "fp8_linear", "int8_linear", "ops", "text_block"]
