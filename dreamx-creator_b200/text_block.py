@@ -3,7 +3,8 @@
 A stack of pre-norm blocks refines video tokens by attending to a prompt's encoder states,
 every Linear an ``Int8Linear``. Per block:
 
-  add_rms_quant(x, y)    x + y -> x,  RMS norm, int8 rows      (y: the block before's output)
+  add_rms_quant(x, y)    x + y, RMS norm, int8 rows   (y: the block before's output; in a
+                         stack the sum takes its place)
   int8_gemm              q = W_q n
   cross_attn             q over the prompt's k | v, each sample its own length
   quant_rows, int8_gemm  y = W_o a
@@ -41,14 +42,15 @@ class CrossBlock(nn.Module):
         self.register_buffer("norm", norm_weight.detach().clone(), persistent=False)
         self.q, self.kv, self.o = q, kv, o
 
-    def forward(self, x, y, kv, kv_lens=None, key_mask=None):
+    def forward(self, x, y, kv, kv_lens=None, key_mask=None, *, into_y=False):
         """x [B, L, dim] the residual stream, y [B, L, dim] what is still to be added to it
-        (or None), kv [B, Lk, 2, kv_heads, head_dim]. Returns (x + y, this block's output)."""
+        (or None), kv [B, Lk, 2, kv_heads, head_dim]. Returns (x + y, this block's output);
+        with ``into_y`` the sum takes the place of a contiguous y, else y is left as it is."""
         B, L, D = x.shape
         rows = x.reshape(B * L, D)
         add = None if y is None else y.reshape(B * L, D)
         n, scale, total = ops.add_rms_quant(rows, self.norm, self.eps, residual=add,
-                                            sum_out=None if add is None else add)
+                                            sum_out=add if into_y else None)
         q = self.q.forward_codes(n, scale, x.dtype).view(B, L, self.heads, self.head_dim)
         a = ops.cross_attn(q, kv[:, :, 0], kv[:, :, 1], kv_lens=kv_lens, key_mask=key_mask)
         out = self.o.forward_codes(*ops.quant_rows(a.view(B * L, -1)), x.dtype)
@@ -94,5 +96,5 @@ class CrossStack(nn.Module):
         A row whose prompt has no visible key only gets the output Linears' biases."""
         y = None
         for block, bkv in zip(self.blocks, kv):
-            x, y = block(x, y, bkv, kv_lens, key_mask)
+            x, y = block(x, y, bkv, kv_lens, key_mask, into_y=True)  # y is ours
         return x + y
