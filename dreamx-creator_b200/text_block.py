@@ -53,7 +53,7 @@ class CrossBlock(nn.Module):
                                             sum_out=add if into_y else None)
         q = self.q.forward_codes(n, scale, x.dtype).view(B, L, self.heads, self.head_dim)
         a = ops.cross_attn(q, kv[:, :, 0], kv[:, :, 1], kv_lens=kv_lens, key_mask=key_mask)
-        out = self.o.forward_codes(*ops.quant_rows(a.view(B * L, -1)), x.dtype)
+        out = self.o.forward_codes(*ops.quant_rows(a.view(B * L, self.o.in_features)), x.dtype)
         return (x if total is None else total.view(B, L, D)), out.view(B, L, D)
 
 
@@ -86,8 +86,8 @@ class CrossStack(nn.Module):
     def text_kv(self, states):
         """Every block's k | v [B, Lk, 2, kv_heads, head_dim] of the encoder's states
         [B, Lk, text_dim], once per prompt."""
-        B, Lk, _ = states.shape
-        q, scale = ops.quant_rows(states.reshape(B * Lk, -1))
+        B, Lk, D = states.shape
+        q, scale = ops.quant_rows(states.reshape(B * Lk, D))
         return [b.kv.forward_codes(q, scale, states.dtype).view(B, Lk, 2, b.kv_heads, b.head_dim)
                 for b in self.blocks]
 

@@ -1,0 +1,40 @@
+"""Text-conditioning blocks on the GPU where their inputs are empty, broadcast or views."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def stack(srdit, cuda_device):
+    return srdit.text_block.CrossStack.random_init(dim=128, text_dim=96, heads=2, layers=3, seed=3)
+
+
+def _inputs(B, L, Lk):
+    g = torch.Generator(device="cuda").manual_seed(L + Lk)
+    return tuple(torch.randn(B, n, d, generator=g, device="cuda").to(torch.bfloat16)
+                 for n, d in ((L, 128), (Lk, 96)))
+
+
+@pytest.mark.parametrize("L,Lk", [(1, 0), (300, 0), (0, 7), (0, 0)])
+def test_no_keys_or_no_tokens(stack, L, Lk):
+    """A prompt without states adds the output Linears' biases; no tokens, no output."""
+    x, states = _inputs(2, L, Lk)
+    out = stack(x, stack.text_kv(states))
+    assert out.shape == x.shape and out.dtype == x.dtype
+    want = x
+    for b in stack.blocks:   # an output is the bias alone, each sum rounded to bf16
+        want = want + b.o.bias
+    assert torch.equal(out, want if L else x)
+
+
+@pytest.mark.parametrize("L", (1, 70))
+def test_a_block_leaves_its_arguments(stack, L):
+    x, states = _inputs(2, L, 7)
+    y = x.flip(1).contiguous() * 0.5
+    x0, y0 = x.clone(), y.clone()
+    kv = stack.text_kv(states)
+    total, out = stack.blocks[0](x, y, kv[0])
+    assert torch.equal(x, x0) and torch.equal(y, y0) and torch.equal(total, x0 + y0)
+    over, again = stack.blocks[0](x, y, kv[0], into_y=True)
+    assert over.data_ptr() == y.data_ptr() and torch.equal(over, total) and torch.equal(out, again)

@@ -85,3 +85,13 @@ def test_a_stack_adds_every_output(stack):
     for block, bkv in zip(stack.blocks, kv):
         total, y = block(total, y, bkv)
     assert torch.equal(out, total + y)
+
+
+@pytest.mark.parametrize("L,Lk", [(5, 0), (0, 7), (0, 0)])
+def test_no_keys_or_no_tokens(stack, L, Lk):
+    """A prompt without states adds the output Linears' biases; no tokens, no output."""
+    x, _, states = _inputs(L, Lk)
+    out = stack(x, stack.text_kv(states))
+    assert out.shape == x.shape
+    want = x + sum(b.o.bias for b in stack.blocks) if Lk == 0 else x
+    assert torch.allclose(out, want, atol=1e-5)
