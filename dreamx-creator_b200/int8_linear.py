@@ -53,8 +53,7 @@ class Int8Linear(Fp8Linear):
         if x.shape[-1] != self.in_features:
             raise ValueError(f"Int8Linear expects {self.in_features} input features, "
                              f"got {x.shape[-1]}")
-        rows = x.reshape(-1, self.in_features)
-        q, scale = ops.quant_rows(rows if rows.stride(-1) == 1 else rows.contiguous())
+        q, scale = ops.quant_rows(ops.as_rows(x, self.in_features))
         return self.forward_codes(q, scale, x.dtype).view(*x.shape[:-1], self.out_features)
 
     def forward_codes(self, q, scale, dtype=torch.bfloat16, out=None):

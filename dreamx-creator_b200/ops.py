@@ -62,12 +62,23 @@ def _need_cuda(*ts):
 
 
 def _rows(t: torch.Tensor):
-    """(row stride in elements) of a 2-D row-major view with unit inner stride."""
+    """(row stride in elements) of a 2-D row-major view with unit inner stride; of a single
+    row, whose stride may be anything, its width at least."""
     st = t.stride()
     if len(st) != 2 or st[1] != 1:
         raise _lib.SrditError(f"expected a 2-D row-major tensor, got shape {tuple(t.shape)} "
                               f"strides {st}")
-    return st[0]
+    return st[0] if t.shape[0] > 1 else max(st[0], t.shape[1])
+
+
+def as_rows(x, K):
+    """x [..., K] as rows [M, K] that the row kernels take (unit inner stride, no row over
+    another): a view where x is laid out so, else (expanded or transposed inputs) a copy."""
+    rows = x.reshape(-1, K)
+    st = rows.stride()
+    if st[1] != 1 or (st[0] < K and rows.shape[0] > 1):
+        rows = rows.clone(memory_format=torch.contiguous_format)
+    return rows
 
 
 def fp8_gemm(a_fp8, a_scale, w_fp8, w_scale, bias=None, out=None, *, epilogue="store",

@@ -47,8 +47,8 @@ class CrossBlock(nn.Module):
         (or None), kv [B, Lk, 2, kv_heads, head_dim]. Returns (x + y, this block's output);
         with ``into_y`` the sum takes the place of a contiguous y, else y is left as it is."""
         B, L, D = x.shape
-        rows = x.reshape(B * L, D)
-        add = None if y is None else y.reshape(B * L, D)
+        rows = ops.as_rows(x, D)
+        add = None if y is None else ops.as_rows(y, D)
         n, scale, total = ops.add_rms_quant(rows, self.norm, self.eps, residual=add,
                                             sum_out=add if into_y else None)
         q = self.q.forward_codes(n, scale, x.dtype).view(B, L, self.heads, self.head_dim)
@@ -87,7 +87,7 @@ class CrossStack(nn.Module):
         """Every block's k | v [B, Lk, 2, kv_heads, head_dim] of the encoder's states
         [B, Lk, text_dim], once per prompt."""
         B, Lk, D = states.shape
-        q, scale = ops.quant_rows(states.reshape(B * Lk, D))
+        q, scale = ops.quant_rows(ops.as_rows(states, D))
         return [b.kv.forward_codes(q, scale, states.dtype).view(B, Lk, 2, b.kv_heads, b.head_dim)
                 for b in self.blocks]
 

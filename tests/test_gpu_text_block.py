@@ -38,3 +38,27 @@ def test_a_block_leaves_its_arguments(stack, L):
     assert torch.equal(x, x0) and torch.equal(y, y0) and torch.equal(total, x0 + y0)
     over, again = stack.blocks[0](x, y, kv[0], into_y=True)
     assert over.data_ptr() == y.data_ptr() and torch.equal(over, total) and torch.equal(out, again)
+
+
+def test_broadcast_inputs_and_single_rows(stack, srdit):
+    """Rows expanded over tokens or samples, and single rows of any stride, as their copies."""
+    x, states = _inputs(2, 5, 7)
+    xe, se = x[:1, :1].expand(2, 5, 128), states[:1].expand(2, 7, 96)
+    out = stack(xe, stack.text_kv(se))
+    assert torch.equal(out, stack(xe.clone(), stack.text_kv(se.clone())))
+    kv = stack.text_kv(states)
+    for a, b in zip(stack.blocks[0](xe, x[:, 1:2].expand(2, 5, 128), kv[0]),
+                    stack.blocks[0](xe.clone(), x[:, 1:2].expand(2, 5, 128).clone(), kv[0])):
+        assert torch.equal(a, b)
+    lin = stack.blocks[0].kv
+    row = states[0, :1]
+    want = lin(row)
+    assert torch.equal(lin(row.expand(4, 96)), want.expand(4, -1))
+    column = row.t().contiguous().t()   # [1, 96], both strides 1
+    assert column.stride() == (1, 1) and torch.equal(lin(column), want)
+    one = x[0, :1]
+    column = one.t().contiguous().t()
+    w = torch.ones(128, device="cuda", dtype=torch.bfloat16)
+    for got, ref in zip(srdit.ops.add_rms_quant(column, w, residual=column),
+                        srdit.ops.add_rms_quant(one, w, residual=one)):
+        assert torch.equal(got, ref)

@@ -95,3 +95,47 @@ def test_no_keys_or_no_tokens(stack, L, Lk):
     assert out.shape == x.shape
     want = x + sum(b.o.bias for b in stack.blocks) if Lk == 0 else x
     assert torch.allclose(out, want, atol=1e-5)
+
+
+# ------------------------------------------------------------------ rows of other layouts
+def test_the_pitch_of_one_row_is_its_width_at_least(srdit):
+    """A single row may have any stride over rows: nothing is read by it."""
+    for t, want in ((torch.zeros(8, 1).t(), 8), (torch.zeros(1, 8).expand(1, 8), 8),
+                    (torch.zeros(1, 16)[:, :8], 16), (torch.zeros(3, 16)[:, :8], 16),
+                    (torch.zeros(0, 8), 8)):
+        assert srdit.ops._rows(t) == want
+    with pytest.raises(srdit._lib.SrditError):
+        srdit.ops._rows(torch.zeros(8, 3).t())
+
+
+@pytest.mark.parametrize("x", [
+    torch.randn(1, 48).expand(4, 48), torch.randn(2, 1, 48).expand(2, 3, 48),
+    torch.randn(1, 3, 48).expand(2, 3, 48), torch.randn(48, 3).t(), torch.randn(48, 1).t(),
+    torch.randn(4, 6, 48)[:, 1], torch.randn(100).as_strided((4, 48), (5, 1)),
+    torch.randn(0, 48), torch.randn(48)])
+def test_the_linear_takes_rows_of_any_layout(srdit, stack, monkeypatch, x):
+    """Expanded, transposed and overlapping rows reach the quantiser as rows a pitch of their
+    width apart at least."""
+    seen = []
+    plain = srdit.ops.quant_rows
+    monkeypatch.setattr(srdit.ops, "quant_rows", lambda r, **kw: (seen.append(r), plain(r))[1])
+    lin = stack.blocks[0].kv
+    y = lin(x)
+    assert y.shape == (*x.shape[:-1], lin.out_features)
+    assert srdit.ops._rows(seen[0]) >= 48 and torch.equal(seen[0], x.reshape(-1, 48))
+    assert torch.equal(y, lin(x.clone(memory_format=torch.contiguous_format)))
+
+
+def test_a_stack_takes_broadcast_inputs(stack, srdit, monkeypatch):
+    x, _, states = _inputs()
+    pitches = []
+    for name in ("add_rms_quant", "quant_rows"):
+        fn = getattr(srdit.ops, name)
+        monkeypatch.setattr(srdit.ops, name, lambda r, *a, fn=fn, **kw: (
+            pitches.append((srdit.ops._rows(r), r.shape[1])), fn(r, *a, **kw))[1])
+    xe, se = x[:1, :1].expand(2, 5, 64), states[:1].expand(2, 7, 48)
+    out = stack(xe, stack.text_kv(se))
+    assert torch.equal(out, stack(xe.clone(), stack.text_kv(se.clone())))
+    ye = x[:1, 1:2].expand(2, 5, 64)
+    stack.blocks[0](xe, ye, stack.text_kv(se)[0])
+    assert all(p >= k for p, k in pitches)
