@@ -54,10 +54,10 @@ def test_broadcast_inputs_and_single_rows(stack, srdit):
     row = states[0, :1]
     want = lin(row)
     assert torch.equal(lin(row.expand(4, 96)), want.expand(4, -1))
-    column = row.t().contiguous().t()   # [1, 96], both strides 1
+    column = row.as_strided((1, 96), (1, 1))   # a transposed column
     assert column.stride() == (1, 1) and torch.equal(lin(column), want)
     one = x[0, :1]
-    column = one.t().contiguous().t()
+    column = one.as_strided((1, 128), (1, 1))
     w = torch.ones(128, device="cuda", dtype=torch.bfloat16)
     for got, ref in zip(srdit.ops.add_rms_quant(column, w, residual=column),
                         srdit.ops.add_rms_quant(one, w, residual=one)):
