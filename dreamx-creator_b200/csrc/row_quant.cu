@@ -13,7 +13,8 @@
 // computed here is rounded twice.
 //
 // A row with a NaN, or an infinity, has the scale NaN (max.NaN keeps it), so what
-// its codes stand for is NaN; int8 codes of it are 0.
+// its codes stand for is NaN; int8 codes of it are 0. A finite row whose sum of squares is
+// not finite (values from 2^56 on) is no such row: far_rstd.
 #include "sm100.cuh"
 #include "srdit_internal.h"
 
@@ -146,11 +147,36 @@ SRDIT_DEV void accumulate(float (&s)[V], const float (&w)[V], uint64_t& ss2, flo
   }
 }
 
+// 1 / sqrt(mean(s^2) + eps) of a finite row x [+ r] whose sum of squares is beyond fp32 (values
+// from 2^56 on): of the values times 2^-72, whose squares' sum is not, read once more by each
+// of the row's warps.
+template <typename T>
+SRDIT_DEV float far_rstd(const T* x, const T* r, int K, float inv_k, float eps) {
+  constexpr float down = 0x1p-72f;
+  float ss = 0.f;
+  __syncwarp();
+#pragma unroll 1
+  for (int c = threadIdx.x & 31; c < K; c += 32) {
+    const float v = (to_f<T>(x[c]) + (r ? to_f<T>(r[c]) : 0.f)) * down;
+    ss = fmaf(v, v, ss);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  return rsqrtf(fmaf(ss, inv_k, eps * down * down)) * down;
+}
+
+// (a call where the code inlined would cost a row of narrow vectors 6 registers)
+template <typename T>
+__device__ __noinline__ float far_rstd_call(const T* x, const T* r, int K, float inv_k, float eps) {
+  return far_rstd<T>(x, r, K, inv_k, eps);
+}
+
 // The row's sums over its `warps` warps, the first of them `warp0` of the block, in the same
-// order in every thread; then its scale and the factor from values to codes.
-template <bool kInt8, bool kNorm>
+// order in every thread; then its scale and the factor from values to codes. far(): the norm's
+// factor where the sum is beyond fp32.
+template <typename T, bool kInt8, bool kNorm, typename F>
 SRDIT_DEV void row_scale(const Args& a, uint64_t ss2, float mx, int warps, int warp0, float2* part,
-                         float& scale, float& inv) {
+                         float& scale, float& inv, F far) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float2 sp = f2_split(ss2);
   float ss = sp.x + sp.y;
@@ -173,7 +199,11 @@ SRDIT_DEV void row_scale(const Args& a, uint64_t ss2, float mx, int warps, int w
     }
   }
   // Approximate root and quotient, 2 units in the last place: every thread computes these.
-  const float rstd = kNorm ? rsqrtf(fmaf(ss, a.inv_k, a.eps)) : 1.0f;
+  float rstd = kNorm ? rsqrtf(fmaf(ss, a.inv_k, a.eps)) : 1.0f;
+  if constexpr (kNorm && !__is_same(T, __half)) {  // (fp16 has no such rows)
+    constexpr float inf = __builtin_huge_valf();
+    if (ss == inf && mx < inf) rstd = far();
+  }
   scale = max_nan(mx * rstd * (kInt8 ? 1.f / 127.f : 1.f / 448.f), 1e-12f);
   inv = __fdividef(rstd, scale);
 }
@@ -181,11 +211,11 @@ SRDIT_DEV void row_scale(const Args& a, uint64_t ss2, float mx, int warps, int w
 // Rows of up to 8192: one row per `warps` warps of the block, 8 values of it in a thread's
 // registers as vectors of V (V = 8: 16-byte loads of 16-bit values; 2 and 1 for rows whose
 // width, pitch or base is not so aligned), vector i of thread t at (i * threads + t) * V.
-// Bounded by memory: 6912 x 3072 bf16 with the residual takes 27.3 us, 5.45 TB/s, what a
+// Bounded by memory: 6912 x 3072 bf16 with the residual takes 27.5 us, 5.41 TB/s, what a
 // copy of as many bytes reaches. (With scalar arithmetic, an exact root and quotients in every
 // thread it took 34 instructions a value, 70% of the issue slots, and 30.9 us. With 16, 24
 // and 32 values in a thread this one takes 29.3, 29.5 and 31.2 us, and a single row of 4096
-// 2.9, 3.3 and 3.8 us in place of 2.5.)
+// 2.9, 3.3 and 3.8 us in place of 2.5. Without far_rstd: 27.3.)
 template <typename T, bool kInt8, bool kNorm, bool kRes, int V>
 __global__ void __launch_bounds__(1024) rows_kernel(const Args a) {
   pdl_begin();
@@ -227,7 +257,13 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Args a) {
     }
   }
   float scale, inv;
-  row_scale<kInt8, kNorm>(a, ss2, mx, a.warps, sub * a.warps, part, scale, inv);
+  row_scale<T, kInt8, kNorm>(a, ss2, mx, a.warps, sub * a.warps, part, scale, inv, [&] {
+    // (of the sum as it was stored, rounded: it may have taken the place of x or of r)
+    const T* far = kRes ? static_cast<const T*>(a.sum) + row * a.lds
+                        : static_cast<const T*>(a.x) + row * a.ldx;
+    return V == 8 ? far_rstd<T>(far, nullptr, a.K, a.inv_k, a.eps)
+                  : far_rstd_call<T>(far, nullptr, a.K, a.inv_k, a.eps);
+  });
   if (!on) return;
   const bool zero = !(scale < __int_as_float(0x7f800000));
   if (t == 0) a.scale[row] = scale;
@@ -241,8 +277,10 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Args a) {
 
 // Wider rows: one block of 512 threads a row, which it reads twice, the second time out of
 // the caches. The sum is stored in the second pass, since it may be x or the residual.
+// Four blocks an SM: 6912 x 14336 bf16 67 us, with the residual 115, 5.2 TB/s (with what the
+// compiler takes by itself, 32 to 44 registers: 66, and 122 to 138).
 template <typename T, bool kInt8, bool kNorm, bool kRes, int V>
-__global__ void __launch_bounds__(512) wide_rows_kernel(const Args a) {
+__global__ void __launch_bounds__(512, 4) wide_rows_kernel(const Args a) {
   pdl_begin();
   __shared__ float2 part[16];
   const long long row = blockIdx.x;
@@ -268,7 +306,11 @@ __global__ void __launch_bounds__(512) wide_rows_kernel(const Args a) {
     accumulate<kNorm, V>(s, ww, ss2, mx);
   }
   float scale, inv;
-  row_scale<kInt8, kNorm>(a, ss2, mx, 16, 0, part, scale, inv);
+  row_scale<T, kInt8, kNorm>(a, ss2, mx, 16, 0, part, scale, inv, [&] {
+    const float rstd = far_rstd<T>(x, r, a.K, a.inv_k, a.eps);
+    __syncthreads();  // every warp has read the row: the sum may take the place of x or of r
+    return rstd;
+  });
   const bool zero = !(scale < __int_as_float(0x7f800000));
   if (threadIdx.x == 0) a.scale[row] = scale;
   uint8_t* q = a.q + row * a.ldq;

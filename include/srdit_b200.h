@@ -556,7 +556,9 @@ int srdit_winattn_fwd(const void* q, const void* k_hr, const void* v_hr, const v
  * bytes; row pitches ld* in elements, any alignment of the element type (rows of 16-byte
  * aligned base, pitch and width are the fast ones). K at most 32768. residual and
  * sum are given together or both NULL (then s = x); sum may be x or residual itself.
- * A row holding a NaN or an infinity gets the scale NaN.
+ * A row holding a NaN or an infinity gets the scale NaN; one with an s * weight beyond fp32
+ * infinity or NaN. Finite rows get finite scales even where their squares' sum is beyond fp32
+ * (16-bit ones with a residual by the rounded sum).
  * Replaces: WanRMSNorm.forward (video_refiner/wan/modules/sr_dit/models.py:424-440) after a
  *   residual addition (models.py:1257) and before Fp8Linear's row-wise quantiser
  *   (fp8_linear.py:93-103); the integer codes have no counterpart there.
