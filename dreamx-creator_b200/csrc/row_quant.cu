@@ -12,9 +12,10 @@
 // the fp32 sum, not on the rounded one: sum_out is rounded once and nothing
 // computed here is rounded twice.
 //
-// A row with a NaN, or an infinity, has the scale NaN (max.NaN keeps it), so what
-// its codes stand for is NaN; int8 codes of it are 0. A finite row whose sum of squares is
-// not finite (values from 2^56 on) is no such row: far_rstd.
+// What cannot be held: a row with a NaN has the scale NaN (max.NaN keeps it). One with an
+// infinity has the scale NaN after a norm (inf * 0) and infinity without one, and int8 codes
+// 0. Either way what its codes stand for is NaN. A finite row whose sum of squares is not
+// finite (values from 2^56 on) is no such row: far_rstd.
 #include "sm100.cuh"
 #include "srdit_internal.h"
 

@@ -558,7 +558,9 @@ int srdit_winattn_fwd(const void* q, const void* k_hr, const void* v_hr, const v
  * sum are given together or both NULL (then s = x); sum may be x or residual itself.
  * A row holding a NaN or an infinity gets the scale NaN; one with an s * weight beyond fp32
  * infinity or NaN. Finite rows get finite scales even where their squares' sum is beyond fp32
- * (16-bit ones with a residual by the rounded sum).
+ * (16-bit ones with a residual by the rounded sum). The root and the quotients are approximate
+ * (2 units in the last place of fp32): a y / scale that lies as near as that to the middle of
+ * two codes may get either.
  * Replaces: WanRMSNorm.forward (video_refiner/wan/modules/sr_dit/models.py:424-440) after a
  *   residual addition (models.py:1257) and before Fp8Linear's row-wise quantiser
  *   (fp8_linear.py:93-103); the integer codes have no counterpart there.
@@ -570,7 +572,9 @@ int srdit_add_rms_quant(const void* x, long long ldx, int M, int K, int dtype,
 
 /*
  * The same row-wise quantiser without the norm (y = x), for any width up to 32768, type and
- * code type: scale[m] = max(max|x| / Q, 1e-12), q = round(x / scale).
+ * code type: scale[m] = max(max|x| / Q, 1e-12), q = round(x / scale), with approximate quotients
+ * as above. A row holding a NaN gets the scale NaN, one with an infinity the scale infinity;
+ * int8 codes of both are 0, and what their codes stand for is NaN.
  * Replaces: quantize_rowwise (fp8_linear.py:93-103, :146-171) where srdit_quant_rowwise's
  *   types or alignments do not fit.
  */

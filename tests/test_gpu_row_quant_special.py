@@ -57,3 +57,33 @@ def test_finite_rows_whose_squares_are_not(srdit, cuda_device, dtype, qdtype, K,
         assert (err <= 0.5 + 127 * 80 * U32).all()
     else:
         assert (err <= torch.clamp(t.abs() * (2.0 ** -4 + 80 * U32), min=2.0 ** -10 * 1.001)).all()
+
+
+@pytest.mark.parametrize("qdtype", CODES)
+@pytest.mark.parametrize("K", (5, 264, 9000))
+@pytest.mark.parametrize("norm", (False, True))
+def test_special_rows(srdit, cuda_device, qdtype, K, norm):
+    """Zeros, values below the smallest scale, a NaN, infinities."""
+    x = torch.ones(6, K, device="cuda")
+    x[0] = 0
+    x[1] = 1e-30
+    x[2, 3] = float("nan")
+    x[3, 4] = float("inf")
+    x[4, 0] = -float("inf")
+    x[5, 2] = -50
+    if norm:
+        q, scale, _ = srdit.ops.add_rms_quant(x, torch.ones(K, device="cuda"), 1e-6, qdtype=qdtype)
+    else:
+        q, scale = srdit.ops.quant_rows(x, qdtype=qdtype)
+    v = q.float() * scale[:, None]
+    # 1e-30 is 1e-27 after the norm, far below half a step of the smallest scale
+    assert (scale[:2] == 1e-12).all() and (q[:2].float() == 0).all()
+    assert scale[2].isnan() and v[2:5].isnan().all()
+    if norm:
+        assert scale[3:5].isnan().all()
+    else:
+        assert scale[3:5].isposinf().all()
+    if qdtype == torch.int8:
+        assert (q[2:5] == 0).all() and q[5, 2] == -127
+    else:
+        assert q[5, 2].float() == -448
