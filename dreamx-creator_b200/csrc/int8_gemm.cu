@@ -650,9 +650,8 @@ static int launch_pair(const Operands& o, Params& p, int dev, cudaStream_t strea
   }
   const int tiles = ((p.M + 255) / 256) * ((p.N + BN - 1) / BN);
   const int pairs = num_sms(dev) / 2;
-  SRDIT_LAUNCH((kern), 2 * (tiles < pairs ? tiles : pairs), NUM_THREADS, C::SMEM, stream, ta, tw,
-               to, p);
-  return static_cast<int>(cudaGetLastError());
+  return launch_plain(kern, 2 * (tiles < pairs ? tiles : pairs), NUM_THREADS, C::SMEM, stream, ta,
+                      tw, to, p);
 }
 
 template <typename T>

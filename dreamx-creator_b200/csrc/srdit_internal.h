@@ -62,8 +62,11 @@ int launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
 }
 
-// A launch as clusters of `cluster` CTAs along x. Never programmatic: one program that let
-// clusters of the next launch start early lost its context, and no cause was found.
+// The clusters of the int8 products (split_kernel, pair_kernel) and of single-token attention
+// (token_kernel) are never launched programmatically, whatever SRDIT_PDL says: one program that
+// let such clusters of the next launch start early, with barriers set up before the dependency
+// wait, lost its context, and no cause was found. launch_clusters: as clusters of `cluster` CTAs
+// along x; launch_plain: without attributes, with the clusters that the kernel declares.
 template <typename... KArgs, typename... Args>
 int launch_clusters(int cluster, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
                     cudaStream_t stream, Args&&... args) {
@@ -79,6 +82,17 @@ int launch_clusters(int cluster, void (*kern)(KArgs...), dim3 grid, dim3 block, 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
+}
+
+template <typename... KArgs, typename... Args>
+int launch_plain(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                 Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
 }
 
