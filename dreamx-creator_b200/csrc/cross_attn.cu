@@ -579,7 +579,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     const uint64_t c2 = f2_pack(a.c, a.c);
     uint8_t* stg = smem + C::OFF_STG + (warp - 4) * 4096;
     int ns = 0, no = 0, idx = 0;
-    bool ok = true;
+    // A wait that runs out sets the abort flag, and those after it end at once: the warp goes
+    // through the rest of its item without a branch, so that no lane of it stays behind, and
+    // leaves at the item's end. (A vote at every wait: 24 heads of 64, 4096 queries on 8192 keys
+    // 296 us in place of 286.)
     Walk walk(a, blockIdx.x, gridDim.x, a.B <= MAX_LENS ? lens : nullptr);
     Item it;
     if (a.ranged && threadIdx.x == 128) reinterpret_cast<Cut*>(a.cuts)[blockIdx.x].parts = 0;
@@ -611,11 +614,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             // the values of unseen keys are zeroed: thread r of tile 0 has key r
             if (t == 0) {
               const int u = idx + 2 * j + 1;
-              if (!mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
-                             abort_flag)) {
-                ok = false;
-                break;
-              }
+              mbar_wait(&full[u % STAGES], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
+                        abort_flag);
               const uint32_t mine =
                   sub == 0 ? vis[0] : sub == 1 ? vis[1] : sub == 2 ? vis[2] : vis[3];
               if (!((mine >> lane) & 1u)) {
@@ -628,10 +628,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
               fence_proxy_async_smem();
             }
           }
-          if (!mbar_wait(&s_full[t], static_cast<uint32_t>(ns) & 1u, a.status, abort_flag)) {
-            ok = false;
-            break;
-          }
+          mbar_wait(&s_full[t], static_cast<uint32_t>(ns) & 1u, a.status, abort_flag);
           ++ns;
           tc_fence_after();
           uint32_t s[4][32];
@@ -714,11 +711,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[t]);
         }
-        if (!ok) break;
-        if (!mbar_wait(&o_full[t], static_cast<uint32_t>(no) & 1u, a.status, abort_flag)) {
-          ok = false;
-          break;
-        }
+        mbar_wait(&o_full[t], static_cast<uint32_t>(no) & 1u, a.status, abort_flag);
+        if (__any_sync(0xffffffffu, *abort_flag != 0u)) break;
         ++no;
         tc_fence_after();
         // O / l (or, of a part, O, m and l): the warp's 32 rows go through its staging
@@ -1054,7 +1048,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, TokenCfg<DP, NT>::PER_SM)
       const int key = key0 + (lane & 15);
       vis = __ballot_sync(0xffffffffu, key < len && (!mrow || __ldg(mrow + key) != 0)) & 0xffffu;
     }
-    if (!mbar_wait(&full[slot], phase, a.status)) {
+    if (!mbar_wait_warp(&full[slot], phase, a.status)) {
       // having given up, let the loads in flight land before the ring is used again
       for (int i = 0; i < 200; ++i) __nanosleep(1000);
       break;

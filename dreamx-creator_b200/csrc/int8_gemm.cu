@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(NUM_THREADS)
   const bool n_on = sub * 32 + lane < p.tile_n && n < p.N;
   T* out = static_cast<T*>(p.out) + n;
   if (p.splits == 1) {
-    if (warp >= 2 && mbar_wait(done, 0u, p.status, abort_flag)) {
+    if (warp >= 2 && mbar_wait_warp(done, 0u, p.status, abort_flag)) {
       tc_fence_after();
       const float sw = n_on ? p.w_scale[n] : 0.f;
       const float b = n_on ? bias_at<T>(p, n) : 0.f;
@@ -239,9 +239,12 @@ __global__ void __launch_bounds__(NUM_THREADS)
     // CTA's columns to it; the copies are counted on that CTA's barrier for the warp. (Stores
     // into the other CTAs' memory, 4 bytes a lane, took 40 ns each.)
     bool got = true;
-    if (warp >= 2) got = mbar_wait(done, 0u, p.status, abort_flag);
+    if (warp >= 2) got = mbar_wait_warp(done, 0u, p.status, abort_flag);
     __syncwarp();
     cluster_wait();
+    // having given up, let the copies in flight to this CTA land
+    if (!got)
+      for (int i = 0; i < 200; ++i) __nanosleep(1000);
     if (warp >= 2 && got) {
       tc_fence_after();
       int* send = reinterpret_cast<int*>(smem) + sub * BT * 32;
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(NUM_THREADS)
             : "memory");
       }
       __syncwarp();
-      if (mine > 0 && mbar_wait(&recv[sub], 0u, p.status, abort_flag)) {
+      if (mine > 0 && mbar_wait_warp(&recv[sub], 0u, p.status, abort_flag)) {
         const float sw = n_on ? p.w_scale[n] : 0.f;
         const float b = n_on ? bias_at<T>(p, n) : 0.f;
         const int* part = reinterpret_cast<const int*>(part_smem) + sub * per * 32 + lane;
@@ -464,6 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     const uint32_t tempty_even = mapa_shared(smem_u32(&tempty[0]), 0);
     int stores = 0;
     int local = 0;
+    bool ok = true;
     for (int tile = cid; tile < num_tiles; tile += ncl, ++local) {
       const int acc = local & 1;
       const int mt = tile / num_n, nt = tile % num_n;
@@ -474,9 +478,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         col_s[acc * 256 + c] = col < p.N ? __ldg(p.w_scale + col) : 0.f;
         col_b[acc * 256 + c] = col < p.N ? bias_at<T>(p, col) : 0.f;
       }
-      named_barrier_sync(1, 128);
-      if (!mbar_wait(&tfull[acc], static_cast<uint32_t>(local >> 1) & 1u, p.status, abort_flag))
-        break;
+      if (!named_barrier_all(1, 128, ok)) break;
+      ok = mbar_wait_warp(&tfull[acc], static_cast<uint32_t>(local >> 1) & 1u, p.status,
+                          abort_flag);
+      if (!ok) continue;  // to the barrier, where all four warps learn of it
       tc_fence_after();
       const int row0 = mt * 256 + static_cast<int>(rank) * 128 + sub * 32;
       const float sa = row0 + lane < p.M ? p.a_scale[row0 + lane] : 0.f;

@@ -121,6 +121,13 @@ SRDIT_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* status,
   }
 }
 
+// mbar_wait by a whole warp: one answer for all lanes, so that none of them goes on to
+// warp-wide instructions that another has given up on.
+SRDIT_DEV bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint32_t* status,
+                              volatile uint32_t* abort_flag = nullptr) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort_flag));
+}
+
 // ---------------------------------------------------------------- cross-GPU flags
 // Monotonic uint32 counters in a rank's memory, written by its peers over
 // NVLink. A writer makes its data visible at system scope, then release-adds;
@@ -264,6 +271,19 @@ SRDIT_DEV void bulk_wait_group_read1() {
 SRDIT_DEV void bulk_wait_group_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 SRDIT_DEV void named_barrier_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+// the same, true where every thread came with true: warps that may give up leave together
+SRDIT_DEV bool named_barrier_all(uint32_t id, uint32_t nthreads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.and.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(nthreads), "r"(v ? 1u : 0u)
+      : "memory");
+  return r != 0;
 }
 
 // ---------------------------------------------------------------- tcgen05 / TMEM
