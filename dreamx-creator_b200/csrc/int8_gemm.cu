@@ -42,7 +42,7 @@ struct Params {
   int splits;  // split_kernel: CTAs of a cluster along K
   int tile_n;  // split_kernel: weight rows of a tile, up to 128
   int stages;  // split_kernel: blocks of K in flight
-  int o_tma;   // pair_kernel: tmO is valid (out and its pitch are 16-byte aligned)
+  int o_tma;   // pair_kernel: tmO is valid (out, its pitch and its width are 16-byte aligned)
   uint32_t* status;
 };
 
@@ -645,7 +645,9 @@ static int launch_pair(const Operands& o, Params& p, int dev, cudaStream_t strea
   if (rc) return rc;
   rc = make_tmap_2d(&tw, o.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, o.ldw, BK, BN / 2);
   if (rc) return rc;
-  p.o_tma = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && (p.ldo * sizeof(T)) % 16 == 0;
+  // A TMA store of a box that reaches past column N writes the rest of N's 16-byte piece too:
+  // only outputs whose rows end with such a piece are stored by it.
+  p.o_tma = (reinterpret_cast<uintptr_t>(p.out) | p.ldo * sizeof(T) | p.N * sizeof(T)) % 16 == 0;
   to = ta;
   if (p.o_tma) {
     const CUtensorMapDataType dt = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
