@@ -148,8 +148,10 @@ SIGNATURES = {
     "srdit_quant_rows": [c_vp, c_ll, c_int, c_int, c_int, c_vp, c_ll, c_int, c_vp, c_vp],
     "srdit_int8_gemm": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_ll,
                         c_ll, c_ll, c_vp, c_vp],
+    "srdit_int8_gemm_columns": [c_int, c_int, c_int],
     "srdit_cross_attn": [ctypes.POINTER(CrossAttnArgs), c_vp],
     "srdit_cross_attn_workspace": [ctypes.POINTER(CrossAttnArgs)],
+    "srdit_cross_attn_items": [ctypes.POINTER(CrossAttnArgs)],
     "srdit_winattn_plan": [c_vp, c_int, c_int, c_int, ctypes.POINTER(WinattnTiling)],
     "srdit_winattn_fwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int,
                           ctypes.POINTER(WinattnGeom), ctypes.POINTER(WinattnTiling), c_vp,

@@ -1505,6 +1505,12 @@ extern "C" int srdit_cross_attn_workspace(const srdit_cross_attn_args* args) {
   return static_cast<int>((p.ws_floats(*args) + 255) / 256);
 }
 
+extern "C" int srdit_cross_attn_items(const srdit_cross_attn_args* args) {
+  if (!args || xattn::check(*args) != 0) return 0;
+  const xattn::Plan p = xattn::make_plan(*args, xattn::sms_here());
+  return p.token ? 0 : p.nq * p.nhp * args->B;
+}
+
 extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t stream) {
   if (!args) return SRDIT_EINVAL;
   const srdit_cross_attn_args& u = *args;

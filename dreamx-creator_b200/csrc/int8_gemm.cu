@@ -661,10 +661,8 @@ static int launch_pair(const Operands& o, Params& p, int dev, cudaStream_t strea
                       tw, to, p);
 }
 
-template <typename T>
-static int launch(const Operands& o, Params& p, cudaStream_t stream) {
-  int dev = 0;
-  cudaGetDevice(&dev);
+// Columns of pair_kernel's tiles for a product, or 0 where split_kernel takes it.
+static int pair_columns(int M, int N, int K, int sms) {
   // split_kernel and pair_kernel, K x N = 4096 x 4096: one token 9.0 and 16.0 us, 16 9.2 and
   // 14.3, 48 10.5 and 10.6, 64 11.4 and 11.1, 72 11.4 and 11.1.
   // From 33 to 64 tokens what the clusters' exchange costs grows with the tokens, what a pair
@@ -672,19 +670,16 @@ static int launch(const Operands& o, Params& p, cudaStream_t stream) {
   // tokens, 1024 x 1024 6.4 and 5.6, 1024 x 4096 8.2 and 7.6, 2048 x 2048 8.0 and 8.3; 64 tokens,
   // 1024 x 1024 6.9 and 5.7, 2048 x 8192 10.3 and 9.6, 3072 x 3072 10.4 and 9.4, 4096 x 1024 8.8
   // and 10.3, 3072 x 14336 14.2 and 15.7, 16384 x 4096 19.2 and 27.3.
-  if (p.M <= 16) return launch_split<T, 16>(o, p, dev, stream);
-  if (p.M <= 32) return launch_split<T, 32>(o, p, dev, stream);
-  if (p.M <= 64 && (p.K > 48 * p.M || static_cast<long long>(p.K) * p.N > 24ll << 20))
-    return launch_split<T, 64>(o, p, dev, stream);
+  if (M <= 32 || (M <= 64 && (K > 48 * M || static_cast<long long>(K) * N > 24ll << 20))) return 0;
   // The tile width with the least time: rounds of tiles over the pairs, times the cycles of
   // a block of K, which are the products' (two per column) or the loads' (60 bytes a cycle
   // and SM), whichever is more.
-  const int pairs = num_sms(dev) / 2;
-  const long long m_tiles = (p.M + 255) / 256;
+  const int pairs = sms / 2;
+  const long long m_tiles = (M + 255) / 256;
   int best = 0;
   long long best_cost = 0;
   for (int bn : {256, 192, 128, 64}) {
-    const long long rounds = (m_tiles * ((p.N + bn - 1) / bn) + pairs - 1) / pairs;
+    const long long rounds = (m_tiles * ((N + bn - 1) / bn) + pairs - 1) / pairs;
     const int mma = 2 * bn, load = (128 + bn / 2) * BK / 60;
     const long long cost = rounds * (mma > load ? mma : load);
     if (!best || cost < best_cost) {
@@ -692,18 +687,38 @@ static int launch(const Operands& o, Params& p, cudaStream_t stream) {
       best_cost = cost;
     }
   }
-  switch (best) {
+  return best;
+}
+
+static int device_here() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
+}
+
+template <typename T>
+static int launch(const Operands& o, Params& p, cudaStream_t stream) {
+  const int dev = device_here();
+  switch (pair_columns(p.M, p.N, p.K, num_sms(dev))) {
+    case 0: break;
     case 256: return launch_pair<T, 256>(o, p, dev, stream);
     case 192: return launch_pair<T, 192>(o, p, dev, stream);
     case 128: return launch_pair<T, 128>(o, p, dev, stream);
     default: return launch_pair<T, 64>(o, p, dev, stream);
   }
+  if (p.M <= 16) return launch_split<T, 16>(o, p, dev, stream);
+  if (p.M <= 32) return launch_split<T, 32>(o, p, dev, stream);
+  return launch_split<T, 64>(o, p, dev, stream);
 }
 
 }  // namespace i8
 }  // namespace srdit
 
 using namespace srdit;
+
+extern "C" int srdit_int8_gemm_columns(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return i8::pair_columns(M, N, K, num_sms(i8::device_here()));
+}
 
 extern "C" int srdit_int8_gemm(const void* a, const float* a_scale, const void* w,
                                const float* w_scale, const void* bias, void* out, int dtype, int M,

@@ -593,6 +593,10 @@ int srdit_quant_rows(const void* x, long long ldx, int M, int K, int dtype, void
 int srdit_int8_gemm(const void* a, const float* a_scale, const void* w, const float* w_scale,
                     const void* bias, void* out, int dtype, int M, int N, int K, long long lda,
                     long long ldw, long long ldo, uint32_t* status, cudaStream_t stream);
+/* How a product of these sizes is run on the current device: the columns of its 256-row tiles, or
+ * 0 where the weights take the rows (few tokens). Nothing is launched; without a device, a
+ * B200's. */
+int srdit_int8_gemm_columns(int M, int N, int K);
 
 /*
  * Attention of queries over an encoder's keys and values of another length:
@@ -628,6 +632,9 @@ typedef struct srdit_cross_attn_args {
 } srdit_cross_attn_args;
 int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t stream);
 int srdit_cross_attn_workspace(const srdit_cross_attn_args* args);
+/* How these arguments are run on the current device: the pairs of query tiles that its SMs go
+ * through, or 0 for few rows (a ring of keys per warp) and where nothing is to do. */
+int srdit_cross_attn_items(const srdit_cross_attn_args* args);
 
 #ifdef __cplusplus
 }
