@@ -727,6 +727,12 @@ extern "C" int srdit_int8_gemm(const void* a, const float* a_scale, const void* 
   if (M < 0 || N < 0 || K <= 0) return SRDIT_EINVAL;
   if (M == 0 || N == 0) return 0;
   if (!a || !a_scale || !w || !w_scale || !out) return SRDIT_EINVAL;
+  // the pitch of one row may be anything
+  if (M == 1) {
+    lda = (K + 15ll) / 16 * 16;
+    ldo = N;
+  }
+  if (N == 1) ldw = (K + 15ll) / 16 * 16;
   if (lda < K || ldw < K || ldo < N) return SRDIT_EINVAL;
   if (K >= 131072) return SRDIT_EUNSUPPORTED;
   if ((lda % 16) || (ldw % 16) || (reinterpret_cast<uintptr_t>(a) & 15u) ||

@@ -370,6 +370,7 @@ static int launch_n(Args& a, cudaStream_t stream) {
 
 template <bool kNorm>
 static int run(Args& a, int dtype, int q_type, cudaStream_t stream) {
+  if (a.M == 1) a.ldx = a.ldr = a.lds = a.ldq = a.K;  // of one row they may be anything
   const bool i8 = q_type == SRDIT_Q_INT8;
   if (!i8 && q_type != SRDIT_Q_E4M3) return SRDIT_EINVAL;
   switch (dtype) {
@@ -399,7 +400,7 @@ static int check_rows(const void* x, long long ldx, int M, int K, int dtype, con
                       long long ldq, const float* scale) {
   if (M < 0 || K <= 0 || !x || !q || !scale || dtype < SRDIT_BF16 || dtype > SRDIT_FP32)
     return SRDIT_EINVAL;
-  if (ldx < K || ldq < K) return SRDIT_EINVAL;
+  if (M > 1 && (ldx < K || ldq < K)) return SRDIT_EINVAL;
   if (!elem_aligned(x, dtype) || (reinterpret_cast<uintptr_t>(scale) & 3u)) return SRDIT_EALIGN;
   if (K > 32768) return SRDIT_EUNSUPPORTED;
   return 0;
@@ -413,7 +414,7 @@ extern "C" int srdit_add_rms_quant(const void* x, long long ldx, int M, int K, i
   const int rc = check_rows(x, ldx, M, K, dtype, q, ldq, scale);
   if (rc) return rc;
   if (!weight || !(eps >= 0.f) || (residual == nullptr) != (sum == nullptr)) return SRDIT_EINVAL;
-  if (residual && (ldr < K || ld_sum < K)) return SRDIT_EINVAL;
+  if (residual && M > 1 && (ldr < K || ld_sum < K)) return SRDIT_EINVAL;
   if (!elem_aligned(weight, dtype) || !elem_aligned(residual, dtype) || !elem_aligned(sum, dtype))
     return SRDIT_EALIGN;
   rq::Args a = {};

@@ -62,13 +62,12 @@ def _need_cuda(*ts):
 
 
 def _rows(t: torch.Tensor):
-    """(row stride in elements) of a 2-D row-major view with unit inner stride; of a single
-    row, whose stride may be anything, its width at least."""
+    """(row stride in elements) of a 2-D row-major view with unit inner stride."""
     st = t.stride()
     if len(st) != 2 or st[1] != 1:
         raise _lib.SrditError(f"expected a 2-D row-major tensor, got shape {tuple(t.shape)} "
                               f"strides {st}")
-    return st[0] if t.shape[0] > 1 else max(st[0], t.shape[1])
+    return st[0]
 
 
 def as_rows(x, K):

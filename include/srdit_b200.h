@@ -553,14 +553,14 @@ int srdit_winattn_fwd(const void* q, const void* k_hr, const void* v_hr, const v
  *   scale[m] = max(max_k |y[m,k]| / Q, 1e-12), Q = 127 (SRDIT_Q_INT8) or 448 (SRDIT_Q_E4M3)
  *   q[m,k] = round(y[m,k] / scale[m]), ties to even
  * x, residual, sum [M, K] and weight [K] of type dtype (SRDIT_BF16 / FP16 / FP32), q [M, K]
- * bytes; row pitches ld* in elements, any alignment of the element type (rows of 16-byte
- * aligned base, pitch and width are the fast ones). K at most 32768. residual and
- * sum are given together or both NULL (then s = x); sum may be x or residual itself.
- * A row holding a NaN or an infinity gets the scale NaN; one with an s * weight beyond fp32
- * infinity or NaN. Finite rows get finite scales even where their squares' sum is beyond fp32
- * (16-bit ones with a residual by the rounded sum). The root and the quotients are approximate
- * (2 units in the last place of fp32): a y / scale that lies as near as that to the middle of
- * two codes may get either.
+ * bytes; row pitches ld* in elements (anything for a single row), any alignment of the element
+ * type (rows of 16-byte aligned base, pitch and width are the fast ones). K at most 32768.
+ * residual and sum are given together or both NULL (then s = x); sum may be x or residual
+ * itself. A row holding a NaN or an infinity gets the scale NaN; one with an s * weight beyond
+ * fp32 infinity or NaN. Other finite rows get finite scales (with eps > 0) even where their
+ * squares' sum is beyond fp32 (16-bit ones with a residual by the rounded sum). The root and the
+ * quotients are approximate (a few units in the last place of fp32): a y / scale that lies as
+ * near as that to the middle of two codes may get either.
  * Replaces: WanRMSNorm.forward (video_refiner/wan/modules/sr_dit/models.py:424-440) after a
  *   residual addition (models.py:1257) and before Fp8Linear's row-wise quantiser
  *   (fp8_linear.py:93-103); the integer codes have no counterpart there.
@@ -585,8 +585,9 @@ int srdit_quant_rows(const void* x, long long ldx, int M, int K, int dtype, void
  * Row-wise scaled int8 GEMM:
  *   out[m,n] = a_scale[m] * w_scale[n] * sum_k A[m,k] W[n,k] + bias[n]
  * A [M, lda] and W [N, ldw] int8 (W is the nn.Linear [out, in] weight), lda and ldw multiples
- * of 16 and both bases 16-byte aligned; the sum is exact in int32 (K below 131072); scales
- * fp32; bias [N] (optional) and out [M, ldo] of type dtype. Any M, N, K, ldo.
+ * of 16 (anything for a single row) and both bases 16-byte aligned; the sum is exact in int32
+ * (K below 131072); scales fp32; bias [N] (optional) and out [M, ldo] of type dtype. Any M, N,
+ * K, ldo.
  * Replaces: Fp8Linear.forward's scaled product (fp8_linear.py:282-297) for weights held as
  *   integers.
  */

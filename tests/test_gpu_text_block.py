@@ -62,3 +62,20 @@ def test_broadcast_inputs_and_single_rows(stack, srdit):
     for got, ref in zip(srdit.ops.add_rms_quant(column, w, residual=column),
                         srdit.ops.add_rms_quant(one, w, residual=one)):
         assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("K", (64, 100))
+def test_products_of_single_rows(srdit, cuda_device, K):
+    """One token, one output channel: a pitch that is not a multiple of 16 is not used."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    a, w = (torch.randint(-128, 128, (n, (K + 15) // 16 * 16), generator=g, device="cuda")
+            .to(torch.int8)[:, :K] for n in (5, 7))
+    one = torch.ones(7, device="cuda")
+    y = srdit.ops.int8_gemm(a, one[:5], w, one, out_dtype=torch.float32)
+    for pitch in (1, K, K + 1):
+        row, column = a[2:3].as_strided((1, K), (pitch, 1)), w[:1].as_strided((1, K), (pitch, 1))
+        out = torch.empty(7, device="cuda").as_strided((1, 7), (1, 1))
+        srdit.ops.int8_gemm(row, one[:1], w, one, out=out)
+        assert torch.equal(out[0], y[2])
+        assert torch.equal(srdit.ops.int8_gemm(a, one[:5], column, one[:1],
+                                               out_dtype=torch.float32), y[:, :1])

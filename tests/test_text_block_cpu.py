@@ -98,16 +98,6 @@ def test_no_keys_or_no_tokens(stack, L, Lk):
 
 
 # ------------------------------------------------------------------ rows of other layouts
-def test_the_pitch_of_one_row_is_its_width_at_least(srdit):
-    """A single row may have any stride over rows: nothing is read by it."""
-    for t, want in ((torch.zeros(8, 1).t(), 8), (torch.zeros(1, 8).expand(1, 8), 8),
-                    (torch.zeros(1, 16)[:, :8], 16), (torch.zeros(3, 16)[:, :8], 16),
-                    (torch.zeros(0, 8), 8)):
-        assert srdit.ops._rows(t) == want
-    with pytest.raises(srdit._lib.SrditError):
-        srdit.ops._rows(torch.zeros(8, 3).t())
-
-
 @pytest.mark.parametrize("x", [
     torch.randn(1, 48).expand(4, 48), torch.randn(2, 1, 48).expand(2, 3, 48),
     torch.randn(1, 3, 48).expand(2, 3, 48), torch.randn(48, 3).t(), torch.randn(48, 1).t(),
@@ -122,7 +112,9 @@ def test_the_linear_takes_rows_of_any_layout(srdit, stack, monkeypatch, x):
     lin = stack.blocks[0].kv
     y = lin(x)
     assert y.shape == (*x.shape[:-1], lin.out_features)
-    assert srdit.ops._rows(seen[0]) >= 48 and torch.equal(seen[0], x.reshape(-1, 48))
+    rows = seen[0]
+    assert srdit.ops._rows(rows) >= 48 or rows.shape[0] == 1   # whose pitch is not used
+    assert torch.equal(rows, x.reshape(-1, 48))
     assert torch.equal(y, lin(x.clone(memory_format=torch.contiguous_format)))
 
 
