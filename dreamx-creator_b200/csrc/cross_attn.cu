@@ -23,11 +23,8 @@
 // join_ranges_kernel).
 #include <atomic>
 
-#include "sm100.cuh"
+#include "elem.cuh"
 #include "srdit_internal.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace srdit {
 namespace xattn {
@@ -56,7 +53,7 @@ struct Args {
   const void* k;
   const void* v;
   void* out;
-  long long qs[3], ks[3], vs[3], os[3];  // {batch, token, head}, elements
+  long long qs[3], os[3];  // {batch, token, head}, elements (k and v go by tensor maps)
   int B, Lq, Lk, H, Hkv, D;
   int group;       // H / Hkv
   int pack;        // tile_kernel: heads of a group side by side in a query tile
@@ -93,16 +90,6 @@ SRDIT_DEV float max3(float x, float y, float z) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
-}
-SRDIT_DEV uint32_t pack2(float x, float y, __nv_bfloat16) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(y), "f"(x));
-  return d;
-}
-SRDIT_DEV uint32_t pack2(float x, float y, __half) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(y), "f"(x));
-  return d;
 }
 SRDIT_DEV int key_count(const Args& a, int b) {
   return a.kv_lens ? min(max(__ldg(a.kv_lens + b), 0), a.Lk) : a.Lk;
@@ -1355,12 +1342,6 @@ static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   return p;
 }
 
-static int sms_here() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  return num_sms(dev);
-}
-
 // a tensor map over [batch, token, head, D] with the given box of heads and tokens;
 // dimensions of one entry, and repeated ones (stride 0), have the extent 1
 static int map_of(CUtensorMap* m, const void* p, const long long st[3], int B, int L, int H, int D,
@@ -1380,19 +1361,6 @@ static int kv_maps(CUtensorMap* tk, CUtensorMap* tv, const srdit_cross_attn_args
   const int B = kv ? u.B : 1;
   const int rc = map_of(tk, kv ? u.k : u.q, u.k_stride, B, u.Lk, u.Hkv, u.D, 1, rows);
   return rc ? rc : map_of(tv, kv ? u.v : u.q, u.v_stride, B, u.Lk, u.Hkv, u.D, 1, rows);
-}
-
-// the kernel's shared memory, set once per device
-template <typename Kern>
-static int set_smem(Kern kern, int bytes, std::atomic<bool>* done) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return 0;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
-  return 0;
 }
 
 template <typename T, int DP>
@@ -1501,13 +1469,13 @@ using namespace srdit;
 
 extern "C" int srdit_cross_attn_workspace(const srdit_cross_attn_args* args) {
   if (!args || xattn::check(*args) != 0) return 0;
-  const xattn::Plan p = xattn::make_plan(*args, xattn::sms_here());
+  const xattn::Plan p = xattn::make_plan(*args, num_sms(device_here()));
   return static_cast<int>((p.ws_floats(*args) + 255) / 256);
 }
 
 extern "C" int srdit_cross_attn_items(const srdit_cross_attn_args* args) {
   if (!args || xattn::check(*args) != 0) return 0;
-  const xattn::Plan p = xattn::make_plan(*args, xattn::sms_here());
+  const xattn::Plan p = xattn::make_plan(*args, num_sms(device_here()));
   return p.token ? 0 : p.nq * p.nhp * args->B;
 }
 
@@ -1516,7 +1484,7 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   const srdit_cross_attn_args& u = *args;
   const int rc = xattn::check(u);
   if (rc) return rc < 0 ? rc : 0;
-  const xattn::Plan p = xattn::make_plan(u, xattn::sms_here());
+  const xattn::Plan p = xattn::make_plan(u, num_sms(device_here()));
   const long long need = 4 * p.ws_floats(u);
   if (need > 0) {
     if (!u.workspace || u.workspace_bytes < need) return SRDIT_EINVAL;
@@ -1529,8 +1497,6 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.out = u.out;
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = u.q_stride[i];
-    a.ks[i] = u.k_stride[i];
-    a.vs[i] = u.v_stride[i];
     a.os[i] = u.o_stride[i];
   }
   a.B = u.B;

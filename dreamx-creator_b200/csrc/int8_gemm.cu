@@ -20,11 +20,8 @@
 //                  workspace, no atomics, no second launch.
 #include <atomic>
 
-#include "sm100.cuh"
+#include "elem.cuh"
 #include "srdit_internal.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace srdit {
 namespace i8 {
@@ -47,26 +44,12 @@ struct Params {
 };
 
 template <typename T>
-SRDIT_DEV float to_f(T v) {
-  return static_cast<float>(v);
-}
-template <typename T>
 SRDIT_DEV float bias_at(const Params& p, int n) {
   return p.bias ? to_f(static_cast<const T*>(p.bias)[n]) : 0.f;
 }
 // acc * sa * sw + bias: the conversion, one product and one fma, a rounding each
 SRDIT_DEV float scaled(uint32_t acc, float sa, float sw, float b) {
   return fmaf(static_cast<float>(static_cast<int>(acc)) * sa, sw, b);
-}
-SRDIT_DEV uint32_t pack2(float x, float y, __nv_bfloat16) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(y), "f"(x));
-  return d;
-}
-SRDIT_DEV uint32_t pack2(float x, float y, __half) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(y), "f"(x));
-  return d;
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -565,16 +548,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 }
 
 // ---------------------------------------------------------------- launch
-template <typename Kern>
-static int set_smem(Kern kern, int bytes, std::atomic<bool>* done, int dev) {
-  if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return 0;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
-  return 0;
-}
-
 struct Operands {
   const void* a;
   const void* w;
@@ -586,7 +559,7 @@ static int launch_split(const Operands& o, Params& p, int dev, cudaStream_t stre
   using C = SplitCfg<BT>;
   auto kern = split_kernel<T, BT>;
   static std::atomic<bool> attr_done[kMaxDevices] = {};
-  int rc = set_smem(kern, 232448, attr_done, dev);
+  int rc = set_smem(kern, 232448, attr_done);
   if (rc) return rc;
   // The tile's weight rows and the splits of K with the least time, in cycles: what an SM's
   // CTAs read at 38 bytes a cycle (an SM's share of the memory is 23; the latency of 2000
@@ -638,7 +611,7 @@ static int launch_pair(const Operands& o, Params& p, int dev, cudaStream_t strea
   using C = PairCfg<BN>;
   auto kern = pair_kernel<T, BN>;
   static std::atomic<bool> attr_done[kMaxDevices] = {};
-  int rc = set_smem(kern, C::SMEM, attr_done, dev);
+  int rc = set_smem(kern, C::SMEM, attr_done);
   if (rc) return rc;
   CUtensorMap ta, tw, to;
   rc = make_tmap_2d(&ta, o.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, o.lda, BK, 128);
@@ -690,11 +663,6 @@ static int pair_columns(int M, int N, int K, int sms) {
   return best;
 }
 
-static int device_here() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
-}
-
 template <typename T>
 static int launch(const Operands& o, Params& p, cudaStream_t stream) {
   const int dev = device_here();
@@ -717,7 +685,7 @@ using namespace srdit;
 
 extern "C" int srdit_int8_gemm_columns(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return i8::pair_columns(M, N, K, num_sms(i8::device_here()));
+  return i8::pair_columns(M, N, K, num_sms(device_here()));
 }
 
 extern "C" int srdit_int8_gemm(const void* a, const float* a_scale, const void* w,

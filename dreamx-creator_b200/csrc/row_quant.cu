@@ -16,11 +16,8 @@
 // infinity has the scale NaN after a norm (inf * 0) and infinity without one, and int8 codes
 // 0. Either way what its codes stand for is NaN. A finite row whose sum of squares is not
 // finite (values from 2^56 on) is no such row: far_rstd.
-#include "sm100.cuh"
+#include "elem.cuh"
 #include "srdit_internal.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace srdit {
 namespace rq {
@@ -39,14 +36,6 @@ struct Args {
   float eps, inv_k;
 };
 
-template <typename T>
-SRDIT_DEV float to_f(T v);
-template <>
-SRDIT_DEV float to_f(float v) { return v; }
-template <>
-SRDIT_DEV float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-SRDIT_DEV float to_f(__half v) { return __half2float(v); }
 template <typename T>
 SRDIT_DEV T from_f(float v);
 template <>
@@ -67,7 +56,7 @@ template <typename T, int V>
 SRDIT_DEV void load(const T* p, float (&o)[V]) {
   const Vec<T, V> t = *reinterpret_cast<const Vec<T, V>*>(p);
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = to_f<T>(t.v[i]);
+  for (int i = 0; i < V; ++i) o[i] = to_f(t.v[i]);
 }
 template <typename T, int V>
 SRDIT_DEV void store(T* p, const float (&o)[V]) {
@@ -158,7 +147,7 @@ SRDIT_DEV float far_rstd(const T* x, const T* r, int K, float inv_k, float eps) 
   __syncwarp();
 #pragma unroll 1
   for (int c = threadIdx.x & 31; c < K; c += 32) {
-    const float v = (to_f<T>(x[c]) + (r ? to_f<T>(r[c]) : 0.f)) * down;
+    const float v = (to_f(x[c]) + (r ? to_f(r[c]) : 0.f)) * down;
     ss = fmaf(v, v, ss);
   }
 #pragma unroll

@@ -3,6 +3,7 @@
 // the runtime's driver entry point, so the library does not link libcuda), and
 // per-device caches.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -23,6 +24,24 @@ enum EpiKind : int {
 
 // Number of SMs of `dev` (cached).
 int num_sms(int dev);
+
+// The current device (0 where there is none).
+inline int device_here() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
+}
+
+// A kernel's dynamic shared memory on the current device, set once: `done` has a flag for each.
+template <typename Kern>
+int set_smem(Kern kern, int bytes, std::atomic<bool>* done) {
+  const int dev = device_here();
+  if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return 0;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
+  return 0;
+}
 
 // 2-D tiled tensor map over a row-major [rows, cols] matrix with `ld` elements
 // per row, box [box_rows, box_cols], 128-byte swizzle. Returns 0 or an SRDIT_E*
