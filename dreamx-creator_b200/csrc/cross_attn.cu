@@ -908,8 +908,8 @@ SRDIT_DEV uint4 lds16(uint32_t src) {
 // A warp alone on its scheduler takes 1300 cycles for a block's 230 instructions, nearly all of
 // it their latency, so an SM gets three CTAs (168 registers; two of 16 rows), and a warp's
 // ring 2 or 3 blocks of 128-wide heads, twice that of 64-wide ones. (Two CTAs with 3 blocks: 4
-// x 32768 keys, 32 heads over 8, 87.6 us in place of 81.1, 8 x 512 keys, 24 heads 17.6 in place
-// of 12.7; one with 6: 136 and 22; of small grids none is better.)
+// x 32768 keys, 32 heads over 8, 86.0 us in place of 80.5, 8 x 512 keys, 24 heads 11.4 in place
+// of 10.9; one with 6: 136 and 17.2.)
 constexpr int TOKEN_WARPS = 4;
 
 template <int DP, int NT>
@@ -1282,8 +1282,8 @@ struct Plan {
 static Plan make_plan(const srdit_cross_attn_args& a, int sms) {
   Plan p = {};
   const int group = a.H / a.Hkv;
-  // 16 rows, token_kernel and tile_kernel: 8 x 512 keys, 24 heads 16.3 and 20.9 us (one row
-  // 12.7); 4 x 32768 keys, 8 heads 93.2 and 107.8 (four rows 81.0)
+  // 16 rows, token_kernel and tile_kernel: 8 x 512 keys, 24 heads 15.7 and 20.4 us (one row
+  // 10.9); 4 x 32768 keys, 8 heads 91 and 118 (four rows 80.7)
   p.token = static_cast<long long>(a.Lq) * group <= 16;
   p.splits = p.cluster = p.parts = 1;
   if (p.token) {

@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Args a) {
 
 // Wider rows: one block of 512 threads a row, which it reads twice, the second time out of
 // the caches. The sum is stored in the second pass, since it may be x or the residual.
-// Four blocks an SM: 6912 x 14336 bf16 67 us, with the residual 115, 5.2 TB/s (with what the
-// compiler takes by itself, 32 to 44 registers: 66, and 122 to 138).
+// Four blocks an SM: 6912 x 14336 bf16 67 to 70 us, with the residual 115 to 128 (with what the
+// compiler takes by itself, 32 to 44 registers: 66 to 73, and 122 to 140).
 template <typename T, bool kInt8, bool kNorm, bool kRes, int V>
 __global__ void __launch_bounds__(512, 4) wide_rows_kernel(const Args a) {
   pdl_begin();

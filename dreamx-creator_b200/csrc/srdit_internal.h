@@ -55,7 +55,7 @@ int make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
                  const long long dims[4], const long long strides_bytes[3], const int box[4]);
 
 // Programmatic dependent launch: every kernel of the library starts with
-// pdl_wait() (sm100.cuh) before it touches global memory, so a launch may be
+// pdl_begin() (sm100.cuh) before it touches global memory, so a launch may be
 // issued with programmatic stream serialization -- its CTAs are scheduled,
 // allocate shared memory / TMEM and set up their barriers while the previous
 // kernel of the stream drains, and then wait for that kernel's completion and

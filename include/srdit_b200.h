@@ -70,6 +70,8 @@ const char* srdit_strerror(int code);
  * A [M, lda] e4m3 row-major (K contiguous), B [N, ldb] e4m3 (the nn.Linear
  * [out, in] weight), a_scale [M] fp32 per token, b_scale [N] fp32 per output
  * channel, bias [N] bf16 or NULL, out [M, ldo] bf16. lda/ldb multiples of 16.
+ * Where N is not a multiple of 8, out's columns from N to the next multiple of 8
+ * are overwritten too.
  * residual [M, ldr] bf16 (EPI_RES / EPI_GATED_RES), gate [N] fp32
  * (EPI_GATED_RES), row_amax [M] fp32 zero-initialised by the caller (EPI_GELU).
  * Replaces: Fp8Linear.forward's torch._scaled_mm(xq, w_fp8.t(), scale_a=xs,
