@@ -375,6 +375,8 @@ def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, st
         fill(a, 0, *fields, ws.data_ptr(), kib << 10, st)
     _launch("srdit_cross_attn", ref, stream, kind="cross_attn",
             work=4 * B * Lq * H * D * Lk)
+    if kib:
+        Stats.launches += 1   # a second kernel joins the parts
     return out
 
 

@@ -116,7 +116,8 @@ def test_strides_of_single_entries(srdit, cuda_device, Lq):
 @pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [
     (1, 1, 300, 128, 1, 64), (2, 1, 513, 48, 2, 128), (1, 2, 700, 60, 3, 64),
     (2, 5, 257, 21, 3, 72), (1, 33, 400, 192, 1, 128), (3, 1, 140, 17, 1, 128),
-    (2, 100, 300, 12, 1, 64), (1, 16, 2000, 1, 1, 128), (1, 17, 2000, 1, 1, 128), (1, 4, 2000, 4, 1, 64)])
+    (2, 100, 300, 12, 1, 64), (1, 16, 2000, 1, 1, 128), (1, 17, 2000, 1, 1, 128),
+    (1, 4, 2000, 4, 1, 64)])
 def test_groups_of_any_size(srdit, cuda_device, dtype, B, Lq, Lk, H, Hkv, D):
     """One to 192 heads on a key head, powers of two and not, with lengths and a mask."""
     g = _gen(H + Lk)
@@ -155,3 +156,13 @@ def test_status_words_stay_clear(srdit, cuda_device, M):
     srdit.ops.int8_gemm(a, one[:M], w, one[:128], status=status)
     srdit.ops.cross_attn(*_qkv(g, 1, M, 3000, 2, 1, 64, torch.bfloat16), status=status)
     assert status.item() == 0
+
+
+@pytest.mark.parametrize("Lq,Lk,kernels", [(1, 300, 1), (1, 40000, 2), (300, 300, 1),
+                                           (300, 9000, 2)])
+def test_every_kernel_is_counted(srdit, cuda_device, Lq, Lk, kernels):
+    """A call whose parts are joined by a second kernel counts as two launches."""
+    q, k, v = _qkv(_gen(Lk), 1, Lq, Lk, 1, 1, 64, torch.bfloat16)
+    before = srdit.ops.Stats.launches
+    srdit.ops.cross_attn(q, k, v)
+    assert srdit.ops.Stats.launches - before == kernels
