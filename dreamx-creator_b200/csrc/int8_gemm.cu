@@ -16,8 +16,8 @@
 //   split_kernel   up to 64 tokens: bounded by the weights' bytes. The weights take the
 //                  MMA's 128 rows and the tokens its columns (16, 32 or 64), so one token
 //                  wastes 15 columns and not 255 rows. K is split over a cluster of up to 8
-//                  CTAs, whose int32 partial sums meet in shared memory of the cluster: no
-//                  workspace, no atomics, no second launch.
+//                  CTAs, which read one another's int32 partial sums out of shared memory:
+//                  no workspace, no atomics, no second launch.
 #include <atomic>
 
 #include "elem.cuh"
@@ -53,25 +53,29 @@ SRDIT_DEV float scaled(uint32_t acc, float sa, float sw, float b) {
 }
 
 // ---------------------------------------------------------------- few tokens
-// Measured: 1 x 3072 x 14336 11.5 us, 3.8 TB/s; 37 x 4096 x 4096 9.8 us, 1.8 TB/s, of which
-// the launch, the first block's latency and the cluster's exchange are 6 (a product of
-// 128 x 128 takes that). Memory is read at its
-// rate for the few microseconds between only. (Stores of 4 bytes into the other CTAs'
-// memory took 40 ns each, scales loaded a token at a time as long as the sums; 128 tokens a
-// tile in this kernel are slower than pair_kernel's 64-column tiles.)
+// Measured: 1 x 3072 x 14336 10.9 us, 4.1 TB/s; 37 x 4096 x 4096 8.8 us, 2.0 TB/s; a product of
+// 1 x 128 x 128, which is launch and latency, takes 3.3. Memory is read at its rate for a few
+// microseconds between only. One CTA goes through a block of K in 400 cycles at least (four
+// MMAs in a row), so without clusters 1 x 14336 x 3072 takes 24 us in place of 12. (Scales
+// loaded a token at a time took as long as the sums; 128 tokens a tile in this kernel are slower
+// than pair_kernel's 64-column tiles. Bulk copies of the sums into the other CTAs' memory were
+// slower, 37 x 4096 x 4096 9.8 us, and not sound: in a process that had run many other products
+// 11 x 2832 x 4077 ended in an illegal access, which range checks on every index of the kernel
+// did not explain. With loads between two barriers of the cluster it has not been seen in 17000
+// products of random sizes.)
 //
-// Shared memory: a ring of p.stages stages (weight rows, then tokens), the other CTAs'
-// partial sums, barriers. An MMA reads 128 weight rows of a stage whatever tile_n is; past
-// the last stage that is still inside this CTA's memory.
+// Shared memory: a ring of p.stages stages (weight rows, then tokens), barriers. An MMA reads
+// 128 weight rows of a stage whatever tile_n is: PAST bytes behind the last stage keep that
+// inside this CTA's memory. The partial sums take the ring's place.
 constexpr int MAX_STAGES = 16;
 template <int BT>
 struct SplitCfg {
-  static constexpr int PART = BT * 512;  // int32 [splits][4 warps][BT / splits][32]
-  static constexpr int BARS = (2 * MAX_STAGES + 5) * 8 + 8;
-  static constexpr int MOST = 232448 - 1024 - PART - BARS;  // for the ring
+  static constexpr int PAST = (128 - 64 - BT) * BK;  // tile_n is 64 at least
+  static constexpr int BARS = (2 * MAX_STAGES + 1) * 8 + 8;
+  static constexpr int MOST = 232448 - 1024 - PAST - BARS;  // for the ring
   static constexpr uint32_t TMEM_COLS = BT < 32 ? 32 : BT;
   static int smem(int stages, int tile_n) {
-    return stages * (tile_n + BT) * BK + PART + BARS + 1024;
+    return stages * (tile_n + BT) * BK + PAST + BARS + 1024;
   }
 };
 
@@ -86,18 +90,15 @@ __global__ void __launch_bounds__(NUM_THREADS)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* part_smem = smem + STAGES * stage_bytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(part_smem + C::PART);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * stage_bytes + C::PAST);
   uint64_t* empty = full + MAX_STAGES;
   uint64_t* done = empty + MAX_STAGES;
-  uint64_t* recv = done + 1;  // [4] the other CTAs' partial sums, for each epilogue warp
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(recv + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int n0 = (static_cast<int>(blockIdx.x) / p.splits) * p.tile_n;
-  const int m0 = static_cast<int>(blockIdx.y) * BT;
   const int num_kb = (p.K + BK - 1) / BK;
   const int kb0 = static_cast<int>(static_cast<long long>(num_kb) * split / p.splits);
   const int kb1 = static_cast<int>(static_cast<long long>(num_kb) * (split + 1) / p.splits);
@@ -106,12 +107,9 @@ __global__ void __launch_bounds__(NUM_THREADS)
     uint8_t* st = smem + s * stage_bytes;
     mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(stage_bytes));
     tma_load_2d(st, &tmW, &full[s], (kb0 + i) * BK, n0);
-    tma_load_2d(st + w_bytes, &tmA, &full[s], (kb0 + i) * BK, m0);
+    tma_load_2d(st + w_bytes, &tmA, &full[s], (kb0 + i) * BK, 0);
   };
   const int n_kb = kb1 - kb0;
-  // token columns of this CTA in its cluster: [split * per, split * per + mine)
-  const int per = BT / p.splits;
-  const int mine = min(max(p.M - m0 - split * per, 0), per);
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmW);
     tma_prefetch_desc(&tmA);
@@ -120,12 +118,9 @@ __global__ void __launch_bounds__(NUM_THREADS)
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
-    for (int x = 0; x < 4; ++x) mbar_init(&recv[x], 1);
     *abort_flag = 0u;
     fence_barrier_init();
     fence_proxy_async_smem();
-    for (int x = 0; x < 4 && p.splits > 1; ++x)
-      mbar_arrive_expect_tx(&recv[x], static_cast<uint32_t>((p.splits - 1) * mine * 128));
     // the first loads need none of what the other warps still set up
     for (int i = 0; i < STAGES && i < n_kb; ++i) load(i, i);
   }
@@ -137,7 +132,6 @@ __global__ void __launch_bounds__(NUM_THREADS)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (p.splits > 1) cluster_arrive();  // waited for before the first remote store
   const uint32_t tmem_base = *tmem_slot;
 
   bool ok = true;
@@ -193,100 +187,92 @@ __global__ void __launch_bounds__(NUM_THREADS)
   // buffer held)
   const int sub = warp & 3;
   const uint32_t t_row = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
-  const int n = n0 + sub * 32 + lane;
-  const bool n_on = sub * 32 + lane < p.tile_n && n < p.N;
-  T* out = static_cast<T*>(p.out) + n;
   if (p.splits == 1) {
     if (warp >= 2 && mbar_wait_warp(done, 0u, p.status, abort_flag)) {
       tc_fence_after();
+      const int n = n0 + sub * 32 + lane;
+      const bool n_on = sub * 32 + lane < p.tile_n && n < p.N;
       const float sw = n_on ? p.w_scale[n] : 0.f;
       const float b = n_on ? bias_at<T>(p, n) : 0.f;
+      T* out = static_cast<T*>(p.out) + n;
 #pragma unroll 1
-      for (int c = 0; c < BT && m0 + c < p.M; c += 16) {
+      for (int c = 0; c < BT && c < p.M; c += 16) {
         uint32_t r[16];
         tmem_ld16(t_row + c, r);
         float sa[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sa[e] = m0 + c + e < p.M ? __ldg(p.a_scale + m0 + c + e) : 0.f;
+        for (int e = 0; e < 16; ++e) sa[e] = c + e < p.M ? __ldg(p.a_scale + c + e) : 0.f;
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int m = m0 + c + e;
-          if (m < p.M && n_on) out[m * p.ldo] = static_cast<T>(scaled(r[e], sa[e], sw, b));
-        }
+        for (int e = 0; e < 16; ++e)
+          if (c + e < p.M && n_on)
+            out[(c + e) * p.ldo] = static_cast<T>(scaled(r[e], sa[e], sw, b));
       }
     }
-  } else {
-    // Token column c belongs to CTA c / per of the cluster. Each epilogue warp lays its 32
-    // rows' partial sums out as [c][32] over the ring, which is done with, and copies each
-    // CTA's columns to it; the copies are counted on that CTA's barrier for the warp. (Stores
-    // into the other CTAs' memory, 4 bytes a lane, took 40 ns each.)
-    bool got = true;
-    if (warp >= 2) got = mbar_wait_warp(done, 0u, p.status, abort_flag);
     __syncwarp();
-    cluster_wait();
-    // having given up, let the copies in flight to this CTA land
-    if (!got)
-      for (int i = 0; i < 200; ++i) __nanosleep(1000);
-    if (warp >= 2 && got) {
+  } else {
+    // Each epilogue warp lays its 32 rows' partial sums out over the ring, which is done with,
+    // as [4 tokens][32 rows][4]. After the cluster's barrier 32 rows of 4 tokens are joined by
+    // one warp of the cluster, out of all its CTAs' memory. (Stores into the other CTAs'
+    // memory, 4 bytes a lane, took 40 ns each.) Both sides are the threads' own accesses, ordered
+    // by the barrier.
+    const uint32_t sums = smem_u32(smem);
+    if (warp >= 2 && mbar_wait_warp(done, 0u, p.status, abort_flag)) {
       tc_fence_after();
-      int* send = reinterpret_cast<int*>(smem) + sub * BT * 32;
 #pragma unroll 1
-      for (int c = 0; c < BT && m0 + c < p.M; c += 16) {
+      for (int c = 0; c < BT && c < p.M; c += 16) {
         uint32_t r[16];
         tmem_ld16(t_row + c, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) send[(c + e) * 32 + lane] = static_cast<int>(r[e]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      const int theirs = min(max(p.M - m0 - lane * per, 0), per);  // of CTA `lane`
-      if (lane < p.splits && lane != split && theirs > 0) {
-        const uint32_t dst = smem_u32(part_smem) +
-                             static_cast<uint32_t>((split * 4 + sub) * per * 128);
-        asm volatile(
-            "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes "
-            "[%0], [%1], %2, [%3];" ::"r"(mapa_shared(dst, static_cast<uint32_t>(lane))),
-            "r"(smem_u32(send + lane * per * 32)), "r"(theirs * 128),
-            "r"(mapa_shared(smem_u32(&recv[sub]), static_cast<uint32_t>(lane)))
-            : "memory");
-      }
-      __syncwarp();
-      if (mine > 0 && mbar_wait_warp(&recv[sub], 0u, p.status, abort_flag)) {
-        const float sw = n_on ? p.w_scale[n] : 0.f;
-        const float b = n_on ? bias_at<T>(p, n) : 0.f;
-        const int* part = reinterpret_cast<const int*>(part_smem) + sub * per * 32 + lane;
-        const int* own = send + split * per * 32 + lane;
-        const int m1 = m0 + split * per;
-        for (int a0 = 0; a0 < mine; a0 += 8) {
-          // eight tokens together: their scales, and their sums over the splits
-          float sa[8];
-          int acc[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool on = a0 + e < mine;
-            sa[e] = on ? __ldg(p.a_scale + m1 + a0 + e) : 0.f;
-            acc[e] = on ? own[(a0 + e) * 32] : 0;
-          }
-          for (int s = 0; s < p.splits; ++s) {
-            if (s == split) continue;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (a0 + e < mine) acc[e] += part[(s * 4 * per + a0 + e) * 32];
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (a0 + e < mine && n_on)
-              out[(m1 + a0 + e) * p.ldo] =
-                  static_cast<T>(scaled(static_cast<uint32_t>(acc[e]), sa[e], sw, b));
-        }
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<uint4*>(smem + ((sub * (BT / 4) + (c + e) / 4) * 32 + lane) * 16) =
+              make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
       }
     }
     __syncwarp();
-    // no CTA leaves while another copies from or to its memory
-    cluster_arrive();
-    cluster_wait();
+    cluster_sync();  // every CTA's sums are in its memory
+    if (warp >= 2) {
+      for (int it = split * 4 + (warp - 2); it < BT; it += p.splits * 4) {
+        const int quad = it >> 2, rows = it & 3;
+        if (quad * 4 >= p.M) break;
+        if (rows * 32 >= p.tile_n) continue;
+        uint4 v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          v[x] = make_uint4(0u, 0u, 0u, 0u);
+          if (x < p.splits)
+            asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v[x].x), "=r"(v[x].y), "=r"(v[x].z), "=r"(v[x].w)
+                         : "r"(mapa_shared(sums + ((rows * (BT / 4) + quad) * 32 + lane) * 16,
+                                           static_cast<uint32_t>(x)))
+                         : "memory");
+        }
+        const int row = rows * 32 + lane, n = n0 + row;
+        const bool n_on = row < p.tile_n && n < p.N;
+        const float sw = n_on ? p.w_scale[n] : 0.f;
+        const float b = n_on ? bias_at<T>(p, n) : 0.f;
+        float sa[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sa[e] = quad * 4 + e < p.M ? __ldg(p.a_scale + quad * 4 + e) : 0.f;
+        uint32_t acc[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          acc[0] += v[x].x;
+          acc[1] += v[x].y;
+          acc[2] += v[x].z;
+          acc[3] += v[x].w;
+        }
+        T* out = static_cast<T*>(p.out) + n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (quad * 4 + e < p.M && n_on)
+            out[(quad * 4 + e) * p.ldo] = static_cast<T>(scaled(acc[e], sa[e], sw, b));
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while another reads its memory
   }
   tc_fence_before();
   __syncthreads();
@@ -566,11 +552,11 @@ static int launch_split(const Operands& o, Params& p, int dev, cudaStream_t stre
   // cycles wants 76 KB in flight), each wave's start and end, the cluster's exchange.
   // Clusters of large CTAs do not fill every SM.
   const int sms = num_sms(dev);
-  const int m_tiles = (p.M + BT - 1) / BT, num_kb = (p.K + BK - 1) / BK;
+  const int num_kb = (p.K + BK - 1) / BK;
   long long best = -1;
   for (int tile = 128; tile >= 64; tile -= 16) {
     for (int splits = 1; splits <= 8 && (splits == 1 || splits * 2 <= num_kb); splits *= 2) {
-      const long long ctas = static_cast<long long>((p.N + tile - 1) / tile) * m_tiles * splits;
+      const long long ctas = static_cast<long long>((p.N + tile - 1) / tile) * splits;
       const int n_kb = (num_kb + splits - 1) / splits, stage = (tile + BT) * BK;
       int stages = C::MOST / stage < MAX_STAGES ? C::MOST / stage : MAX_STAGES;
       if (stages > n_kb) stages = n_kb;
@@ -601,7 +587,7 @@ static int launch_split(const Operands& o, Params& p, int dev, cudaStream_t stre
   if (rc) return rc;
   rc = make_tmap_2d(&tw, o.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, o.ldw, BK, p.tile_n);
   if (rc) return rc;
-  const dim3 grid(static_cast<unsigned>(n_tiles * p.splits), static_cast<unsigned>(m_tiles));
+  const dim3 grid(static_cast<unsigned>(n_tiles * p.splits));
   return launch_clusters(p.splits, kern, grid, NUM_THREADS,
                          static_cast<size_t>(C::smem(p.stages, p.tile_n)), stream, ta, tw, p);
 }
@@ -636,13 +622,13 @@ static int launch_pair(const Operands& o, Params& p, int dev, cudaStream_t strea
 
 // Columns of pair_kernel's tiles for a product, or 0 where split_kernel takes it.
 static int pair_columns(int M, int N, int K, int sms) {
-  // split_kernel and pair_kernel, K x N = 4096 x 4096: one token 9.0 and 16.0 us, 16 9.2 and
-  // 14.3, 48 10.5 and 10.6, 64 11.4 and 11.1, 72 11.4 and 11.1.
-  // From 33 to 64 tokens what the clusters' exchange costs grows with the tokens, what a pair
-  // without a split of K loses with K, and large weights want split_kernel's deeper loads: 40
-  // tokens, 1024 x 1024 6.4 and 5.6, 1024 x 4096 8.2 and 7.6, 2048 x 2048 8.0 and 8.3; 64 tokens,
-  // 1024 x 1024 6.9 and 5.7, 2048 x 8192 10.3 and 9.6, 3072 x 3072 10.4 and 9.4, 4096 x 1024 8.8
-  // and 10.3, 3072 x 14336 14.2 and 15.7, 16384 x 4096 19.2 and 27.3.
+  // split_kernel and pair_kernel, K x N = 4096 x 4096: one token 6.7 and 16.2 us, 16 6.9 and
+  // 13.6, 48 8.6 and 9.4, 64 8.8 and 9.4.
+  // From 33 to 64 tokens the clusters' exchange grows with the tokens, what a pair without a
+  // split of K loses grows with K, and large weights want split_kernel's deeper loads: 40 tokens,
+  // 1024 x 1024 5.5 and 5.7, 1024 x 4096 6.8 and 6.8, 2048 x 2048 6.9 and 7.3; 64 tokens, 1024 x
+  // 1024 6.1 and 5.7, 2048 x 8192 8.7 and 7.6, 3072 x 3072 8.5 and 8.2, 4096 x 1024 7.1 and 9.3,
+  // 3072 x 14336 10.5 and 13.1, 16384 x 4096 12.7 and 23.7.
   if (M <= 32 || (M <= 64 && (K > 48 * M || static_cast<long long>(K) * N > 24ll << 20))) return 0;
   // The tile width with the least time: rounds of tiles over the pairs, times the cycles of
   // a block of K, which are the products' (two per column) or the loads' (60 bytes a cycle

@@ -84,8 +84,10 @@ int launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
 // The clusters of the int8 products (split_kernel, pair_kernel) and of single-token attention
 // (token_kernel) are never launched programmatically, whatever SRDIT_PDL says: one program that
 // let such clusters of the next launch start early, with barriers set up before the dependency
-// wait, lost its context, and no cause was found. launch_clusters: as clusters of `cluster` CTAs
-// along x; launch_plain: without attributes, with the clusters that the kernel declares.
+// wait, lost its context. (split_kernel then exchanged its sums by bulk copies, which are gone
+// since and may have been the cause; the form was not tried again.) launch_clusters: as clusters
+// of `cluster` CTAs along x; launch_plain: without attributes, with the clusters that the kernel
+// declares.
 template <typename... KArgs, typename... Args>
 int launch_clusters(int cluster, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
                     cudaStream_t stream, Args&&... args) {

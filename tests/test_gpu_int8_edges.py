@@ -166,3 +166,20 @@ def test_every_kernel_is_counted(srdit, cuda_device, Lq, Lk, kernels):
     before = srdit.ops.Stats.launches
     srdit.ops.cross_attn(q, k, v)
     assert srdit.ops.Stats.launches - before == kernels
+
+
+@pytest.mark.parametrize("M,N,K", [
+    (11, 4077, 2832), (57, 4452, 4934), (6, 2640, 4829), (22, 1362, 2675), (9, 2953, 2467),
+    (64, 33, 3211), (33, 2, 3084), (1, 10, 4724), (45, 2296, 2789), (16, 4077, 4096)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_products_of_few_tokens_and_a_long_axis(srdit, cuda_device, dtype, M, N, K):
+    """Sums shared out over the CTAs of a cluster, some of them without a token to join, of odd
+    sizes and in rows wider than they are long; five times over, the same bits."""
+    g = _gen(M + N + K)
+    a, w = (torch.randint(-128, 128, (n, (K + 15) // 16 * 16 + 32), generator=g, device="cuda")
+            .to(torch.int8)[:, :K] for n in (M, N))
+    _check_gemm(srdit, a, w, dtype, True, g)
+    s = torch.rand(max(M, N), generator=g, device="cuda")
+    first = srdit.ops.int8_gemm(a, s[:M], w, s[:N], out_dtype=dtype)
+    for _ in range(4):
+        assert torch.equal(srdit.ops.int8_gemm(a, s[:M], w, s[:N], out_dtype=dtype), first)
