@@ -55,13 +55,13 @@ SRDIT_DEV float scaled(uint32_t acc, float sa, float sw, float b) {
 // ---------------------------------------------------------------- few tokens
 // Measured: 1 x 3072 x 14336 10.9 us, 4.1 TB/s; 37 x 4096 x 4096 8.8 us, 2.0 TB/s; a product of
 // 1 x 128 x 128, which is launch and latency, takes 3.3. Memory is read at its rate for a few
-// microseconds between only. One CTA goes through a block of K in 400 cycles at least (four
-// MMAs in a row), so without clusters 1 x 14336 x 3072 takes 24 us in place of 12. (Scales
+// microseconds between only. A CTA takes 400 cycles for a block of K, tiles of 32 rows and of
+// 112 alike, so without clusters 1 x 14336 x 3072 takes 24 us in place of 9. (Scales
 // loaded a token at a time took as long as the sums; 128 tokens a tile in this kernel are slower
 // than pair_kernel's 64-column tiles. Bulk copies of the sums into the other CTAs' memory were
 // slower, 37 x 4096 x 4096 9.8 us, and not sound: in a process that had run many other products
 // 11 x 2832 x 4077 ended in an illegal access, which range checks on every index of the kernel
-// did not explain. With loads between two barriers of the cluster it has not been seen in 17000
+// did not explain. With loads between two barriers of the cluster it has not been seen in 43000
 // products of random sizes.)
 //
 // Shared memory: a ring of p.stages stages (weight rows, then tokens), barriers. An MMA reads
