@@ -103,6 +103,34 @@ CROSS_ATTN_LAYOUT = struct.Struct("@4P7i12q2PqfPqP")
 assert CROSS_ATTN_LAYOUT.size == ctypes.sizeof(CrossAttnArgs)
 
 
+SRDIT_KV_PLAIN = -1
+
+
+class KvPages(ctypes.Structure):
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("code", c_int),
+                ("dtype", c_int), ("pages", c_int), ("page_size", c_int), ("Hkv", c_int),
+                ("D", c_int), ("k_stride", c_ll * 3), ("v_stride", c_ll * 3),
+                ("ks_stride", c_ll * 3), ("vs_stride", c_ll * 3), ("table", c_vp),
+                ("table_stride", c_ll), ("table_width", c_int), ("B", c_int)]
+
+
+class SeqAttnArgs(ctypes.Structure):
+    _fields_ = [("pages", c_vp), ("q", c_vp), ("k", c_vp), ("v", c_vp), ("out", c_vp),
+                ("dtype", c_int), ("T", c_int), ("Tk", c_int), ("B", c_int), ("H", c_int),
+                ("Hkv", c_int), ("D", c_int), ("q_stride", c_ll * 2), ("k_stride", c_ll * 2),
+                ("v_stride", c_ll * 2), ("o_stride", c_ll * 2), ("cu_q", c_vp), ("cu_k", c_vp),
+                ("kv_lens", c_vp), ("max_q", c_int), ("max_kv", c_int), ("causal", c_int),
+                ("scale", c_float), ("workspace", c_vp), ("workspace_bytes", c_ll),
+                ("status", c_vp)]
+
+
+KV_PAGES_LAYOUT = struct.Struct("@4P6i12qPq2i")
+SEQ_ATTN_LAYOUT = struct.Struct("@5P7i8q3P3ifPqP")
+KV_STRIDES = struct.Struct("@4q")   # {token, head} of k, then of v
+assert KV_PAGES_LAYOUT.size == ctypes.sizeof(KvPages)
+assert SEQ_ATTN_LAYOUT.size == ctypes.sizeof(SeqAttnArgs)
+
+
 # name -> argtypes (every function returns int)
 SIGNATURES = {
     "srdit_version": [],
@@ -152,6 +180,10 @@ SIGNATURES = {
     "srdit_cross_attn": [ctypes.POINTER(CrossAttnArgs), c_vp],
     "srdit_cross_attn_workspace": [ctypes.POINTER(CrossAttnArgs)],
     "srdit_cross_attn_items": [ctypes.POINTER(CrossAttnArgs)],
+    "srdit_kv_write": [ctypes.POINTER(KvPages), c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp],
+    "srdit_kv_read": [ctypes.POINTER(KvPages), c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
+    "srdit_seq_attn": [ctypes.POINTER(SeqAttnArgs), c_vp],
+    "srdit_seq_attn_workspace": [ctypes.POINTER(SeqAttnArgs)],
     "srdit_winattn_plan": [c_vp, c_int, c_int, c_int, ctypes.POINTER(WinattnTiling)],
     "srdit_winattn_fwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int,
                           ctypes.POINTER(WinattnGeom), ctypes.POINTER(WinattnTiling), c_vp,

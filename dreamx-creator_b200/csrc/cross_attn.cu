@@ -23,30 +23,13 @@
 // join_ranges_kernel).
 #include <atomic>
 
-#include "elem.cuh"
+#include "attn.cuh"
 #include "srdit_internal.h"
 
 namespace srdit {
 namespace xattn {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int TILE = 128;
-
-// n / d and n % d for 0 <= n < 2^31 by a product: mul = ceil(2^(31 + l) / d), 2^l >= d
-struct Divisor {
-  uint32_t mul, shift;
-  int d;
-  static Divisor of(int d) {
-    uint32_t l = 0;
-    while ((1ll << l) < d) ++l;
-    const uint64_t two = 1ull << (31 + l);
-    return {static_cast<uint32_t>((two + d - 1) / d), 31 + l, d};
-  }
-  SRDIT_DEV int div(int n) const {
-    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
-  }
-  SRDIT_DEV int mod(int n) const { return n - div(n) * d; }
-};
 
 struct Args {
   const void* q;
@@ -74,23 +57,6 @@ struct Args {
   uint32_t* status;
 };
 
-SRDIT_DEV float neg_inf() { return -__int_as_float(0x7f800000); }
-SRDIT_DEV float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// the larger of two, the largest of three; NaN if one is
-SRDIT_DEV float max2(float x, float y) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
-}
-SRDIT_DEV float max3(float x, float y, float z) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
 SRDIT_DEV int key_count(const Args& a, int b) {
   return a.kv_lens ? min(max(__ldg(a.kv_lens + b), 0), a.Lk) : a.Lk;
 }
@@ -878,33 +844,6 @@ __global__ void __launch_bounds__(256) join_ranges_kernel(const __grid_constant_
 // thread c of a quad holds dims 16c..16c+15 of each 64 (16-byte loads) for both operands;
 // O's rows may be numbered in any order, so lane group g holds value columns 8g..8g+7 of
 // each 64. The weights change from accumulator to operand layout by movmatrix.
-template <typename T>
-SRDIT_DEV void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                        uint32_t b0, uint32_t b1) {
-  if constexpr (__is_same(T, __nv_bfloat16))
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-SRDIT_DEV uint32_t transpose8x8(uint32_t v) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
-  return d;
-}
-SRDIT_DEV uint4 lds16(uint32_t src) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(src));
-  return v;
-}
-
 // A warp alone on its scheduler takes 1300 cycles for a block's 230 instructions, nearly all of
 // it their latency, so an SM gets three CTAs (168 registers; two of 16 rows), and a warp's
 // ring 2 or 3 blocks of 128-wide heads, twice that of 64-wide ones. (Two CTAs with 3 blocks: 4
@@ -1511,9 +1450,9 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.nq = p.nq;
   a.nhp = p.nhp;
   if (!p.token) {
-    a.by_ctas = xattn::Divisor::of(p.ctas);
-    a.by_per = xattn::Divisor::of(p.nq * p.nhp);
-    a.by_nq = xattn::Divisor::of(p.nq);
+    a.by_ctas = Divisor::of(p.ctas);
+    a.by_per = Divisor::of(p.nq * p.nhp);
+    a.by_nq = Divisor::of(p.nq);
   }
   a.splits = p.splits;
   a.ranged = p.ranged;
@@ -1525,7 +1464,7 @@ extern "C" int srdit_cross_attn(const srdit_cross_attn_args* args, cudaStream_t 
   a.kv_lens = u.kv_lens;
   a.mask = u.key_mask;
   a.mask_stride = u.mask_stride;
-  a.c = u.scale * xattn::kLog2e;
+  a.c = u.scale * kLog2e;
   a.ws = static_cast<float*>(u.workspace);
   if (p.token) {
     a.ml = a.ws + static_cast<long long>(p.parts) * u.B * u.Lq * u.H * u.D;

@@ -380,6 +380,192 @@ def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, st
     return out
 
 
+def _int32(t, n, what):
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise _lib.SrditError(f"{what} must be contiguous int32 [{n}]")
+    return t.data_ptr()
+
+
+def _pages(k_pages, v_pages, table, k_scale, v_scale, dtype):
+    """The C view of a cache's pages (``_lib.KvPages``) whose rows go to or from ``dtype``."""
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise _lib.SrditError(f"pages {tuple(k_pages.shape)} {k_pages.dtype}, "
+                              f"{tuple(v_pages.shape)} {v_pages.dtype}: "
+                              "[pages, page_size, kv_heads, D] of one type each")
+    n, size, Hkv, D = k_pages.shape
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise _lib.SrditError(f"pages need unit stride over D, have {ks}, {vs}")
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1
+                                                          and table.stride(1) != 1):
+        raise _lib.SrditError("the page table must be int32 [sequences, pages] with unit stride")
+    dt = _code(HALF_TYPES, dtype, "rows of a cache")
+    if k_pages.dtype == dtype:
+        code = _lib.SRDIT_KV_PLAIN
+        if k_scale is not None or v_scale is not None:
+            raise _lib.SrditError(f"scales for pages of {dtype}")
+        scales, ss = (0, 0), (0, 0, 0, 0, 0, 0)
+    else:
+        code = _code(CODES, k_pages.dtype, f"pages for rows of {dtype}, other than that type,")
+        if k_scale is None or v_scale is None:
+            raise _lib.SrditError(f"pages of {k_pages.dtype} need k_scale and v_scale")
+        for t in (k_scale, v_scale):
+            if t.dtype != torch.float32 or t.shape != (n, size, Hkv):
+                raise _lib.SrditError(f"scales must be float32 {(n, size, Hkv)}")
+        scales = (k_scale.data_ptr(), v_scale.data_ptr())
+        ss = (*k_scale.stride(), *v_scale.stride())
+    p = _lib.KvPages()
+    _lib.KV_PAGES_LAYOUT.pack_into(
+        p, 0, k_pages.data_ptr(), v_pages.data_ptr(), *scales, code, dt, n, size, Hkv, D,
+        *ks[:3], *vs[:3], *ss, table.data_ptr(), table.stride(0), table.shape[1], table.shape[0])
+    return p
+
+
+def _kv_rows(k, v, Hkv, D):
+    """The strides {token, head} of packed k, v [T, Hkv, D] as the C entries take them."""
+    if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (Hkv, D) or k.dtype != v.dtype:
+        raise _lib.SrditError(f"k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}: "
+                              f"[tokens, {Hkv}, {D}] of one type each")
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or vs[2] != 1:
+        raise _lib.SrditError(f"k, v need unit stride over D, have {ks}, {vs}")
+    st = ctypes.create_string_buffer(32)
+    _lib.KV_STRIDES.pack_into(st, 0, ks[0], ks[1], vs[0], vs[1])
+    return st, ctypes.addressof(st)
+
+
+def kv_write(k, v, k_pages, v_pages, page_table, kv_lens, *, cu_q=None, k_scale=None,
+             v_scale=None):
+    """Write new tokens' k, v [T, Hkv, D] (bf16 or fp16) into a cache's pages.
+
+    k_pages, v_pages [pages, page_size, Hkv, D]: of k's type, or int8 / float8_e4m3fn codes with
+    float32 scales [pages, page_size, Hkv] (any strides). ``page_table`` int32 [B, width]: token
+    p of sequence b lies in row p % page_size of page ``page_table[b, p // page_size]``.
+    ``cu_q`` (int32 [B + 1]): sequence b's new tokens are the rows cu_q[b] to cu_q[b + 1] of k
+    and v (default: T / B each); ``kv_lens`` (int32 [B]): its length with them. D a multiple of
+    8 (16 for codes) up to 128, page_size 16, 32, 64 or a multiple of 128. A token whose page
+    the table does not have is left out."""
+    stream = _same_device(k, v, k_pages, v_pages, page_table, kv_lens, cu_q, k_scale, v_scale)
+    p = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
+    B, (_, _, Hkv, D) = page_table.shape[0], k_pages.shape
+    st, at = _kv_rows(k, v, Hkv, D)
+    T = k.shape[0]
+    _launch("srdit_kv_write", ctypes.byref(p), k.data_ptr(), at, v.data_ptr(), at + 16, T,
+            None if cu_q is None else _int32(cu_q, B + 1, "cu_q"), _int32(kv_lens, B, "kv_lens"),
+            stream, kind="kv_write", work=2 * T * Hkv * D * (2 + k_pages.element_size()))
+
+
+def kv_read(k_pages, v_pages, page_table, cu_k, k=None, v=None, *, total=None, dtype=None,
+            k_scale=None, v_scale=None):
+    """Read the first tokens of every sequence back: (k, v) [T, Hkv, D], sequence b's in the rows
+    cu_k[b] to cu_k[b + 1] (int32 [B + 1]), codes times their scales. Without ``k`` and ``v``
+    they are made, of ``total`` rows and ``dtype`` (bf16, or the pages' own). Rows behind the
+    last sequence are left as they were; tokens without a page are zeros."""
+    if k is None:
+        if total is None or v is not None:
+            raise _lib.SrditError("kv_read needs k and v, or total")
+        dtype = dtype or (k_pages.dtype if k_pages.dtype in HALF_TYPES else torch.bfloat16)
+        k, v = (torch.empty(total, *k_pages.shape[2:], dtype=dtype, device=k_pages.device)
+                for _ in range(2))
+    elif v is None or (dtype is not None and k.dtype != dtype) or (
+            total is not None and k.shape[0] != total):
+        raise _lib.SrditError("k and v do not go with total and dtype")
+    stream = _same_device(k, v, k_pages, v_pages, page_table, cu_k, k_scale, v_scale)
+    p = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
+    _, _, Hkv, D = k_pages.shape
+    st, at = _kv_rows(k, v, Hkv, D)
+    T = k.shape[0]
+    _launch("srdit_kv_read", ctypes.byref(p), k.data_ptr(), at, v.data_ptr(), at + 16, T,
+            _int32(cu_k, page_table.shape[0] + 1, "cu_k"), stream, kind="kv_read",
+            work=2 * T * Hkv * D * (2 + k_pages.element_size()))
+    return k, v
+
+
+def _seq_attn(kind, q, out, Hkv, B, pages, k, v, Tk, kv_strides, cu_q, cu_k, kv_lens, max_q,
+              max_kv, causal, scale, status, stream):
+    T, H, D = q.shape
+    dt = _code(HALF_TYPES, q.dtype, kind)
+    if Hkv == 0 or H % Hkv:
+        raise _lib.SrditError(f"{H} heads over {Hkv} key heads")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise _lib.SrditError(f"out must be {q.dtype} {tuple(q.shape)}")
+    qs, os = q.stride(), out.stride()
+    if qs[2] != 1 or os[2] != 1:
+        raise _lib.SrditError(f"q, out need unit stride over D, have {qs}, {os}")
+    a = _lib.SeqAttnArgs()
+    fill = _lib.SEQ_ATTN_LAYOUT.pack_into
+    fields = (ctypes.addressof(pages) if pages is not None else 0, q.data_ptr(), k, v,
+              out.data_ptr(), dt, T, Tk, B, H, Hkv, D, *qs[:2], *kv_strides, *os[:2], cu_q, cu_k,
+              kv_lens, int(max_q), int(max_kv), bool(causal), D ** -0.5 if scale is None else scale)
+    st = 0 if status is None else status.data_ptr()
+    fill(a, 0, *fields, 0, 0, st)
+    ref = ctypes.byref(a)
+    kib = _lib.count("srdit_seq_attn_workspace", ref)
+    if kib:
+        ws = torch.empty(kib << 10, dtype=torch.uint8, device=q.device)
+        fill(a, 0, *fields, ws.data_ptr(), kib << 10, st)
+    _launch("srdit_seq_attn", ref, stream, kind=kind, work=4 * T * H * D * (max_kv or Tk))
+    if kib:
+        Stats.launches += 1   # a second kernel joins the parts
+    return out
+
+
+def paged_attn(q, k_pages, v_pages, page_table, kv_lens, out=None, *, cu_q=None, max_q=None,
+               max_kv=None, causal=True, k_scale=None, v_scale=None, scale=None, status=None):
+    """Attention of new tokens' q [T, H, D] over their sequences' cached tokens, which
+    ``kv_write`` has put there, the new ones included. Returns out [T, H, D].
+
+    Pages, table, ``kv_lens`` and ``cu_q`` as in ``kv_write``; H a multiple of the pages' heads.
+    Sequence b's n new tokens are its last ones: with ``causal`` each sees the tokens up to its
+    own, else all kv_lens[b] of them. One that sees none gets zeros; rows of out behind the last
+    sequence are left as they were. ``max_q``: no sequence has more new tokens (default: T / B
+    without ``cu_q``, else T; steps of one token each say 1); ``max_kv``: about the longest
+    sequence (default: what the table holds), by which work is split. ``scale``: D ** -0.5."""
+    stream = _same_device(q, k_pages, v_pages, page_table, kv_lens, out, cu_q, k_scale, v_scale,
+                          status)
+    if q.dim() != 3 or k_pages.dim() != 4 or q.shape[2] != k_pages.shape[3]:
+        raise _lib.SrditError(f"q {tuple(q.shape)} [tokens, heads, D] does not go with pages "
+                              f"{tuple(k_pages.shape)}")
+    p = _pages(k_pages, v_pages, page_table, k_scale, v_scale, q.dtype)
+    B = page_table.shape[0]
+    if max_q is None:
+        max_q = q.shape[0] if cu_q is not None or B == 0 else q.shape[0] // B
+    return _seq_attn("paged_attn", q, out, k_pages.shape[2], B, p, 0, 0, 0, (0, 0, 0, 0),
+                     0 if cu_q is None else _int32(cu_q, B + 1, "cu_q"), 0,
+                     _int32(kv_lens, B, "kv_lens"), max_q,
+                     page_table.shape[1] * k_pages.shape[1] if max_kv is None else max_kv,
+                     causal, scale, status, stream)
+
+
+def packed_attn(q, k, v, cu_q, out=None, *, cu_k=None, causal=True, scale=None, status=None):
+    """Attention of whole packed sequences: q [T, H, D] (bf16 or fp16) over k, v [Tk, Hkv, D],
+    sequence b's rows being cu_q[b] to cu_q[b + 1] of q (int32 [B + 1] on the device) and, with
+    ``cu_k``, cu_k[b] to cu_k[b + 1] of k and v (default: cu_q). Returns out [T, H, D].
+
+    With ``causal`` a sequence's queries are its last tokens: query i of n sees the keys up to
+    L - n + i of its L. Views whose strides are multiples of 8 are read in place (k and v of one
+    projection side by side). A query that sees no key gets zeros; rows of out behind the last
+    sequence are left as they were. ``scale``: D ** -0.5."""
+    stream = _same_device(q, k, v, cu_q, out, cu_k, status)
+    if q.dim() != 3 or k.dim() != 3 or q.shape[2] != k.shape[2] or k.dtype != q.dtype:
+        raise _lib.SrditError(f"q {tuple(q.shape)} {q.dtype} [tokens, heads, D] does not go with k "
+                              f"{tuple(k.shape)} {k.dtype}")
+    Tk, Hkv, D = k.shape
+    ks, vs = k.stride(), v.stride()
+    if v.shape != k.shape or v.dtype != k.dtype or ks[2] != 1 or vs[2] != 1:
+        raise _lib.SrditError(f"k {tuple(k.shape)} {ks}, v {tuple(v.shape)} {vs}: one shape and "
+                              "type, unit stride over D")
+    B = cu_q.numel() - 1
+    if B < 0 or (cu_k is None and Tk != q.shape[0]):
+        raise _lib.SrditError(f"{B} sequences; without cu_k k and v have q's {q.shape[0]} rows")
+    return _seq_attn("packed_attn", q, out, Hkv, B, None, k.data_ptr(), v.data_ptr(), Tk,
+                     (*ks[:2], *vs[:2]), _int32(cu_q, B + 1, "cu_q"),
+                     0 if cu_k is None else _int32(cu_k, B + 1, "cu_k"), 0, 0, 0, causal, scale,
+                     status, stream)
+
+
 def row_reduce(x, op, out=None):
     """Per-row sum of squares (op "sumsq") or max |x| (op "absmax") of a bf16 [M, K]."""
     _need_cuda(x, out)

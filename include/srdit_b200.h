@@ -639,6 +639,95 @@ int srdit_cross_attn_workspace(const srdit_cross_attn_args* args);
  * through, or 0 for few rows (a ring of keys per warp) and where nothing is to do. */
 int srdit_cross_attn_items(const srdit_cross_attn_args* args);
 
+/*
+ * A key/value cache in pages, and the sequences that it holds: token p of sequence b lies in row
+ * p % page_size of page table[b * table_stride + p / page_size]. k, v [pages, page_size, Hkv, D]
+ * with strides {page, token, head} in elements and unit stride over D: of type dtype (SRDIT_BF16
+ * / FP16; code SRDIT_KV_PLAIN), or 8-bit codes (SRDIT_Q_INT8 / E4M3) with fp32 scales k_scale,
+ * v_scale [pages, page_size, Hkv], strides ks_stride, vs_stride. Bases and strides of k and v in
+ * units of 16 bytes. D a multiple of 8 (16 for codes), at most 128; page_size 16, 32, 64 or a
+ * multiple of 128; Hkv at most 1024. The table (int32, on the device) may hold anything where a
+ * sequence has no page yet. A page out of [0, pages) is none: nothing is written to it, it reads
+ * as zeros, and its keys are not seen.
+ */
+#define SRDIT_KV_PLAIN (-1)
+typedef struct srdit_kv_pages {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int code, dtype;
+  int pages, page_size, Hkv, D;
+  long long k_stride[3], v_stride[3], ks_stride[3], vs_stride[3];
+  const int32_t* table;
+  long long table_stride;
+  int table_width, B;
+} srdit_kv_pages;
+
+/*
+ * Write the keys and values of new tokens into their pages. k, v [T, Hkv, D] of the pages' dtype
+ * with strides {token, head} (multiples of 8; 16-byte bases): sequence b's n are the rows
+ * [cu_q[b], cu_q[b+1]) (optional int32 [B+1] on the device; NULL: T / B each), and they are its
+ * tokens kv_lens[b] - n to kv_lens[b] - 1 (int32 [B] on the device: its length with them; tokens
+ * before 0 are left out). As codes, per token and head:
+ *   scale = max(max_d |x_d| * (1/Q), 1e-12), Q = 127 or 448;  code = round(x * (1/scale))
+ * each operation rounded to fp32, ties to even: every caller that computes so gets the same
+ * codes. NaN and infinities as with srdit_quant_rows. No token may be written twice in a call.
+ * Replaces: the cache's append (video_refiner/wan/modules/sr_dit/attention.py:964-974), for
+ *   caches in pages.
+ */
+int srdit_kv_write(const srdit_kv_pages* pages, const void* k, const long long* k_stride,
+                   const void* v, const long long* v_stride, int T, const int32_t* cu_q,
+                   const int32_t* kv_lens, cudaStream_t stream);
+/*
+ * Read the first tokens of every sequence back into packed rows: k, v [T, Hkv, D] of the pages'
+ * dtype, sequence b's tokens 0, 1, ... in the rows [cu_k[b], cu_k[b+1]) (NULL: T / B each), codes
+ * times their scales in fp32, rounded once. Rows behind the last sequence are left as they were.
+ */
+int srdit_kv_read(const srdit_kv_pages* pages, void* k, const long long* k_stride, void* v,
+                  const long long* v_stride, int T, const int32_t* cu_k, cudaStream_t stream);
+
+/*
+ * Attention of packed sequences:
+ *   o[i,h] = sum_j p_j v[j,g] / sum_j p_j,  p_j = exp(scale * q[i,h].k[j,g] - max),
+ *   g = h / (H / Hkv)
+ * q, out [T, H, D] of type dtype (SRDIT_BF16 / FP16), strides {token, head}: sequence b's n
+ * queries are the rows [cu_q[b], cu_q[b+1]) (optional int32 [B+1] on the device; NULL: T / B
+ * each). Its L keys are either
+ *   pages != NULL: its first kv_lens[b] tokens of the cache (int32 [B] on the device; of the
+ *     pages' dtype, or codes; the queries' own tokens are written before), or
+ *   pages == NULL: the rows [cu_k[b], cu_k[b+1]) (NULL: cu_q's) of k, v [Tk, Hkv, D].
+ * causal: the queries are its last n tokens, query i sees the keys j <= L - n + i; else all. A
+ * query that sees no key gets 0; rows behind the last sequence are left as they were. What lies
+ * behind a sequence's length does not matter, NaN included; the value of a key that some queries
+ * of the sequence see and a causal mask hides from others has to be finite for those.
+ * max_q: no sequence has more queries (0: T; a sequence's further rows may be left as they were);
+ * max_kv (pages): about the longest sequence (0: what the table holds), which the work's split goes by and no result.
+ * Views as in srdit_cross_attn (bases 16-byte aligned, strides multiples of 8). scale > 0.
+ * workspace: where srdit_seq_attn_workspace (which reads the arguments, not the tensors) returns
+ * n > 0, n KiB, 16-byte aligned. T * H at most 2^26, B * Hkv at most 65535.
+ * Replaces: flash_attention over packed sequences (attention.py:61-168), with a cache in pages.
+ */
+typedef struct srdit_seq_attn_args {
+  const srdit_kv_pages* pages;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int dtype, T, Tk, B, H, Hkv, D;
+  long long q_stride[2], k_stride[2], v_stride[2], o_stride[2];
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* kv_lens;
+  int max_q, max_kv, causal;
+  float scale;
+  void* workspace;
+  long long workspace_bytes;
+  uint32_t* status;
+} srdit_seq_attn_args;
+int srdit_seq_attn(const srdit_seq_attn_args* args, cudaStream_t stream);
+int srdit_seq_attn_workspace(const srdit_seq_attn_args* args);
+
 #ifdef __cplusplus
 }
 #endif

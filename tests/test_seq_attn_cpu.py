@@ -1,0 +1,156 @@
+"""The paged cache's and the packed attention's C entries without a GPU: their structures, what
+they refuse, and that there is no CPU path."""
+import ctypes
+import re
+
+import pytest
+import torch
+
+EINVAL, EALIGN, EUNSUPPORTED = -1, -2, -3
+
+
+@pytest.mark.parametrize("name,cls,layout", [
+    ("srdit_kv_pages", "KvPages", "KV_PAGES_LAYOUT"),
+    ("srdit_seq_attn_args", "SeqAttnArgs", "SEQ_ATTN_LAYOUT")])
+def test_structs_match_the_header(srdit, name, cls, layout):
+    lib = srdit._lib
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), lib.HEADER.read_text(),
+                     re.S).group(1)
+    names = re.findall(r"(\w+)(?:\[\d\])?\s*[,;]", body)
+    fields = getattr(lib, cls)._fields_
+    assert names == [f[0] for f in fields]
+    # the packed layout puts the n-th value into the n-th field
+    a, st = getattr(lib, cls)(), getattr(lib, layout)
+    width = [f[1]._length_ if hasattr(f[1], "_length_") else 1 for f in fields]
+    st.pack_into(a, 0, *range(1, sum(width) + 1))
+    at = 1
+    for (f, _), w in zip(fields, width):
+        got = getattr(a, f)
+        assert (list(got) if w > 1 else got) == (list(range(at, at + w)) if w > 1 else at), f
+        at += w
+
+
+def _pages(lib, **kw):
+    v = dict(k=1 << 20, v=2 << 20, k_scale=3 << 20, v_scale=4 << 20, code=0, dtype=0, pages=9,
+             page_size=16, Hkv=2, D=64, k_stride=(2048, 128, 64), v_stride=(2048, 128, 64),
+             ks_stride=(32, 2, 1), vs_stride=(32, 1, 16), table=5 << 20, table_stride=4,
+             table_width=4, B=3)
+    v.update(kw)
+    return _fill(lib.KvPages(), v)
+
+
+def _fill(a, v):
+    for name, x in v.items():
+        if isinstance(x, tuple):
+            getattr(a, name)[:] = x
+        else:
+            setattr(a, name, x)
+    return a
+
+
+PAGES = [
+    (dict(B=-1), EINVAL), (dict(pages=-1), EINVAL), (dict(Hkv=0), EINVAL), (dict(D=0), EINVAL),
+    (dict(page_size=0), EINVAL), (dict(table_width=-1), EINVAL), (dict(dtype=2), EINVAL),
+    (dict(code=2), EINVAL), (dict(k=None), EINVAL), (dict(v_scale=None), EINVAL),
+    (dict(table=None), EINVAL), (dict(D=136), EUNSUPPORTED), (dict(D=72), EUNSUPPORTED),
+    (dict(code=-1, D=60), EUNSUPPORTED), (dict(page_size=8), EUNSUPPORTED),
+    (dict(page_size=48), EUNSUPPORTED), (dict(page_size=192), EUNSUPPORTED),
+    (dict(Hkv=1025), EUNSUPPORTED), (dict(table_width=1 << 28), EUNSUPPORTED),
+    (dict(k=(1 << 20) + 8), EALIGN), (dict(v_stride=(2048, 120, 64)), EALIGN),
+    (dict(table=(5 << 20) + 2), EALIGN), (dict(k_scale=(3 << 20) + 2), EALIGN),
+    (dict(k_stride=(2048, 0, 64)), EINVAL), (dict(v_stride=(-2048, 128, 64)), EINVAL),
+    (dict(ks_stride=(32, 2, 0)), EINVAL)]
+
+
+def _rows_call(lib, write, pages=None, **kw):
+    v = dict(k=6 << 20, k_stride=(128, 64), v=7 << 20, v_stride=(128, 64), T=5, cu=8 << 20,
+             lens=9 << 20)
+    v.update(kw)
+    p = _pages(lib, **(pages or {}))
+    st = [(ctypes.c_longlong * 2)(*v[x]) if v[x] else None for x in ("k_stride", "v_stride")]
+    args = [ctypes.byref(p), v["k"], st[0], v["v"], st[1], v["T"], v["cu"]]
+    if write:
+        return lib.lib().srdit_kv_write(*args, v["lens"], None)
+    return lib.lib().srdit_kv_read(*args, None)
+
+
+@pytest.mark.parametrize("write", (True, False))
+@pytest.mark.parametrize("pages,rc", PAGES)
+def test_page_refusals(srdit, write, pages, rc):
+    assert _rows_call(srdit._lib, write, pages) == rc
+
+
+@pytest.mark.parametrize("write", (True, False))
+@pytest.mark.parametrize("kw,rc", [
+    (dict(T=0), 0), (dict(T=-1), EINVAL), (dict(k=None), EINVAL), (dict(v=None), EINVAL),
+    (dict(k_stride=None), EINVAL), (dict(cu=None), EINVAL), (dict(k=(6 << 20) + 8), EALIGN),
+    (dict(v_stride=(128, 60)), EALIGN), (dict(cu=2), EALIGN)])
+def test_row_refusals(srdit, write, kw, rc):
+    assert _rows_call(srdit._lib, write, **kw) == rc
+
+
+def test_read_and_write_differ(srdit):
+    lib = srdit._lib
+    assert _rows_call(lib, True, lens=None) == EINVAL
+    assert _rows_call(lib, True, lens=3) == EALIGN
+    assert _rows_call(lib, False, k_stride=(0, 64)) == EINVAL   # two tokens in one place
+    assert _rows_call(lib, True, pages=dict(B=0)) == 0
+    assert lib.lib().srdit_kv_write(None, *[None] * 4, 5, None, None, None) == EINVAL
+
+
+def _attn(lib, pages=None, workspace=False, **kw):
+    v = dict(q=10 << 20, k=11 << 20, v=12 << 20, out=13 << 20, dtype=0, T=6, Tk=6, B=3, H=4, Hkv=2,
+             D=64, q_stride=(256, 64), k_stride=(128, 64), v_stride=(128, 64), o_stride=(256, 64),
+             cu_q=14 << 20, kv_lens=15 << 20, max_q=2, scale=0.125)
+    v.update(kw)
+    a = _fill(lib.SeqAttnArgs(), v)
+    if pages is not None:
+        p = _pages(lib, **pages)
+        a.pages = ctypes.addressof(p)
+    if workspace:
+        return lib.lib().srdit_seq_attn_workspace(ctypes.byref(a))
+    return lib.lib().srdit_seq_attn(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("pages", (None, {}))
+@pytest.mark.parametrize("kw,rc", [
+    (dict(T=0), 0), (dict(H=0), 0), (dict(T=-1), EINVAL), (dict(Hkv=0), EINVAL),
+    (dict(H=3), EINVAL), (dict(dtype=2), EINVAL), (dict(max_q=-1), EINVAL),
+    (dict(max_kv=-1), EINVAL), (dict(q=None), EINVAL), (dict(out=None), EINVAL),
+    (dict(scale=0.0), EINVAL), (dict(scale=float("nan")), EINVAL), (dict(scale=float("inf")), EINVAL),
+    (dict(cu_q=None, T=7), EINVAL), (dict(q=(10 << 20) + 8), EALIGN), (dict(cu_q=2), EALIGN),
+    (dict(q_stride=(256, 60)), EALIGN), (dict(o_stride=(256, 0)), EINVAL),
+    (dict(q_stride=(0, 64)), EINVAL), (dict(q_stride=(-256, 64)), EALIGN),
+    (dict(T=1 << 25), EUNSUPPORTED)])
+def test_attention_refusals(srdit, pages, kw, rc):
+    assert _attn(srdit._lib, pages, **kw) == rc
+    assert _attn(srdit._lib, pages, workspace=True, **kw) == 0
+
+
+@pytest.mark.parametrize("pages,rc", PAGES)
+def test_attention_page_refusals(srdit, pages, rc):
+    assert _attn(srdit._lib, pages) == rc
+
+
+@pytest.mark.parametrize("pages,kw,rc", [
+    (dict(Hkv=1), {}, EINVAL), (dict(B=2), {}, EINVAL), (dict(D=32), {}, EINVAL),
+    (dict(dtype=1), {}, EINVAL), ({}, dict(kv_lens=None), EINVAL), ({}, dict(kv_lens=2), EALIGN),
+    (None, dict(k=None), EINVAL), (None, dict(v=None), EINVAL), (None, dict(Tk=-1), EINVAL),
+    (None, dict(D=60), EUNSUPPORTED), (None, dict(D=136), EUNSUPPORTED),
+    (None, dict(k_stride=(128, 60)), EALIGN), (None, dict(v_stride=(0, 64)), EINVAL),
+    (None, dict(cu_k=2), EALIGN), (None, dict(cu_q=None, Tk=7), EINVAL)])
+def test_attention_key_refusals(srdit, pages, kw, rc):
+    assert _attn(srdit._lib, pages, **kw) == rc
+
+
+def test_no_cpu_path(srdit):
+    err, ops = srdit._lib.SrditError, srdit.ops
+    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    pool = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
+    i = torch.zeros(2, 1, dtype=torch.int32)
+    for call in (lambda: ops.kv_write(x, x, pool, pool, i, i[:, 0]),
+                 lambda: ops.kv_read(pool, pool, i, i[:, 0], total=2),
+                 lambda: ops.paged_attn(x, pool, pool, i, i[:, 0]),
+                 lambda: ops.packed_attn(x, x, x, i[:, 0])):
+        with pytest.raises(err):
+            call()
