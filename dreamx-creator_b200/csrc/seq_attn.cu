@@ -6,113 +6,25 @@
 // over the L keys of the query's sequence, or with a causal mask over those up to its own
 // token, j <= L - n + i for query i of n; g = h / (H / Hkv). A row that sees no key is 0.
 // The softmax is one pass over the keys with a running maximum m and sum l, in fp32 and base
-// 2: p = 2^(s c - m) with c = scale log2(e).
-#include <atomic>
-
-#include "seq.cuh"
+// 2: p = 2^(s c - m) with c = scale log2(e). seq_step.cu has the kernel of few rows,
+// seq_chunk.cu that of many; this file checks the arguments.
+#include "seq_attn.cuh"
 
 namespace srdit {
 namespace sattn {
 
-struct Args {
-  const void* q;
-  void* out;
-  long long qs[2], os[2];
-  const void* kv[2];
-  long long ps[2][3], ss[2][3];  // strides {page, token, head}; packed keys are one page
-  const float* scale[2];
-  Table table;
-  Offsets rows, keys;
-  Divisor by_each;
-  const int32_t* lens;
-  int B, H, Hkv, D, group, paged, causal;
-  float c;
-};
-
-// The simplest form: a warp per query row, a lane four of its values, key after key.
-template <typename T, int CODE>
-__global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ Args a) {
-  pdl_begin();
-  const int lane = threadIdx.x & 31, col = lane * 4;
-  const long long task = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int t = static_cast<int>(task / a.H), h = static_cast<int>(task % a.H);
-  if (t >= a.rows.rows) return;
-  const int b = find_sequence(a.rows, a.B, t, a.by_each);
-  if (b >= a.B) return;
-  const bool on = col < a.D;
-  const int len = a.paged ? a.table.clamp_len(__ldg(a.lens + b)) : a.keys.end(b) - a.keys.begin(b);
-  const int last = a.causal ? min(len, len - (a.rows.end(b) - t) + 1) : len;
-  auto four = [&](const void* p, long long at, float (&f)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[e] = 0.f;
-      if (!on) continue;
-      if constexpr (CODE == SRDIT_KV_PLAIN) {
-        f[e] = to_f(static_cast<const T*>(p)[at + e]);
-      } else if constexpr (CODE == SRDIT_Q_INT8) {
-        f[e] = static_cast<const int8_t*>(p)[at + e];
-      } else {
-        uint32_t h2;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
-            : "=r"(h2)
-            : "h"(static_cast<uint16_t>(static_cast<const uint8_t*>(p)[at + e])));
-        f[e] = __low2float(*reinterpret_cast<const __half2*>(&h2));
-      }
-    }
-  };
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = neg_inf(), l = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    q[e] = on ? to_f(static_cast<const T*>(a.q)[t * a.qs[0] + h * a.qs[1] + col + e]) : 0.f;
-  for (int j = 0; j < last; ++j) {
-    long long page = 0, row = a.keys.begin(b) + j;
-    if (a.paged) {
-      const int n = a.table.by_page.div(j);
-      page = a.table.page(b, n);
-      if (page < 0) continue;
-      row = j - n * a.table.page_size;
-    }
-    const int g = h / a.group;
-    float k[4], v[4], s = 0.f;
-    four(a.kv[0], page * a.ps[0][0] + row * a.ps[0][1] + g * a.ps[0][2] + col, k);
-    four(a.kv[1], page * a.ps[1][0] + row * a.ps[1][1] + g * a.ps[1][2] + col, v);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(q[e], k[e], s);
-#pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    float f = 1.f;
-    if constexpr (CODE != SRDIT_KV_PLAIN) {
-      s *= a.scale[0][page * a.ss[0][0] + row * a.ss[0][1] + g * a.ss[0][2]];
-      f = a.scale[1][page * a.ss[1][0] + row * a.ss[1][1] + g * a.ss[1][2]];
-    }
-    s *= a.c;
-    const float mn = max2(m, s), neg = mn == neg_inf() ? 0.f : -mn;
-    const float alpha = ex2(m + neg), p = ex2(s + neg);
-    m = mn;
-    l = fmaf(l, alpha, p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(p * f, v[e], o[e] * alpha);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (on)
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + t * a.os[0] + h * a.os[1] + col) =
-        make_uint2(pack2(o[0] * inv, o[1] * inv, T{}), pack2(o[2] * inv, o[3] * inv, T{}));
+// Up to 16 query rows per key head over pages go to step_kernel, which streams the cache.
+static Plan make_plan(const srdit_seq_attn_args& u, int max_q, int sms) {
+  if (u.pages && static_cast<long long>(max_q) * (u.H / u.Hkv) <= 16) return plan_step(u, sms);
+  return plan_chunk(u, sms);
 }
 
-template <typename T, int CODE>
-static int run(const Args& a, cudaStream_t stream) {
-  const long long tasks = static_cast<long long>(a.rows.rows) * a.H;
-  SRDIT_LAUNCH((row_kernel<T, CODE>), static_cast<unsigned>((tasks + 7) / 8), 256, 0, stream, a);
-  return static_cast<int>(cudaGetLastError());
-}
-
-template <typename T>
-static int run_code(const Args& a, int code, cudaStream_t stream) {
-  switch (code) {
-    case SRDIT_Q_INT8: return run<T, SRDIT_Q_INT8>(a, stream);
-    case SRDIT_Q_E4M3: return run<T, SRDIT_Q_E4M3>(a, stream);
-    default: return run<T, SRDIT_KV_PLAIN>(a, stream);
-  }
+// the arguments with max_q as it is used: 0 is all rows
+static srdit_seq_attn_args with_max_q(const srdit_seq_attn_args& u) {
+  srdit_seq_attn_args v = u;
+  const int most = u.cu_q ? u.T : u.T / u.B;
+  if (v.max_q == 0 || v.max_q > most) v.max_q = most;
+  return v;
 }
 
 // 16-byte rows: base and the strides that are used; entries of an output are one place each
@@ -169,41 +81,34 @@ using namespace srdit;
 
 extern "C" int srdit_seq_attn_workspace(const srdit_seq_attn_args* args) {
   if (!args || sattn::check(*args) != 0) return 0;
-  return 0;
+  const srdit_seq_attn_args u = sattn::with_max_q(*args);
+  const sattn::Plan p = sattn::make_plan(u, u.max_q, num_sms(device_here()));
+  return static_cast<int>((p.ws_floats + 255) / 256);
 }
 
 extern "C" int srdit_seq_attn(const srdit_seq_attn_args* args, cudaStream_t stream) {
   if (!args) return SRDIT_EINVAL;
-  const srdit_seq_attn_args& u = *args;
-  const int rc = sattn::check(u);
+  const int rc = sattn::check(*args);
   if (rc) return rc < 0 ? rc : 0;
+  const srdit_seq_attn_args u = sattn::with_max_q(*args);
+  const sattn::Plan p = sattn::make_plan(u, u.max_q, num_sms(device_here()));
+  if (p.ws_floats > 0) {
+    if (!u.workspace || u.workspace_bytes < 4 * p.ws_floats) return SRDIT_EINVAL;
+    if (reinterpret_cast<uintptr_t>(u.workspace) & 15u) return SRDIT_EALIGN;
+  }
   sattn::Args a = {};
   a.q = u.q;
   a.out = u.out;
-  a.paged = u.pages != nullptr;
-  const long long* const st[2] = {u.k_stride, u.v_stride};
   if (u.pages) {
-    const srdit_kv_pages& p = *u.pages;
-    a.table = table_of(p);
-    const void* const kv[2] = {p.k, p.v};
-    const long long* const ps[2] = {p.k_stride, p.v_stride};
-    const long long* const ss[2] = {p.ks_stride, p.vs_stride};
-    const float* const scale[2] = {p.k_scale, p.v_scale};
-    for (int i = 0; i < 2; ++i) {
-      a.kv[i] = kv[i];
-      a.scale[i] = scale[i];
-      for (int d = 0; d < 3; ++d) {
-        a.ps[i][d] = ps[i][d];
-        a.ss[i][d] = ss[i][d];
-      }
+    const srdit_kv_pages& c = *u.pages;
+    a.table = table_of(c);
+    a.scale[0] = c.k_scale;
+    a.scale[1] = c.v_scale;
+    for (int d = 0; d < 3; ++d) {
+      a.ss[0][d] = c.ks_stride[d];
+      a.ss[1][d] = c.vs_stride[d];
     }
   } else {
-    a.kv[0] = u.k;
-    a.kv[1] = u.v;
-    for (int i = 0; i < 2; ++i) {
-      a.ps[i][1] = st[i][0];
-      a.ps[i][2] = st[i][1];
-    }
     a.keys = {u.cu_k ? u.cu_k : u.cu_q, u.Tk, u.Tk / u.B};
   }
   for (int i = 0; i < 2; ++i) {
@@ -213,14 +118,16 @@ extern "C" int srdit_seq_attn(const srdit_seq_attn_args* args, cudaStream_t stre
   a.rows = {u.cu_q, u.T, u.T / u.B};
   a.by_each = Divisor::of(u.cu_q ? 1 : u.T / u.B);
   a.lens = u.kv_lens;
+  a.T = u.T;
   a.B = u.B;
   a.H = u.H;
   a.Hkv = u.Hkv;
   a.D = u.D;
   a.group = u.H / u.Hkv;
   a.causal = u.causal;
+  a.max_q = u.max_q;
   a.c = u.scale * kLog2e;
-  const int code = u.pages ? u.pages->code : SRDIT_KV_PLAIN;
-  return u.dtype == SRDIT_BF16 ? sattn::run_code<__nv_bfloat16>(a, code, stream)
-                               : sattn::run_code<__half>(a, code, stream);
+  a.ws = static_cast<float*>(u.workspace);
+  a.status = u.status;
+  return p.step ? sattn::run_step(u, a, p, stream) : sattn::run_chunk(u, a, p, stream);
 }

@@ -1,0 +1,1116 @@
+// seq_chunk.cu -- attention of many query rows per key head: whole prompts, and chunks of new
+// tokens over the pages of a cache. Bounded by the tensor cores and the exponentials.
+//
+// A work item is up to 2 rt tokens of one sequence with `pack` heads of one group side by side,
+// as two query tiles of 128 rows that share every key tile; while one is in its softmax the other
+// has the tensor core. A causal item ends at the key tile of its last token, each query tile at
+// its own.
+//
+// Warps: 0 loads keys, values and queries by TMA, 1 issues the products, 2 finds the CTA's items
+// and passes them on as records, 3 (16-bit keys) looks over the values of tiles that are partly
+// hidden, 4 to 7 and 8 to 11 are the softmax of one query tile each, a row a thread, and with codes
+// 12 to 15 widen them: codes come through a ring of their own and go to the tensor core as fp16,
+// which holds them exactly, and so do the queries. A key's scale then multiplies its scores, a
+// value's its weights, both in fp32. The running maximum is that of score + log2(largest scale of
+// the tile's values), so that weight times scale stays at 2^8 or below.
+#include <atomic>
+
+#include "seq_attn.cuh"
+
+namespace srdit {
+namespace sattn {
+
+constexpr int ROWS = 2 * TILE;    // of an item
+constexpr int MAX_SLOTS = 256;    // pieces of sequences of a ranged launch
+constexpr int MIN_SHARE = 4;      // key tiles that a ranged CTA takes at least
+constexpr int RECORDS = 4;
+
+template <int DP, int CODE>
+struct ChunkCfg {
+  static constexpr bool CODES = CODE != SRDIT_KV_PLAIN;
+  static constexpr int THREADS = CODES ? 512 : 384;
+  static constexpr int SLAB = TILE * 128;  // 128 rows x 64 values
+  static constexpr int BYTES = SLAB * (DP / 64);
+  static constexpr int STAGES = CODES ? (DP == 128 ? 3 : 6) : (DP == 128 ? 4 : 8);
+  static constexpr int RAW = 2;            // tiles of codes
+  static constexpr int OFF_KV = 2 * BYTES;
+  static constexpr int OFF_RAW = OFF_KV + STAGES * BYTES;
+  static constexpr int OFF_STG = OFF_RAW + (CODES ? RAW * SLAB : 0);  // 32 rows x 64 bytes a warp
+  static constexpr int SCALES = 4;         // tiles whose scales are kept: [2][128] each
+  static constexpr int OFF_SC = OFF_STG + 8 * 2048;
+  static constexpr int OFF_Q = OFF_SC + (CODES ? SCALES * 1024 : 0);  // queries' factors [2][256]
+  static constexpr int OFF_REC = OFF_Q + (CODES ? 2048 : 0);
+  static constexpr int OFF_STEPS = OFF_REC + RECORDS * 64;  // ranged: where each piece begins
+  static constexpr int OFF_GAPS = OFF_STEPS + MAX_SLOTS * 4;  // keys without a page, 8 tiles
+  static constexpr int GAPS = 8;
+  static constexpr int OFF_BAD = OFF_GAPS + GAPS * 16;        // values that are not finite
+  static constexpr int OFF_BAR = OFF_BAD + STAGES * 16;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  // What is noted of tile x is written when the stage of its K tile is free. If that was
+  // tile y's K tile, the softmax is done with tile y - 1 then, if it was y's V tile, with y.
+  static_assert((!CODES || 2 * SCALES >= STAGES + 2) && 2 * GAPS >= STAGES + 2,
+                "notes outlive their tile");
+  // 16-bit keys: V tiles have stages of their own, whose phases `full` counts
+  static_assert(CODES || STAGES % 2 == 0, "K and V tiles alternate");
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+// What a CTA does next.
+struct Record {
+  int row0, tokens;  // first query row; tokens (0: nothing more)
+  int h0, b;
+  int pos0;          // the first token's place in its sequence
+  int len, kv0;      // keys; packed: the first one's row
+  int t0, e0, e1;    // key tiles: from t0 to the ends of the two query tiles
+  int part;          // -1: all of the keys; else where in the workspace the part goes
+  int parts;         // of an item that this CTA begins and others end: in how many it is
+  int pad[4];
+  SRDIT_DEV int steps() const { return max(e0, e1) - t0; }
+};
+
+// What a CTA leaves for join_chunk_kernel: the item that it begins and does not end.
+struct Cut {
+  int parts, row0, tokens, h0;
+};
+
+// The pieces of sequences: piece n of sequence b is number begin(b) / (2 rt) + b + n, so that a
+// sequence of any length has enough numbers and a search finds it; numbers behind a sequence's
+// end are empty.
+struct Pieces {
+  const Args& a;
+  SRDIT_DEV int base(int b) const {
+    return a.by_piece.div(a.rows.at ? a.rows.begin(b) : b * a.rows.each) + b;
+  }
+  // the last sequence whose base is not above n, by one thread
+  SRDIT_DEV int find(int n) const {
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (base(mid) <= n) lo = mid; else hi = mid;
+    }
+    return lo;
+  }
+  // the same by a warp
+  SRDIT_DEV int find_warp(int n) const {
+    int lo = 0, count = a.B;
+    while (count > 1) {
+      const int each = (count + 31) >> 5, at = lo + static_cast<int>(threadIdx.x & 31) * each;
+      const unsigned le = __ballot_sync(0xffffffffu, at < lo + count && base(at) <= n);
+      const int k = le ? 31 - __clz(le) : 0;
+      count = min(each, count - k * each);
+      lo += k * each;
+    }
+    return lo;
+  }
+  // the item of piece n of sequence b; false: there is none
+  SRDIT_DEV bool item(int b, int n, Record& r) const {
+    const int begin = a.rows.begin(b), tokens = a.rows.end(b) - begin;
+    const int at = (n - base(b)) * 2 * a.rt;
+    if (at < 0 || at >= tokens) return false;
+    r.b = b;
+    r.row0 = begin + at;
+    r.tokens = min(2 * a.rt, tokens - at);
+    r.len = a.key_count(b);
+    r.kv0 = a.paged() ? 0 : a.keys.begin(b);
+    r.pos0 = r.len - tokens + at;
+    r.t0 = 0;
+    const int tiles = (r.len + TILE - 1) / TILE;
+    auto end = [&](int last) {
+      return !a.causal ? tiles : last < 0 ? 0 : min(tiles, last / TILE + 1);
+    };
+    r.e0 = end(r.pos0 + min(r.tokens, a.rt) - 1);
+    r.e1 = r.tokens > a.rt ? end(r.pos0 + r.tokens - 1) : 0;
+    r.part = -1;
+    r.parts = 0;
+    return true;
+  }
+};
+
+template <typename T, int DP, int CODE>
+__global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Args a,
+                 int k_one_head, int v_one_head) {
+  pdl_begin();
+  using C = ChunkCfg<DP, CODE>;
+  using E = typename Compute<T, CODE>::type;
+  constexpr int STAGES = C::STAGES, RAW = C::RAW;
+  constexpr bool CODES = C::CODES;
+  constexpr bool TURN_Q = CODES && !__is_same(T, __half);  // queries become fp16
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // 16-bit keys: by TMA
+  uint64_t* full = loaded + STAGES;     // ready for the products
+  uint64_t* empty = full + STAGES;
+  uint64_t* raw_full = empty + STAGES;  // codes
+  uint64_t* raw_empty = raw_full + RAW;
+  uint64_t* q_loaded = raw_empty + RAW;  // [2], one per query tile
+  uint64_t* q_full = q_loaded + 2;
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;     // scores of a tile ready
+  uint64_t* p_full = s_full + 2;      // its weights written (one arrival per warp)
+  uint64_t* p_half = p_full + 2;      // the first half of them
+  uint64_t* o_full = p_half + 2;      // its last product done
+  uint64_t* rec_full = o_full + 2;
+  uint64_t* rec_empty = rec_full + RECORDS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rec_empty + RECORDS);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  static_assert((3 * STAGES + 2 * RAW + 14 + 2 * RECORDS) * 8 + 8 <= 512, "barrier area");
+  Record* records = reinterpret_cast<Record*>(smem + C::OFF_REC);
+  int* starts = reinterpret_cast<int*>(smem + C::OFF_STEPS);
+  uint4* gaps = reinterpret_cast<uint4*>(smem + C::OFF_GAPS);  // by tiles, a bit a key
+  uint4* bad = reinterpret_cast<uint4*>(smem + C::OFF_BAD);    // by stages
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&loaded[s], 1);
+      mbar_init(&full[s], CODES ? 4 : 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < RAW; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], 4);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_loaded[t], 1);
+      mbar_init(&q_full[t], 4);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&p_half[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    for (int s = 0; s < RECORDS; ++s) {
+      mbar_init(&rec_full[s], 1);
+      mbar_init(&rec_empty[s], 10 + (CODES ? 4 : 1));
+    }
+    *abort_flag = 0u;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // tensor memory: S0 @0, S1 @128 (weights over the first 64 columns), O0 @256, O1 @384
+  const uint32_t tmem_base = *tmem_slot;
+  // a tile that some query of the item does not see whole by place
+  auto partly = [&](const Record& r, int key0) {
+    return key0 + TILE > r.len || (a.causal && key0 + TILE - 1 > r.pos0);
+  };
+  if (warp < 4) {
+    if constexpr (CODES)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      // the pages' boxes of a tile side by side: lane l has the box of keys l * box on
+      int idx = 0, tiles = 0;   // ring uses, key tiles
+      int nq[2] = {0, 0};       // query tiles loaded
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int at = n % RECORDS;
+        ok = mbar_wait_warp(&rec_full[at], static_cast<uint32_t>(n / RECORDS) & 1u, a.status,
+                            abort_flag);
+        if (!ok) break;
+        const Record r = records[at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&rec_empty[at]);
+        if (r.tokens == 0) break;
+        if (r.steps() <= 0) continue;
+        const int g = r.h0 / a.group;
+        const int boxes = TILE >> a.box_log;
+        auto load_q = [&](int t) {
+          if (!mbar_wait_warp(&q_empty[t], (static_cast<uint32_t>(nq[t]) & 1u) ^ 1u, a.status,
+                              abort_flag))
+            return false;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_loaded[t], C::BYTES);
+            for (int d = 0; d < DP / 64; ++d)
+              tma_load_4d(smem + t * C::BYTES + d * C::SLAB, &tmQ, &q_loaded[t], d * 64, r.h0,
+                          r.row0 + t * a.rt, 0);
+          }
+          ++nq[t];
+          return true;
+        };
+        // this lane's box of a tile: its page (-1: none) and row; whether keys have no page
+        auto place = [&](int tile, int& page, int& row, bool& gap) {
+          page = 0;
+          row = r.kv0 + tile * TILE;
+          gap = false;
+          if (a.paged()) {
+            const int key = tile * TILE + (lane << a.box_log);
+            const int p = a.table.by_page.div(key);
+            const bool on = lane < boxes && key < r.len;
+            row = key - p * a.table.page_size;
+            page = on ? a.table.page(r.b, p) : -1;
+            gap = on && page < 0;
+          }
+        };
+        auto load_kv = [&](bool v, int page, int row, bool gap) {
+          const CUtensorMap* tm = v ? &tmV : &tmK;
+          const int h = (v ? v_one_head : k_one_head) ? 0 : g;
+          const int at_page = page >= 0 ? page : max(a.table.pages, 1);  // past the pages: zeros
+          const unsigned gap_boxes = __ballot_sync(0xffffffffu, gap);
+          if constexpr (CODES) {
+            const int s = idx % RAW;
+            if (!mbar_wait_warp(&raw_empty[s], (static_cast<uint32_t>(idx / RAW) & 1u) ^ 1u,
+                                a.status, abort_flag))
+              return false;
+            if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], C::SLAB);
+            __syncwarp();
+            if (lane < boxes)
+              tma_load_4d(smem + C::OFF_RAW + s * C::SLAB + (lane << a.box_log) * 128, tm,
+                          &raw_full[s], 0, h, row, at_page);
+          } else {
+            const int s = idx % STAGES;
+            if (!mbar_wait_warp(&empty[s], (static_cast<uint32_t>(idx / STAGES) & 1u) ^ 1u,
+                                a.status, abort_flag))
+              return false;
+            if (!v) {
+              if (lane < 4) {
+                const uint32_t lo = (gap_boxes >> ((lane * 32) >> a.box_log)) & 1u;
+                const uint32_t hi = (gap_boxes >> ((lane * 32 + 16) >> a.box_log)) & 1u;
+                reinterpret_cast<uint32_t*>(gaps + tiles % C::GAPS)[lane] =
+                    (lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u);
+              }
+              ++tiles;
+              __syncwarp();
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&loaded[s], C::BYTES);
+            __syncwarp();
+            if (lane < boxes)
+              for (int d = 0; d < DP / 64; ++d)
+                tma_load_4d(smem + C::OFF_KV + s * C::BYTES + d * C::SLAB +
+                                (lane << a.box_log) * 128,
+                            tm, &loaded[s], d * 64, h, row, at_page);
+          }
+          ++idx;
+          return true;
+        };
+        int page, row, page1 = 0, row1 = 0;
+        bool gap, gap1 = false;
+        place(r.t0, page, row, gap);
+        ok = (r.e0 <= r.t0 || load_q(0)) && load_kv(false, page, row, gap) &&
+             (r.e1 <= r.t0 || load_q(1));
+        const int end = max(r.e0, r.e1);
+        for (int j = r.t0; j < end && ok; ++j) {
+          if (j + 1 < end) place(j + 1, page1, row1, gap1);
+          ok = load_kv(true, page, row, false) &&
+               (j + 1 == end || load_kv(false, page1, row1, gap1));
+          page = page1;
+          row = row1;
+        }
+      }
+      // having given up, let the loads in flight land before the CTA exits
+      if (!ok)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      // S0 S1 | PV0 S0' PV1 S1' | ...: a tile's next scores follow its product, so the
+      // weights that share their columns have been read (the tensor core runs in order)
+      if (elect_one()) {
+        constexpr uint32_t fmt = __is_same(E, __nv_bfloat16) ? 1u : 0u;
+        const uint32_t idesc_s = idesc_make(fmt, fmt, 0u, 0u, 128u, 128u);
+        const uint32_t idesc_o = idesc_make(fmt, fmt, 0u, 1u, 128u, static_cast<uint32_t>(DP));
+        int idx = 0, nrec = 0;
+        int nq[2] = {0, 0}, np[2] = {0, 0};
+        auto kv_wait = [&](int u, bool v) {
+          return mbar_wait((CODES || v ? full : loaded) + u % STAGES,
+                           static_cast<uint32_t>(u / STAGES) & 1u, a.status, abort_flag);
+        };
+        auto q_wait = [&](int t) {
+          return mbar_wait((TURN_Q ? q_full : q_loaded) + t, static_cast<uint32_t>(nq[t]++) & 1u,
+                           a.status, abort_flag);
+        };
+        auto scores = [&](int t, int u) {  // S_t = Q_t K^T, K in ring use u
+          const uint32_t q_addr = smem_u32(smem + t * C::BYTES);
+          const uint32_t k_addr = smem_u32(smem + C::OFF_KV + (u % STAGES) * C::BYTES);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = static_cast<uint32_t>((k >> 2) * C::SLAB + (k & 3) * 32);
+            mma_bf16_ss(tmem_base + t * 128u, sdesc_sw128(q_addr + off, 16, 1024),
+                        sdesc_sw128(k_addr + off, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[t]);
+        };
+        // O_t (+)= P_t V over the keys 16 k0 to 16 k1, V in ring use u
+        auto product = [&](int t, int u, bool first, int k0, int k1) {
+          const uint32_t v_addr = smem_u32(smem + C::OFF_KV + (u % STAGES) * C::BYTES);
+#pragma unroll
+          for (int k = k0; k < k1; ++k)
+            mma_bf16_ts(tmem_base + 256u + t * 128u, tmem_base + t * 128u + k * 8u,
+                        sdesc_sw128(v_addr + k * 16 * 128, C::SLAB, 1024), idesc_o,
+                        (!first || k > 0) ? 1u : 0u);
+        };
+        bool ok = true;
+        struct Now {
+          int t0, e[2], end;
+        };
+        // the next item with key tiles, or false
+        auto next = [&](Now& r) {
+          while (true) {
+            const int at = nrec % RECORDS;
+            if (!mbar_wait(&rec_full[at], static_cast<uint32_t>(nrec / RECORDS) & 1u, a.status,
+                           abort_flag)) {
+              ok = false;
+              return false;
+            }
+            const int tokens = records[at].tokens;
+            r.t0 = records[at].t0;
+            r.e[0] = records[at].e0;
+            r.e[1] = records[at].e1;
+            r.end = max(r.e[0], r.e[1]);
+            mbar_arrive(&rec_empty[at]);
+            ++nrec;
+            if (tokens == 0) return false;
+            if (r.end > r.t0) return true;
+          }
+        };
+        Now it = {};
+        bool on = next(it);
+        int j = it.t0;
+        if (on) {
+          ok = kv_wait(0, false);
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (it.e[t] <= it.t0) continue;
+            ok = q_wait(t);
+            if (!ok) break;
+            tc_fence_after();
+            scores(t, 0);
+            if (it.e[t] - it.t0 == 1) tc_commit(&q_empty[t]);
+          }
+          if (ok) tc_commit(&empty[0]);
+        }
+        while (ok && on) {
+          // the step after (it, j): the item's next key tile, or another item's first
+          Now nx = it;
+          int nj = j + 1;
+          const bool last = nj == it.end;
+          bool more = true;
+          if (last) {
+            more = next(nx);
+            nj = nx.t0;
+            if (!ok) break;
+          }
+          const int uv = idx + 1, uk = idx + 2;
+          ok = kv_wait(uv, true);
+          bool k_ready = false;
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (j < it.e[t]) {
+              ok = mbar_wait(&p_half[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              product(t, uv, j == it.t0, 0, 4);
+              ok = mbar_wait(&p_full[t], static_cast<uint32_t>(np[t]) & 1u, a.status, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              ++np[t];
+              product(t, uv, j == it.t0, 4, 8);
+              if (j + 1 == it.e[t]) tc_commit(&o_full[t]);
+            }
+            if (more && nj < nx.e[t]) {
+              if (!k_ready) ok = kv_wait(uk, false);
+              k_ready = true;
+              if (ok && last) ok = q_wait(t);
+              if (!ok) break;
+              tc_fence_after();
+              scores(t, uk);
+              if (nj + 1 == nx.e[t]) tc_commit(&q_empty[t]);
+            }
+          }
+          if (!ok) break;
+          tc_commit(&empty[uv % STAGES]);
+          if (more) tc_commit(&empty[uk % STAGES]);
+          idx += 2;
+          it = nx;
+          on = more;
+          j = nj;
+        }
+      }
+      __syncwarp();
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ items
+      const Pieces pieces{a};
+      int n = 0;
+      auto pass = [&](const Record& r) {
+        const int at = n % RECORDS;
+        if (!mbar_wait_warp(&rec_empty[at], (static_cast<uint32_t>(n / RECORDS) & 1u) ^ 1u,
+                            a.status, abort_flag))
+          return false;
+        if (lane == 0) {
+          records[at] = r;
+          mbar_arrive(&rec_full[at]);
+        }
+        __syncwarp();
+        ++n;
+        return true;
+      };
+      Record r = {};
+      bool ok = true;
+      if (!a.ranged) {
+        // whole items, every gridDim-th one. Causal: the last pieces first (the longest), all heads
+        // of a piece side by side; else a head's pieces, which share its keys, side by side.
+        const int items = a.slots * a.nhp;
+        for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
+          int slot, hp;
+          if (a.causal) {
+            slot = a.by_nhp.div(x);
+            hp = x - slot * a.nhp;
+            slot = a.slots - 1 - slot;
+          } else {
+            hp = a.by_slots.div(x);
+            slot = x - hp * a.slots;
+          }
+          if (!pieces.item(pieces.find_warp(slot), slot, r)) continue;
+          r.h0 = hp * a.pack;
+          ok = pass(r);
+        }
+      } else {
+        // an equal share of all items' key tiles, head pack by head pack (an item without any
+        // counts as one). starts[]: where each piece begins.
+        int total = 0;
+        for (int s0 = 0; s0 < a.slots; s0 += 32) {
+          const int s = s0 + lane;
+          int w = 0;
+          if (s < a.slots && pieces.item(pieces.find(s), s, r)) w = max(1, max(r.e0, r.e1));
+          int sum = w;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+          }
+          if (s < a.slots) starts[s] = total + sum - w;
+          total += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        __syncwarp();
+        const int all = total * a.nhp;
+        const int share = max((all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x),
+                              MIN_SHARE);
+        int s = blockIdx.x * share;
+        const int s1 = min(s + share, all);
+        if (lane == 0) static_cast<Cut*>(a.cuts)[blockIdx.x].parts = 0;
+        if (s < s1) {
+          int hp = s / total, x = s - hp * total;
+          int slot = 0;  // the last piece that does not begin behind x
+          for (int o = 128; o; o >>= 1)
+            if (slot + o < a.slots && starts[slot + o] <= x) slot += o;
+          while (s < s1 && ok) {
+            const bool found = pieces.item(pieces.find_warp(slot), slot, r);
+            const int w = found ? max(1, max(r.e0, r.e1)) : 0;
+            if (x < starts[slot] + w) {
+              const int t0 = x - starts[slot], t1 = min(w, t0 + (s1 - s));
+              r.h0 = hp * a.pack;
+              r.t0 = t0;
+              r.e0 = max(t0, min(r.e0, t1));
+              r.e1 = max(t0, min(r.e1, t1));
+              const int cta = static_cast<int>(blockIdx.x);
+              r.part = t0 > 0 ? 2 * cta : t1 < w ? 2 * cta + 1 : -1;
+              if (t0 == 0 && t1 < w) r.parts = (s + w - 1) / share - cta + 1;
+              ok = pass(r);
+              s += t1 - t0;
+              x += t1 - t0;
+            }
+            if (++slot == a.slots) {
+              slot = 0;
+              x = 0;
+              ++hp;
+            }
+          }
+        }
+      }
+      r.tokens = 0;
+      if (ok) pass(r);
+    } else if constexpr (!CODES) {
+      // ------------------------------------------------------------ values of partly hidden tiles
+      // Rows behind the sequence become zeros (a weight of 0 times a NaN would be a NaN). Where a
+      // causal mask hides some of the tile, so does a row that is not finite, and the queries
+      // that see it are told.
+      int idx = 0;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int at = n % RECORDS;
+        ok = mbar_wait_warp(&rec_full[at], static_cast<uint32_t>(n / RECORDS) & 1u, a.status,
+                            abort_flag);
+        if (!ok) break;
+        const Record r = records[at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&rec_empty[at]);
+        if (r.tokens == 0) break;
+        const int steps = r.steps();
+        for (int j = 0; j < steps && ok; ++j) {
+          const int u = idx + 2 * j + 1, s = u % STAGES;
+          ok = mbar_wait_warp(&loaded[s], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
+                              abort_flag);
+          if (!ok) break;
+          const int key0 = (r.t0 + j) * TILE;
+          if (partly(r, key0)) {
+#pragma unroll 1
+            for (int w = 0; w < 4; ++w) {
+              uint8_t* vrow = smem + C::OFF_KV + s * C::BYTES + (w * 32 + lane) * 128;
+              const bool behind = key0 + w * 32 + lane >= r.len;
+              uint32_t m = 0;
+              if (!behind && a.causal) {
+#pragma unroll
+                for (int x = 0; x < DP / 8; ++x) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(
+                      vrow + (x >> 3) * C::SLAB + (((x + lane) & 7) << 4));
+                  m = max_bits(max_bits(max_bits(max_bits(m, v.x), v.y), v.z), v.w);
+                }
+              }
+              const bool off = not_finite<E>(m);
+              if (behind || off) {
+#pragma unroll
+                for (int x = 0; x < DP / 8; ++x)
+                  *reinterpret_cast<uint4*>(vrow + (x >> 3) * C::SLAB +
+                                            (((x + lane) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+              }
+              const unsigned all = __ballot_sync(0xffffffffu, off);
+              if (lane == 0) reinterpret_cast<uint32_t*>(bad + s)[w] = all;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
+        idx += 2 * max(steps, 0);
+      }
+    }
+  } else if (warp < 12) {
+    if constexpr (CODES)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ------------------------------------------------------------ softmax
+    const int t = (warp - 4) >> 2;  // query tile
+    const int sub = warp & 3;       // tensor-memory lane quarter
+    const int row = sub * 32 + lane;
+    const uint32_t t_lane = static_cast<uint32_t>(sub * 32) << 16;
+    const uint32_t s_tmem = tmem_base + t_lane + t * 128u;
+    const uint32_t o_tmem = tmem_base + t_lane + 256u + t * 128u;
+    uint8_t* stg = smem + C::OFF_STG + (warp - 4) * 2048;
+    const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SC);
+    const float* q_back = reinterpret_cast<const float*>(smem + C::OFF_Q);
+    const int my_token = t * a.rt + row / a.pack;
+    const int warp_token = t * a.rt + sub * 32 / a.pack;
+    int ns = 0, no = 0, idx = 0, tiles = 0;
+    // A wait that runs out sets the abort flag, and those after it end at once: the warp goes
+    // through the rest of its item without a branch, so that no lane of it stays behind, and
+    // leaves at the item's end.
+    for (int n = 0;; ++n) {
+      const int at = n % RECORDS;
+      if (!mbar_wait_warp(&rec_full[at], static_cast<uint32_t>(n / RECORDS) & 1u, a.status,
+                          abort_flag))
+        break;
+      const Record& rec = records[at];
+      const int t0 = rec.t0, e = t ? rec.e1 : rec.e0, steps = rec.steps();
+      const int len = rec.len, pos0 = rec.pos0, tokens = rec.tokens, part = rec.part;
+      const int row0 = rec.row0, h0 = rec.h0, parts = rec.parts;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&rec_empty[at]);
+      if (tokens == 0) break;
+      const int n_tiles = e - t0;
+      float m = neg_inf(), l = 0.f, c = a.c;
+      // the last key that this row sees, and the least of its warp's
+      const int lim = a.causal ? min(len - 1, pos0 + my_token) : len - 1;
+      const int lim0 = a.causal ? min(len - 1, pos0 + warp_token) : len - 1;
+      for (int j = 0; j < n_tiles; ++j) {
+        const int key0 = (t0 + j) * TILE, u = idx + 2 * j;
+        mbar_wait(&s_full[t], static_cast<uint32_t>(ns) & 1u, a.status, abort_flag);
+        ++ns;
+        tc_fence_after();
+        // what was noted before the products that are done now
+        if (TURN_Q && j == 0) c = q_back[(n & 1) * 256 + t * 128 + row];
+        const uint64_t c2 = f2_pack(c, c);
+        const uint4 gap = gaps[tiles % C::GAPS];
+        const bool masked = key0 + TILE - 1 > lim0 || (gap.x | gap.y | gap.z | gap.w) != 0u;
+        uint32_t vis[4];
+        if (masked) {
+          const uint32_t none[4] = {gap.x, gap.y, gap.z, gap.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int count = lim - key0 + 1 - 32 * w;
+            vis[w] = (count >= 32 ? 0xffffffffu : count <= 0 ? 0u : (1u << count) - 1u) & ~none[w];
+          }
+        }
+        uint32_t s[4][32];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) tmem_ld32(s_tmem + w * 32, s[w]);
+        tmem_ld_wait();
+        const float* sc = scales + (tiles % C::SCALES) * 256;
+        if constexpr (CODES) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) {
+              const float4 k = *reinterpret_cast<const float4*>(sc + w * 32 + x);
+              const float2 y0 =
+                  f2_split(f2_mul(u64_of(s[w][x], s[w][x + 1]), f2_pack(k.x, k.y)));
+              const float2 y1 =
+                  f2_split(f2_mul(u64_of(s[w][x + 2], s[w][x + 3]), f2_pack(k.z, k.w)));
+              s[w][x] = __float_as_uint(y0.x);
+              s[w][x + 1] = __float_as_uint(y0.y);
+              s[w][x + 2] = __float_as_uint(y1.x);
+              s[w][x + 3] = __float_as_uint(y1.y);
+            }
+        }
+        if (masked) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (!((vis[w] >> x) & 1u)) s[w][x] = __float_as_uint(neg_inf());
+        }
+        float mx[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          mx[w] = __uint_as_float(s[w][0]);
+#pragma unroll
+          for (int x = 1; x < 31; x += 2)
+            mx[w] = max3(mx[w], __uint_as_float(s[w][x]), __uint_as_float(s[w][x + 1]));
+          mx[w] = max2(mx[w], __uint_as_float(s[w][31]));
+        }
+        float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
+        if constexpr (CODES) {  // the values' scales are there with the V tile
+          mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u, a.status,
+                    abort_flag);
+          float most = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float v = sc[128 + w * 32 + lane];
+            most = fmaxf(most, v < 3e38f ? v : 0.f);
+          }
+          most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+          top += __log2f(fmaxf(most, 1e-30f));
+        }
+        // the maximum moves (and O is rescaled) only when a tile's is 8 above it:
+        // weights stay below 2^8 and the quotient is the same
+        // (written so that a NaN raises it too, and stays in l and O)
+        const bool raise = !(top <= m + 8.f) && top != neg_inf();
+        const float m_new = raise ? top : m;
+        const float alpha = raise ? ex2(m - m_new) : 1.f;
+        m = m_new;
+        const float neg_m = m == neg_inf() ? 0.f : -m;
+        const uint64_t neg_m2 = f2_pack(neg_m, neg_m);
+        if (j > 0 && __any_sync(0xffffffffu, raise)) {
+          // scores of this tile are ready, so the product before it is done
+#pragma unroll 1
+          for (int w = 0; w < DP / 16; ++w) {
+            uint32_t o[16];
+            tmem_ld16(o_tmem + w * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+            tmem_st16(o_tmem + w * 16, o);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            const float2 y = f2_split(f2_fma(u64_of(s[w][x], s[w][x + 1]), c2, neg_m2));
+            s[w][x] = __float_as_uint(y.x);
+            s[w][x + 1] = __float_as_uint(y.y);
+          }
+        uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t pw[16];
+          if constexpr (CODES) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(sc + 128 + w * 32 + x);
+              const uint64_t p0 =
+                  f2_pack(ex2(__uint_as_float(s[w][x])), ex2(__uint_as_float(s[w][x + 1])));
+              const uint64_t p1 =
+                  f2_pack(ex2(__uint_as_float(s[w][x + 2])), ex2(__uint_as_float(s[w][x + 3])));
+              sum[0] = f2_add(sum[0], p0);
+              sum[1] = f2_add(sum[1], p1);
+              float2 y0 = f2_split(f2_mul(p0, f2_pack(v.x, v.y)));
+              float2 y1 = f2_split(f2_mul(p1, f2_pack(v.z, v.w)));
+              if (masked) {  // (a scale of NaN stays with the rows that see its key)
+                if (!((vis[w] >> x) & 1u)) y0.x = 0.f;
+                if (!((vis[w] >> (x + 1)) & 1u)) y0.y = 0.f;
+                if (!((vis[w] >> (x + 2)) & 1u)) y1.x = 0.f;
+                if (!((vis[w] >> (x + 3)) & 1u)) y1.y = 0.f;
+              }
+              pw[x >> 1] = pack2(y0.x, y0.y, E{});
+              pw[(x >> 1) + 1] = pack2(y1.x, y1.y, E{});
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; x += 2) {
+              const uint64_t p2 =
+                  f2_pack(ex2(__uint_as_float(s[w][x])), ex2(__uint_as_float(s[w][x + 1])));
+              sum[(x >> 1) & 1] = f2_add(sum[(x >> 1) & 1], p2);
+              const float2 p = f2_split(p2);
+              pw[x >> 1] = pack2(p.x, p.y, E{});
+            }
+          }
+          if (w == 2) {  // the first 64 keys' weights, stored by now: their product can begin
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[t]);
+          }
+          tmem_st16(s_tmem + w * 16, pw);
+        }
+        const float2 sp = f2_split(f2_add(sum[0], sum[1]));
+        l = l * alpha + (sp.x + sp.y);
+        if constexpr (!CODES) {
+          if (a.causal && key0 + TILE - 1 > pos0) {  // values taken out, as not finite
+            mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u,
+                      a.status, abort_flag);
+            uint4 off = bad[(u + 1) % STAGES];
+            if (masked)
+              off = make_uint4(off.x & vis[0], off.y & vis[1], off.z & vis[2], off.w & vis[3]);
+            if (off.x | off.y | off.z | off.w) l = __int_as_float(0x7fc00000);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+        ++tiles;
+      }
+      tiles += max(steps, 0) - max(n_tiles, 0);
+      if (n_tiles > 0) {
+        mbar_wait(&o_full[t], static_cast<uint32_t>(no) & 1u, a.status, abort_flag);
+        ++no;
+      }
+      if (__any_sync(0xffffffffu, *abort_flag != 0u)) break;
+      tc_fence_after();
+      idx += 2 * max(steps, 0);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (part < 0) {
+        // O / l: the warp's 32 rows go through its staging buffer 64 bytes of each at a time
+#pragma unroll 1
+        for (int d = 0; d < DP; d += 32) {
+          uint32_t o[32];
+          if (n_tiles > 0) {
+            tmem_ld32(o_tmem + d, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = 0u;
+          }
+          __syncwarp();  // the rows before have left the buffer
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              w[y] = pack2(__uint_as_float(o[x * 8 + y * 2]) * inv,
+                           __uint_as_float(o[x * 8 + y * 2 + 1]) * inv, T{});
+            *reinterpret_cast<uint4*>(stg + lane * 64 + ((x ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+          const int piece = lane & 3, col = d + piece * 8;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int r = y * 8 + (lane >> 2), tr = sub * 32 + r;
+            const int token = t * a.rt + tr / a.pack;
+            if (token < tokens && col < a.D)
+              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (row0 + token) * a.os[0] +
+                                        (h0 + tr % a.pack) * a.os[1] + col) =
+                  *reinterpret_cast<const uint4*>(stg + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+          }
+        }
+      } else {
+        // a part: [D][256 rows], a row a lane
+        float* ws = a.ws + static_cast<long long>(part) * DP * ROWS + t * TILE + row;
+        reinterpret_cast<float2*>(a.ml)[part * ROWS + t * TILE + row] = make_float2(m, l);
+        if (t == 0 && row == 0 && parts) {
+          const Cut cut = {parts, row0, tokens, h0};
+          static_cast<Cut*>(a.cuts)[blockIdx.x] = cut;
+        }
+        if (n_tiles > 0) {
+#pragma unroll 1
+          for (int d = 0; d < DP; d += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_tmem + d, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) ws[(d + x) * ROWS] = __uint_as_float(o[x]);
+          }
+        }
+      }
+      // the next item's first weights, published after this, free O
+      tc_fence_before();
+    }
+  } else if constexpr (CODES) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    // ------------------------------------------------------------ codes to fp16
+    const int w = warp - 12;
+    const int r8 = lane & 7, y0 = lane >> 3;  // a lane's row of 8, its pieces of 16 bytes
+    const int key = w * 32 + lane;            // whose scales this lane fetches
+    float* scales = reinterpret_cast<float*>(smem + C::OFF_SC);
+    float* q_back = reinterpret_cast<float*>(smem + C::OFF_Q);
+    int idx = 0, tiles = 0, nq[2] = {0, 0};
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int at = n % RECORDS;
+      ok = mbar_wait_warp(&rec_full[at], static_cast<uint32_t>(n / RECORDS) & 1u, a.status,
+                          abort_flag);
+      if (!ok) break;
+      const Record r = records[at];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&rec_empty[at]);
+      if (r.tokens == 0) break;
+      const int steps = r.steps();
+      if (steps <= 0) continue;
+      const int g = r.h0 / a.group;
+      // the scales of a tile's keys, 0 where there is none; whether a key has no page
+      bool here = false;
+      auto scales_of = [&](int tile, float& k, float& v) {
+        const int x = tile * TILE + key;
+        k = v = 0.f;
+        here = true;
+        if (x >= r.len) return;
+        const int p = a.table.by_page.div(x), in = x - p * a.table.page_size;
+        const long long page = a.table.page(r.b, p);
+        here = page >= 0;
+        if (!here) return;
+        k = __ldg(a.scale[0] + page * a.ss[0][0] + in * a.ss[0][1] + g * a.ss[0][2]);
+        v = __ldg(a.scale[1] + page * a.ss[1][0] + in * a.ss[1][1] + g * a.ss[1][2]);
+      };
+      float ks, vs;
+      scales_of(r.t0, ks, vs);
+      auto turn_q = [&](int t) {
+        if (!mbar_wait_warp(&q_loaded[t], static_cast<uint32_t>(nq[t]) & 1u, a.status, abort_flag))
+          return false;
+        ++nq[t];
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int row = w * 32 + i * 8 + r8;
+          uint8_t* q = smem + t * C::BYTES + row * 128;
+          uint4 v[DP / 32];
+          uint32_t mx = 0;
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x) {
+            const int piece = (x & 1) * 4 + y0;
+            v[x] = *reinterpret_cast<const uint4*>(q + (x >> 1) * C::SLAB + ((piece ^ r8) << 4));
+            mx = max_bits(max_bits(max_bits(max_bits(mx, v[x].x), v[x].y), v[x].z), v[x].w);
+          }
+          mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const int k = fp16_exponent(max(mx & 0xffffu, mx >> 16));
+          const float f = exp2_int(k);
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x) {
+            const int piece = (x & 1) * 4 + y0;
+            *reinterpret_cast<uint4*>(q + (x >> 1) * C::SLAB + ((piece ^ r8) << 4)) =
+                make_uint4(bf16x2_as_fp16(v[x].x, f), bf16x2_as_fp16(v[x].y, f),
+                           bf16x2_as_fp16(v[x].z, f), bf16x2_as_fp16(v[x].w, f));
+          }
+          if (y0 == 0) q_back[(n & 1) * 256 + t * 128 + row] = a.c * exp2_int(-k);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[t]);
+        return true;
+      };
+      auto turn = [&](bool v, int tile, float scale, bool there) {
+        const int u = idx, s = u % STAGES, x = u % RAW;
+        ++idx;
+        if (!mbar_wait_warp(&empty[s], (static_cast<uint32_t>(u / STAGES) & 1u) ^ 1u, a.status,
+                            abort_flag) ||
+            !mbar_wait_warp(&raw_full[x], static_cast<uint32_t>(u / RAW) & 1u, a.status, abort_flag))
+          return false;
+        float* sc = scales + (tiles % C::SCALES) * 256 + (v ? 128 : 0);
+        sc[key] = scale;
+        if (!v) {
+          const unsigned none = __ballot_sync(0xffffffffu, !there);
+          if (lane == 0) reinterpret_cast<uint32_t*>(gaps + tiles % C::GAPS)[w] = none;
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int row = w * 32 + i * 8 + r8;
+          const uint8_t* from = smem + C::OFF_RAW + x * C::SLAB + row * 128;
+          uint8_t* to = smem + C::OFF_KV + s * C::BYTES + row * 128;
+#pragma unroll
+          for (int k = 0; k < DP / 64; ++k) {
+            const int piece = k * 4 + y0;
+            uint4 codes = *reinterpret_cast<const uint4*>(from + ((piece ^ r8) << 4));
+            if (CODE == SRDIT_Q_E4M3 && v) {
+              // a NaN code makes its token's value one; behind the sequence it is nothing
+              if (nan_codes(codes.x) || nan_codes(codes.y) || nan_codes(codes.z) ||
+                  nan_codes(codes.w)) {
+                codes = make_uint4(0, 0, 0, 0);
+                if (tile * TILE + row < r.len) sc[row] = __int_as_float(0x7fc00000);
+              }
+            }
+            uint32_t h[8];
+            widen_codes<CODE>(codes, h);
+            uint8_t* slab = to + k * C::SLAB;
+            *reinterpret_cast<uint4*>(slab + (((2 * y0) ^ r8) << 4)) =
+                make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(slab + (((2 * y0 + 1) ^ r8) << 4)) =
+                make_uint4(h[4], h[5], h[6], h[7]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&full[s]);
+          mbar_arrive(&raw_empty[x]);
+        }
+        return true;
+      };
+      const int end = max(r.e0, r.e1);
+      if (TURN_Q && r.e0 > r.t0) ok = turn_q(0);
+      for (int j = r.t0; j < end && ok; ++j) {
+        const bool there = here;
+        const float k = ks, v = vs;
+        ok = turn(false, j, k, there);
+        if (TURN_Q && ok && j == r.t0 && r.e1 > r.t0) ok = turn_q(1);
+        if (j + 1 < end) scales_of(j + 1, ks, vs);
+        ok = ok && turn(true, j, v, there);
+        ++tiles;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// One block per 32 rows of the items that the CTAs' shares cut: joins their parts, 8 columns a
+// thread, a row a lane.
+template <typename T, int DP>
+__global__ void __launch_bounds__(DP / 8 * 32) join_chunk_kernel(const __grid_constant__ Args a) {
+  pdl_begin();
+  const Cut cut = static_cast<const Cut*>(a.cuts)[blockIdx.x];
+  if (cut.parts == 0) return;
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), d = (threadIdx.x >> 5) * 8;
+  const int token = row / a.pack, head = cut.h0 + row % a.pack;
+  if (token >= cut.tokens || d >= a.D) return;
+  float m = neg_inf(), l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int p = 0; p < cut.parts; ++p) {
+    const int cta = static_cast<int>(blockIdx.x) + p, part = p == 0 ? 2 * cta + 1 : 2 * cta;
+    const float2 q = reinterpret_cast<const float2*>(a.ml)[part * ROWS + row];
+    if (q.x == neg_inf()) continue;  // it saw no key
+    const float* ws = a.ws + (static_cast<long long>(part) * DP + d) * ROWS + row;
+    float v[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = ws[x * ROWS];
+    const float mn = max2(m, q.x);
+    const float f0 = ex2(m - mn), f1 = ex2(q.x - mn);
+    m = mn;
+    l = l * f0 + q.y * f1;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) acc[x] = acc[x] * f0 + v[x] * f1;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t w[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) w[x] = pack2(acc[2 * x] * inv, acc[2 * x + 1] * inv, T{});
+  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (cut.row0 + token) * a.os[0] +
+                            head * a.os[1] + d) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// ---------------------------------------------------------------- launch
+Plan plan_chunk(const srdit_seq_attn_args& u, int sms) {
+  Plan p = {};
+  const int group = u.H / u.Hkv;
+  // heads of a group side by side in a query tile, a power of two of them
+  p.pack = 1;
+  while (p.pack < TILE && group % (2 * p.pack) == 0) p.pack *= 2;
+  p.rt = TILE / p.pack;
+  p.slots = u.T / (2 * p.rt) + u.B;
+  p.nhp = u.H / p.pack;
+  const long long items = static_cast<long long>(p.slots) * p.nhp;
+  long long keys = u.Tk;
+  if (u.pages) {
+    const long long held = static_cast<long long>(u.pages->table_width) * u.pages->page_size;
+    keys = u.max_kv > 0 && u.max_kv < held ? u.max_kv : held;
+  }
+  const long long tiles = (keys + TILE - 1) / TILE;
+  // few items of many key tiles: shared out by key tiles (items x tiles in 32 bits)
+  p.ranged = items < 2 * sms && p.slots <= MAX_SLOTS && tiles > 8 && items * tiles < (1ll << 30);
+  p.ctas = static_cast<int>(p.ranged || items > sms ? sms : items);
+  p.ws_floats = p.ranged ? 2ll * p.ctas * ROWS * ((u.D <= 64 ? 64 : 128) + 2) + 4 * p.ctas : 0;
+  return p;
+}
+
+template <typename T, int DP, int CODE>
+static int launch(const srdit_seq_attn_args& u, const Args& a, const Plan& p, cudaStream_t stream) {
+  using C = ChunkCfg<DP, CODE>;
+  auto kern = chunk_kernel<T, DP, CODE>;
+  static std::atomic<bool> attr_done[kMaxDevices] = {};
+  int rc = set_smem(kern, C::SMEM, attr_done);
+  if (rc) return rc;
+  CUtensorMap tq, tk, tv;
+  {
+    const long long row = (u.D + 7) / 8 * 16;
+    const bool ut = u.T > 1, uh = u.H > 1 && u.q_stride[1] > 0;
+    const long long dims[4] = {u.D, uh ? u.H : 1, u.T, 1};
+    const long long strides[3] = {uh ? u.q_stride[1] * 2 : row, ut ? u.q_stride[0] * 2 : row, row};
+    const int box[4] = {64, p.pack, p.rt, 1};
+    rc = make_tmap_4d(&tq, u.q, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, dims, strides, box);
+  }
+  const int cols = C::CODES ? 128 : 64;
+  if (!rc) rc = key_map(&tk, u, false, cols, 1 << a.box_log);
+  if (!rc) rc = key_map(&tv, u, true, cols, 1 << a.box_log);
+  if (rc) return rc;
+  const bool packed = u.pages == nullptr;
+  SRDIT_LAUNCH((kern), p.ctas, C::THREADS, C::SMEM, stream, tq, tk, tv, a,
+               packed && u.k_stride[1] == 0, packed && u.v_stride[1] == 0);
+  rc = static_cast<int>(cudaGetLastError());
+  if (rc || !p.ranged) return rc;
+  SRDIT_LAUNCH((join_chunk_kernel<T, DP>), dim3(p.ctas, ROWS / 32), DP / 8 * 32, 0, stream, a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int CODE>
+static int launch_size(const srdit_seq_attn_args& u, const Args& a, const Plan& p,
+                       cudaStream_t stream) {
+  return u.D <= 64 ? launch<T, 64, CODE>(u, a, p, stream) : launch<T, 128, CODE>(u, a, p, stream);
+}
+
+template <typename T>
+static int run_typed(const srdit_seq_attn_args& u, const Args& a, const Plan& p,
+                     cudaStream_t stream) {
+  switch (u.pages ? u.pages->code : SRDIT_KV_PLAIN) {
+    case SRDIT_Q_INT8: return launch_size<T, SRDIT_Q_INT8>(u, a, p, stream);
+    case SRDIT_Q_E4M3: return launch_size<T, SRDIT_Q_E4M3>(u, a, p, stream);
+    default: return launch_size<T, SRDIT_KV_PLAIN>(u, a, p, stream);
+  }
+}
+
+int run_chunk(const srdit_seq_attn_args& u, Args& a, const Plan& p, cudaStream_t stream) {
+  a.pack = p.pack;
+  a.rt = p.rt;
+  a.slots = p.slots;
+  a.nhp = p.nhp;
+  a.by_nhp = Divisor::of(p.nhp);
+  a.by_slots = Divisor::of(p.slots);
+  a.by_piece = Divisor::of(2 * p.rt);
+  a.ranged = p.ranged;
+  const int page = u.pages ? u.pages->page_size : TILE;
+  a.box_log = page >= TILE ? 7 : page == 64 ? 6 : page == 32 ? 5 : 4;
+  const long long rows = 2ll * p.ctas * ROWS;
+  a.ml = a.ws + rows * (u.D <= 64 ? 64 : 128);
+  a.cuts = a.ml + 2 * rows;
+  return u.dtype == SRDIT_BF16 ? run_typed<__nv_bfloat16>(u, a, p, stream)
+                               : run_typed<__half>(u, a, p, stream);
+}
+
+}  // namespace sattn
+}  // namespace srdit

@@ -380,3 +380,59 @@ def test_refusals(srdit, cuda_device):
                dict(k=x[..., :60], v=x[..., :60], q=x[..., :60]), dict(scale=-1.0)):
         with pytest.raises(err):
             pk(**kw)
+
+
+# ------------------------------------------------------------------ values that are not finite
+def _poison(g, cache, code, b, token, what):
+    """Make a cached token's value of key head 1 not finite: an element, a scale, a code."""
+    page, row = cache.places(b, token, token + 1)
+    if code is None:
+        cache.v[page, row, 1, 3] = what
+    elif code == torch.float8_e4m3fn and what != what:
+        cache.v.view(torch.uint8)[page, row, 1, 3] = 0x7F
+    else:
+        cache.vs[page, row, 1] = what
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("what", (float("nan"), float("inf")))
+@pytest.mark.parametrize("new,lens,at", [
+    ([4, 3], [70, 35], 68), ([7, 1], [23, 9], 17), ([130, 20], [400, 90], 300),
+    ([260, 5], [260, 300], 129), ([200, 77], [1000, 77], 999)])
+def test_hidden_values_may_be_anything(srdit, cuda_device, code, what, new, lens, at):
+    """A value that a causal mask hides from a query is not in its answer, finite or not; the
+    queries that see it get no finite one."""
+    g, dt = gen(50), torch.bfloat16
+    cache = Cache(g, lens, 2, 64, 16, code or dt).fill(g, dt)
+    cu, H = offsets(new), 4
+    q = randn(g, sum(new), H, 64).to(dt)
+
+    def call():
+        return srdit.ops.paged_attn(q, cache.k, cache.v, cache.table, cache.lens_dev, cu_q=cu,
+                                    max_q=max(new), **cache.scales)
+
+    want = call()
+    check_paged(cache, q, cu, want, True, 64 ** -0.5)
+    _poison(g, cache, code, 0, at, what)
+    got = call()
+    see = at - (lens[0] - new[0])   # the first query that sees it
+    rest = torch.ones(sum(new), H, dtype=torch.bool, device="cuda")
+    rest[max(see, 0):new[0], 2:] = False
+    assert torch.equal(got[rest], want[rest])
+    assert (~got[~rest].isfinite()).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("what", (float("nan"), -float("inf")))
+@pytest.mark.parametrize("at", (0, 100, 255, 256, 511))
+def test_hidden_values_of_a_prompt(srdit, cuda_device, dtype, what, at):
+    g = gen(51)
+    q, k, v = (randn(g, 512, 2, 64).to(dtype) for _ in range(3))
+    cu = offsets([512])
+    want = srdit.ops.packed_attn(q, k, v, cu)
+    v[at, 1, 7] = what
+    got = srdit.ops.packed_attn(q, k, v, cu)
+    rest = torch.ones(512, 2, dtype=torch.bool, device="cuda")
+    rest[at:, 1] = False
+    assert torch.equal(got[rest], want[rest])
+    assert (~got[~rest].isfinite()).any(-1).all()

@@ -154,3 +154,27 @@ def test_no_cpu_path(srdit):
                  lambda: ops.packed_attn(x, x, x, i[:, 0])):
         with pytest.raises(err):
             call()
+
+
+# ------------------------------------------------------------------ the kernels' sources
+from tests.test_bounded_waits_cpu import _code, _without_single_threads  # noqa: E402
+
+
+@pytest.mark.parametrize("name", ("seq_step.cu", "seq_chunk.cu"))
+def test_a_warp_gives_up_as_one(name):
+    """As tests/test_bounded_waits_cpu.py has it for the other kernels: a wait of a whole warp
+    has one answer, or none is asked for and the abort flag is voted on."""
+    text = _code(name)
+    assert "mbar_wait" in text and "named_barrier" not in text
+    shared = _without_single_threads(text)
+    for m in re.finditer(r"\bmbar_wait\(", shared):
+        assert re.search(r"[;{}]\s*$", shared[:m.start()]), shared[m.start() - 40:m.end() + 60]
+        assert shared[m.start():shared.index(";", m.end())].endswith("abort_flag)")
+        assert "if (__any_sync(0xffffffffu, *abort_flag != 0u)) break;" in shared
+
+
+def test_clusters_are_never_launched_programmatically(srdit):
+    text = (srdit._lib.PKG / "csrc" / "seq_step.cu").read_text()
+    body = re.search(r"^static int launch\(.*?^\}", text, re.S | re.M).group(0)
+    assert "launch_clusters(" in body and "SRDIT_LAUNCH" not in body
+    assert text.count("step_kernel<T, DP, NT, CODE>") == 2   # its shared memory, its launch
