@@ -45,7 +45,7 @@ struct Plan {
   bool step;                    // step_kernel (few rows per key head), else chunk_kernel
   int splits, cluster, parts;   // step_kernel; parts in the workspace per row (1: none)
   int pack, rt, slots, nhp;     // chunk_kernel
-  bool ranged;
+  int ranged;                   // 0: whole items, 1: shared out by key tiles, 2: the last round
   int ctas;
   long long ws_floats;
 };

@@ -9,10 +9,15 @@
 // Warps: 0 loads keys, values and queries by TMA, 1 issues the products, 2 finds the CTA's items
 // and passes them on as records, 3 (16-bit keys) looks over the values of tiles that are partly
 // hidden, 4 to 7 and 8 to 11 are the softmax of one query tile each, a row a thread, and with codes
-// 12 to 15 widen them: codes come through a ring of their own and go to the tensor core as fp16,
-// which holds them exactly, and so do the queries. A key's scale then multiplies its scores, a
-// value's its weights, both in fp32. The running maximum is that of score + log2(largest scale of
-// the tile's values), so that weight times scale stays at 2^8 or below.
+// 12 to 15 widen them in place.
+//
+// Codes go to the tensor core as fp16, which holds them exactly, and so do the queries.
+//   fp16 queries   a key's scale multiplies its scores, a value's its weights, both in fp32
+//   bf16 queries   become fp16 times a power of two per row; code times scale is rounded once to
+//                  fp16 (an eighth of the answer's rounding), in units that are a power of two per 32
+//                  keys
+// Either way the running maximum is that of score + log2(unit of the values), so that the weights
+// stay at 2^8 or below, and the sum is of weights in the unit of one.
 #include <atomic>
 
 #include "seq_attn.cuh"
@@ -24,6 +29,7 @@ constexpr int ROWS = 2 * TILE;    // of an item
 constexpr int MAX_SLOTS = 256;    // pieces of sequences of a ranged launch
 constexpr int MIN_SHARE = 4;      // key tiles that a ranged CTA takes at least
 constexpr int RECORDS = 4;
+constexpr int MAX_SEQS = 64;      // sequences that are kept in shared memory
 
 template <int DP, int CODE>
 struct ChunkCfg {
@@ -31,17 +37,18 @@ struct ChunkCfg {
   static constexpr int THREADS = CODES ? 512 : 384;
   static constexpr int SLAB = TILE * 128;  // 128 rows x 64 values
   static constexpr int BYTES = SLAB * (DP / 64);
-  static constexpr int STAGES = CODES ? (DP == 128 ? 3 : 6) : (DP == 128 ? 4 : 8);
-  static constexpr int RAW = 2;            // tiles of codes
+  static constexpr int STAGES = DP == 128 ? 4 : CODES ? 6 : 8;
+  static constexpr int RAW = BYTES - SLAB;  // where in a stage codes land: its last slab
   static constexpr int OFF_KV = 2 * BYTES;
-  static constexpr int OFF_RAW = OFF_KV + STAGES * BYTES;
-  static constexpr int OFF_STG = OFF_RAW + (CODES ? RAW * SLAB : 0);  // 32 rows x 64 bytes a warp
+  static constexpr int OFF_STG = OFF_KV + STAGES * BYTES;  // 32 rows x 64 bytes a warp
   static constexpr int SCALES = 4;         // tiles whose scales are kept: [2][128] each
   static constexpr int OFF_SC = OFF_STG + 8 * 2048;
-  static constexpr int OFF_Q = OFF_SC + (CODES ? SCALES * 1024 : 0);  // queries' factors [2][256]
+  static constexpr int OFF_UNITS = OFF_SC + (CODES ? SCALES * 1024 : 0);  // ... and units [2][4]
+  static constexpr int OFF_Q = OFF_UNITS + (CODES ? SCALES * 32 : 0);  // queries' factors [2][256]
   static constexpr int OFF_REC = OFF_Q + (CODES ? 2048 : 0);
-  static constexpr int OFF_STEPS = OFF_REC + RECORDS * 64;  // ranged: where each piece begins
-  static constexpr int OFF_GAPS = OFF_STEPS + MAX_SLOTS * 4;  // keys without a page, 8 tiles
+  static constexpr int OFF_STEPS = OFF_REC + RECORDS * 64;  // ranged: the pieces
+  static constexpr int OFF_SEQS = OFF_STEPS + (2 * MAX_SLOTS + 4) * 4;
+  static constexpr int OFF_GAPS = OFF_SEQS + MAX_SEQS * 16;  // keys without a page, 8 tiles
   static constexpr int GAPS = 8;
   static constexpr int OFF_BAD = OFF_GAPS + GAPS * 16;        // values that are not finite
   static constexpr int OFF_BAR = OFF_BAD + STAGES * 16;
@@ -78,8 +85,14 @@ struct Cut {
 // end are empty.
 struct Pieces {
   const Args& a;
+  const int4* seqs;  // {begin, end, keys, first key's row} in shared memory, or null
+
+  static SRDIT_DEV int4 sequence(const Args& a, int b) {
+    return make_int4(a.rows.begin(b), a.rows.end(b), a.key_count(b),
+                     a.paged() ? 0 : a.keys.begin(b));
+  }
   SRDIT_DEV int base(int b) const {
-    return a.by_piece.div(a.rows.at ? a.rows.begin(b) : b * a.rows.each) + b;
+    return a.by_piece.div(seqs ? seqs[b].x : a.rows.begin(b)) + b;
   }
   // the last sequence whose base is not above n, by one thread
   SRDIT_DEV int find(int n) const {
@@ -104,14 +117,15 @@ struct Pieces {
   }
   // the item of piece n of sequence b; false: there is none
   SRDIT_DEV bool item(int b, int n, Record& r) const {
-    const int begin = a.rows.begin(b), tokens = a.rows.end(b) - begin;
-    const int at = (n - base(b)) * 2 * a.rt;
+    const int4 q = seqs ? seqs[b] : sequence(a, b);
+    const int tokens = q.y - q.x;
+    const int at = (n - a.by_piece.div(q.x) - b) * 2 * a.rt;
     if (at < 0 || at >= tokens) return false;
     r.b = b;
-    r.row0 = begin + at;
+    r.row0 = q.x + at;
     r.tokens = min(2 * a.rt, tokens - at);
-    r.len = a.key_count(b);
-    r.kv0 = a.paged() ? 0 : a.keys.begin(b);
+    r.len = q.z;
+    r.kv0 = q.w;
     r.pos0 = r.len - tokens + at;
     r.t0 = 0;
     const int tiles = (r.len + TILE - 1) / TILE;
@@ -134,18 +148,17 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   pdl_begin();
   using C = ChunkCfg<DP, CODE>;
   using E = typename Compute<T, CODE>::type;
-  constexpr int STAGES = C::STAGES, RAW = C::RAW;
+  constexpr int STAGES = C::STAGES;
   constexpr bool CODES = C::CODES;
-  constexpr bool TURN_Q = CODES && !__is_same(T, __half);  // queries become fp16
+  // bf16 queries and codes: the queries become fp16, and codes times their scales too
+  constexpr bool FOLD = CODES && !__is_same(T, __half);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // 16-bit keys: by TMA
+  uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // by TMA
   uint64_t* full = loaded + STAGES;     // ready for the products
   uint64_t* empty = full + STAGES;
-  uint64_t* raw_full = empty + STAGES;  // codes
-  uint64_t* raw_empty = raw_full + RAW;
-  uint64_t* q_loaded = raw_empty + RAW;  // [2], one per query tile
+  uint64_t* q_loaded = empty + STAGES;  // [2], one per query tile
   uint64_t* q_full = q_loaded + 2;
   uint64_t* q_empty = q_full + 2;
   uint64_t* s_full = q_empty + 2;     // scores of a tile ready
@@ -154,11 +167,14 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   uint64_t* o_full = p_half + 2;      // its last product done
   uint64_t* rec_full = o_full + 2;
   uint64_t* rec_empty = rec_full + RECORDS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rec_empty + RECORDS);
+  uint64_t* sc_full = rec_empty + RECORDS;  // codes: a tile's scales are there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_full + C::SCALES);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  static_assert((3 * STAGES + 2 * RAW + 14 + 2 * RECORDS) * 8 + 8 <= 512, "barrier area");
+  static_assert((3 * STAGES + 14 + 2 * RECORDS + C::SCALES) * 8 + 8 <= 512, "barrier area");
   Record* records = reinterpret_cast<Record*>(smem + C::OFF_REC);
-  int* starts = reinterpret_cast<int*>(smem + C::OFF_STEPS);
+  int* starts = reinterpret_cast<int*>(smem + C::OFF_STEPS);  // first key tile of each piece
+  int* numbers = starts + MAX_SLOTS + 4;                      // ... and its number
+  int4* seqs = reinterpret_cast<int4*>(smem + C::OFF_SEQS);
   uint4* gaps = reinterpret_cast<uint4*>(smem + C::OFF_GAPS);  // by tiles, a bit a key
   uint4* bad = reinterpret_cast<uint4*>(smem + C::OFF_BAD);    // by stages
 
@@ -168,10 +184,6 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       mbar_init(&loaded[s], 1);
       mbar_init(&full[s], CODES ? 4 : 1);
       mbar_init(&empty[s], 1);
-    }
-    for (int s = 0; s < RAW; ++s) {
-      mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], 4);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_loaded[t], 1);
@@ -184,8 +196,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     }
     for (int s = 0; s < RECORDS; ++s) {
       mbar_init(&rec_full[s], 1);
-      mbar_init(&rec_empty[s], 10 + (CODES ? 4 : 1));
+      mbar_init(&rec_empty[s], CODES ? 15 : 11);
     }
+    for (int s = 0; s < C::SCALES; ++s) mbar_init(&sc_full[s], 1);
     *abort_flag = 0u;
     fence_barrier_init();
   }
@@ -198,6 +211,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if (warp >= 4 && static_cast<int>(threadIdx.x) - 128 < min(a.B, MAX_SEQS))
+    seqs[threadIdx.x - 128] = Pieces::sequence(a, threadIdx.x - 128);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -206,6 +221,16 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   // a tile that some query of the item does not see whole by place
   auto partly = [&](const Record& r, int key0) {
     return key0 + TILE > r.len || (a.causal && key0 + TILE - 1 > r.pos0);
+  };
+  // FOLD: 32 keys' scales over 2^e, in [2^6, 2^7) for the largest finite one, so that code times
+  // scale, at most 448 x 2^7, is one of fp16; and f = 2^e
+  auto in_units = [](float scale, float& f, float& e) {
+    const uint32_t top = __reduce_max_sync(
+        0xffffffffu, scale < 3e38f ? __float_as_uint(fmaxf(scale, 0.f)) : 0u);
+    const int x = max(static_cast<int>(top >> 23) - 133, -100);
+    f = exp2_int(x);
+    e = static_cast<float>(x);
+    return scale * exp2_int(-x);
   };
   if (warp < 4) {
     if constexpr (CODES)
@@ -262,38 +287,30 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           const int h = (v ? v_one_head : k_one_head) ? 0 : g;
           const int at_page = page >= 0 ? page : max(a.table.pages, 1);  // past the pages: zeros
           const unsigned gap_boxes = __ballot_sync(0xffffffffu, gap);
-          if constexpr (CODES) {
-            const int s = idx % RAW;
-            if (!mbar_wait_warp(&raw_empty[s], (static_cast<uint32_t>(idx / RAW) & 1u) ^ 1u,
-                                a.status, abort_flag))
-              return false;
-            if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], C::SLAB);
-            __syncwarp();
-            if (lane < boxes)
-              tma_load_4d(smem + C::OFF_RAW + s * C::SLAB + (lane << a.box_log) * 128, tm,
-                          &raw_full[s], 0, h, row, at_page);
-          } else {
-            const int s = idx % STAGES;
-            if (!mbar_wait_warp(&empty[s], (static_cast<uint32_t>(idx / STAGES) & 1u) ^ 1u,
-                                a.status, abort_flag))
-              return false;
-            if (!v) {
-              if (lane < 4) {
-                const uint32_t lo = (gap_boxes >> ((lane * 32) >> a.box_log)) & 1u;
-                const uint32_t hi = (gap_boxes >> ((lane * 32 + 16) >> a.box_log)) & 1u;
-                reinterpret_cast<uint32_t*>(gaps + tiles % C::GAPS)[lane] =
-                    (lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u);
-              }
-              ++tiles;
-              __syncwarp();
+          const int s = idx % STAGES;
+          if (!mbar_wait_warp(&empty[s], (static_cast<uint32_t>(idx / STAGES) & 1u) ^ 1u, a.status,
+                              abort_flag))
+            return false;
+          if (!CODES && !v) {
+            if (lane < 4) {
+              const uint32_t lo = (gap_boxes >> ((lane * 32) >> a.box_log)) & 1u;
+              const uint32_t hi = (gap_boxes >> ((lane * 32 + 16) >> a.box_log)) & 1u;
+              reinterpret_cast<uint32_t*>(gaps + tiles % C::GAPS)[lane] =
+                  (lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u);
             }
-            if (lane == 0) mbar_arrive_expect_tx(&loaded[s], C::BYTES);
+            ++tiles;
             __syncwarp();
-            if (lane < boxes)
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&loaded[s], CODES ? C::SLAB : C::BYTES);
+          __syncwarp();
+          uint8_t* dst = smem + C::OFF_KV + s * C::BYTES + (lane << a.box_log) * 128;
+          if (lane < boxes) {
+            if constexpr (CODES) {
+              tma_load_4d(dst + C::RAW, tm, &loaded[s], 0, h, row, at_page);
+            } else {
               for (int d = 0; d < DP / 64; ++d)
-                tma_load_4d(smem + C::OFF_KV + s * C::BYTES + d * C::SLAB +
-                                (lane << a.box_log) * 128,
-                            tm, &loaded[s], d * 64, h, row, at_page);
+                tma_load_4d(dst + d * C::SLAB, tm, &loaded[s], d * 64, h, row, at_page);
+            }
           }
           ++idx;
           return true;
@@ -330,7 +347,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                            static_cast<uint32_t>(u / STAGES) & 1u, a.status, abort_flag);
         };
         auto q_wait = [&](int t) {
-          return mbar_wait((TURN_Q ? q_full : q_loaded) + t, static_cast<uint32_t>(nq[t]++) & 1u,
+          return mbar_wait((FOLD ? q_full : q_loaded) + t, static_cast<uint32_t>(nq[t]++) & 1u,
                            a.status, abort_flag);
         };
         auto scores = [&](int t, int u) {  // S_t = Q_t K^T, K in ring use u
@@ -441,7 +458,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       __syncwarp();
     } else if (warp == 2) {
       // ------------------------------------------------------------ items
-      const Pieces pieces{a};
+      const Pieces pieces{a, a.B <= MAX_SEQS ? seqs : nullptr};
       int n = 0;
       auto pass = [&](const Record& r) {
         const int at = n % RECORDS;
@@ -459,10 +476,12 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       Record r = {};
       bool ok = true;
       if (!a.ranged) {
-        // whole items, every gridDim-th one. Causal: the last pieces first (the longest), all heads
-        // of a piece side by side; else a head's pieces, which share its keys, side by side.
-        const int items = a.slots * a.nhp;
-        for (int x = blockIdx.x; x < items && ok; x += gridDim.x) {
+        // Whole items, one of every gridDim. Causal: the last pieces first (the longest), all heads
+        // of a piece side by side, in rounds that go forth and back, so that no CTA has the longest
+        // of every round; else a head's pieces, which share its keys, side by side.
+        const int items = a.slots * a.nhp, ctas = static_cast<int>(gridDim.x);
+        int at = blockIdx.x, step = 2 * (ctas - 1 - at) + 1;
+        for (int x = at; x < items && ok;) {
           int slot, hp;
           if (a.causal) {
             slot = a.by_nhp.div(x);
@@ -472,57 +491,79 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             hp = a.by_slots.div(x);
             slot = x - hp * a.slots;
           }
+          if (a.causal) {
+            x += step;
+            step = 2 * ctas - step;
+          } else {
+            x += ctas;
+          }
           if (!pieces.item(pieces.find_warp(slot), slot, r)) continue;
           r.h0 = hp * a.pack;
           ok = pass(r);
         }
       } else {
-        // an equal share of all items' key tiles, head pack by head pack (an item without any
-        // counts as one). starts[]: where each piece begins.
-        int total = 0;
+        // The pieces that there are, head pack by head pack, are the items. Whole ones in rounds as
+        // long as every CTA gets one (a.ranged 2), whose CTAs share keys; of the others an equal
+        // share of the key tiles (an item without any counts as one).
+        int total = 0, count = 0;
         for (int s0 = 0; s0 < a.slots; s0 += 32) {
           const int s = s0 + lane;
           int w = 0;
           if (s < a.slots && pieces.item(pieces.find(s), s, r)) w = max(1, max(r.e0, r.e1));
+          const unsigned found = __ballot_sync(0xffffffffu, w > 0);
           int sum = w;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += y;
           }
-          if (s < a.slots) starts[s] = total + sum - w;
+          if (w > 0) {
+            const int at = count + __popc(found & ((1u << lane) - 1u));
+            starts[at] = total + sum - w;
+            numbers[at] = s;
+          }
           total += __shfl_sync(0xffffffffu, sum, 31);
+          count += __popc(found);
         }
+        if (lane == 0) starts[count] = total;
         __syncwarp();
-        const int all = total * a.nhp;
-        const int share = max((all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x),
-                              MIN_SHARE);
-        int s = blockIdx.x * share;
+        const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
+        auto load = [&](int n, int hp) {
+          pieces.item(pieces.find_warp(numbers[n]), numbers[n], r);
+          r.h0 = hp * a.pack;
+        };
+        int whole = a.ranged == 2 ? count * a.nhp / ctas * ctas : 0;
+        for (int x = cta; x < whole && ok; x += ctas) {
+          load(x % count, x / count);
+          ok = pass(r);
+        }
+        if (count == 0) whole = 0;
+        const int hp0 = count > 0 ? whole / count : 0, n0 = whole - hp0 * count;
+        const int s0 = hp0 * total + (count > 0 ? starts[n0] : 0);
+        const int all = total * a.nhp - s0;
+        const int share = max((all + ctas - 1) / ctas, MIN_SHARE);
+        int s = cta * share;
         const int s1 = min(s + share, all);
-        if (lane == 0) static_cast<Cut*>(a.cuts)[blockIdx.x].parts = 0;
-        if (s < s1) {
-          int hp = s / total, x = s - hp * total;
-          int slot = 0;  // the last piece that does not begin behind x
-          for (int o = 128; o; o >>= 1)
-            if (slot + o < a.slots && starts[slot + o] <= x) slot += o;
+        if (lane == 0) static_cast<Cut*>(a.cuts)[cta].parts = 0;
+        if (s < s1 && ok) {
+          int hp = (s0 + s) / total, x = s0 + s - hp * total;
+          int n = 0;  // the piece that key tile x is of
+          for (int o = MAX_SLOTS / 2; o; o >>= 1)
+            if (n + o < count && starts[n + o] <= x) n += o;
           while (s < s1 && ok) {
-            const bool found = pieces.item(pieces.find_warp(slot), slot, r);
-            const int w = found ? max(1, max(r.e0, r.e1)) : 0;
-            if (x < starts[slot] + w) {
-              const int t0 = x - starts[slot], t1 = min(w, t0 + (s1 - s));
-              r.h0 = hp * a.pack;
-              r.t0 = t0;
-              r.e0 = max(t0, min(r.e0, t1));
-              r.e1 = max(t0, min(r.e1, t1));
-              const int cta = static_cast<int>(blockIdx.x);
-              r.part = t0 > 0 ? 2 * cta : t1 < w ? 2 * cta + 1 : -1;
-              if (t0 == 0 && t1 < w) r.parts = (s + w - 1) / share - cta + 1;
-              ok = pass(r);
-              s += t1 - t0;
-              x += t1 - t0;
-            }
-            if (++slot == a.slots) {
-              slot = 0;
+            load(n, hp);
+            const int w = starts[n + 1] - starts[n];
+            const int t0 = x - starts[n], t1 = min(w, t0 + (s1 - s));
+            r.t0 = t0;
+            r.e0 = max(t0, min(r.e0, t1));
+            r.e1 = max(t0, min(r.e1, t1));
+            r.part = t0 > 0 ? 2 * cta : t1 < w ? 2 * cta + 1 : -1;
+            if (t0 == 0 && t1 < w) r.parts = (s + w - 1) / share - cta + 1;
+            ok = pass(r);
+            s += t1 - t0;
+            x += t1 - t0;
+            if (++n == count) {
+              n = 0;
               x = 0;
               ++hp;
             }
@@ -585,6 +626,84 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         }
         idx += 2 * max(steps, 0);
       }
+    } else {
+      // ------------------------------------------------------------ scales of codes
+      // The scales of a tile's keys, 0 where there is none, four keys a lane; pages are read two
+      // tiles ahead, scales one.
+      float* scales = reinterpret_cast<float*>(smem + C::OFF_SC);
+      float* units = reinterpret_cast<float*>(smem + C::OFF_UNITS);
+      int idx = 0, tiles = 0;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int at = n % RECORDS;
+        ok = mbar_wait_warp(&rec_full[at], static_cast<uint32_t>(n / RECORDS) & 1u, a.status,
+                            abort_flag);
+        if (!ok) break;
+        const int t0 = records[at].t0, steps = records[at].steps(), len = records[at].len;
+        const int b = records[at].b, g = records[at].h0 / a.group, tokens = records[at].tokens;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&rec_empty[at]);
+        if (tokens == 0) break;
+        const float* ks = a.scale[0] + g * a.ss[0][2];
+        const float* vs = a.scale[1] + g * a.ss[1][2];
+        auto page_of = [&](int j, int w) {
+          const int x = (t0 + j) * TILE + w * 32 + lane;
+          return j < steps && x < len ? a.table.page(b, a.table.by_page.div(x)) : -1;
+        };
+        int page[4], page1[4];
+        float k[4], v[4];
+        auto fetch = [&](int j) {  // page[]: tile j's
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            k[w] = v[w] = 0.f;
+            if (page[w] < 0) continue;
+            const int x = (t0 + j) * TILE + w * 32 + lane;
+            const long long in = x - a.table.by_page.div(x) * a.table.page_size;
+            k[w] = __ldg(ks + page[w] * a.ss[0][0] + in * a.ss[0][1]);
+            v[w] = __ldg(vs + page[w] * a.ss[1][0] + in * a.ss[1][1]);
+          }
+        };
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          page[w] = page_of(0, w);
+          page1[w] = page_of(1, w);
+        }
+        fetch(0);
+        for (int j = 0; j < steps && ok; ++j) {
+          // the tile's K stage is taken: nobody reads what its place held before
+          const int s = idx % STAGES;
+          ok = mbar_wait_warp(&loaded[s], static_cast<uint32_t>(idx / STAGES) & 1u, a.status,
+                              abort_flag);
+          if (!ok) break;
+          idx += 2;
+          const int place = tiles % C::SCALES;
+          float* sc = scales + place * 256;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const unsigned gap = __ballot_sync(
+                0xffffffffu, page[w] < 0 && (t0 + j) * TILE + w * 32 + lane < len);
+            if (lane == 0) reinterpret_cast<uint32_t*>(gaps + tiles % C::GAPS)[w] = gap;
+            if constexpr (FOLD) {
+              float f, e;
+              k[w] = in_units(k[w], f, e);
+              if (lane == 0) units[place * 8 + w] = f;
+              v[w] = in_units(v[w], f, e);
+              if (lane == 0) units[place * 8 + 4 + w] = e;
+            }
+            sc[w * 32 + lane] = k[w];
+            sc[128 + w * 32 + lane] = v[w];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[place]);
+          ++tiles;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            page[w] = page1[w];
+            page1[w] = page_of(j + 2, w);
+          }
+          fetch(j + 1);
+        }
+      }
     }
   } else if (warp < 12) {
     if constexpr (CODES)
@@ -630,8 +749,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         ++ns;
         tc_fence_after();
         // what was noted before the products that are done now
-        if (TURN_Q && j == 0) c = q_back[(n & 1) * 256 + t * 128 + row];
-        const uint64_t c2 = f2_pack(c, c);
+        if (FOLD && j == 0) c = q_back[(n & 1) * 256 + t * 128 + row];
         const uint4 gap = gaps[tiles % C::GAPS];
         const bool masked = key0 + TILE - 1 > lim0 || (gap.x | gap.y | gap.z | gap.w) != 0u;
         uint32_t vis[4];
@@ -648,7 +766,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         for (int w = 0; w < 4; ++w) tmem_ld32(s_tmem + w * 32, s[w]);
         tmem_ld_wait();
         const float* sc = scales + (tiles % C::SCALES) * 256;
-        if constexpr (CODES) {
+        if constexpr (CODES && !FOLD) {
 #pragma unroll
           for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -680,8 +798,27 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             mx[w] = max3(mx[w], __uint_as_float(s[w][x]), __uint_as_float(s[w][x + 1]));
           mx[w] = max2(mx[w], __uint_as_float(s[w][31]));
         }
-        float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
-        if constexpr (CODES) {  // the values' scales are there with the V tile
+        // per 32 keys: the scores' factor, and log2 of the unit that the values are in
+        float cw[4], lv[4];
+        float top;
+        if constexpr (FOLD) {
+          const float* units = reinterpret_cast<const float*>(smem + C::OFF_UNITS) +
+                               tiles % C::SCALES * 8;
+          const float4 f = *reinterpret_cast<const float4*>(units);
+          const float4 v = *reinterpret_cast<const float4*>(units + 4);
+          const float u[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) cw[w] = fmaxf(c * u[w], 1.2e-38f);  // (0 times -inf is NaN)
+          lv[0] = v.x, lv[1] = v.y, lv[2] = v.z, lv[3] = v.w;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) mx[w] = fmaf(mx[w], cw[w], lv[w]);
+          top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) cw[w] = c, lv[w] = 0.f;
+          top = max2(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
+        }
+        if constexpr (CODES && !FOLD) {  // the values' scales are there with the V tile
           mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u, a.status,
                     abort_flag);
           float most = 0.f;
@@ -701,7 +838,6 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         const float alpha = raise ? ex2(m - m_new) : 1.f;
         m = m_new;
         const float neg_m = m == neg_inf() ? 0.f : -m;
-        const uint64_t neg_m2 = f2_pack(neg_m, neg_m);
         if (j > 0 && __any_sync(0xffffffffu, raise)) {
           // scores of this tile are ready, so the product before it is done
 #pragma unroll 1
@@ -715,18 +851,22 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           }
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 4; ++w) {
+          const uint64_t c2 = f2_pack(cw[w], cw[w]);
+          const uint64_t neg_m2 = f2_pack(neg_m + lv[w], neg_m + lv[w]);
 #pragma unroll
           for (int x = 0; x < 32; x += 2) {
             const float2 y = f2_split(f2_fma(u64_of(s[w][x], s[w][x + 1]), c2, neg_m2));
             s[w][x] = __float_as_uint(y.x);
             s[w][x + 1] = __float_as_uint(y.y);
           }
+        }
         uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+        l *= alpha;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t pw[16];
-          if constexpr (CODES) {
+          if constexpr (CODES && !FOLD) {
 #pragma unroll
             for (int x = 0; x < 32; x += 4) {
               const float4 v = *reinterpret_cast<const float4*>(sc + 128 + w * 32 + x);
@@ -757,6 +897,11 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               pw[x >> 1] = pack2(p.x, p.y, E{});
             }
           }
+          if constexpr (FOLD) {  // the sum of weights in the unit of one
+            const float2 sp = f2_split(f2_add(sum[0], sum[1]));
+            l = fmaf(sp.x + sp.y, ex2(-lv[w]), l);
+            sum[0] = sum[1] = f2_pack(0.f, 0.f);
+          }
           if (w == 2) {  // the first 64 keys' weights, stored by now: their product can begin
             tmem_st_wait();
             tc_fence_before();
@@ -765,9 +910,11 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           }
           tmem_st16(s_tmem + w * 16, pw);
         }
-        const float2 sp = f2_split(f2_add(sum[0], sum[1]));
-        l = l * alpha + (sp.x + sp.y);
-        if constexpr (!CODES) {
+        if constexpr (!FOLD) {
+          const float2 sp = f2_split(f2_add(sum[0], sum[1]));
+          l += sp.x + sp.y;
+        }
+        if constexpr (!CODES || FOLD) {
           if (a.causal && key0 + TILE - 1 > pos0) {  // values taken out, as not finite
             mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u,
                       a.status, abort_flag);
@@ -854,7 +1001,6 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     // ------------------------------------------------------------ codes to fp16
     const int w = warp - 12;
     const int r8 = lane & 7, y0 = lane >> 3;  // a lane's row of 8, its pieces of 16 bytes
-    const int key = w * 32 + lane;            // whose scales this lane fetches
     float* scales = reinterpret_cast<float*>(smem + C::OFF_SC);
     float* q_back = reinterpret_cast<float*>(smem + C::OFF_Q);
     int idx = 0, tiles = 0, nq[2] = {0, 0};
@@ -870,23 +1016,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       if (r.tokens == 0) break;
       const int steps = r.steps();
       if (steps <= 0) continue;
-      const int g = r.h0 / a.group;
-      // the scales of a tile's keys, 0 where there is none; whether a key has no page
-      bool here = false;
-      auto scales_of = [&](int tile, float& k, float& v) {
-        const int x = tile * TILE + key;
-        k = v = 0.f;
-        here = true;
-        if (x >= r.len) return;
-        const int p = a.table.by_page.div(x), in = x - p * a.table.page_size;
-        const long long page = a.table.page(r.b, p);
-        here = page >= 0;
-        if (!here) return;
-        k = __ldg(a.scale[0] + page * a.ss[0][0] + in * a.ss[0][1] + g * a.ss[0][2]);
-        v = __ldg(a.scale[1] + page * a.ss[1][0] + in * a.ss[1][1] + g * a.ss[1][2]);
-      };
-      float ks, vs;
-      scales_of(r.t0, ks, vs);
+      const int end = max(r.e0, r.e1);
       auto turn_q = [&](int t) {
         if (!mbar_wait_warp(&q_loaded[t], static_cast<uint32_t>(nq[t]) & 1u, a.status, abort_flag))
           return false;
@@ -921,63 +1051,91 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if (lane == 0) mbar_arrive(&q_full[t]);
         return true;
       };
-      auto turn = [&](bool v, int tile, float scale, bool there) {
-        const int u = idx, s = u % STAGES, x = u % RAW;
+      auto turn = [&](bool v, int tile) {
+        const int u = idx, s = u % STAGES;
         ++idx;
-        if (!mbar_wait_warp(&empty[s], (static_cast<uint32_t>(u / STAGES) & 1u) ^ 1u, a.status,
-                            abort_flag) ||
-            !mbar_wait_warp(&raw_full[x], static_cast<uint32_t>(u / RAW) & 1u, a.status, abort_flag))
+        if (!mbar_wait_warp(&loaded[s], static_cast<uint32_t>(u / STAGES) & 1u, a.status,
+                            abort_flag))
           return false;
-        float* sc = scales + (tiles % C::SCALES) * 256 + (v ? 128 : 0);
-        sc[key] = scale;
-        if (!v) {
-          const unsigned none = __ballot_sync(0xffffffffu, !there);
-          if (lane == 0) reinterpret_cast<uint32_t*>(gaps + tiles % C::GAPS)[w] = none;
-        }
-        __syncwarp();
+        const int place = tiles % C::SCALES;
+        if (!v && !mbar_wait_warp(&sc_full[place], static_cast<uint32_t>(tiles / C::SCALES) & 1u,
+                                  a.status, abort_flag))
+          return false;
+        float* sc = scales + place * 256 + (v ? 128 : 0);
+        constexpr int NP = DP / 64;
+        // The rows of codes lie where the same rows of the last slab go: a row is read before it is
+        // written.
+        uint8_t* to = smem + C::OFF_KV + s * C::BYTES + (w * 32 + r8) * 128;
+        const uint8_t* from = to + C::RAW;
+        const bool look = v && (CODE == SRDIT_Q_E4M3 || FOLD) && partly(r, tile * TILE);
+        uint32_t off = 0;  // rows that are not finite, by their scale or a NaN code
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
           const int row = w * 32 + i * 8 + r8;
-          const uint8_t* from = smem + C::OFF_RAW + x * C::SLAB + row * 128;
-          uint8_t* to = smem + C::OFF_KV + s * C::BYTES + row * 128;
+          uint4 c[NP];
 #pragma unroll
-          for (int k = 0; k < DP / 64; ++k) {
-            const int piece = k * 4 + y0;
-            uint4 codes = *reinterpret_cast<const uint4*>(from + ((piece ^ r8) << 4));
-            if (CODE == SRDIT_Q_E4M3 && v) {
-              // a NaN code makes its token's value one; behind the sequence it is nothing
-              if (nan_codes(codes.x) || nan_codes(codes.y) || nan_codes(codes.z) ||
-                  nan_codes(codes.w)) {
-                codes = make_uint4(0, 0, 0, 0);
-                if (tile * TILE + row < r.len) sc[row] = __int_as_float(0x7fc00000);
+          for (int k = 0; k < NP; ++k)
+            c[k] = *reinterpret_cast<const uint4*>(from + i * 1024 + (((k * 4 + y0) ^ r8) << 4));
+          float scale = FOLD ? sc[row] : 1.f;
+          if (look) {
+            // Zeros in place of rows behind the sequence, and of those that are not finite: the
+            // queries that see these are told, or have the scale for it.
+            bool nan = FOLD && !(fabsf(scale) < 3e38f);
+            if constexpr (CODE == SRDIT_Q_E4M3) {
+#pragma unroll
+              for (int k = 0; k < NP; ++k)
+                nan |= nan_codes(c[k].x) || nan_codes(c[k].y) || nan_codes(c[k].z) ||
+                       nan_codes(c[k].w);
+            }
+            uint32_t rows = __ballot_sync(0xffffffffu, nan);
+            rows |= rows >> 16;
+            rows = (rows | rows >> 8) & 0xffu;
+            off |= rows << (8 * i);
+            if (((rows >> r8) & 1u) || tile * TILE + row >= r.len) {
+#pragma unroll
+              for (int k = 0; k < NP; ++k) c[k] = make_uint4(0, 0, 0, 0);
+              if (FOLD) scale = 0.f;
+              if (!FOLD && tile * TILE + row < r.len) sc[row] = __int_as_float(0x7fc00000);
+            }
+          }
+          __syncwarp();
+          // the scale in two terms, so that the product is rounded once
+          const __half hi = __float2half_rn(scale);
+          const __half2 f = __half2half2(hi);
+          const __half2 rest = __half2half2(__float2half_rn(scale - __half2float(hi)));
+#pragma unroll
+          for (int k = 0; k < NP; ++k) {
+            uint32_t h[8];
+            widen_codes<CODE>(c[k], h);
+            if constexpr (FOLD) {
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const __half2 n = *reinterpret_cast<const __half2*>(&h[x]);
+                const __half2 y = __hfma2(n, f, __hmul2(n, rest));
+                h[x] = *reinterpret_cast<const uint32_t*>(&y);
               }
             }
-            uint32_t h[8];
-            widen_codes<CODE>(codes, h);
-            uint8_t* slab = to + k * C::SLAB;
+            uint8_t* slab = to + k * C::SLAB + i * 1024;
             *reinterpret_cast<uint4*>(slab + (((2 * y0) ^ r8) << 4)) =
                 make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4*>(slab + (((2 * y0 + 1) ^ r8) << 4)) =
                 make_uint4(h[4], h[5], h[6], h[7]);
           }
         }
+        if (FOLD && look && lane == 0) reinterpret_cast<uint32_t*>(bad + s)[w] = off;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&full[s]);
-          mbar_arrive(&raw_empty[x]);
-        }
+        if (lane == 0) mbar_arrive(&full[s]);
         return true;
       };
-      const int end = max(r.e0, r.e1);
-      if (TURN_Q && r.e0 > r.t0) ok = turn_q(0);
       for (int j = r.t0; j < end && ok; ++j) {
-        const bool there = here;
-        const float k = ks, v = vs;
-        ok = turn(false, j, k, there);
-        if (TURN_Q && ok && j == r.t0 && r.e1 > r.t0) ok = turn_q(1);
-        if (j + 1 < end) scales_of(j + 1, ks, vs);
-        ok = ok && turn(true, j, v, there);
+        // (one copy of the code for keys and values: two are more than the instruction caches hold
+        // beside the softmax)
+#pragma unroll 1
+        for (int x = 0; x < 2 && ok; ++x) {
+          if (FOLD && j == r.t0 && (x ? r.e1 : r.e0) > r.t0) ok = turn_q(x);
+          ok = ok && turn(x != 0, j);
+        }
         ++tiles;
       }
     }
@@ -1042,8 +1200,22 @@ Plan plan_chunk(const srdit_seq_attn_args& u, int sms) {
     keys = u.max_kv > 0 && u.max_kv < held ? u.max_kv : held;
   }
   const long long tiles = (keys + TILE - 1) / TILE;
-  // few items of many key tiles: shared out by key tiles (items x tiles in 32 bits)
-  p.ranged = items < 2 * sms && p.slots <= MAX_SLOTS && tiles > 8 && items * tiles < (1ll << 30);
+  // Few items of many key tiles are shared out by key tiles, and so is what a last round of whole
+  // items would leave idle (items x tiles in 32 bits); joining the parts costs what several do.
+  const long long some =
+      (u.B == 1 ? (u.T + 2 * p.rt - 1) / (2 * p.rt) : p.slots - u.B / 2) * static_cast<long long>(p.nhp);
+  if (p.slots <= MAX_SLOTS && items * tiles < (1ll << 30)) {
+    // CTAs of shares go through keys at different places and miss what others have fetched: a step
+    // takes a quarter more
+    const long long rounds = (some + sms - 1) / sms, steps = some * tiles;
+    const long long whole = rounds * tiles, shared = steps / sms * 5 / 4 + 7;
+    if (some < sms || u.causal) {
+      p.ranged = some < 2 * sms && shared < whole;
+    } else {
+      const long long last = some % sms;
+      p.ranged = last && last * tiles / sms * 5 / 4 + 7 < tiles ? 2 : 0;
+    }
+  }
   p.ctas = static_cast<int>(p.ranged || items > sms ? sms : items);
   p.ws_floats = p.ranged ? 2ll * p.ctas * ROWS * ((u.D <= 64 ? 64 : 128) + 2) + 4 * p.ctas : 0;
   return p;

@@ -12,6 +12,12 @@ Tolerances, with u the unit roundoff of a type (2^-8 bf16, 2^-11 fp16):
   of the output. Weights below the smallest fp16 step add 2^-25 |v_j| each; with codes they
   are held in units of at most twice the largest scale of a value, so 2^-24 of that scale times
   |code_j|.
+- with bf16 queries many rows' codes are multiplied by their scales and rounded once to fp16 (2^-11
+  of each key and value): the values add 2^-11 sum_j p_j |v_j| / sum_j p_j, and the keys move the
+  score of key j by up to e_j = 2^-11 scale sum_d |q_d k_jd|, its weight by that part of itself,
+  and so the answer by sum_j p_j e_j |v_j| + |o| sum_j p_j e_j over sum_j p_j. What rounds to less
+  than fp16's smallest step is 2^-25 of a unit in which the largest scale is 2^6 or more: far
+  below the 2^-24 of that scale that stands for the weights.
 """
 import torch
 
@@ -148,6 +154,10 @@ def attention(q, k, v, scale, causal, u_p, out_dtype, codes=None, vs=None, hide=
         o, a = p @ v[:, g], p @ v[:, g].abs()
         out[:, h] = o
         tol[:, h] = (u_p + 2.0 ** -11) * a + U[out_dtype] * o.abs() * (1 + 2.0 ** -6) + 1e-30
+        if codes is not None and out_dtype == torch.bfloat16:
+            e = 2.0 ** -11 * scale * (q[:, h].double().abs() @ k[:, g].abs().t())
+            pe = p * torch.where(seen, e, 0.0)
+            tol[:, h] += 2.0 ** -11 * a + pe @ v[:, g].abs() + o.abs() * pe.sum(1, keepdim=True)
         if codes is not None:
             tol[:, h] += 2.0 ** -24 * vs[:, g].max() * codes[:, g].abs().sum(0) if L else 0
         elif u_p == U[torch.float16]:
