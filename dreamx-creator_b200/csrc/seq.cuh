@@ -17,18 +17,37 @@ struct Offsets {
 };
 
 // The sequence among B that packed row t belongs to, by one warp (B: behind the last one).
-// Rows before the first offset are no sequence's either.
-SRDIT_DEV int find_sequence(const Offsets& o, int B, int t, Divisor by_each) {
-  if (!o.at) return by_each.div(t);
+// Rows before the first offset are no sequence's either. With `lens`, len is its entry of it, and
+// begin and end are the sequence's rows: all of them come with one trip to memory.
+SRDIT_DEV int find_sequence(const Offsets& o, int B, int t, Divisor by_each, const int32_t* lens,
+                            int& len, int& begin, int& end) {
+  if (!o.at) {
+    const int b = by_each.div(t);
+    begin = b * o.each;
+    end = begin + o.each;
+    len = lens ? __ldg(lens + b) : 0;
+    return b;
+  }
   const int lane = threadIdx.x & 31;
-  int b = 0;
   for (int base = 0; base < B; base += 32) {  // offsets that are not above t
     const int n = base + lane;
-    const unsigned below = __ballot_sync(0xffffffffu, n < B && __ldg(o.at + n + 1) <= t);
-    b = base + __popc(below);
-    if (below != 0xffffffffu) break;
+    const bool on = n < B;
+    const int to = on ? __ldg(o.at + n + 1) : 0x7fffffff, from = on ? __ldg(o.at + n) : 0;
+    const int l = on && lens ? __ldg(lens + n) : 0;
+    const unsigned below = __ballot_sync(0xffffffffu, to <= t);
+    if (below == 0xffffffffu) continue;
+    const int x = __popc(below);  // (of ascending offsets)
+    const int b = base + x;
+    begin = max(__shfl_sync(0xffffffffu, from, x), 0);
+    end = min(__shfl_sync(0xffffffffu, to, x), o.rows);
+    len = __shfl_sync(0xffffffffu, l, x);
+    return b < B && t >= begin ? b : B;
   }
-  return b < B && t >= __ldg(o.at) ? b : B;
+  return B;
+}
+SRDIT_DEV int find_sequence(const Offsets& o, int B, int t, Divisor by_each) {
+  int len, begin, end;
+  return find_sequence(o, B, t, by_each, nullptr, len, begin, end);
 }
 
 // A sequence's pages.

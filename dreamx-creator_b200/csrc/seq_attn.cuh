@@ -31,7 +31,7 @@ struct Args {
   int ranged, box_log;      // items shared out by key tiles; log2 of the keys of a page's box
   void* cuts;
   // step_kernel
-  int splits;
+  int splits, shared;       // parts of the keys; shares of all keys
   Divisor by_group;
 
   SRDIT_DEV bool paged() const { return table.page_size > 0; }
@@ -44,6 +44,7 @@ struct Args {
 struct Plan {
   bool step;                    // step_kernel (few rows per key head), else chunk_kernel
   int splits, cluster, parts;   // step_kernel; parts in the workspace per row (1: none)
+  bool shared;                  // ... all keys in equal shares
   int pack, rt, slots, nhp;     // chunk_kernel
   int ranged;                   // 0: whole items, 1: shared out by key tiles, 2: the last round
   int ctas;
