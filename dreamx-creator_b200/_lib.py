@@ -126,7 +126,7 @@ class SeqAttnArgs(ctypes.Structure):
 
 KV_PAGES_LAYOUT = struct.Struct("@4P6i12qPq2i")
 SEQ_ATTN_LAYOUT = struct.Struct("@5P7i8q3P3ifPqP")
-KV_STRIDES = struct.Struct("@4q")   # {token, head} of k, then of v
+KvStrides = c_ll * 4   # {token, head} of k, then of v
 assert KV_PAGES_LAYOUT.size == ctypes.sizeof(KvPages)
 assert SEQ_ATTN_LAYOUT.size == ctypes.sizeof(SeqAttnArgs)
 

@@ -25,7 +25,7 @@ struct Args {
   float* ml;                // ... their {m, l}
   uint32_t* status;
   // chunk_kernel
-  int pack, rt;             // heads of a group side by side in a query tile, its tokens
+  int pack, pack_log, rt;   // heads of a group side by side in a query tile (2^n), its tokens
   int slots, nhp;           // pieces of 2 rt tokens (some empty), head packs
   Divisor by_nhp, by_slots, by_piece;  // ... and 2 rt
   int ranged, box_log;      // items shared out by key tiles; log2 of the keys of a page's box

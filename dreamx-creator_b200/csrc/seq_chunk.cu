@@ -30,6 +30,7 @@ constexpr int MAX_SLOTS = 256;    // pieces of sequences of a ranged launch
 constexpr int MIN_SHARE = 4;      // key tiles that a ranged CTA takes at least
 constexpr int RECORDS = 4;
 constexpr int MAX_SEQS = 64;      // sequences that are kept in shared memory
+constexpr int MAX_SORTED = 64;    // pieces whose items are taken by length
 
 template <int DP, int CODE>
 struct ChunkCfg {
@@ -476,25 +477,50 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       Record r = {};
       bool ok = true;
       if (!a.ranged) {
-        // Whole items, one of every gridDim. Causal: the last pieces first (the longest), all heads
-        // of a piece side by side, in rounds that go forth and back, so that no CTA has the longest
-        // of every round; else a head's pieces, which share its keys, side by side.
-        const int items = a.slots * a.nhp, ctas = static_cast<int>(gridDim.x);
-        int at = blockIdx.x, step = 2 * (ctas - 1 - at) + 1;
-        for (int x = at; x < items && ok;) {
+        // Whole items, one of every gridDim. A few pieces: by their key tiles, the longest first;
+        // causal: the last pieces first; all heads of a piece side by side, in rounds that go forth
+        // and back, so that no CTA has the longest of every round. Else a head's pieces, which share
+        // its keys, side by side.
+        const int ctas = static_cast<int>(gridDim.x);
+        const bool sorted = a.slots <= MAX_SORTED && a.B > 1, by_length = sorted || a.causal;
+        int slots = a.slots;
+        if (sorted) {
+          int w[MAX_SORTED / 32];
+          slots = 0;
+#pragma unroll
+          for (int y = 0; y < MAX_SORTED / 32; ++y) {
+            const int s = y * 32 + lane;
+            w[y] = 0;
+            if (s < a.slots && pieces.item(pieces.find(s), s, r)) w[y] = max(1, max(r.e0, r.e1));
+            if (s < a.slots) starts[s] = w[y];
+            slots += __popc(__ballot_sync(0xffffffffu, w[y] > 0));
+          }
+          __syncwarp();
+          int rank[MAX_SORTED / 32] = {};
+          for (int x = 0; x < a.slots; ++x) {
+            const int v = starts[x];
+#pragma unroll
+            for (int y = 0; y < MAX_SORTED / 32; ++y)
+              rank[y] += v > w[y] || (v == w[y] && x < y * 32 + lane);
+          }
+#pragma unroll
+          for (int y = 0; y < MAX_SORTED / 32; ++y)
+            if (w[y] > 0) numbers[rank[y]] = y * 32 + lane;
+          __syncwarp();
+        }
+        const int items = slots * a.nhp;
+        int step = 2 * (ctas - 1 - static_cast<int>(blockIdx.x)) + 1;
+        for (int x = blockIdx.x; x < items && ok;) {
           int slot, hp;
-          if (a.causal) {
+          if (by_length) {
             slot = a.by_nhp.div(x);
             hp = x - slot * a.nhp;
-            slot = a.slots - 1 - slot;
-          } else {
-            hp = a.by_slots.div(x);
-            slot = x - hp * a.slots;
-          }
-          if (a.causal) {
+            slot = sorted ? numbers[slot] : a.slots - 1 - slot;
             x += step;
             step = 2 * ctas - step;
           } else {
+            hp = a.by_slots.div(x);
+            slot = x - hp * a.slots;
             x += ctas;
           }
           if (!pieces.item(pieces.find_warp(slot), slot, r)) continue;
@@ -720,8 +746,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     uint8_t* stg = smem + C::OFF_STG + (warp - 4) * 2048;
     const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SC);
     const float* q_back = reinterpret_cast<const float*>(smem + C::OFF_Q);
-    const int my_token = t * a.rt + row / a.pack;
-    const int warp_token = t * a.rt + sub * 32 / a.pack;
+    const int my_token = t * a.rt + (row >> a.pack_log);
+    const int warp_token = t * a.rt + (sub * 32 >> a.pack_log);
     int ns = 0, no = 0, idx = 0, tiles = 0;
     // A wait that runs out sets the abort flag, and those after it end at once: the warp goes
     // through the rest of its item without a branch, so that no lane of it stays behind, and
@@ -941,8 +967,19 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (part < 0) {
         // O / l: the warp's 32 rows go through its staging buffer 64 bytes of each at a time
+        const int piece = lane & 3;
+        T* to[4];
+        bool on[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int r = sub * 32 + y * 8 + (lane >> 2), token = t * a.rt + (r >> a.pack_log);
+          on[y] = token < tokens;
+          to[y] = static_cast<T*>(a.out) + (row0 + token) * a.os[0] +
+                  (h0 + (r & (a.pack - 1))) * a.os[1] + piece * 8;
+        }
+        const bool any = warp_token < tokens;
 #pragma unroll 1
-        for (int d = 0; d < DP; d += 32) {
+        for (int d = 0; d < DP && any; d += 32) {
           uint32_t o[32];
           if (n_tiles > 0) {
             tmem_ld32(o_tmem + d, o);
@@ -963,14 +1000,11 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
           __syncwarp();
-          const int piece = lane & 3, col = d + piece * 8;
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const int r = y * 8 + (lane >> 2), tr = sub * 32 + r;
-            const int token = t * a.rt + tr / a.pack;
-            if (token < tokens && col < a.D)
-              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (row0 + token) * a.os[0] +
-                                        (h0 + tr % a.pack) * a.os[1] + col) =
+            const int r = y * 8 + (lane >> 2);
+            if (on[y] && d + piece * 8 < a.D)
+              *reinterpret_cast<uint4*>(to[y] + d) =
                   *reinterpret_cast<const uint4*>(stg + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
           }
         }
@@ -1156,7 +1190,7 @@ __global__ void __launch_bounds__(DP / 8 * 32) join_chunk_kernel(const __grid_co
   const Cut cut = static_cast<const Cut*>(a.cuts)[blockIdx.x];
   if (cut.parts == 0) return;
   const int row = blockIdx.y * 32 + (threadIdx.x & 31), d = (threadIdx.x >> 5) * 8;
-  const int token = row / a.pack, head = cut.h0 + row % a.pack;
+  const int token = row >> a.pack_log, head = cut.h0 + (row & (a.pack - 1));
   if (token >= cut.tokens || d >= a.D) return;
   float m = neg_inf(), l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
@@ -1268,6 +1302,8 @@ static int run_typed(const srdit_seq_attn_args& u, const Args& a, const Plan& p,
 
 int run_chunk(const srdit_seq_attn_args& u, Args& a, const Plan& p, cudaStream_t stream) {
   a.pack = p.pack;
+  a.pack_log = 0;
+  while ((1 << a.pack_log) < p.pack) ++a.pack_log;
   a.rt = p.rt;
   a.slots = p.slots;
   a.nhp = p.nhp;

@@ -387,51 +387,56 @@ def _int32(t, n, what):
 
 
 def _pages(k_pages, v_pages, table, k_scale, v_scale, dtype):
-    """The C view of a cache's pages (``_lib.KvPages``) whose rows go to or from ``dtype``."""
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
-        raise _lib.SrditError(f"pages {tuple(k_pages.shape)} {k_pages.dtype}, "
-                              f"{tuple(v_pages.shape)} {v_pages.dtype}: "
-                              "[pages, page_size, kv_heads, D] of one type each")
-    n, size, Hkv, D = k_pages.shape
-    ks, vs = k_pages.stride(), v_pages.stride()
+    """The C view (``_lib.KvPages``) of a cache's pages, whose rows go to or from ``dtype``; the
+    sequences, key heads and their width."""
+    shape, held, ks, vs = k_pages.shape, k_pages.dtype, k_pages.stride(), v_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != held:
+        raise _lib.SrditError(f"pages {tuple(shape)} {held}, {tuple(v_pages.shape)} "
+                              f"{v_pages.dtype}: [pages, page_size, kv_heads, D] of one type each")
+    n, size, Hkv, D = shape
     if ks[3] != 1 or vs[3] != 1:
         raise _lib.SrditError(f"pages need unit stride over D, have {ks}, {vs}")
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1
-                                                          and table.stride(1) != 1):
+    entries, ts = table.shape, table.stride()
+    if len(entries) != 2 or table.dtype != torch.int32 or (ts[1] != 1 and entries[1] > 1):
         raise _lib.SrditError("the page table must be int32 [sequences, pages] with unit stride")
-    dt = _code(HALF_TYPES, dtype, "rows of a cache")
-    if k_pages.dtype == dtype:
-        code = _lib.SRDIT_KV_PLAIN
+    dt = HALF_TYPES.get(dtype)
+    if dt is None:
+        _code(HALF_TYPES, dtype, "rows of a cache")
+    if held == dtype:
         if k_scale is not None or v_scale is not None:
             raise _lib.SrditError(f"scales for pages of {dtype}")
-        scales, ss = (0, 0), (0, 0, 0, 0, 0, 0)
+        code, scales, ss = _lib.SRDIT_KV_PLAIN, (0, 0), (0, 0, 0, 0, 0, 0)
     else:
-        code = _code(CODES, k_pages.dtype, f"pages for rows of {dtype}, other than that type,")
+        code = CODES.get(held)
+        if code is None:
+            _code(CODES, held, f"pages for rows of {dtype}, other than that type,")
         if k_scale is None or v_scale is None:
-            raise _lib.SrditError(f"pages of {k_pages.dtype} need k_scale and v_scale")
-        for t in (k_scale, v_scale):
-            if t.dtype != torch.float32 or t.shape != (n, size, Hkv):
-                raise _lib.SrditError(f"scales must be float32 {(n, size, Hkv)}")
+            raise _lib.SrditError(f"pages of {held} need k_scale and v_scale")
+        rows = (n, size, Hkv)
+        if (k_scale.shape != rows or v_scale.shape != rows or k_scale.dtype != torch.float32
+                or v_scale.dtype != torch.float32):
+            raise _lib.SrditError(f"scales must be float32 {rows}")
         scales = (k_scale.data_ptr(), v_scale.data_ptr())
-        ss = (*k_scale.stride(), *v_scale.stride())
+        ss = k_scale.stride() + v_scale.stride()
     p = _lib.KvPages()
+    B = entries[0]
     _lib.KV_PAGES_LAYOUT.pack_into(
         p, 0, k_pages.data_ptr(), v_pages.data_ptr(), *scales, code, dt, n, size, Hkv, D,
-        *ks[:3], *vs[:3], *ss, table.data_ptr(), table.stride(0), table.shape[1], table.shape[0])
-    return p
+        *ks[:3], *vs[:3], *ss, table.data_ptr(), ts[0], entries[1], B)
+    return p, B, Hkv, D
 
 
 def _kv_rows(k, v, Hkv, D):
-    """The strides {token, head} of packed k, v [T, Hkv, D] as the C entries take them."""
-    if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (Hkv, D) or k.dtype != v.dtype:
-        raise _lib.SrditError(f"k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}: "
+    """The tokens of packed k, v [T, Hkv, D], and the address of their strides {token, head} as the
+    C entries take them, in a buffer that is to be kept."""
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if v.shape != shape or len(shape) != 3 or shape[1] != Hkv or shape[2] != D or k.dtype != v.dtype:
+        raise _lib.SrditError(f"k {tuple(shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}: "
                               f"[tokens, {Hkv}, {D}] of one type each")
-    ks, vs = k.stride(), v.stride()
     if ks[2] != 1 or vs[2] != 1:
         raise _lib.SrditError(f"k, v need unit stride over D, have {ks}, {vs}")
-    st = ctypes.create_string_buffer(32)
-    _lib.KV_STRIDES.pack_into(st, 0, ks[0], ks[1], vs[0], vs[1])
-    return st, ctypes.addressof(st)
+    st = _lib.KvStrides(ks[0], ks[1], vs[0], vs[1])
+    return shape[0], st, ctypes.addressof(st)
 
 
 def kv_write(k, v, k_pages, v_pages, page_table, kv_lens, *, cu_q=None, k_scale=None,
@@ -446,13 +451,11 @@ def kv_write(k, v, k_pages, v_pages, page_table, kv_lens, *, cu_q=None, k_scale=
     8 (16 for codes) up to 128, page_size 16, 32, 64 or a multiple of 128. A token whose page
     the table does not have is left out."""
     stream = _same_device(k, v, k_pages, v_pages, page_table, kv_lens, cu_q, k_scale, v_scale)
-    p = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
-    B, (_, _, Hkv, D) = page_table.shape[0], k_pages.shape
-    st, at = _kv_rows(k, v, Hkv, D)
-    T = k.shape[0]
+    p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
+    T, st, at = _kv_rows(k, v, Hkv, D)
     _launch("srdit_kv_write", ctypes.byref(p), k.data_ptr(), at, v.data_ptr(), at + 16, T,
             None if cu_q is None else _int32(cu_q, B + 1, "cu_q"), _int32(kv_lens, B, "kv_lens"),
-            stream, kind="kv_write", work=2 * T * Hkv * D * (2 + k_pages.element_size()))
+            stream, kind="kv_write", work=6 * T * Hkv * D)
 
 
 def kv_read(k_pages, v_pages, page_table, cu_k, k=None, v=None, *, total=None, dtype=None,
@@ -471,34 +474,35 @@ def kv_read(k_pages, v_pages, page_table, cu_k, k=None, v=None, *, total=None, d
             total is not None and k.shape[0] != total):
         raise _lib.SrditError("k and v do not go with total and dtype")
     stream = _same_device(k, v, k_pages, v_pages, page_table, cu_k, k_scale, v_scale)
-    p = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
-    _, _, Hkv, D = k_pages.shape
-    st, at = _kv_rows(k, v, Hkv, D)
-    T = k.shape[0]
+    p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
+    T, st, at = _kv_rows(k, v, Hkv, D)
     _launch("srdit_kv_read", ctypes.byref(p), k.data_ptr(), at, v.data_ptr(), at + 16, T,
-            _int32(cu_k, page_table.shape[0] + 1, "cu_k"), stream, kind="kv_read",
-            work=2 * T * Hkv * D * (2 + k_pages.element_size()))
+            _int32(cu_k, B + 1, "cu_k"), stream, kind="kv_read", work=6 * T * Hkv * D)
     return k, v
 
 
-def _seq_attn(kind, q, out, Hkv, B, pages, k, v, Tk, kv_strides, cu_q, cu_k, kv_lens, max_q,
+def _seq_attn(kind, q, out, Hkv, width, B, pages, k, v, Tk, kv_strides, cu_q, cu_k, kv_lens, max_q,
               max_kv, causal, scale, status, stream):
-    T, H, D = q.shape
-    dt = _code(HALF_TYPES, q.dtype, kind)
-    if Hkv == 0 or H % Hkv:
-        raise _lib.SrditError(f"{H} heads over {Hkv} key heads")
+    shape, dtype, qs = q.shape, q.dtype, q.stride()
+    if len(shape) != 3 or shape[2] != width or Hkv == 0 or shape[1] % Hkv:
+        raise _lib.SrditError(f"q {tuple(shape)} [tokens, heads, D] does not go with {Hkv} key heads "
+                              f"of {width}")
+    T, H, D = shape
+    dt = HALF_TYPES.get(dtype)
+    if dt is None:
+        _code(HALF_TYPES, dtype, kind)
     if out is None:
-        out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise _lib.SrditError(f"out must be {q.dtype} {tuple(q.shape)}")
-    qs, os = q.stride(), out.stride()
+        out = torch.empty(T, H, D, dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype != dtype:
+        raise _lib.SrditError(f"out must be {dtype} {tuple(shape)}")
+    os = out.stride()
     if qs[2] != 1 or os[2] != 1:
         raise _lib.SrditError(f"q, out need unit stride over D, have {qs}, {os}")
     a = _lib.SeqAttnArgs()
     fill = _lib.SEQ_ATTN_LAYOUT.pack_into
-    fields = (ctypes.addressof(pages) if pages is not None else 0, q.data_ptr(), k, v,
-              out.data_ptr(), dt, T, Tk, B, H, Hkv, D, *qs[:2], *kv_strides, *os[:2], cu_q, cu_k,
-              kv_lens, int(max_q), int(max_kv), bool(causal), D ** -0.5 if scale is None else scale)
+    fields = (pages, q.data_ptr(), k, v, out.data_ptr(), dt, T, Tk, B, H, Hkv, D, qs[0], qs[1],
+              *kv_strides, os[0], os[1], cu_q, cu_k, kv_lens, max_q, max_kv, bool(causal),
+              D ** -0.5 if scale is None else scale)
     st = 0 if status is None else status.data_ptr()
     fill(a, 0, *fields, 0, 0, st)
     ref = ctypes.byref(a)
@@ -525,18 +529,14 @@ def paged_attn(q, k_pages, v_pages, page_table, kv_lens, out=None, *, cu_q=None,
     sequence (default: what the table holds), by which work is split. ``scale``: D ** -0.5."""
     stream = _same_device(q, k_pages, v_pages, page_table, kv_lens, out, cu_q, k_scale, v_scale,
                           status)
-    if q.dim() != 3 or k_pages.dim() != 4 or q.shape[2] != k_pages.shape[3]:
-        raise _lib.SrditError(f"q {tuple(q.shape)} [tokens, heads, D] does not go with pages "
-                              f"{tuple(k_pages.shape)}")
-    p = _pages(k_pages, v_pages, page_table, k_scale, v_scale, q.dtype)
-    B = page_table.shape[0]
+    p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, q.dtype)
     if max_q is None:
         max_q = q.shape[0] if cu_q is not None or B == 0 else q.shape[0] // B
-    return _seq_attn("paged_attn", q, out, k_pages.shape[2], B, p, 0, 0, 0, (0, 0, 0, 0),
+    return _seq_attn("paged_attn", q, out, Hkv, D, B, ctypes.addressof(p), 0, 0, 0, (0, 0, 0, 0),
                      0 if cu_q is None else _int32(cu_q, B + 1, "cu_q"), 0,
                      _int32(kv_lens, B, "kv_lens"), max_q,
-                     page_table.shape[1] * k_pages.shape[1] if max_kv is None else max_kv,
-                     causal, scale, status, stream)
+                     p.table_width * p.page_size if max_kv is None else max_kv, causal, scale,
+                     status, stream)
 
 
 def packed_attn(q, k, v, cu_q, out=None, *, cu_k=None, causal=True, scale=None, status=None):
@@ -549,19 +549,16 @@ def packed_attn(q, k, v, cu_q, out=None, *, cu_k=None, causal=True, scale=None, 
     projection side by side). A query that sees no key gets zeros; rows of out behind the last
     sequence are left as they were. ``scale``: D ** -0.5."""
     stream = _same_device(q, k, v, cu_q, out, cu_k, status)
-    if q.dim() != 3 or k.dim() != 3 or q.shape[2] != k.shape[2] or k.dtype != q.dtype:
-        raise _lib.SrditError(f"q {tuple(q.shape)} {q.dtype} [tokens, heads, D] does not go with k "
-                              f"{tuple(k.shape)} {k.dtype}")
-    Tk, Hkv, D = k.shape
-    ks, vs = k.stride(), v.stride()
-    if v.shape != k.shape or v.dtype != k.dtype or ks[2] != 1 or vs[2] != 1:
-        raise _lib.SrditError(f"k {tuple(k.shape)} {ks}, v {tuple(v.shape)} {vs}: one shape and "
-                              "type, unit stride over D")
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if (len(shape) != 3 or v.shape != shape or k.dtype != q.dtype or v.dtype != q.dtype
+            or ks[2] != 1 or vs[2] != 1):
+        raise _lib.SrditError(f"k {tuple(shape)} {k.dtype} {ks}, v {tuple(v.shape)} {v.dtype} {vs}: "
+                              f"[tokens, kv_heads, D] of {q.dtype} with unit stride over D")
     B = cu_q.numel() - 1
-    if B < 0 or (cu_k is None and Tk != q.shape[0]):
+    if B < 0 or (cu_k is None and shape[0] != q.shape[0]):
         raise _lib.SrditError(f"{B} sequences; without cu_k k and v have q's {q.shape[0]} rows")
-    return _seq_attn("packed_attn", q, out, Hkv, B, None, k.data_ptr(), v.data_ptr(), Tk,
-                     (*ks[:2], *vs[:2]), _int32(cu_q, B + 1, "cu_q"),
+    return _seq_attn("packed_attn", q, out, shape[1], shape[2], B, 0, k.data_ptr(), v.data_ptr(),
+                     shape[0], (ks[0], ks[1], vs[0], vs[1]), _int32(cu_q, B + 1, "cu_q"),
                      0 if cu_k is None else _int32(cu_k, B + 1, "cu_k"), 0, 0, 0, causal, scale,
                      status, stream)
 
