@@ -234,10 +234,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     return scale * exp2_int(-x);
   };
   if (warp < 4) {
-    if constexpr (CODES)
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    else
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if constexpr (!CODES) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0) {
       // ------------------------------------------------------------ producer
       // the pages' boxes of a tile side by side: lane l has the box of keys l * box on
@@ -732,10 +729,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       }
     }
   } else if (warp < 12) {
-    if constexpr (CODES)
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    else
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    if constexpr (!CODES) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------ softmax
     const int t = (warp - 4) >> 2;  // query tile
     const int sub = warp & 3;       // tensor-memory lane quarter
@@ -778,142 +772,199 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if (FOLD && j == 0) c = q_back[(n & 1) * 256 + t * 128 + row];
         const uint4 gap = gaps[tiles % C::GAPS];
         const bool masked = key0 + TILE - 1 > lim0 || (gap.x | gap.y | gap.z | gap.w) != 0u;
-        uint32_t vis[4];
-        if (masked) {
-          const uint32_t none[4] = {gap.x, gap.y, gap.z, gap.w};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int count = lim - key0 + 1 - 32 * w;
-            vis[w] = (count >= 32 ? 0xffffffffu : count <= 0 ? 0u : (1u << count) - 1u) & ~none[w];
-          }
-        }
-        uint32_t s[4][32];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) tmem_ld32(s_tmem + w * 32, s[w]);
-        tmem_ld_wait();
-        const float* sc = scales + (tiles % C::SCALES) * 256;
-        if constexpr (CODES && !FOLD) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int x = 0; x < 32; x += 4) {
-              const float4 k = *reinterpret_cast<const float4*>(sc + w * 32 + x);
-              const float2 y0 =
-                  f2_split(f2_mul(u64_of(s[w][x], s[w][x + 1]), f2_pack(k.x, k.y)));
-              const float2 y1 =
-                  f2_split(f2_mul(u64_of(s[w][x + 2], s[w][x + 3]), f2_pack(k.z, k.w)));
-              s[w][x] = __float_as_uint(y0.x);
-              s[w][x + 1] = __float_as_uint(y0.y);
-              s[w][x + 2] = __float_as_uint(y1.x);
-              s[w][x + 3] = __float_as_uint(y1.y);
-            }
-        }
-        if (masked) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (!((vis[w] >> x) & 1u)) s[w][x] = __float_as_uint(neg_inf());
-        }
-        float mx[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          mx[w] = __uint_as_float(s[w][0]);
-#pragma unroll
-          for (int x = 1; x < 31; x += 2)
-            mx[w] = max3(mx[w], __uint_as_float(s[w][x]), __uint_as_float(s[w][x + 1]));
-          mx[w] = max2(mx[w], __uint_as_float(s[w][31]));
-        }
-        // per 32 keys: the scores' factor, and log2 of the unit that the values are in
-        float cw[4], lv[4];
-        float top;
-        if constexpr (FOLD) {
-          const float* units = reinterpret_cast<const float*>(smem + C::OFF_UNITS) +
-                               tiles % C::SCALES * 8;
-          const float4 f = *reinterpret_cast<const float4*>(units);
-          const float4 v = *reinterpret_cast<const float4*>(units + 4);
-          const float u[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) cw[w] = fmaxf(c * u[w], 1.2e-38f);  // (0 times -inf is NaN)
-          lv[0] = v.x, lv[1] = v.y, lv[2] = v.z, lv[3] = v.w;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) mx[w] = fmaf(mx[w], cw[w], lv[w]);
-          top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
-        } else {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) cw[w] = c, lv[w] = 0.f;
-          top = max2(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
-        }
-        if constexpr (CODES && !FOLD) {  // the values' scales are there with the V tile
-          mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u, a.status,
-                    abort_flag);
-          float most = 0.f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float v = sc[128 + w * 32 + lane];
-            most = fmaxf(most, v < 3e38f ? v : 0.f);
-          }
-          most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-          top += __log2f(fmaxf(most, 1e-30f));
-        }
-        // the maximum moves (and O is rescaled) only when a tile's is 8 above it:
-        // weights stay below 2^8 and the quotient is the same
-        // (written so that a NaN raises it too, and stays in l and O)
-        const bool raise = !(top <= m + 8.f) && top != neg_inf();
-        const float m_new = raise ? top : m;
-        const float alpha = raise ? ex2(m - m_new) : 1.f;
-        m = m_new;
-        const float neg_m = m == neg_inf() ? 0.f : -m;
-        if (j > 0 && __any_sync(0xffffffffu, raise)) {
-          // scores of this tile are ready, so the product before it is done
+        // The maximum moves (and O is rescaled) only when a tile's is 8 above it: weights stay below
+        // 2^8 and the quotient is the same. (Written so that a NaN raises it too, and stays in l
+        // and O.) Scores of this tile are ready, so the product before it is done.
+        auto new_max = [&](float top) {
+          const bool raise = !(top <= m + 8.f) && top != neg_inf();
+          const float m_new = raise ? top : m;
+          const float alpha = raise ? ex2(m - m_new) : 1.f;
+          m = m_new;
+          l *= alpha;
+          if (j > 0 && __any_sync(0xffffffffu, raise)) {
 #pragma unroll 1
-          for (int w = 0; w < DP / 16; ++w) {
-            uint32_t o[16];
-            tmem_ld16(o_tmem + w * 16, o);
-            tmem_ld_wait();
+            for (int w = 0; w < DP / 16; ++w) {
+              uint32_t o[16];
+              tmem_ld16(o_tmem + w * 16, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-            tmem_st16(o_tmem + w * 16, o);
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint64_t c2 = f2_pack(cw[w], cw[w]);
-          const uint64_t neg_m2 = f2_pack(neg_m + lv[w], neg_m + lv[w]);
-#pragma unroll
-          for (int x = 0; x < 32; x += 2) {
-            const float2 y = f2_split(f2_fma(u64_of(s[w][x], s[w][x + 1]), c2, neg_m2));
-            s[w][x] = __float_as_uint(y.x);
-            s[w][x + 1] = __float_as_uint(y.y);
-          }
-        }
-        uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-        l *= alpha;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t pw[16];
-          if constexpr (CODES && !FOLD) {
-#pragma unroll
-            for (int x = 0; x < 32; x += 4) {
-              const float4 v = *reinterpret_cast<const float4*>(sc + 128 + w * 32 + x);
-              const uint64_t p0 =
-                  f2_pack(ex2(__uint_as_float(s[w][x])), ex2(__uint_as_float(s[w][x + 1])));
-              const uint64_t p1 =
-                  f2_pack(ex2(__uint_as_float(s[w][x + 2])), ex2(__uint_as_float(s[w][x + 3])));
-              sum[0] = f2_add(sum[0], p0);
-              sum[1] = f2_add(sum[1], p1);
-              float2 y0 = f2_split(f2_mul(p0, f2_pack(v.x, v.y)));
-              float2 y1 = f2_split(f2_mul(p1, f2_pack(v.z, v.w)));
-              if (masked) {  // (a scale of NaN stays with the rows that see its key)
-                if (!((vis[w] >> x) & 1u)) y0.x = 0.f;
-                if (!((vis[w] >> (x + 1)) & 1u)) y0.y = 0.f;
-                if (!((vis[w] >> (x + 2)) & 1u)) y1.x = 0.f;
-                if (!((vis[w] >> (x + 3)) & 1u)) y1.y = 0.f;
-              }
-              pw[x >> 1] = pack2(y0.x, y0.y, E{});
-              pw[(x >> 1) + 1] = pack2(y1.x, y1.y, E{});
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+              tmem_st16(o_tmem + w * 16, o);
             }
-          } else {
+          }
+        };
+        // the first 64 keys' weights, stored by now: their product can begin
+        auto publish_half = [&] {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[t]);
+        };
+        // the keys from key0 + 32 w on that this row sees
+        auto seen = [&](int w) {
+          const int count = lim - key0 + 1 - 32 * w;
+          const uint32_t none = w == 0 ? gap.x : w == 1 ? gap.y : w == 2 ? gap.z : gap.w;
+          return (count >= 32 ? 0xffffffffu : count <= 0 ? 0u : (1u << count) - 1u) & ~none;
+        };
+        if constexpr (CODES) {
+          // Two passes over the scores, 64 of them at a time, so that the code is short: with all 128
+          // in registers at once, as below, it does not fit the instruction caches beside that of the
+          // warps that widen codes (PASSES).
+          const float* sc = scales + (tiles % C::SCALES) * 256;
+          const float* units =
+              reinterpret_cast<const float*>(smem + C::OFF_UNITS) + tiles % C::SCALES * 8;
+          // the scores of keys 64 h on, which have been asked for, as they count
+          auto finish = [&](int h, uint32_t (&s)[2][32]) {
+            tmem_ld_wait();
+            if constexpr (!FOLD) {
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) {
+                  const float4 k = *reinterpret_cast<const float4*>(sc + h * 64 + y * 32 + x);
+                  const float2 y0 = f2_split(f2_mul(u64_of(s[y][x], s[y][x + 1]), f2_pack(k.x, k.y)));
+                  const float2 y1 =
+                      f2_split(f2_mul(u64_of(s[y][x + 2], s[y][x + 3]), f2_pack(k.z, k.w)));
+                  s[y][x] = __float_as_uint(y0.x);
+                  s[y][x + 1] = __float_as_uint(y0.y);
+                  s[y][x + 2] = __float_as_uint(y1.x);
+                  s[y][x + 3] = __float_as_uint(y1.y);
+                }
+            }
+            if (masked) {
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const uint32_t vis = seen(2 * h + y);
+#pragma unroll
+                for (int x = 0; x < 32; ++x)
+                  if (!((vis >> x) & 1u)) s[y][x] = __float_as_uint(neg_inf());
+              }
+            }
+          };
+          auto ask = [&](int h, uint32_t (&s)[2][32]) {
+            tmem_ld32(s_tmem + h * 64, s[0]);
+            tmem_ld32(s_tmem + h * 64 + 32, s[1]);
+          };
+          // per 32 keys: the scores' factor, and log2 of the unit that the values are in
+          auto factor = [&](int w) {
+            return FOLD ? fmaxf(c * units[w], 1.2e-38f) : c;  // (0 times -inf is NaN)
+          };
+          float top = neg_inf();
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t s[2][32];
+            ask(h, s);
+            finish(h, s);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float mx = __uint_as_float(s[y][0]);
+#pragma unroll
+              for (int x = 1; x < 31; x += 2)
+                mx = max3(mx, __uint_as_float(s[y][x]), __uint_as_float(s[y][x + 1]));
+              mx = max2(mx, __uint_as_float(s[y][31]));
+              top = max2(top, fmaf(mx, factor(2 * h + y), FOLD ? units[4 + 2 * h + y] : 0.f));
+            }
+          }
+          if constexpr (!FOLD) {  // the values' scales are there with the V tile
+            mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u,
+                      a.status, abort_flag);
+            float most = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const float v = sc[128 + w * 32 + lane];
+              most = fmaxf(most, v < 3e38f ? v : 0.f);
+            }
+            most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+            top += __log2f(fmaxf(most, 1e-30f));
+          }
+          new_max(top);
+          const float neg_m = m == neg_inf() ? 0.f : -m;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t s[2][32];
+            ask(h, s);
+            if (h) publish_half();
+            finish(h, s);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              uint32_t pw[16];
+              const float lv = FOLD ? units[4 + 2 * h + y] : 0.f, cw = factor(2 * h + y);
+              const uint64_t c2 = f2_pack(cw, cw), neg_m2 = f2_pack(neg_m + lv, neg_m + lv);
+              uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+              const uint32_t vis = !FOLD && masked ? seen(2 * h + y) : 0u;
+#pragma unroll
+              for (int x = 0; x < 32; x += 2) {
+                const float2 z = f2_split(f2_fma(u64_of(s[y][x], s[y][x + 1]), c2, neg_m2));
+                s[y][x] = __float_as_uint(z.x);
+                s[y][x + 1] = __float_as_uint(z.y);
+              }
+#pragma unroll
+              for (int x = 0; x < 32; x += 4) {
+                const uint64_t p0 =
+                    f2_pack(ex2(__uint_as_float(s[y][x])), ex2(__uint_as_float(s[y][x + 1])));
+                const uint64_t p1 =
+                    f2_pack(ex2(__uint_as_float(s[y][x + 2])), ex2(__uint_as_float(s[y][x + 3])));
+                sum[0] = f2_add(sum[0], p0);
+                sum[1] = f2_add(sum[1], p1);
+                float2 y0 = f2_split(p0), y1 = f2_split(p1);
+                if constexpr (!FOLD) {
+                  const float4 v =
+                      *reinterpret_cast<const float4*>(sc + 128 + h * 64 + y * 32 + x);
+                  y0 = f2_split(f2_mul(p0, f2_pack(v.x, v.y)));
+                  y1 = f2_split(f2_mul(p1, f2_pack(v.z, v.w)));
+                  if (masked) {  // (a scale of NaN stays with the rows that see its key)
+                    if (!((vis >> x) & 1u)) y0.x = 0.f;
+                    if (!((vis >> (x + 1)) & 1u)) y0.y = 0.f;
+                    if (!((vis >> (x + 2)) & 1u)) y1.x = 0.f;
+                    if (!((vis >> (x + 3)) & 1u)) y1.y = 0.f;
+                  }
+                }
+                pw[x >> 1] = pack2(y0.x, y0.y, E{});
+                pw[(x >> 1) + 1] = pack2(y1.x, y1.y, E{});
+              }
+              const float2 sp = f2_split(f2_add(sum[0], sum[1]));
+              l = fmaf(sp.x + sp.y, FOLD ? ex2(-lv) : 1.f, l);  // in the unit of one
+              tmem_st16(s_tmem + h * 32 + y * 16, pw);
+            }
+          }
+        } else {
+          uint32_t s[4][32];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) tmem_ld32(s_tmem + w * 32, s[w]);
+          tmem_ld_wait();
+          if (masked) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t vis = seen(w);
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (!((vis >> x) & 1u)) s[w][x] = __float_as_uint(neg_inf());
+            }
+          }
+          float mx[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            mx[w] = __uint_as_float(s[w][0]);
+#pragma unroll
+            for (int x = 1; x < 31; x += 2)
+              mx[w] = max3(mx[w], __uint_as_float(s[w][x]), __uint_as_float(s[w][x + 1]));
+            mx[w] = max2(mx[w], __uint_as_float(s[w][31]));
+          }
+          new_max(max2(max3(mx[0], mx[1], mx[2]), mx[3]) * c);
+          const float neg_m = m == neg_inf() ? 0.f : -m;
+          const uint64_t c2 = f2_pack(c, c), neg_m2 = f2_pack(neg_m, neg_m);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int x = 0; x < 32; x += 2) {
+              const float2 y = f2_split(f2_fma(u64_of(s[w][x], s[w][x + 1]), c2, neg_m2));
+              s[w][x] = __float_as_uint(y.x);
+              s[w][x + 1] = __float_as_uint(y.y);
+            }
+          uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t pw[16];
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
               const uint64_t p2 =
@@ -922,21 +973,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               const float2 p = f2_split(p2);
               pw[x >> 1] = pack2(p.x, p.y, E{});
             }
+            if (w == 2) publish_half();
+            tmem_st16(s_tmem + w * 16, pw);
           }
-          if constexpr (FOLD) {  // the sum of weights in the unit of one
-            const float2 sp = f2_split(f2_add(sum[0], sum[1]));
-            l = fmaf(sp.x + sp.y, ex2(-lv[w]), l);
-            sum[0] = sum[1] = f2_pack(0.f, 0.f);
-          }
-          if (w == 2) {  // the first 64 keys' weights, stored by now: their product can begin
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_half[t]);
-          }
-          tmem_st16(s_tmem + w * 16, pw);
-        }
-        if constexpr (!FOLD) {
           const float2 sp = f2_split(f2_add(sum[0], sum[1]));
           l += sp.x + sp.y;
         }
@@ -946,7 +985,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                       a.status, abort_flag);
             uint4 off = bad[(u + 1) % STAGES];
             if (masked)
-              off = make_uint4(off.x & vis[0], off.y & vis[1], off.z & vis[2], off.w & vis[3]);
+              off = make_uint4(off.x & seen(0), off.y & seen(1), off.z & seen(2), off.w & seen(3));
             if (off.x | off.y | off.z | off.w) l = __int_as_float(0x7fc00000);
           }
         }
@@ -1031,7 +1070,6 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       tc_fence_before();
     }
   } else if constexpr (CODES) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ------------------------------------------------------------ codes to fp16
     const int w = warp - 12;
     const int r8 = lane & 7, y0 = lane >> 3;  // a lane's row of 8, its pieces of 16 bytes
