@@ -864,7 +864,12 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               mx = max2(mx, __uint_as_float(s[y][31]));
               top = max2(top, fmaf(mx, factor(2 * h + y), FOLD ? units[4 + 2 * h + y] : 0.f));
             }
+            if constexpr (!FOLD) {  // as they count: the scales are read once
+              tmem_st32(s_tmem + h * 64, s[0]);
+              tmem_st32(s_tmem + h * 64 + 32, s[1]);
+            }
           }
+          if constexpr (!FOLD) tmem_st_wait();
           if constexpr (!FOLD) {  // the values' scales are there with the V tile
             mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u,
                       a.status, abort_flag);
@@ -884,7 +889,10 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             uint32_t s[2][32];
             ask(h, s);
             if (h) publish_half();
-            finish(h, s);
+            if constexpr (FOLD)
+              finish(h, s);
+            else
+              tmem_ld_wait();
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               uint32_t pw[16];
