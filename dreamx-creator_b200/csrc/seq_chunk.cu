@@ -26,11 +26,11 @@ namespace srdit {
 namespace sattn {
 
 constexpr int ROWS = 2 * TILE;    // of an item
-constexpr int MAX_SLOTS = 256;    // pieces of sequences of a ranged launch
+constexpr int MAX_SLOTS = 192;    // pieces of sequences that are kept in shared memory
 constexpr int MIN_SHARE = 4;      // key tiles that a ranged CTA takes at least
 constexpr int RECORDS = 4;
 constexpr int MAX_SEQS = 64;      // sequences that are kept in shared memory
-constexpr int MAX_SORTED = 64;    // pieces whose items are taken by length
+constexpr int MAX_SORTED = 64;    // pieces that are taken by length
 
 template <int DP, int CODE>
 struct ChunkCfg {
@@ -47,7 +47,8 @@ struct ChunkCfg {
   static constexpr int OFF_UNITS = OFF_SC + (CODES ? SCALES * 1024 : 0);  // ... and units [2][4]
   static constexpr int OFF_Q = OFF_UNITS + (CODES ? SCALES * 32 : 0);  // queries' factors [2][256]
   static constexpr int OFF_REC = OFF_Q + (CODES ? 2048 : 0);
-  static constexpr int OFF_STEPS = OFF_REC + RECORDS * 64;  // ranged: the pieces
+  static constexpr int OFF_PIECES = OFF_REC + RECORDS * 64;
+  static constexpr int OFF_STEPS = OFF_PIECES + MAX_SLOTS * 32;  // their first key tiles, order
   static constexpr int OFF_SEQS = OFF_STEPS + (2 * MAX_SLOTS + 4) * 4;
   static constexpr int OFF_GAPS = OFF_SEQS + MAX_SEQS * 16;  // keys without a page, 8 tiles
   static constexpr int GAPS = 8;
@@ -63,17 +64,24 @@ struct ChunkCfg {
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
-// What a CTA does next.
-struct Record {
-  int row0, tokens;  // first query row; tokens (0: nothing more)
-  int h0, b;
-  int pos0;          // the first token's place in its sequence
+// Up to 2 rt tokens of a sequence.
+struct Piece {
+  int row0, tokens;  // first query row; tokens
+  int b, pos0;       // sequence; the first token's place in it
   int len, kv0;      // keys; packed: the first one's row
-  int t0, e0, e1;    // key tiles: from t0 to the ends of the two query tiles
+  int e0, e1;        // the ends of the two query tiles' key tiles
+  SRDIT_DEV int weight() const { return max(1, max(e0, e1)); }  // key tiles; one without any
+};
+
+// What a CTA does next: a piece (tokens 0: nothing more) for a pack of heads, and of its key tiles
+// those from t0 on.
+struct Record {
+  Piece p;
+  int h0, t0;
   int part;          // -1: all of the keys; else where in the workspace the part goes
   int parts;         // of an item that this CTA begins and others end: in how many it is
   int pad[4];
-  SRDIT_DEV int steps() const { return max(e0, e1) - t0; }
+  SRDIT_DEV int steps() const { return max(p.e0, p.e1) - t0; }
 };
 
 // What a CTA leaves for join_chunk_kernel: the item that it begins and does not end.
@@ -116,8 +124,8 @@ struct Pieces {
     }
     return lo;
   }
-  // the item of piece n of sequence b; false: there is none
-  SRDIT_DEV bool item(int b, int n, Record& r) const {
+  // number n, of sequence b; false: it is empty
+  SRDIT_DEV bool piece(int b, int n, Piece& r) const {
     const int4 q = seqs ? seqs[b] : sequence(a, b);
     const int tokens = q.y - q.x;
     const int at = (n - a.by_piece.div(q.x) - b) * 2 * a.rt;
@@ -128,15 +136,12 @@ struct Pieces {
     r.len = q.z;
     r.kv0 = q.w;
     r.pos0 = r.len - tokens + at;
-    r.t0 = 0;
     const int tiles = (r.len + TILE - 1) / TILE;
     auto end = [&](int last) {
       return !a.causal ? tiles : last < 0 ? 0 : min(tiles, last / TILE + 1);
     };
     r.e0 = end(r.pos0 + min(r.tokens, a.rt) - 1);
     r.e1 = r.tokens > a.rt ? end(r.pos0 + r.tokens - 1) : 0;
-    r.part = -1;
-    r.parts = 0;
     return true;
   }
 };
@@ -173,8 +178,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   volatile uint32_t* abort_flag = tmem_slot + 1;
   static_assert((3 * STAGES + 14 + 2 * RECORDS + C::SCALES) * 8 + 8 <= 512, "barrier area");
   Record* records = reinterpret_cast<Record*>(smem + C::OFF_REC);
+  Piece* kept = reinterpret_cast<Piece*>(smem + C::OFF_PIECES);
   int* starts = reinterpret_cast<int*>(smem + C::OFF_STEPS);  // first key tile of each piece
-  int* numbers = starts + MAX_SLOTS + 4;                      // ... and its number
+  int* order = starts + MAX_SLOTS + 4;
   int4* seqs = reinterpret_cast<int4*>(smem + C::OFF_SEQS);
   uint4* gaps = reinterpret_cast<uint4*>(smem + C::OFF_GAPS);  // by tiles, a bit a key
   uint4* bad = reinterpret_cast<uint4*>(smem + C::OFF_BAD);    // by stages
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   const uint32_t tmem_base = *tmem_slot;
   // a tile that some query of the item does not see whole by place
   auto partly = [&](const Record& r, int key0) {
-    return key0 + TILE > r.len || (a.causal && key0 + TILE - 1 > r.pos0);
+    return key0 + TILE > r.p.len || (a.causal && key0 + TILE - 1 > r.p.pos0);
   };
   // FOLD: 32 keys' scales over 2^e, in [2^6, 2^7) for the largest finite one, so that code times
   // scale, at most 448 x 2^7, is one of fp16; and f = 2^e
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         const Record r = records[at];
         __syncwarp();
         if (lane == 0) mbar_arrive(&rec_empty[at]);
-        if (r.tokens == 0) break;
+        if (r.p.tokens == 0) break;
         if (r.steps() <= 0) continue;
         const int g = r.h0 / a.group;
         const int boxes = TILE >> a.box_log;
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             mbar_arrive_expect_tx(&q_loaded[t], C::BYTES);
             for (int d = 0; d < DP / 64; ++d)
               tma_load_4d(smem + t * C::BYTES + d * C::SLAB, &tmQ, &q_loaded[t], d * 64, r.h0,
-                          r.row0 + t * a.rt, 0);
+                          r.p.row0 + t * a.rt, 0);
           }
           ++nq[t];
           return true;
@@ -269,14 +275,14 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         // this lane's box of a tile: its page (-1: none) and row; whether keys have no page
         auto place = [&](int tile, int& page, int& row, bool& gap) {
           page = 0;
-          row = r.kv0 + tile * TILE;
+          row = r.p.kv0 + tile * TILE;
           gap = false;
           if (a.paged()) {
             const int key = tile * TILE + (lane << a.box_log);
             const int p = a.table.by_page.div(key);
-            const bool on = lane < boxes && key < r.len;
+            const bool on = lane < boxes && key < r.p.len;
             row = key - p * a.table.page_size;
-            page = on ? a.table.page(r.b, p) : -1;
+            page = on ? a.table.page(r.p.b, p) : -1;
             gap = on && page < 0;
           }
         };
@@ -316,9 +322,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         int page, row, page1 = 0, row1 = 0;
         bool gap, gap1 = false;
         place(r.t0, page, row, gap);
-        ok = (r.e0 <= r.t0 || load_q(0)) && load_kv(false, page, row, gap) &&
-             (r.e1 <= r.t0 || load_q(1));
-        const int end = max(r.e0, r.e1);
+        ok = (r.p.e0 <= r.t0 || load_q(0)) && load_kv(false, page, row, gap) &&
+             (r.p.e1 <= r.t0 || load_q(1));
+        const int end = max(r.p.e0, r.p.e1);
         for (int j = r.t0; j < end && ok; ++j) {
           if (j + 1 < end) place(j + 1, page1, row1, gap1);
           ok = load_kv(true, page, row, false) &&
@@ -381,10 +387,10 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               ok = false;
               return false;
             }
-            const int tokens = records[at].tokens;
+            const int tokens = records[at].p.tokens;
             r.t0 = records[at].t0;
-            r.e[0] = records[at].e0;
-            r.e[1] = records[at].e1;
+            r.e[0] = records[at].p.e0;
+            r.e[1] = records[at].p.e1;
             r.end = max(r.e[0], r.e[1]);
             mbar_arrive(&rec_empty[at]);
             ++nrec;
@@ -456,63 +462,138 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       __syncwarp();
     } else if (warp == 2) {
       // ------------------------------------------------------------ items
+      // (The code up to the first record is met cold by every CTA, so it is short.)
       const Pieces pieces{a, a.B <= MAX_SEQS ? seqs : nullptr};
+      const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
       int n = 0;
-      auto pass = [&](const Record& r) {
+      // piece p for head pack hp, key tiles t0 to t1; by lane 0
+      auto pass = [&](const Piece& p, int hp, int t0, int t1, int part, int parts) {
         const int at = n % RECORDS;
         if (!mbar_wait_warp(&rec_empty[at], (static_cast<uint32_t>(n / RECORDS) & 1u) ^ 1u,
                             a.status, abort_flag))
           return false;
         if (lane == 0) {
-          records[at] = r;
+          Record& r = records[at];
+          r.p = p;
+          r.p.e0 = max(t0, min(p.e0, t1));
+          r.p.e1 = max(t0, min(p.e1, t1));
+          r.h0 = hp * a.pack;
+          r.t0 = t0;
+          r.part = part;
+          r.parts = parts;
           mbar_arrive(&rec_full[at]);
         }
         __syncwarp();
         ++n;
         return true;
       };
-      Record r = {};
       bool ok = true;
-      if (!a.ranged) {
-        // Whole items, one of every gridDim. A few pieces: by their key tiles, the longest first;
-        // causal: the last pieces first; all heads of a piece side by side, in rounds that go forth
-        // and back, so that no CTA has the longest of every round. Else a head's pieces, which share
-        // its keys, side by side.
-        const int ctas = static_cast<int>(gridDim.x);
-        const bool sorted = a.slots <= MAX_SORTED && a.B > 1, by_length = sorted || a.causal;
-        int slots = a.slots;
-        if (sorted) {
-          int w[MAX_SORTED / 32];
-          slots = 0;
+      constexpr int all_tiles = 0x7fffffff;
+      if (a.slots <= MAX_SLOTS) {
+        // the pieces that there are
+        int total = 0, count = 0;
+#pragma unroll 1
+        for (int s0 = 0; s0 < a.slots; s0 += 32) {
+          const int s = s0 + lane;
+          Piece p;
+          const bool on = s < a.slots && pieces.piece(pieces.find(s), s, p);
+          const int w = on ? p.weight() : 0;
+          const unsigned found = __ballot_sync(0xffffffffu, on);
+          int sum = w;
 #pragma unroll
-          for (int y = 0; y < MAX_SORTED / 32; ++y) {
-            const int s = y * 32 + lane;
-            w[y] = 0;
-            if (s < a.slots && pieces.item(pieces.find(s), s, r)) w[y] = max(1, max(r.e0, r.e1));
-            if (s < a.slots) starts[s] = w[y];
-            slots += __popc(__ballot_sync(0xffffffffu, w[y] > 0));
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
           }
-          __syncwarp();
-          int rank[MAX_SORTED / 32] = {};
-          for (int x = 0; x < a.slots; ++x) {
-            const int v = starts[x];
-#pragma unroll
-            for (int y = 0; y < MAX_SORTED / 32; ++y)
-              rank[y] += v > w[y] || (v == w[y] && x < y * 32 + lane);
+          if (on) {
+            const int at = count + __popc(found & ((1u << lane) - 1u));
+            kept[at] = p;
+            starts[at] = total + sum - w;
           }
-#pragma unroll
-          for (int y = 0; y < MAX_SORTED / 32; ++y)
-            if (w[y] > 0) numbers[rank[y]] = y * 32 + lane;
-          __syncwarp();
+          total += __shfl_sync(0xffffffffu, sum, 31);
+          count += __popc(found);
         }
-        const int items = slots * a.nhp;
-        int step = 2 * (ctas - 1 - static_cast<int>(blockIdx.x)) + 1;
-        for (int x = blockIdx.x; x < items && ok;) {
+        if (lane == 0) starts[count] = total;
+        __syncwarp();
+        const int items = count * a.nhp;
+        if (!a.ranged) {
+          // Whole items, one of every gridDim. A few pieces: the longest first; causal: the last ones
+          // first; all heads of a piece side by side, in rounds that go forth and back, so that no
+          // CTA has the longest of every round. Else a head's pieces, which share its keys, side by
+          // side.
+          const bool sorted = count <= MAX_SORTED && a.B > 1;
+          if (sorted) {
+#pragma unroll 1
+            for (int k = lane; k < count; k += 32) {
+              const int w = starts[k + 1] - starts[k];
+              int rank = 0;
+              for (int x = 0; x < count; ++x) {
+                const int v = starts[x + 1] - starts[x];
+                rank += v > w || (v == w && x < k);
+              }
+              order[rank] = k;
+            }
+            __syncwarp();
+          }
+          int step = 2 * (ctas - 1 - cta) + 1;
+          for (int x = cta; x < items && ok;) {
+            int k, hp;
+            if (sorted || a.causal) {
+              k = a.by_nhp.div(x);
+              hp = x - k * a.nhp;
+              k = sorted ? order[k] : count - 1 - k;
+              x += step;
+              step = 2 * ctas - step;
+            } else {
+              hp = x / count;
+              k = x - hp * count;
+              x += ctas;
+            }
+            ok = pass(kept[k], hp, 0, all_tiles, -1, 0);
+          }
+        } else {
+          // Head pack by head pack. Whole items in rounds as long as every CTA gets one (a.ranged 2),
+          // whose CTAs share keys; of the others an equal share of the key tiles.
+          const int whole = a.ranged == 2 ? items / ctas * ctas : 0;
+          for (int x = cta; x < whole && ok; x += ctas)
+            ok = pass(kept[x % count], x / count, 0, all_tiles, -1, 0);
+          const int hp0 = count > 0 ? whole / count : 0;
+          const int s0 = hp0 * total + starts[whole - hp0 * count];
+          const int all = total * a.nhp - s0;
+          const int share = max((all + ctas - 1) / ctas, MIN_SHARE);
+          int s = cta * share;
+          const int s1 = min(s + share, all);
+          if (lane == 0) static_cast<Cut*>(a.cuts)[cta].parts = 0;
+          if (s < s1 && ok) {
+            int hp = (s0 + s) / total, x = s0 + s - hp * total;
+            int k = 0;  // the piece that key tile x is of
+            for (int o = 128; o; o >>= 1)
+              if (k + o < count && starts[k + o] <= x) k += o;
+            while (s < s1 && ok) {
+              const int w = starts[k + 1] - starts[k];
+              const int t0 = x - starts[k], t1 = min(w, t0 + (s1 - s));
+              ok = pass(kept[k], hp, t0, t1, t0 > 0 ? 2 * cta : t1 < w ? 2 * cta + 1 : -1,
+                        t0 == 0 && t1 < w ? (s + w - 1) / share - cta + 1 : 0);
+              s += t1 - t0;
+              x += t1 - t0;
+              if (++k == count) {
+                k = 0;
+                x = 0;
+                ++hp;
+              }
+            }
+          }
+        }
+      } else {
+        // more pieces than are kept: whole items, causal the last pieces first, as above
+        const int items = a.slots * a.nhp;
+        int step = 2 * (ctas - 1 - cta) + 1;
+        for (int x = cta; x < items && ok;) {
           int slot, hp;
-          if (by_length) {
+          if (a.causal) {
             slot = a.by_nhp.div(x);
             hp = x - slot * a.nhp;
-            slot = sorted ? numbers[slot] : a.slots - 1 - slot;
+            slot = a.slots - 1 - slot;
             x += step;
             step = 2 * ctas - step;
           } else {
@@ -520,81 +601,14 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             slot = x - hp * a.slots;
             x += ctas;
           }
-          if (!pieces.item(pieces.find_warp(slot), slot, r)) continue;
-          r.h0 = hp * a.pack;
-          ok = pass(r);
-        }
-      } else {
-        // The pieces that there are, head pack by head pack, are the items. Whole ones in rounds as
-        // long as every CTA gets one (a.ranged 2), whose CTAs share keys; of the others an equal
-        // share of the key tiles (an item without any counts as one).
-        int total = 0, count = 0;
-        for (int s0 = 0; s0 < a.slots; s0 += 32) {
-          const int s = s0 + lane;
-          int w = 0;
-          if (s < a.slots && pieces.item(pieces.find(s), s, r)) w = max(1, max(r.e0, r.e1));
-          const unsigned found = __ballot_sync(0xffffffffu, w > 0);
-          int sum = w;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += y;
-          }
-          if (w > 0) {
-            const int at = count + __popc(found & ((1u << lane) - 1u));
-            starts[at] = total + sum - w;
-            numbers[at] = s;
-          }
-          total += __shfl_sync(0xffffffffu, sum, 31);
-          count += __popc(found);
-        }
-        if (lane == 0) starts[count] = total;
-        __syncwarp();
-        const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
-        auto load = [&](int n, int hp) {
-          pieces.item(pieces.find_warp(numbers[n]), numbers[n], r);
-          r.h0 = hp * a.pack;
-        };
-        int whole = a.ranged == 2 ? count * a.nhp / ctas * ctas : 0;
-        for (int x = cta; x < whole && ok; x += ctas) {
-          load(x % count, x / count);
-          ok = pass(r);
-        }
-        if (count == 0) whole = 0;
-        const int hp0 = count > 0 ? whole / count : 0, n0 = whole - hp0 * count;
-        const int s0 = hp0 * total + (count > 0 ? starts[n0] : 0);
-        const int all = total * a.nhp - s0;
-        const int share = max((all + ctas - 1) / ctas, MIN_SHARE);
-        int s = cta * share;
-        const int s1 = min(s + share, all);
-        if (lane == 0) static_cast<Cut*>(a.cuts)[cta].parts = 0;
-        if (s < s1 && ok) {
-          int hp = (s0 + s) / total, x = s0 + s - hp * total;
-          int n = 0;  // the piece that key tile x is of
-          for (int o = MAX_SLOTS / 2; o; o >>= 1)
-            if (n + o < count && starts[n + o] <= x) n += o;
-          while (s < s1 && ok) {
-            load(n, hp);
-            const int w = starts[n + 1] - starts[n];
-            const int t0 = x - starts[n], t1 = min(w, t0 + (s1 - s));
-            r.t0 = t0;
-            r.e0 = max(t0, min(r.e0, t1));
-            r.e1 = max(t0, min(r.e1, t1));
-            r.part = t0 > 0 ? 2 * cta : t1 < w ? 2 * cta + 1 : -1;
-            if (t0 == 0 && t1 < w) r.parts = (s + w - 1) / share - cta + 1;
-            ok = pass(r);
-            s += t1 - t0;
-            x += t1 - t0;
-            if (++n == count) {
-              n = 0;
-              x = 0;
-              ++hp;
-            }
-          }
+          Piece p;
+          if (pieces.piece(pieces.find_warp(slot), slot, p)) ok = pass(p, hp, 0, all_tiles, -1, 0);
         }
       }
-      r.tokens = 0;
-      if (ok) pass(r);
+      if (ok) {
+        Piece p = {};
+        pass(p, 0, 0, 0, -1, 0);
+      }
     } else if constexpr (!CODES) {
       // ------------------------------------------------------------ values of partly hidden tiles
       // Rows behind the sequence become zeros (a weight of 0 times a NaN would be a NaN). Where a
@@ -610,7 +624,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         const Record r = records[at];
         __syncwarp();
         if (lane == 0) mbar_arrive(&rec_empty[at]);
-        if (r.tokens == 0) break;
+        if (r.p.tokens == 0) break;
         const int steps = r.steps();
         for (int j = 0; j < steps && ok; ++j) {
           const int u = idx + 2 * j + 1, s = u % STAGES;
@@ -622,7 +636,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
 #pragma unroll 1
             for (int w = 0; w < 4; ++w) {
               uint8_t* vrow = smem + C::OFF_KV + s * C::BYTES + (w * 32 + lane) * 128;
-              const bool behind = key0 + w * 32 + lane >= r.len;
+              const bool behind = key0 + w * 32 + lane >= r.p.len;
               uint32_t m = 0;
               if (!behind && a.causal) {
 #pragma unroll
@@ -662,8 +676,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         ok = mbar_wait_warp(&rec_full[at], static_cast<uint32_t>(n / RECORDS) & 1u, a.status,
                             abort_flag);
         if (!ok) break;
-        const int t0 = records[at].t0, steps = records[at].steps(), len = records[at].len;
-        const int b = records[at].b, g = records[at].h0 / a.group, tokens = records[at].tokens;
+        const int t0 = records[at].t0, steps = records[at].steps(), len = records[at].p.len;
+        const int b = records[at].p.b, g = records[at].h0 / a.group, tokens = records[at].p.tokens;
         __syncwarp();
         if (lane == 0) mbar_arrive(&rec_empty[at]);
         if (tokens == 0) break;
@@ -752,9 +766,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                           abort_flag))
         break;
       const Record& rec = records[at];
-      const int t0 = rec.t0, e = t ? rec.e1 : rec.e0, steps = rec.steps();
-      const int len = rec.len, pos0 = rec.pos0, tokens = rec.tokens, part = rec.part;
-      const int row0 = rec.row0, h0 = rec.h0, parts = rec.parts;
+      const int t0 = rec.t0, e = t ? rec.p.e1 : rec.p.e0, steps = rec.steps();
+      const int len = rec.p.len, pos0 = rec.p.pos0, tokens = rec.p.tokens, part = rec.part;
+      const int row0 = rec.p.row0, h0 = rec.h0, parts = rec.parts;
       __syncwarp();
       if (lane == 0) mbar_arrive(&rec_empty[at]);
       if (tokens == 0) break;
@@ -1093,10 +1107,10 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       const Record r = records[at];
       __syncwarp();
       if (lane == 0) mbar_arrive(&rec_empty[at]);
-      if (r.tokens == 0) break;
+      if (r.p.tokens == 0) break;
       const int steps = r.steps();
       if (steps <= 0) continue;
-      const int end = max(r.e0, r.e1);
+      const int end = max(r.p.e0, r.p.e1);
       auto turn_q = [&](int t) {
         if (!mbar_wait_warp(&q_loaded[t], static_cast<uint32_t>(nq[t]) & 1u, a.status, abort_flag))
           return false;
@@ -1171,11 +1185,11 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             rows |= rows >> 16;
             rows = (rows | rows >> 8) & 0xffu;
             off |= rows << (8 * i);
-            if (((rows >> r8) & 1u) || tile * TILE + row >= r.len) {
+            if (((rows >> r8) & 1u) || tile * TILE + row >= r.p.len) {
 #pragma unroll
               for (int k = 0; k < NP; ++k) c[k] = make_uint4(0, 0, 0, 0);
               if (FOLD) scale = 0.f;
-              if (!FOLD && tile * TILE + row < r.len) sc[row] = __int_as_float(0x7fc00000);
+              if (!FOLD && tile * TILE + row < r.p.len) sc[row] = __int_as_float(0x7fc00000);
             }
           }
           __syncwarp();
@@ -1213,7 +1227,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         // beside the softmax)
 #pragma unroll 1
         for (int x = 0; x < 2 && ok; ++x) {
-          if (FOLD && j == r.t0 && (x ? r.e1 : r.e0) > r.t0) ok = turn_q(x);
+          if (FOLD && j == r.t0 && (x ? r.p.e1 : r.p.e0) > r.t0) ok = turn_q(x);
           ok = ok && turn(x != 0, j);
         }
         ++tiles;
