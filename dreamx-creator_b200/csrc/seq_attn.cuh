@@ -66,29 +66,32 @@ struct Compute<T, SRDIT_KV_PLAIN> {
   using type = T;
 };
 
-// 16 codes as 16 fp16 values, exactly, in order (word i: values 2i and 2i + 1)
+// 4 codes as fp16 values, exactly: the first two in x, the others in y
+template <int CODE>
+SRDIT_DEV void widen4(uint32_t u, uint32_t& x, uint32_t& y) {
+  if constexpr (CODE == SRDIT_Q_INT8) {
+    // n + 128 behind the exponent of 1024, less 1152
+    const uint32_t b = u ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t lo = __byte_perm(b, 0x64646464u, 0x4140), hi = __byte_perm(b, 0x64646464u, 0x4342);
+    const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&lo), off);
+    const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&hi), off);
+    x = *reinterpret_cast<const uint32_t*>(&p);
+    y = *reinterpret_cast<const uint32_t*>(&q);
+  } else {
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}"
+        : "=r"(x), "=r"(y)
+        : "r"(u));
+  }
+}
+// 16 codes, in order (word i: values 2i and 2i + 1)
 template <int CODE>
 SRDIT_DEV void widen_codes(uint4 w, uint32_t (&h)[8]) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (CODE == SRDIT_Q_INT8) {
-      // n + 128 behind the exponent of 1024, less 1152
-      const uint32_t b = u[i] ^ 0x80808080u;
-      const __half2 off = __half2half2(__ushort_as_half(0x6480));
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t x = __byte_perm(b, 0x64646464u, e ? 0x4342 : 0x4140);
-        const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
-        h[2 * i + e] = *reinterpret_cast<const uint32_t*>(&y);
-      }
-    } else {
-      asm("{.reg .b16 l, h; mov.b32 {l, h}, %2;\n\t"
-          "cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}"
-          : "=r"(h[2 * i]), "=r"(h[2 * i + 1])
-          : "r"(u[i]));
-    }
-  }
+  widen4<CODE>(w.x, h[0], h[1]);
+  widen4<CODE>(w.y, h[2], h[3]);
+  widen4<CODE>(w.z, h[4], h[5]);
+  widen4<CODE>(w.w, h[6], h[7]);
 }
 // whether one of 4 e4m3 codes is NaN
 SRDIT_DEV bool nan_codes(uint32_t w) {

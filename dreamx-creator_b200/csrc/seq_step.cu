@@ -189,6 +189,8 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
   int page_now = -1, page_next = pages_at(0);
   int fetched = 0;
   uint32_t there = 0;  // two bits a slot: whether the halves' pages are ones
+  const float* k_scale = CODES ? a.scale[0] + kvh * a.ss[0][2] : nullptr;
+  const float* v_scale = CODES ? a.scale[1] + kvh * a.ss[1][2] : nullptr;
   auto fetch = [&](int slot) {
     const int in = fetched & ((32 >> pages_log) - 1);
     if (in == 0) {
@@ -229,8 +231,8 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
       const float* k = a.scale[0];
       const float* v = a.scale[1];
       if (on) {
-        k += p * a.ss[0][0] + in_page * a.ss[0][1] + kvh * a.ss[0][2];
-        v += p * a.ss[1][0] + in_page * a.ss[1][1] + kvh * a.ss[1][2];
+        k = k_scale + (p * a.ss[0][0] + in_page * a.ss[0][1]);
+        v = v_scale + (p * a.ss[1][0] + in_page * a.ss[1][1]);
       }
       cp_async4(smem_u32(&sc[warp][slot][lane]), k, on);
       cp_async4(smem_u32(&sc[warp][slot][KB + lane]), v, on);
@@ -498,35 +500,42 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
     }
 #pragma unroll
     for (int y = 0; y < NB; ++y) {
-      uint4 vf[4][NV];
+      // the operand rows are the lane group's value columns 2w and 2w + 1 of its x-th eight: of each
+      // the keys of rows 2c and 2c + 1 (a0, a1) and those 8 further on side by side
+      if constexpr (CODES) {
+        const uint32_t r0[4] = {vr[y][0][0].x, vr[y][0][0].y, vr[y][0][0].z, vr[y][0][0].w};
+        const uint32_t r1[4] = {vr[y][1][0].x, vr[y][1][0].y, vr[y][1][0].z, vr[y][1][0].w};
+        const uint32_t r2[4] = {vr[y][2][0].x, vr[y][2][0].y, vr[y][2][0].z, vr[y][2][0].w};
+        const uint32_t r3[4] = {vr[y][3][0].x, vr[y][3][0].y, vr[y][3][0].z, vr[y][3][0].w};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (CODES) {
-          uint32_t w[8];
-          widen_codes<CODE>(vr[y][r][0], w);
-          vf[r][0] = make_uint4(w[0], w[1], w[2], w[3]);
-          if constexpr (NV == 2) vf[r][1] = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
+        for (int j = 0; j < 2 * NV; ++j)
 #pragma unroll
-          for (int x = 0; x < NV; ++x) vf[r][x] = vr[y][r][x];
-        }
-      }
+          for (int e = 0; e < 2; ++e) {
+            // (codes of two columns of two rows, by column)
+            uint32_t a0, a1, a2, a3;
+            widen4<CODE>(__byte_perm(r0[j], r1[j], e ? 0x7362 : 0x5140), a0, a1);
+            widen4<CODE>(__byte_perm(r2[j], r3[j], e ? 0x7362 : 0x5140), a2, a3);
 #pragma unroll
-      for (int x = 0; x < NV; ++x) {
-        const uint32_t r0[4] = {vf[0][x].x, vf[0][x].y, vf[0][x].z, vf[0][x].w};
-        const uint32_t r1[4] = {vf[1][x].x, vf[1][x].y, vf[1][x].z, vf[1][x].w};
-        const uint32_t r2[4] = {vf[2][x].x, vf[2][x].y, vf[2][x].z, vf[2][x].w};
-        const uint32_t r3[4] = {vf[3][x].x, vf[3][x].y, vf[3][x].z, vf[3][x].w};
+            for (int n = 0; n < NT; ++n)
+              mma16816<E>(o[n][2 * j + e], a0, a1, a2, a3, pf[n][y][0], pf[n][y][1]);
+          }
+      } else {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          // the lane group's columns 2w (operand row g) and 2w + 1 (row g + 8)
-          const uint32_t a0 = __byte_perm(r0[w], r1[w], 0x5410);
-          const uint32_t a1 = __byte_perm(r0[w], r1[w], 0x7632);
-          const uint32_t a2 = __byte_perm(r2[w], r3[w], 0x5410);
-          const uint32_t a3 = __byte_perm(r2[w], r3[w], 0x7632);
+        for (int x = 0; x < NV; ++x) {
+          const uint32_t r0[4] = {vr[y][0][x].x, vr[y][0][x].y, vr[y][0][x].z, vr[y][0][x].w};
+          const uint32_t r1[4] = {vr[y][1][x].x, vr[y][1][x].y, vr[y][1][x].z, vr[y][1][x].w};
+          const uint32_t r2[4] = {vr[y][2][x].x, vr[y][2][x].y, vr[y][2][x].z, vr[y][2][x].w};
+          const uint32_t r3[4] = {vr[y][3][x].x, vr[y][3][x].y, vr[y][3][x].z, vr[y][3][x].w};
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            mma16816<E>(o[n][x * 4 + w], a0, a1, a2, a3, pf[n][y][0], pf[n][y][1]);
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a0 = __byte_perm(r0[w], r1[w], 0x5410);
+            const uint32_t a1 = __byte_perm(r0[w], r1[w], 0x7632);
+            const uint32_t a2 = __byte_perm(r2[w], r3[w], 0x5410);
+            const uint32_t a3 = __byte_perm(r2[w], r3[w], 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma16816<E>(o[n][x * 4 + w], a0, a1, a2, a3, pf[n][y][0], pf[n][y][1]);
+          }
         }
       }
     }
