@@ -104,6 +104,8 @@ assert CROSS_ATTN_LAYOUT.size == ctypes.sizeof(CrossAttnArgs)
 
 
 SRDIT_KV_PLAIN = -1
+SRDIT_WAY_STEP, SRDIT_WAY_STEP_SHARES = 1, 2
+SRDIT_WAY_CHUNK, SRDIT_WAY_CHUNK_SHARES, SRDIT_WAY_CHUNK_REST = 3, 4, 5
 
 
 class KvPages(ctypes.Structure):
@@ -184,6 +186,7 @@ SIGNATURES = {
     "srdit_kv_read": [ctypes.POINTER(KvPages), c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
     "srdit_seq_attn": [ctypes.POINTER(SeqAttnArgs), c_vp],
     "srdit_seq_attn_workspace": [ctypes.POINTER(SeqAttnArgs)],
+    "srdit_seq_attn_way": [ctypes.POINTER(SeqAttnArgs)],
     "srdit_winattn_plan": [c_vp, c_int, c_int, c_int, ctypes.POINTER(WinattnTiling)],
     "srdit_winattn_fwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int,
                           ctypes.POINTER(WinattnGeom), ctypes.POINTER(WinattnTiling), c_vp,

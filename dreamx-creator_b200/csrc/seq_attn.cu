@@ -86,6 +86,14 @@ extern "C" int srdit_seq_attn_workspace(const srdit_seq_attn_args* args) {
   return static_cast<int>((p.ws_floats + 255) / 256);
 }
 
+extern "C" int srdit_seq_attn_way(const srdit_seq_attn_args* args) {
+  if (!args || sattn::check(*args) != 0) return SRDIT_WAY_NONE;
+  const srdit_seq_attn_args u = sattn::with_max_q(*args);
+  const sattn::Plan p = sattn::make_plan(u, u.max_q, num_sms(device_here()));
+  if (p.step) return p.shared ? SRDIT_WAY_STEP_SHARES : SRDIT_WAY_STEP;
+  return p.ranged == 0 ? SRDIT_WAY_CHUNK : p.ranged == 1 ? SRDIT_WAY_CHUNK_SHARES : SRDIT_WAY_CHUNK_REST;
+}
+
 extern "C" int srdit_seq_attn(const srdit_seq_attn_args* args, cudaStream_t stream) {
   if (!args) return SRDIT_EINVAL;
   const int rc = sattn::check(*args);

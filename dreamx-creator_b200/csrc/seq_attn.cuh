@@ -28,6 +28,7 @@ struct Args {
   int pack, pack_log, rt;   // heads of a group side by side in a query tile (2^n), its tokens
   int slots, nhp;           // pieces of 2 rt tokens (some empty), head packs
   Divisor by_nhp, by_slots, by_piece;  // ... and 2 rt
+  Divisor by_packs, by_ctas;           // ... the packs of a group, the CTAs
   int ranged, box_log;      // items shared out by key tiles; log2 of the keys of a page's box
   void* cuts;
   // step_kernel

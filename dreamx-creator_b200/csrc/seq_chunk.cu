@@ -77,10 +77,10 @@ struct Piece {
 // those from t0 on.
 struct Record {
   Piece p;
-  int h0, t0;
+  int h0, g, t0;     // first head, key head
   int part;          // -1: all of the keys; else where in the workspace the part goes
   int parts;         // of an item that this CTA begins and others end: in how many it is
-  int pad[4];
+  int pad[3];
   SRDIT_DEV int steps() const { return max(p.e0, p.e1) - t0; }
 };
 
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   // scale, at most 448 x 2^7, is one of fp16; and f = 2^e
   auto in_units = [](float scale, float& f, float& e) {
     const uint32_t top = __reduce_max_sync(
-        0xffffffffu, scale < 3e38f ? __float_as_uint(fmaxf(scale, 0.f)) : 0u);
+        0xffffffffu, fabsf(scale) < 3e38f ? __float_as_uint(fabsf(scale)) : 0u);
     const int x = max(static_cast<int>(top >> 23) - 133, -100);
     f = exp2_int(x);
     e = static_cast<float>(x);
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if (lane == 0) mbar_arrive(&rec_empty[at]);
         if (r.p.tokens == 0) break;
         if (r.steps() <= 0) continue;
-        const int g = r.h0 / a.group;
+        const int g = r.g;
         const int boxes = TILE >> a.box_log;
         auto load_q = [&](int t) {
           if (!mbar_wait_warp(&q_empty[t], (static_cast<uint32_t>(nq[t]) & 1u) ^ 1u, a.status,
@@ -478,6 +478,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           r.p.e0 = max(t0, min(p.e0, t1));
           r.p.e1 = max(t0, min(p.e1, t1));
           r.h0 = hp * a.pack;
+          r.g = a.by_packs.div(hp);
           r.t0 = t0;
           r.part = part;
           r.parts = parts;
@@ -545,8 +546,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               x += step;
               step = 2 * ctas - step;
             } else {
-              hp = x / count;
-              k = x - hp * count;
+              for (hp = 0, k = x; k >= count; k -= count) ++hp;
               x += ctas;
             }
             ok = pass(kept[k], hp, 0, all_tiles, -1, 0);
@@ -554,26 +554,35 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         } else {
           // Head pack by head pack. Whole items in rounds as long as every CTA gets one (a.ranged 2),
           // whose CTAs share keys; of the others an equal share of the key tiles.
-          const int whole = a.ranged == 2 ? items / ctas * ctas : 0;
-          for (int x = cta; x < whole && ok; x += ctas)
-            ok = pass(kept[x % count], x / count, 0, all_tiles, -1, 0);
-          const int hp0 = count > 0 ? whole / count : 0;
-          const int s0 = hp0 * total + starts[whole - hp0 * count];
+          // (Loops in place of divisions, which are long code.)
+          int whole = 0, hp0 = 0, k0 = 0;
+          if (a.ranged == 2) {
+            whole = a.by_ctas.div(items) * ctas;
+            for (int x = cta, hp = 0, k = cta; x < whole && ok; x += ctas, k += ctas) {
+              for (; k >= count; k -= count) ++hp;
+              ok = pass(kept[k], hp, 0, all_tiles, -1, 0);
+            }
+            for (k0 = whole; count > 0 && k0 >= count; k0 -= count) ++hp0;
+          }
+          const int s0 = hp0 * total + starts[k0];
           const int all = total * a.nhp - s0;
-          const int share = max((all + ctas - 1) / ctas, MIN_SHARE);
+          const int share = max(a.by_ctas.div(all + ctas - 1), MIN_SHARE);
           int s = cta * share;
           const int s1 = min(s + share, all);
           if (lane == 0) static_cast<Cut*>(a.cuts)[cta].parts = 0;
           if (s < s1 && ok) {
-            int hp = (s0 + s) / total, x = s0 + s - hp * total;
+            int hp = 0, x = s0 + s;
+            for (; x >= total; x -= total) ++hp;
             int k = 0;  // the piece that key tile x is of
             for (int o = 128; o; o >>= 1)
               if (k + o < count && starts[k + o] <= x) k += o;
             while (s < s1 && ok) {
               const int w = starts[k + 1] - starts[k];
               const int t0 = x - starts[k], t1 = min(w, t0 + (s1 - s));
-              ok = pass(kept[k], hp, t0, t1, t0 > 0 ? 2 * cta : t1 < w ? 2 * cta + 1 : -1,
-                        t0 == 0 && t1 < w ? (s + w - 1) / share - cta + 1 : 0);
+              int parts = 0;
+              if (t0 == 0 && t1 < w)
+                for (parts = 2; (cta + parts) * share < s + w;) ++parts;
+              ok = pass(kept[k], hp, t0, t1, t0 > 0 ? 2 * cta : t1 < w ? 2 * cta + 1 : -1, parts);
               s += t1 - t0;
               x += t1 - t0;
               if (++k == count) {
@@ -677,7 +686,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                             abort_flag);
         if (!ok) break;
         const int t0 = records[at].t0, steps = records[at].steps(), len = records[at].p.len;
-        const int b = records[at].p.b, g = records[at].h0 / a.group, tokens = records[at].p.tokens;
+        const int b = records[at].p.b, g = records[at].g, tokens = records[at].p.tokens;
         __syncwarp();
         if (lane == 0) mbar_arrive(&rec_empty[at]);
         if (tokens == 0) break;
@@ -890,7 +899,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             float most = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const float v = sc[128 + w * 32 + lane];
+              const float v = fabsf(sc[128 + w * 32 + lane]);
               most = fmaxf(most, v < 3e38f ? v : 0.f);
             }
             most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
@@ -1288,17 +1297,18 @@ Plan plan_chunk(const srdit_seq_attn_args& u, int sms) {
   p.slots = u.T / (2 * p.rt) + u.B;
   p.nhp = u.H / p.pack;
   const long long items = static_cast<long long>(p.slots) * p.nhp;
-  long long keys = u.Tk;
+  long long keys = u.Tk, held = u.Tk;
   if (u.pages) {
-    const long long held = static_cast<long long>(u.pages->table_width) * u.pages->page_size;
+    held = static_cast<long long>(u.pages->table_width) * u.pages->page_size;
     keys = u.max_kv > 0 && u.max_kv < held ? u.max_kv : held;
   }
   const long long tiles = (keys + TILE - 1) / TILE;
   // Few items of many key tiles are shared out by key tiles, and so is what a last round of whole
-  // items would leave idle (items x tiles in 32 bits); joining the parts costs what several do.
+  // items would leave idle (all key tiles in 32 bits, however long the sequences turn out to be);
+  // joining the parts costs what several do.
   const long long some =
       (u.B == 1 ? (u.T + 2 * p.rt - 1) / (2 * p.rt) : p.slots - u.B / 2) * static_cast<long long>(p.nhp);
-  if (p.slots <= MAX_SLOTS && items * tiles < (1ll << 30)) {
+  if (p.slots <= MAX_SLOTS && items * (held / TILE + 1) < (1ll << 30)) {
     // CTAs of shares go through keys at different places and miss what others have fetched: a step
     // takes a quarter more
     const long long rounds = (some + sms - 1) / sms, steps = some * tiles;
@@ -1370,6 +1380,8 @@ int run_chunk(const srdit_seq_attn_args& u, Args& a, const Plan& p, cudaStream_t
   a.by_nhp = Divisor::of(p.nhp);
   a.by_slots = Divisor::of(p.slots);
   a.by_piece = Divisor::of(2 * p.rt);
+  a.by_packs = Divisor::of(a.group / p.pack);
+  a.by_ctas = Divisor::of(p.ctas);
   a.ranged = p.ranged;
   const int page = u.pages ? u.pages->page_size : TILE;
   a.box_log = page >= TILE ? 7 : page == 64 ? 6 : page == 32 ? 5 : 4;

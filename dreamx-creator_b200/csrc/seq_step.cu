@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
 #pragma unroll
       for (int y = 0; y < NB; ++y)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) top = fmaxf(top, vs[y][h] < 3e38f ? vs[y][h] : 0.f);
+        for (int h = 0; h < 2; ++h)
+          top = fmaxf(top, fabsf(vs[y][h]) < 3e38f ? fabsf(vs[y][h]) : 0.f);
       top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
       lv = __log2f(fmaxf(top, 1e-30f));
     }

@@ -648,7 +648,7 @@ int srdit_cross_attn_items(const srdit_cross_attn_args* args);
  * units of 16 bytes. D a multiple of 8 (16 for codes), at most 128; page_size 16, 32, 64 or a
  * multiple of 128; Hkv at most 1024. The table (int32, on the device) may hold anything where a
  * sequence has no page yet. A page out of [0, pages) is none: nothing is written to it, it reads
- * as zeros, and its keys are not seen.
+ * as zeros, and its keys are not seen. Entry points that read the cache leave it as it is.
  */
 #define SRDIT_KV_PLAIN (-1)
 typedef struct srdit_kv_pages {
@@ -728,6 +728,17 @@ typedef struct srdit_seq_attn_args {
 } srdit_seq_attn_args;
 int srdit_seq_attn(const srdit_seq_attn_args* args, cudaStream_t stream);
 int srdit_seq_attn_workspace(const srdit_seq_attn_args* args);
+/* How these arguments are run on the current device: few query rows per key head, each (sequence,
+ * key head)'s keys split over a cluster of CTAs (SRDIT_WAY_STEP) or all keys in equal shares
+ * (STEP_SHARES); many, in whole items of two query tiles (CHUNK), all key tiles in equal shares
+ * (CHUNK_SHARES) or those of the last round of items (CHUNK_REST). */
+#define SRDIT_WAY_NONE 0
+#define SRDIT_WAY_STEP 1
+#define SRDIT_WAY_STEP_SHARES 2
+#define SRDIT_WAY_CHUNK 3
+#define SRDIT_WAY_CHUNK_SHARES 4
+#define SRDIT_WAY_CHUNK_REST 5
+int srdit_seq_attn_way(const srdit_seq_attn_args* args);
 
 #ifdef __cplusplus
 }

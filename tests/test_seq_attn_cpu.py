@@ -178,3 +178,54 @@ def test_clusters_are_never_launched_programmatically(srdit):
     body = re.search(r"^static int launch\(.*?^\}", text, re.S | re.M).group(0)
     assert "launch_clusters(" in body and "SRDIT_LAUNCH" not in body
     assert text.count("step_kernel<T, DP, NT, CODE>") == 2   # its shared memory, its launch
+
+
+# ------------------------------------------------------------------ how a call is run
+STEP, STEP_SHARES, CHUNK, CHUNK_SHARES, CHUNK_REST = 1, 2, 3, 4, 5
+
+
+def _way(lib, pages, B, T, H, Hkv, kv=0, max_q=0, causal=1, D=128, Tk=0, width=None, code=-1):
+    v = dict(q=10 << 20, k=11 << 20, v=12 << 20, out=13 << 20, T=T, Tk=Tk, B=B, H=H, Hkv=Hkv, D=D,
+             q_stride=(H * D, D), k_stride=(Hkv * D, D), v_stride=(Hkv * D, D), o_stride=(H * D, D),
+             cu_q=14 << 20, kv_lens=15 << 20, max_q=max_q, max_kv=kv, causal=causal, scale=0.125)
+    a = _fill(lib.SeqAttnArgs(), v)
+    if pages:
+        st = (16 * Hkv * D, Hkv * D, D)
+        p = _pages(lib, B=B, Hkv=Hkv, D=D, code=code, k_stride=st, v_stride=st,
+                   ks_stride=(16 * Hkv, Hkv, 1), vs_stride=(16 * Hkv, Hkv, 1),
+                   table_width=width or max(1, -(-kv // 16)))
+        a.pages = ctypes.addressof(p)
+    L = lib.lib()
+    ws = L.srdit_seq_attn_workspace(ctypes.byref(a))
+    way = L.srdit_seq_attn_way(ctypes.byref(a))
+    # parts of rows meet in the workspace (parts of clusters only where they are more than 8)
+    assert way == STEP or (ws > 0) == (way in (STEP_SHARES, CHUNK_SHARES, CHUNK_REST))
+    return way
+
+
+@pytest.mark.parametrize("kw,way", [
+    (dict(B=4, T=4, H=32, Hkv=8, kv=1024, max_q=1), STEP),
+    (dict(B=32, T=32, H=32, Hkv=8, kv=4096, max_q=1), STEP_SHARES),
+    (dict(B=1100, T=1100, H=32, Hkv=8, kv=4096, max_q=1), STEP),           # more than are kept
+    (dict(B=32, T=32, H=32, Hkv=8, kv=4096, max_q=1, code=1), STEP_SHARES),
+    (dict(B=8, T=32, H=16, Hkv=4, kv=64, max_q=4), STEP),                  # 16 rows a key head
+    (dict(B=8, T=40, H=16, Hkv=4, kv=64, max_q=5), CHUNK),
+    (dict(B=1, T=64, H=32, Hkv=8, kv=32768), CHUNK_SHARES),
+    (dict(B=1, T=64, H=32, Hkv=8, kv=300), CHUNK),
+    (dict(B=1, T=6912, H=24, Hkv=24, kv=13824, causal=0), CHUNK_REST),
+    (dict(B=1, T=6912, H=24, Hkv=24, kv=512, causal=0), CHUNK),
+    (dict(B=500, T=6912, H=24, Hkv=24, kv=13824, causal=0), CHUNK),        # more pieces than are kept
+    (dict(B=1, T=1400, H=32, Hkv=8, kv=1 << 20), CHUNK_SHARES),
+    (dict(B=1, T=1400, H=32, Hkv=8, kv=1 << 20, width=1 << 26), CHUNK),    # key tiles beyond 32 bits
+])
+def test_ways_over_pages(srdit, kw, way):
+    assert _way(srdit._lib, True, **kw) == way
+
+
+@pytest.mark.parametrize("kw,way", [
+    (dict(B=1, T=1, H=1, Hkv=1, Tk=1), CHUNK), (dict(B=16, T=4000, H=24, Hkv=24, Tk=4000), CHUNK),
+    (dict(B=1, T=8192, H=32, Hkv=8, Tk=8192), CHUNK),
+    (dict(B=1, T=300, H=4, Hkv=4, Tk=20000), CHUNK_SHARES),
+    (dict(B=1, T=2304, H=24, Hkv=24, Tk=6912, causal=0), CHUNK_REST)])
+def test_ways_of_packed_rows(srdit, kw, way):
+    assert _way(srdit._lib, False, **kw) == way
