@@ -832,7 +832,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if constexpr (CODES) {
           // Two passes over the scores, 64 of them at a time, so that the code is short: with all 128
           // in registers at once, as below, it does not fit the instruction caches beside that of the
-          // warps that widen codes (PASSES).
+          // warps that widen codes. (2 x 512 queries on 16384 e4m3 keys, 32 heads over 8 of 128: 421
+          // us so, 406 in passes of 32, 361 in passes of 64; the same keys in 16 bits 258.)
           const float* sc = scales + (tiles % C::SCALES) * 256;
           const float* units =
               reinterpret_cast<const float*>(smem + C::OFF_UNITS) + tiles % C::SCALES * 8;
@@ -1251,39 +1252,79 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   }
 }
 
-// One block per 32 rows of the items that the CTAs' shares cut: joins their parts, 8 columns a
-// thread, a row a lane.
+// Joins the parts of the items that the CTAs' shares cut: a block takes 32 columns of 32 rows of
+// one, then others, of as many as there are (a block for every CTA's item, rows and columns, most
+// of which have nothing to do, took 10 us to launch); a thread four columns of a row, four parts'
+// loads in flight: bounded by their latency.
+constexpr int JOIN_COLS = 32;
+constexpr int JOIN_CTAS = 256;  // of a launch by shares, at most
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(DP / 8 * 32) join_chunk_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(JOIN_COLS / 4 * 32)
+    join_chunk_kernel(const __grid_constant__ Args a, int ctas) {
   pdl_begin();
-  const Cut cut = static_cast<const Cut*>(a.cuts)[blockIdx.x];
-  if (cut.parts == 0) return;
-  const int row = blockIdx.y * 32 + (threadIdx.x & 31), d = (threadIdx.x >> 5) * 8;
+  __shared__ int cuts_of[JOIN_CTAS];
+  __shared__ int found[JOIN_COLS / 4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Cut* all_cuts = static_cast<const Cut*>(a.cuts);
+  const bool mine = static_cast<int>(threadIdx.x) < ctas && all_cuts[threadIdx.x].parts != 0;
+  const unsigned bits = __ballot_sync(0xffffffffu, mine);
+  if (lane == 0) found[warp] = __popc(bits);
+  __syncthreads();
+  int count = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < JOIN_COLS / 4; ++w) {
+    if (w < warp) before += found[w];
+    count += found[w];
+  }
+  if (mine) cuts_of[before + __popc(bits & ((1u << lane) - 1u))] = threadIdx.x;
+  __syncthreads();
+  const int cols = (a.D + JOIN_COLS - 1) / JOIN_COLS, tasks = count * (ROWS / 32) * cols;
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+  const int which = task / ((ROWS / 32) * cols), rest = task - which * ((ROWS / 32) * cols);
+  const int first = cuts_of[which];  // the CTA that begins the item
+  const Cut cut = all_cuts[first];
+  const int row = rest / cols * 32 + lane;
+  const int d = rest % cols * JOIN_COLS + warp * 4;
   const int token = row >> a.pack_log, head = cut.h0 + (row & (a.pack - 1));
-  if (token >= cut.tokens || d >= a.D) return;
-  float m = neg_inf(), l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int p = 0; p < cut.parts; ++p) {
-    const int cta = static_cast<int>(blockIdx.x) + p, part = p == 0 ? 2 * cta + 1 : 2 * cta;
-    const float2 q = reinterpret_cast<const float2*>(a.ml)[part * ROWS + row];
-    if (q.x == neg_inf()) continue;  // it saw no key
-    const float* ws = a.ws + (static_cast<long long>(part) * DP + d) * ROWS + row;
-    float v[8];
+  if (token >= cut.tokens || d >= a.D) continue;
+  float m = neg_inf(), l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int p0 = 0; p0 < cut.parts; p0 += 4) {
+    float2 q[4];
+    float v[4][4];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = ws[x * ROWS];
-    const float mn = max2(m, q.x);
-    const float f0 = ex2(m - mn), f1 = ex2(q.x - mn);
+    for (int y = 0; y < 4; ++y) {
+      const int p = p0 + y, part = 2 * (first + p) + (p == 0);
+      const bool on = p < cut.parts;
+      const float* ws = a.ws + (static_cast<long long>(part) * DP + d) * ROWS + row;
+      q[y] = on ? __ldg(reinterpret_cast<const float2*>(a.ml) + part * ROWS + row)
+                : make_float2(neg_inf(), 0.f);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[y][x] = on ? __ldg(ws + x * ROWS) : 0.f;
+    }
+    float mn = m;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) mn = max2(mn, q[y].x);
+    if (mn == neg_inf()) continue;  // no key seen yet
+    const float f = ex2(m - mn);
     m = mn;
-    l = l * f0 + q.y * f1;
+    l *= f;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) acc[x] = acc[x] * f0 + v[x] * f1;
+    for (int x = 0; x < 4; ++x) acc[x] *= f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      if (q[y].x == neg_inf()) continue;  // it saw no key
+      const float g = ex2(q[y].x - m);
+      l = fmaf(q[y].y, g, l);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[x] = fmaf(v[y][x], g, acc[x]);
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint32_t w[4];
-#pragma unroll
-  for (int x = 0; x < 4; ++x) w[x] = pack2(acc[2 * x] * inv, acc[2 * x + 1] * inv, T{});
-  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (cut.row0 + token) * a.os[0] +
-                            head * a.os[1] + d) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (cut.row0 + token) * a.os[0] +
+                            head * a.os[1] + d) =
+      make_uint2(pack2(acc[0] * inv, acc[1] * inv, T{}), pack2(acc[2] * inv, acc[3] * inv, T{}));
+  }
 }
 
 // ---------------------------------------------------------------- launch
@@ -1320,6 +1361,7 @@ Plan plan_chunk(const srdit_seq_attn_args& u, int sms) {
       p.ranged = last && last * tiles / sms * 5 / 4 + 7 < tiles ? 2 : 0;
     }
   }
+  if (sms > JOIN_CTAS) sms = JOIN_CTAS;
   p.ctas = static_cast<int>(p.ranged || items > sms ? sms : items);
   p.ws_floats = p.ranged ? 2ll * p.ctas * ROWS * ((u.D <= 64 ? 64 : 128) + 2) + 4 * p.ctas : 0;
   return p;
@@ -1350,7 +1392,7 @@ static int launch(const srdit_seq_attn_args& u, const Args& a, const Plan& p, cu
                packed && u.k_stride[1] == 0, packed && u.v_stride[1] == 0);
   rc = static_cast<int>(cudaGetLastError());
   if (rc || !p.ranged) return rc;
-  SRDIT_LAUNCH((join_chunk_kernel<T, DP>), dim3(p.ctas, ROWS / 32), DP / 8 * 32, 0, stream, a);
+  SRDIT_LAUNCH((join_chunk_kernel<T, DP>), 4 * p.ctas, JOIN_COLS / 4 * 32, 0, stream, a, p.ctas);
   return static_cast<int>(cudaGetLastError());
 }
 
