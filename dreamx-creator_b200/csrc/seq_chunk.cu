@@ -240,7 +240,10 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     return scale * exp2_int(-x);
   };
   if (warp < 4) {
-    if constexpr (!CODES) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if constexpr (!CODES)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    else if constexpr (!FOLD)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0) {
       // ------------------------------------------------------------ producer
       // the pages' boxes of a tile side by side: lane l has the box of keys l * box on
@@ -752,7 +755,12 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       }
     }
   } else if (warp < 12) {
-    if constexpr (!CODES) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // registers, as 128 threads' shares of what the block was launched with: 104 + 2 x 200 of 3 x
+    // 168; fp16 queries over codes 64 + 2 x 192 + 64 of 4 x 128
+    if constexpr (!CODES)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    else if constexpr (!FOLD)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ------------------------------------------------------------ softmax
     const int t = (warp - 4) >> 2;  // query tile
     const int sub = warp & 3;       // tensor-memory lane quarter
@@ -838,17 +846,26 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           const float* units =
               reinterpret_cast<const float*>(smem + C::OFF_UNITS) + tiles % C::SCALES * 8;
           // the scores of keys 64 h on, which have been asked for, as they count
+          // (fp16 queries: the scales of 64 keys or values are read while the scores are on their way)
+          auto read = [&](const float* from, float4 (&f)[16]) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) f[x] = *reinterpret_cast<const float4*>(from + 4 * x);
+          };
           auto finish = [&](int h, uint32_t (&s)[2][32]) {
-            tmem_ld_wait();
-            if constexpr (!FOLD) {
+            if constexpr (FOLD) {
+              tmem_ld_wait();
+            } else {
+              float4 k[16];
+              read(sc + h * 64, k);
+              tmem_ld_wait();
 #pragma unroll
               for (int y = 0; y < 2; ++y)
 #pragma unroll
                 for (int x = 0; x < 32; x += 4) {
-                  const float4 k = *reinterpret_cast<const float4*>(sc + h * 64 + y * 32 + x);
-                  const float2 y0 = f2_split(f2_mul(u64_of(s[y][x], s[y][x + 1]), f2_pack(k.x, k.y)));
+                  const float4 f = k[y * 8 + x / 4];
+                  const float2 y0 = f2_split(f2_mul(u64_of(s[y][x], s[y][x + 1]), f2_pack(f.x, f.y)));
                   const float2 y1 =
-                      f2_split(f2_mul(u64_of(s[y][x + 2], s[y][x + 3]), f2_pack(k.z, k.w)));
+                      f2_split(f2_mul(u64_of(s[y][x + 2], s[y][x + 3]), f2_pack(f.z, f.w)));
                   s[y][x] = __float_as_uint(y0.x);
                   s[y][x + 1] = __float_as_uint(y0.y);
                   s[y][x + 2] = __float_as_uint(y1.x);
@@ -874,6 +891,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             return FOLD ? fmaxf(c * units[w], 1.2e-38f) : c;  // (0 times -inf is NaN)
           };
           float top = neg_inf();
+          bool odd = false;  // values of the tile are not finite and hidden from some rows
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             uint32_t s[2][32];
@@ -898,13 +916,16 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u,
                       a.status, abort_flag);
             float most = 0.f;
+            bool not_all = false;  // finite
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               const float v = fabsf(sc[128 + w * 32 + lane]);
               most = fmaxf(most, v < 3e38f ? v : 0.f);
+              not_all |= !(v < 3e38f);
             }
             most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
             top += __log2f(fmaxf(most, 1e-30f));
+            odd = masked && __any_sync(0xffffffffu, not_all);
           }
           new_max(top);
           const float neg_m = m == neg_inf() ? 0.f : -m;
@@ -913,17 +934,19 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             uint32_t s[2][32];
             ask(h, s);
             if (h) publish_half();
-            if constexpr (FOLD)
+            float4 values[16];
+            if constexpr (FOLD) {
               finish(h, s);
-            else
+            } else {
+              read(sc + 128 + h * 64, values);
               tmem_ld_wait();
+            }
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               uint32_t pw[16];
               const float lv = FOLD ? units[4 + 2 * h + y] : 0.f, cw = factor(2 * h + y);
               const uint64_t c2 = f2_pack(cw, cw), neg_m2 = f2_pack(neg_m + lv, neg_m + lv);
               uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-              const uint32_t vis = !FOLD && masked ? seen(2 * h + y) : 0u;
 #pragma unroll
               for (int x = 0; x < 32; x += 2) {
                 const float2 z = f2_split(f2_fma(u64_of(s[y][x], s[y][x + 1]), c2, neg_m2));
@@ -940,19 +963,19 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                 sum[1] = f2_add(sum[1], p1);
                 float2 y0 = f2_split(p0), y1 = f2_split(p1);
                 if constexpr (!FOLD) {
-                  const float4 v =
-                      *reinterpret_cast<const float4*>(sc + 128 + h * 64 + y * 32 + x);
+                  const float4 v = values[y * 8 + x / 4];
                   y0 = f2_split(f2_mul(p0, f2_pack(v.x, v.y)));
                   y1 = f2_split(f2_mul(p1, f2_pack(v.z, v.w)));
-                  if (masked) {  // (a scale of NaN stays with the rows that see its key)
-                    if (!((vis >> x) & 1u)) y0.x = 0.f;
-                    if (!((vis >> (x + 1)) & 1u)) y0.y = 0.f;
-                    if (!((vis >> (x + 2)) & 1u)) y1.x = 0.f;
-                    if (!((vis >> (x + 3)) & 1u)) y1.y = 0.f;
-                  }
                 }
                 pw[x >> 1] = pack2(y0.x, y0.y, E{});
                 pw[(x >> 1) + 1] = pack2(y1.x, y1.y, E{});
+              }
+              if (!FOLD && odd) {  // (a scale that is not finite stays with the rows that see its key)
+                const uint32_t vis = seen(2 * h + y);
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                  pw[x] &= ((vis >> (2 * x)) & 1u ? 0xffffu : 0u) |
+                           ((vis >> (2 * x + 1)) & 1u ? 0xffff0000u : 0u);
               }
               const float2 sp = f2_split(f2_add(sum[0], sum[1]));
               l = fmaf(sp.x + sp.y, FOLD ? ex2(-lv) : 1.f, l);  // in the unit of one
@@ -1102,6 +1125,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       tc_fence_before();
     }
   } else if constexpr (CODES) {
+    if constexpr (!FOLD) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ------------------------------------------------------------ codes to fp16
     const int w = warp - 12;
     const int r8 = lane & 7, y0 = lane >> 3;  // a lane's row of 8, its pieces of 16 bytes
