@@ -233,6 +233,21 @@ def lib() -> ctypes.CDLL:
         return L
 
 
+def calls():
+    """The extension that calls some entry points with torch tensors (csrc/torch_calls.cpp), or
+    None where it is not built: the wrappers then make their checks in Python."""
+    path = LIB_PATH.parent / "_srdit_calls.so"
+    if not path.exists():
+        return None
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("_srdit_calls", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    names = ("srdit_kv_write", "srdit_kv_read", "srdit_seq_attn", "srdit_seq_attn_workspace")
+    module.init(*(ctypes.cast(getattr(lib(), n), c_vp).value for n in names))
+    return module
+
+
 def count(name: str, *args) -> int:
     """Call an entry point that returns a count (not a status)."""
     fn = _fns.get(name)

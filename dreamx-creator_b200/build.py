@@ -2,7 +2,9 @@
 
 Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` only and links them into
 ``lib/libsrdit_b200.so`` inside the package, so the built library travels with
-the source tree. ``python build.py`` or ``build()`` from Python.
+the source tree; and ``csrc/torch_calls.cpp``, the short way from torch tensors to some of
+its entry points, with g++ into ``lib/_srdit_calls.so``. ``python build.py`` or ``build()``
+from Python.
 """
 from __future__ import annotations
 
@@ -16,6 +18,7 @@ PKG = pathlib.Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
 LIB = LIBDIR / "libsrdit_b200.so"
+CALLS = LIBDIR / "_srdit_calls.so"
 INCLUDE = PKG.parent / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -36,11 +39,34 @@ def sources():
 
 
 def up_to_date() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not CALLS.exists():
         return False
-    t = LIB.stat().st_mtime
+    t = min(LIB.stat().st_mtime, CALLS.stat().st_mtime)
     deps = list(CSRC.glob("*")) + list(INCLUDE.glob("*.h"))
     return all(p.stat().st_mtime <= t for p in deps)
+
+
+def build_calls() -> str:
+    """Compile the extension of ``csrc/torch_calls.cpp`` against the installed torch; its log."""
+    import sysconfig
+
+    import torch
+
+    root = pathlib.Path(torch.__file__).parent
+    cuda = pathlib.Path(nvcc_path()).resolve().parents[1]
+    tmp = CALLS.with_suffix(".so.tmp")
+    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+                cuda / "include", sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(x for i in includes for x in ("-isystem", str(i))), str(CSRC / "torch_calls.cpp"),
+           "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-lc10", "-lc10_cuda",
+           f"-Wl,-rpath,{root / 'lib'}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for torch_calls.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, CALLS)
+    return f"$ {' '.join(cmd)}\n{r.stdout}{r.stderr}"
 
 
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
@@ -67,6 +93,7 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    logs.append(build_calls())
     os.replace(tmp, LIB)
     (LIBDIR / "build.log").write_text("\n".join(logs))
     if verbose:

@@ -380,6 +380,26 @@ def cross_attn(q, k, v, out=None, *, kv_lens=None, key_mask=None, scale=None, st
     return out
 
 
+_calls = ()   # the extension that makes a call's checks on the tensors themselves, when loaded
+
+
+def _short(name, entry, *args):
+    """A call by the extension's function ``name``; whether it was one (else the wrapper goes on
+    with its own checks). Launches that are timed one by one go the long way."""
+    global _calls
+    if _calls == ():
+        _calls = _lib.calls()
+    if _calls is None or Stats.events is not None:
+        return False
+    rc = getattr(_calls, name)(*args)
+    if rc is None:
+        return False
+    if rc:
+        _lib.check(rc, entry)
+    Stats.launches += 1
+    return True
+
+
 def _int32(t, n, what):
     if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise _lib.SrditError(f"{what} must be contiguous int32 [{n}]")
@@ -450,6 +470,9 @@ def kv_write(k, v, k_pages, v_pages, page_table, kv_lens, *, cu_q=None, k_scale=
     and v (default: T / B each); ``kv_lens`` (int32 [B]): its length with them. D a multiple of
     8 (16 for codes) up to 128, page_size 16, 32, 64 or a multiple of 128. A token whose page
     the table does not have is left out."""
+    if _short("kv_write", "srdit_kv_write", k, v, k_pages, v_pages, page_table, kv_lens, cu_q,
+              k_scale, v_scale):
+        return
     stream = _same_device(k, v, k_pages, v_pages, page_table, kv_lens, cu_q, k_scale, v_scale)
     p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
     T, st, at = _kv_rows(k, v, Hkv, D)
@@ -473,6 +496,9 @@ def kv_read(k_pages, v_pages, page_table, cu_k, k=None, v=None, *, total=None, d
     elif v is None or (dtype is not None and k.dtype != dtype) or (
             total is not None and k.shape[0] != total):
         raise _lib.SrditError("k and v do not go with total and dtype")
+    if _short("kv_read", "srdit_kv_read", k_pages, v_pages, page_table, cu_k, k, v, k_scale,
+              v_scale):
+        return k, v
     stream = _same_device(k, v, k_pages, v_pages, page_table, cu_k, k_scale, v_scale)
     p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
     T, st, at = _kv_rows(k, v, Hkv, D)
@@ -491,9 +517,7 @@ def _seq_attn(kind, q, out, Hkv, width, B, pages, k, v, Tk, kv_strides, cu_q, cu
     dt = HALF_TYPES.get(dtype)
     if dt is None:
         _code(HALF_TYPES, dtype, kind)
-    if out is None:
-        out = torch.empty(T, H, D, dtype=dtype, device=q.device)
-    elif out.shape != shape or out.dtype != dtype:
+    if out.shape != shape or out.dtype != dtype:
         raise _lib.SrditError(f"out must be {dtype} {tuple(shape)}")
     os = out.stride()
     if qs[2] != 1 or os[2] != 1:
@@ -527,6 +551,11 @@ def paged_attn(q, k_pages, v_pages, page_table, kv_lens, out=None, *, cu_q=None,
     sequence are left as they were. ``max_q``: no sequence has more new tokens (default: T / B
     without ``cu_q``, else T; steps of one token each say 1); ``max_kv``: about the longest
     sequence (default: what the table holds), by which work is split. ``scale``: D ** -0.5."""
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if _short("paged_attn", "srdit_seq_attn", q, k_pages, v_pages, page_table, kv_lens, out, cu_q,
+              max_q, max_kv, causal, k_scale, v_scale, scale, status):
+        return out
     stream = _same_device(q, k_pages, v_pages, page_table, kv_lens, out, cu_q, k_scale, v_scale,
                           status)
     p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, q.dtype)
@@ -548,6 +577,10 @@ def packed_attn(q, k, v, cu_q, out=None, *, cu_k=None, causal=True, scale=None, 
     L - n + i of its L. Views whose strides are multiples of 8 are read in place (k and v of one
     projection side by side). A query that sees no key gets zeros; rows of out behind the last
     sequence are left as they were. ``scale``: D ** -0.5."""
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if _short("packed_attn", "srdit_seq_attn", q, k, v, cu_q, out, cu_k, causal, scale, status):
+        return out
     stream = _same_device(q, k, v, cu_q, out, cu_k, status)
     shape, ks, vs = k.shape, k.stride(), v.stride()
     if (len(shape) != 3 or v.shape != shape or k.dtype != q.dtype or v.dtype != q.dtype

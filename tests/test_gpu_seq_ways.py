@@ -24,6 +24,7 @@ def way(srdit, monkeypatch):
         return real(name, *args, **kw)
 
     monkeypatch.setattr(srdit.ops, "_launch", launch)
+    monkeypatch.setattr(srdit.ops, "_calls", None)   # by way of _launch
     return lambda: seen["way"]
 
 

@@ -229,3 +229,20 @@ def test_ways_over_pages(srdit, kw, way):
     (dict(B=1, T=2304, H=24, Hkv=24, Tk=6912, causal=0), CHUNK_REST)])
 def test_ways_of_packed_rows(srdit, kw, way):
     assert _way(srdit._lib, False, **kw) == way
+
+
+def test_the_extension_leaves_what_it_does_not_know(srdit):
+    """Without CUDA tensors it takes nothing: the wrappers say what is wrong."""
+    ext = srdit._lib.calls()
+    assert ext is not None
+    x, i = torch.zeros(2, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 1, dtype=torch.int32)
+    pool = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
+    assert ext.kv_write(x, x, pool, pool, i, i[:, 0], None, None, None) is None
+    assert ext.kv_read(pool, pool, i, i[:, 0], x, x, None, None) is None
+    assert ext.paged_attn(x, pool, pool, i, i[:, 0], x, None, 1, 1, True, None, None, None,
+                          None) is None
+    assert ext.packed_attn(x, x, x, i[:, 0], x, None, True, None, None) is None
+    for f, n in ((ext.kv_write, 9), (ext.kv_read, 8), (ext.paged_attn, 14), (ext.packed_attn, 9)):
+        assert f() is None and f(*[None] * n) is None and f(*[3] * n) is None
+    with pytest.raises(TypeError):
+        ext.init(1)
