@@ -6,6 +6,8 @@ video_refiner/wan/modules/sr_dit/):
   fp8_linear.Fp8Linear / convert_linears_to_fp8
   int8_linear.Int8Linear / convert_linears_to_int8 (the same interface in 8-bit integers)
   text_block.CrossStack -- text-conditioning blocks on the integer operators
+  ops.kv_write / kv_read / paged_attn / packed_attn -- a key/value cache in pages, and attention
+      of new tokens over it and of packed prompts
   model.SRDiT  -- the 30-block streaming forward, module names as in WanModel
 
 The directory name carries a hyphen, so import it by path:
