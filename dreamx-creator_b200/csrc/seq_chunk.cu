@@ -800,7 +800,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         ++ns;
         tc_fence_after();
         // what was noted before the products that are done now
-        if (FOLD && j == 0) c = q_back[(n & 1) * 256 + t * 128 + row];
+        if (FOLD && j == 0) c = q_back[(no & 1) * 256 + t * 128 + row];
         const uint4 gap = gaps[tiles % C::GAPS];
         const bool masked = key0 + TILE - 1 > lim0 || (gap.x | gap.y | gap.z | gap.w) != 0u;
         // The maximum moves (and O is rescaled) only when a tile's is 8 above it: weights stay below
@@ -1172,7 +1172,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                 make_uint4(bf16x2_as_fp16(v[x].x, f), bf16x2_as_fp16(v[x].y, f),
                            bf16x2_as_fp16(v[x].z, f), bf16x2_as_fp16(v[x].w, f));
           }
-          if (y0 == 0) q_back[(n & 1) * 256 + t * 128 + row] = a.c * exp2_int(-k);
+          // by the uses of this query tile: that of two before has been read, as its weights were
+          // there before the last scores of the one before, which freed the queries
+          if (y0 == 0) q_back[((nq[t] - 1) & 1) * 256 + t * 128 + row] = a.c * exp2_int(-k);
         }
         fence_proxy_async_smem();
         __syncwarp();

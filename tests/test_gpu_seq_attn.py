@@ -82,6 +82,20 @@ def test_many_sequences(srdit, cuda_device, code, causal):
     _paged(srdit, g, cache, new, 8, dt, causal)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("D", (64, 128))
+def test_items_of_one_and_of_two_tiles(srdit, cuda_device, dtype, code, D):
+    """Many short sequences in turn, with the second query tile of an item in use or not, whose
+    query rows are of very different size."""
+    g, n = gen(16), 260
+    new = torch.randint(0, 2, (n,), generator=torch.Generator().manual_seed(3)).mul(160).add(40).tolist()
+    cache = Cache(g, [100 + i % 29 for i in range(n)], 4, D, 16, code or dtype, "heads").fill(g, dtype)
+    q = randn(g, sum(new), 4, D)
+    q = q * torch.exp2(torch.randint(-12, 1, (sum(new), 4, 1), generator=g, device="cuda").float())
+    _paged(srdit, g, cache, new, 4, dtype, False, q.to(dtype))
+
+
 @pytest.mark.parametrize("code", CODES)
 def test_a_chunk_of_frames(srdit, cuda_device, code):
     """Two frames of 2304 tokens over four, every token seen; pages of a frame."""
