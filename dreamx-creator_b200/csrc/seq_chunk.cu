@@ -1035,7 +1035,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           l += sp.x + sp.y;
         }
         if constexpr (!CODES || FOLD) {
-          if (a.causal && key0 + TILE - 1 > pos0) {  // values taken out, as not finite
+          // values taken out, as not finite (of 16 bits, only where a causal mask hides some)
+          if ((a.causal && key0 + TILE - 1 > pos0) || (FOLD && key0 + TILE > len)) {
             mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u,
                       a.status, abort_flag);
             uint4 off = bad[(u + 1) % STAGES];

@@ -450,3 +450,25 @@ def test_hidden_values_of_a_prompt(srdit, cuda_device, dtype, what, at):
     rest[at:, 1] = False
     assert torch.equal(got[rest], want[rest])
     assert (~got[~rest].isfinite()).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("new,lens,at", [
+    ([4, 3], [70, 35], 0), ([4, 3], [70, 35], 66), ([7, 1], [200, 9], 192), ([130, 20], [400, 90], 12),
+    ([130, 20], [400, 90], 390), ([260, 5], [300, 300], 299), ([90, 77], [128, 77], 127)])
+def test_seen_values_that_are_not_finite(srdit, cuda_device, dtype, code, causal, new, lens, at):
+    """A query that sees a value that is not finite does not get a finite answer, whatever else
+    its block of keys has: ends of sequences, whole blocks."""
+    g = gen(52)
+    cache = Cache(g, lens, 2, 64, 16, code or dtype).fill(g, dtype)
+    cu, H = offsets(new), 4
+    q = randn(g, sum(new), H, 64).to(dtype)
+    for what in (float("nan"), float("inf")):
+        _poison(g, cache, code, 0, at, what)
+        out = srdit.ops.paged_attn(q, cache.k, cache.v, cache.table, cache.lens_dev, cu_q=cu,
+                                   max_q=max(new), causal=causal, **cache.scales)
+        see = max(at - (lens[0] - new[0]), 0) if causal else 0
+        assert (~out[see:new[0], 2:].isfinite()).any(-1).all()
+        assert out[:, :2].isfinite().all() and out[new[0]:].isfinite().all()
