@@ -56,12 +56,13 @@ static int check(const srdit_seq_attn_args& a) {
   }
   if (a.B == 0 || a.T == 0 || a.H == 0) return 1;
   if (!a.q || !a.out || !(a.scale > 0.f) || a.scale > 3.4028234e38f) return SRDIT_EINVAL;
+  if (a.H > 1 && a.q_stride[1] == 0) return SRDIT_EINVAL;  // (of the inputs, key heads may be repeated)
   if (!a.cu_q && a.T % a.B) return SRDIT_EINVAL;
   if (paged ? !a.kv_lens : (a.Tk > 0 && (!a.k || !a.v)) || (!a.cu_k && !a.cu_q && a.Tk % a.B))
     return SRDIT_EINVAL;
   if (a.D <= 0 || a.D > 128 || a.D % 8) return SRDIT_EUNSUPPORTED;
   if (static_cast<long long>(a.B) * a.Hkv > 65535 ||
-      static_cast<long long>(a.T) * a.H > (1ll << 26))
+      static_cast<long long>(a.T) * a.H > (1ll << 26) || (!paged && a.Tk > 0x7fffff00))
     return SRDIT_EUNSUPPORTED;
   int rc = check_view(a.q, a.q_stride, a.T, a.H, false);
   if (!rc) rc = check_view(a.out, a.o_stride, a.T, a.H, true);

@@ -116,6 +116,7 @@ PyObject* guarded(F f) {
   try {
     return PyLong_FromLong(f());
   } catch (...) {
+    PyErr_Clear();  // (of an argument's __bool__; the wrapper meets it again)
     Py_RETURN_NONE;
   }
 }

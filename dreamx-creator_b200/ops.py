@@ -469,7 +469,7 @@ def kv_write(k, v, k_pages, v_pages, page_table, kv_lens, *, cu_q=None, k_scale=
     ``cu_q`` (int32 [B + 1]): sequence b's new tokens are the rows cu_q[b] to cu_q[b + 1] of k
     and v (default: T / B each); ``kv_lens`` (int32 [B]): its length with them. D a multiple of
     8 (16 for codes) up to 128, page_size 16, 32, 64 or a multiple of 128. A token whose page
-    the table does not have is left out."""
+    the table does not have is left out; no two tokens of a call may go to one row."""
     if _short("kv_write", "srdit_kv_write", k, v, k_pages, v_pages, page_table, kv_lens, cu_q,
               k_scale, v_scale):
         return

@@ -706,7 +706,7 @@ int srdit_kv_read(const srdit_kv_pages* pages, void* k, const long long* k_strid
  * max_kv (pages): about the longest sequence (0: what the table holds), which the work's split goes by and no result.
  * Views as in srdit_cross_attn (bases 16-byte aligned, strides multiples of 8). scale > 0.
  * workspace: where srdit_seq_attn_workspace (which reads the arguments, not the tensors) returns
- * n > 0, n KiB, 16-byte aligned. T * H at most 2^26, B * Hkv at most 65535.
+ * n > 0, n KiB, 16-byte aligned. T * H at most 2^26, B * Hkv at most 65535, Tk at most 2^31 - 256.
  * Replaces: flash_attention over packed sequences (attention.py:61-168), with a cache in pages.
  */
 typedef struct srdit_seq_attn_args {

@@ -251,6 +251,21 @@ def test_packed_keys_of_other_lengths(srdit, cuda_device, dtype, causal, nq, nk,
     assert (buf == 5).all()
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("causal", (True, False))
+def test_repeated_key_heads(srdit, cuda_device, dtype, causal):
+    """One key head for all by a stride of zero; heads of q are not read so."""
+    g = gen(22)
+    q = randn(g, 500, 6, 64).to(dtype)
+    k, v = (randn(g, 500, 1, 64).to(dtype).expand(500, 3, 64) for _ in range(2))
+    cu = offsets([200, 300])
+    out = srdit.ops.packed_attn(q, k, v.contiguous(), cu, causal=causal)
+    check_packed(q, k, v, cu, cu, out, causal, 64 ** -0.5)
+    assert torch.equal(out, srdit.ops.packed_attn(q, k, v, cu, causal=causal))
+    with pytest.raises(srdit._lib.SrditError):
+        srdit.ops.packed_attn(q[:, :1].expand(500, 6, 64), k, v, cu, causal=causal)
+
+
 @pytest.mark.parametrize("causal", (True, False))
 def test_sequences_do_not_see_each_other(srdit, cuda_device, causal):
     """NaN in one sequence's keys and values leaves its neighbours as they are."""

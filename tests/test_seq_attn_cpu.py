@@ -120,7 +120,8 @@ def _attn(lib, pages=None, workspace=False, **kw):
     (dict(scale=0.0), EINVAL), (dict(scale=float("nan")), EINVAL), (dict(scale=float("inf")), EINVAL),
     (dict(cu_q=None, T=7), EINVAL), (dict(q=(10 << 20) + 8), EALIGN), (dict(cu_q=2), EALIGN),
     (dict(q_stride=(256, 60)), EALIGN), (dict(o_stride=(256, 0)), EINVAL),
-    (dict(q_stride=(0, 64)), EINVAL), (dict(q_stride=(-256, 64)), EALIGN),
+    (dict(q_stride=(0, 64)), EINVAL), (dict(q_stride=(256, 0)), EINVAL),
+    (dict(q_stride=(-256, 64)), EALIGN),
     (dict(T=1 << 25), EUNSUPPORTED)])
 def test_attention_refusals(srdit, pages, kw, rc):
     assert _attn(srdit._lib, pages, **kw) == rc
@@ -138,7 +139,8 @@ def test_attention_page_refusals(srdit, pages, rc):
     (None, dict(k=None), EINVAL), (None, dict(v=None), EINVAL), (None, dict(Tk=-1), EINVAL),
     (None, dict(D=60), EUNSUPPORTED), (None, dict(D=136), EUNSUPPORTED),
     (None, dict(k_stride=(128, 60)), EALIGN), (None, dict(v_stride=(0, 64)), EINVAL),
-    (None, dict(cu_k=2), EALIGN), (None, dict(cu_q=None, Tk=7), EINVAL)])
+    (None, dict(cu_k=2), EALIGN), (None, dict(cu_q=None, Tk=7), EINVAL),
+    (None, dict(cu_k=16 << 20, Tk=2 ** 31 - 255), EUNSUPPORTED)])
 def test_attention_key_refusals(srdit, pages, kw, rc):
     assert _attn(srdit._lib, pages, **kw) == rc
 
