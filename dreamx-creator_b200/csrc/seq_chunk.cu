@@ -17,7 +17,9 @@
 //                  fp16 (an eighth of the answer's rounding), in units that are a power of two per 32
 //                  keys
 // Either way the running maximum is that of score + log2(unit of the values), so that the weights
-// stay at 2^8 or below, and the sum is of weights in the unit of one.
+// stay at 2^8 or below, and the sum is of weights in the unit of one. Scales of very different size,
+// those of keys that a row does not see among them, are units of their own. (Scores in base 2 are to
+// be below 2^28: beyond that the rounding of a maximum is more than an exponential takes.)
 #include <atomic>
 
 #include "seq_attn.cuh"
@@ -44,8 +46,9 @@ struct ChunkCfg {
   static constexpr int OFF_STG = OFF_KV + STAGES * BYTES;  // 32 rows x 64 bytes a warp
   static constexpr int SCALES = 4;         // tiles whose scales are kept: [2][128] each
   static constexpr int OFF_SC = OFF_STG + 8 * 2048;
-  static constexpr int OFF_UNITS = OFF_SC + (CODES ? SCALES * 1024 : 0);  // ... and units [2][4]
-  static constexpr int OFF_Q = OFF_UNITS + (CODES ? SCALES * 32 : 0);  // queries' factors [2][256]
+  static constexpr int OFF_UNITS = OFF_SC + (CODES ? SCALES * 1024 : 0);  // ... and units [3][4]
+  static constexpr int OFF_OWN = OFF_UNITS + (CODES ? SCALES * 64 : 0);  // ... or keys' own [2][128]
+  static constexpr int OFF_Q = OFF_OWN + (CODES ? SCALES * 256 : 0);  // queries' factors [2][256]
   static constexpr int OFF_REC = OFF_Q + (CODES ? 2048 : 0);
   static constexpr int OFF_PIECES = OFF_REC + RECORDS * 64;
   static constexpr int OFF_STEPS = OFF_PIECES + MAX_SLOTS * 32;  // their first key tiles, order
@@ -146,6 +149,47 @@ struct Pieces {
   }
 };
 
+// f(first key, scores) of a row's scores, 16 at a time, which may change them: short code, for what is
+// not done with every tile.
+template <bool kStore, typename F>
+SRDIT_DEV void each16(uint32_t s_tmem, F f) {
+#pragma unroll 1
+  for (int x0 = 0; x0 < TILE; x0 += 16) {
+    uint32_t s[16];
+    tmem_ld16(s_tmem + x0, s);
+    tmem_ld_wait();
+    f(x0, s);
+    if (kStore) tmem_st16(s_tmem + x0, s);
+  }
+  if (kStore) tmem_st_wait();
+}
+// A row's scores of a tile whose keys and values have units of their own (2^own), as those of weights in
+// base 2, where it sees the key (`seen`); returns the sum of the weights in the unit of one, over
+// 2^(the largest score). (Not inlined: hardly ever run, and beside the softmax it would displace code
+// that is. Only from kernels that leave the warps' registers as they are.)
+__device__ __noinline__ float take_by_key(uint32_t s_tmem, uint4 seen, const int8_t* own, float c) {
+  float top = neg_inf(), sum = 0.f;
+  each16<true>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
+    const uint32_t vis = (x0 < 32 ? seen.x : x0 < 64 ? seen.y : x0 < 96 ? seen.z : seen.w) >> (x0 & 16);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const float f = fmaxf(c * exp2_int(own[x0 + x]), 1.2e-38f);  // (0 times -inf is NaN)
+      const float y = (vis >> x) & 1u
+                          ? fmaf(__uint_as_float(s[x]), f, static_cast<float>(own[128 + x0 + x]))
+                          : neg_inf();
+      top = max2(top, y);
+      s[x] = __float_as_uint(y);
+    }
+  });
+  const float neg = top == neg_inf() ? 0.f : -top;
+  each16<false>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
+#pragma unroll
+    for (int x = 0; x < 16; ++x)
+      sum = fmaf(ex2(__uint_as_float(s[x]) + neg), exp2_int(-own[128 + x0 + x]), sum);
+  });
+  return sum;
+}
+
 template <typename T, int DP, int CODE>
 __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -228,16 +272,6 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
   // a tile that some query of the item does not see whole by place
   auto partly = [&](const Record& r, int key0) {
     return key0 + TILE > r.p.len || (a.causal && key0 + TILE - 1 > r.p.pos0);
-  };
-  // FOLD: 32 keys' scales over 2^e, in [2^6, 2^7) for the largest finite one, so that code times
-  // scale, at most 448 x 2^7, is one of fp16; and f = 2^e
-  auto in_units = [](float scale, float& f, float& e) {
-    const uint32_t top = __reduce_max_sync(
-        0xffffffffu, fabsf(scale) < 3e38f ? __float_as_uint(fabsf(scale)) : 0u);
-    const int x = max(static_cast<int>(top >> 23) - 133, -100);
-    f = exp2_int(x);
-    e = static_cast<float>(x);
-    return scale * exp2_int(-x);
   };
   if (warp < 4) {
     if constexpr (!CODES)
@@ -681,6 +715,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       // tiles ahead, scales one.
       float* scales = reinterpret_cast<float*>(smem + C::OFF_SC);
       float* units = reinterpret_cast<float*>(smem + C::OFF_UNITS);
+      int8_t* own_units = reinterpret_cast<int8_t*>(smem + C::OFF_OWN);
       int idx = 0, tiles = 0;
       bool ok = true;
       for (int n = 0; ok; ++n) {
@@ -726,21 +761,56 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           if (!ok) break;
           idx += 2;
           const int place = tiles % C::SCALES;
-          float* sc = scales + place * 256;
+          float x[8];  // 32 keys' scales, 32 values' scales
+          int e[8];
+          unsigned gap[4];
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const unsigned gap = __ballot_sync(
-                0xffffffffu, page[w] < 0 && (t0 + j) * TILE + w * 32 + lane < len);
-            if (lane == 0) reinterpret_cast<uint32_t*>(gaps + tiles % C::GAPS)[w] = gap;
-            if constexpr (FOLD) {
-              float f, e;
-              k[w] = in_units(k[w], f, e);
-              if (lane == 0) units[place * 8 + w] = f;
-              v[w] = in_units(v[w], f, e);
-              if (lane == 0) units[place * 8 + 4 + w] = e;
+            gap[w] = __ballot_sync(0xffffffffu,
+                                   page[w] < 0 && (t0 + j) * TILE + w * 32 + lane < len);
+            x[w] = k[w];
+            x[4 + w] = v[w];
+          }
+          bool wide = false;
+          if constexpr (FOLD) {
+            // 32 keys' scales over 2^e, in [2^6, 2^7) for the largest finite one, so that code times
+            // scale, at most 448 x 2^7, is one of fp16. Where one that is not 0 is less than 2^-16 of
+            // the largest and would lose bits, every key of the tile has a unit of its own.
+            uint32_t top[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const uint32_t bits = fabsf(x[y]) < 3e38f ? __float_as_uint(fabsf(x[y])) : 0u;
+              top[y] = __reduce_max_sync(0xffffffffu, bits);
+              const uint32_t least = __reduce_min_sync(0xffffffffu, bits - 1u) + 1u;
+              wide |= __uint_as_float(top[y]) > 65536.f * __uint_as_float(least);
             }
-            sc[w * 32 + lane] = k[w];
-            sc[128 + w * 32 + lane] = v[w];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const uint32_t bits = wide ? __float_as_uint(fabsf(x[y])) : top[y];
+              e[y] = max(static_cast<int>(bits >> 23) - 133, -100);
+              x[y] *= exp2_int(-e[y]);
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < 8; ++y) scales[place * 256 + y * 32 + lane] = x[y];
+          if (lane == 0) gaps[tiles % C::GAPS] = make_uint4(gap[0], gap[1], gap[2], gap[3]);
+          if constexpr (FOLD) {
+            // units: 2^e of keys; e of values; what makes a sum of weights one in the unit of one, 0
+            // where keys have their own
+            float4* un = reinterpret_cast<float4*>(units + place * 16);
+            if (lane == 0) {
+              un[0] = wide ? make_float4(1.f, 1.f, 1.f, 1.f)
+                           : make_float4(exp2_int(e[0]), exp2_int(e[1]), exp2_int(e[2]), exp2_int(e[3]));
+              un[1] = wide ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(e[4], e[5], e[6], e[7]);
+              un[2] = wide ? make_float4(0.f, 0.f, 0.f, 0.f)
+                           : make_float4(exp2_int(-e[4]), exp2_int(-e[5]), exp2_int(-e[6]),
+                                         exp2_int(-e[7]));
+            }
+            if (wide) {
+#pragma unroll
+              for (int y = 0; y < 8; ++y)
+                own_units[place * 256 + y * 32 + lane] = static_cast<int8_t>(e[y]);
+            }
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[place]);
@@ -841,10 +911,11 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           // Two passes over the scores, 64 of them at a time, so that the code is short: with all 128
           // in registers at once, as below, it does not fit the instruction caches beside that of the
           // warps that widen codes. (2 x 512 queries on 16384 e4m3 keys, 32 heads over 8 of 128: 421
-          // us so, 406 in passes of 32, 361 in passes of 64; the same keys in 16 bits 258.)
+          // us so, 406 in passes of 32, 361 in passes of 64; the same keys in 16 bits 258. Masks, which few
+          // tiles need, go over the scores once before, in a short loop: 366 -> 354.)
           const float* sc = scales + (tiles % C::SCALES) * 256;
           const float* units =
-              reinterpret_cast<const float*>(smem + C::OFF_UNITS) + tiles % C::SCALES * 8;
+              reinterpret_cast<const float*>(smem + C::OFF_UNITS) + tiles % C::SCALES * 16;
           // the scores of keys 64 h on, which have been asked for, as they count
           // (fp16 queries: the scales of 64 keys or values are read while the scores are on their way)
           auto read = [&](const float* from, float4 (&f)[16]) {
@@ -872,7 +943,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                   s[y][x + 3] = __float_as_uint(y1.y);
                 }
             }
-            if (masked) {
+            if (!FOLD && masked) {
 #pragma unroll
               for (int y = 0; y < 2; ++y) {
                 const uint32_t vis = seen(2 * h + y);
@@ -886,9 +957,24 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             tmem_ld32(s_tmem + h * 64, s[0]);
             tmem_ld32(s_tmem + h * 64 + 32, s[1]);
           };
+          const bool wide = FOLD && units[8] == 0.f;  // keys have units of their own
+          float sum_of = 0.f;
+          if (wide) {
+            sum_of = take_by_key(
+                s_tmem, make_uint4(seen(0), seen(1), seen(2), seen(3)),
+                reinterpret_cast<const int8_t*>(smem) + C::OFF_OWN + tiles % C::SCALES * 256, c);
+          } else if (FOLD && masked) {
+            each16<true>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
+              const uint32_t vis = seen(x0 >> 5) >> (x0 & 16);
+#pragma unroll
+              for (int x = 0; x < 16; ++x)
+                if (!((vis >> x) & 1u)) s[x] = __float_as_uint(neg_inf());
+            });
+          }
+          const float cj = wide ? 1.f : c;
           // per 32 keys: the scores' factor, and log2 of the unit that the values are in
           auto factor = [&](int w) {
-            return FOLD ? fmaxf(c * units[w], 1.2e-38f) : c;  // (0 times -inf is NaN)
+            return FOLD ? fmaxf(cj * units[w], 1.2e-38f) : c;  // (0 times -inf is NaN)
           };
           float top = neg_inf();
           bool odd = false;  // values of the tile are not finite and hidden from some rows
@@ -915,20 +1001,37 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           if constexpr (!FOLD) {  // the values' scales are there with the V tile
             mbar_wait(&full[(u + 1) % STAGES], static_cast<uint32_t>((u + 1) / STAGES) & 1u,
                       a.status, abort_flag);
-            float most = 0.f;
-            bool not_all = false;  // finite
+            float most = 0.f, least = 3e38f;  // of the finite ones but 0
+            bool not_all = false;             // finite
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               const float v = fabsf(sc[128 + w * 32 + lane]);
               most = fmaxf(most, v < 3e38f ? v : 0.f);
+              least = fminf(least, v > 0.f ? v : 3e38f);
               not_all |= !(v < 3e38f);
             }
             most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-            top += __log2f(fmaxf(most, 1e-30f));
+            least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
+            auto log2_of = [](float v) { return __log2f(fmaxf(v < 3e38f ? v : 0.f, 1e-30f)); };
+            if (most > 256.f * least) {
+              // Products of weights and scales are to be 2^8 at most, but not all far below it, as
+              // where the largest scale is one that the row does not see: by key.
+              top = neg_inf();
+              each16<false>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
+                const uint32_t vis = seen(x0 >> 5) >> (x0 & 16);
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                  if ((vis >> x) & 1u)
+                    top = max2(top, fmaf(__uint_as_float(s[x]), c, log2_of(fabsf(sc[128 + x0 + x]))));
+              });
+            } else {
+              top += log2_of(most);
+            }
             odd = masked && __any_sync(0xffffffffu, not_all);
           }
           new_max(top);
           const float neg_m = m == neg_inf() ? 0.f : -m;
+          if (FOLD) l = fmaf(sum_of, ex2(top + neg_m), l);
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             uint32_t s[2][32];
@@ -978,7 +1081,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                            ((vis >> (2 * x + 1)) & 1u ? 0xffff0000u : 0u);
               }
               const float2 sp = f2_split(f2_add(sum[0], sum[1]));
-              l = fmaf(sp.x + sp.y, FOLD ? ex2(-lv) : 1.f, l);  // in the unit of one
+              l = fmaf(sp.x + sp.y, FOLD ? units[8 + 2 * h + y] : 1.f, l);  // in the unit of one
               tmem_st16(s_tmem + h * 32 + y * 16, pw);
             }
           }

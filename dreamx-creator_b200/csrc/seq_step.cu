@@ -11,9 +11,9 @@
 //
 // Codes are widened to fp16 in registers, which is exact; a key's scale multiplies its scores, a
 // value's scale its weights, both in fp32, so the only rounding is the weights' to fp16. The
-// weights' running maximum is that of score + log2(largest scale of the block's values): weight
-// times scale stays at 1 or below, whatever size the scales have, and the sum l is of weights in the
-// same unit.
+// weights' running maximum is that of score + log2(scale of the value): weight times scale stays at
+// 1 or below, and some are near it, whatever size the scales have, those of keys that are hidden
+// among them; the sum l is of weights in the same unit.
 //
 // The keys are split in one of two ways. Little work: every (sequence, key head) over a cluster of
 // up to 8 CTAs, which join their parts in shared memory. Much: three CTAs on every SM take equal
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
       m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
       const int k = fp16_exponent(max(m & 0xffffu, m >> 16));
-      const float f = exp2_int(k), back = a.c * exp2_int(-k);
+      const float f = exp2_int(k), back = fmaxf(a.c * exp2_int(-k), 1.2e-38f);  // (0 times -inf is NaN)
 #pragma unroll
       for (int x = 0; x < NC; ++x)
         qf[n][x] = make_uint4(bf16x2_as_fp16(qf[n][x].x, f), bf16x2_as_fp16(qf[n][x].y, f),
@@ -403,16 +403,19 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
           bad[y][h] = ((g & 1) ? all[2 * h + 1] : all[2 * h]) & (0x11111111u << (g >> 1));
       }
     }
-    float lv = 0.f;
-    if constexpr (CODES) {  // log2 of the block's largest scale of a value
-      float top = 0.f;
+    // log2 of a value's scale; what a weight in its unit is in the unit of one; the rest of the scale
+    // (1, or what its sign, 0, NaN or infinity is)
+    float lv[NB][2], one[NB][2];
+    if constexpr (CODES) {
 #pragma unroll
       for (int y = 0; y < NB; ++y)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          top = fmaxf(top, fabsf(vs[y][h]) < 3e38f ? fabsf(vs[y][h]) : 0.f);
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-      lv = __log2f(fmaxf(top, 1e-30f));
+        for (int h = 0; h < 2; ++h) {
+          const float v = fabsf(vs[y][h]);
+          lv[y][h] = __log2f(fmaxf(v < 3e38f ? v : 0.f, 1e-30f));
+          one[y][h] = ex2(-lv[y][h]);
+          vs[y][h] *= one[y][h];
+        }
     }
     float p[NT][NB][4];
 #pragma unroll
@@ -462,11 +465,20 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        // (rounded before the maximum is taken from them: however large they are, that of the
+        // largest is 0)
+#pragma unroll
+        for (int y = 0; y < NB; ++y)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& x = p[n][y][2 * h + e];
+            x = CODES ? __fmaf_rn(x, cq[n][e], lv[y][h]) : __fmul_rn(x, cq[n][e]);
+          }
         float top = max2(p[n][0][e], p[n][0][2 + e]);
         if constexpr (NB == 2) top = max2(top, max2(p[n][1][e], p[n][1][2 + e]));
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) top = max2(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float mn = max2(m[n][e], fmaf(top, cq[n][e], lv));
+        const float mn = max2(m[n][e], top);
         const float neg = mn == neg_inf() ? 0.f : -mn;
         alpha[n][e] = ex2(m[n][e] + neg);
         moved |= mn != m[n][e];
@@ -478,8 +490,8 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
           for (int h = 0; h < 2; ++h) {
             float& x = p[n][y][2 * h + e];
             const bool seen = x != neg_inf();
-            x = ex2(fmaf(x, cq[n][e], neg));
-            sum += x;
+            x = ex2(__fadd_rn(x, neg));
+            sum = CODES ? fmaf(x, one[y][h], sum) : sum + x;
             if constexpr (CODES) x = seen ? x * vs[y][h] : 0.f;
             if (bad[y][h] && seen) sum = __int_as_float(0x7fc00000);
           }

@@ -3,7 +3,7 @@ bits (tests/seq_cases.py has it, with the tolerances)."""
 import pytest
 import torch
 
-from tests.seq_cases import Cache, check_packed, check_paged, gen, offsets, randn
+from tests.seq_cases import U, Cache, attention, check_packed, check_paged, gen, offsets, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -449,6 +449,54 @@ def test_hidden_values_may_be_anything(srdit, cuda_device, code, what, new, lens
     rest[max(see, 0):new[0], 2:] = False
     assert torch.equal(got[rest], want[rest])
     assert (~got[~rest].isfinite()).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("new,lens,at", [
+    ([4, 3], [70, 35], 68), ([7, 1], [23, 9], 17), ([130, 20], [400, 90], 300),
+    ([260, 5], [260, 300], 129), ([200, 77], [1000, 77], 999)])
+@pytest.mark.parametrize("size", (20, 96))
+@pytest.mark.parametrize("D", (64, 128))
+def test_a_token_of_another_size(srdit, cuda_device, dtype, code, new, lens, at, size, D):
+    """A token with values of 2^96 and keys of 2^20 or 2^96 (fp16: 2^14) times the others' size, which
+    a causal mask hides from some queries: those get what they would without it. The others' score
+    of it is beyond all others: it is all of their answer, or none (many rows over keys in 16 bits:
+    where scores are below 2^28)."""
+    g, big = gen(53), 96 if dtype == torch.bfloat16 else 14
+    cache = Cache(g, lens, 2, D, 16, code or dtype).fill(g, dtype)
+    k, v = randn(g, 2, 1, 2, D).clamp(-3, 3)
+    cache.put(0, at, (k * 2.0 ** min(size, big)).to(dtype), (v * 2.0 ** big).to(dtype))
+    cu, H, n, scale = offsets(new), 4, new[0], D ** -0.5
+    q = randn(g, sum(new), H, D).to(dtype)
+    out = srdit.ops.paged_attn(q, cache.k, cache.v, cache.table, cache.lens_dev, cu_q=cu,
+                               max_q=max(new), **cache.scales)
+    K, _, _ = cache.rows(0, "k")
+    V, codes, vs = cache.rows(0, "v")
+    s = torch.stack([q[:n, h].double() @ K[at, h // 2] for h in range(H)], 1) * scale
+    see = torch.arange(n, device="cuda")[:, None] >= at - (lens[0] - n)
+    none, all_ = ~see | (s < -300), see & (s > 300)
+    if code is None and max(new) > 8 and s.abs().max() > 2.0 ** 28:
+        none, all_ = (~see).expand(n, H), torch.zeros_like(all_)
+    else:
+        assert (none | all_).sum() > 0.7 * n * H and (all_.any() or see.sum() < 8)
+    # without the token: the formula, and no term of its size in the tolerance
+    gone = torch.zeros(lens[0], dtype=torch.bool, device="cuda")
+    gone[at] = True
+    K0, V0 = (x.masked_fill(gone[:, None, None], 0) for x in (K, V))
+    if vs is not None:
+        vs = vs.masked_fill(gone[:, None], 0)
+    u_p = U[dtype if code is None else torch.float16]
+    ref, tol = attention(q[:n], K0, V0, scale, True, u_p, dtype, codes, vs, gone)
+    err = (out[:n].double() - ref).abs()
+    assert (err <= tol)[none].all(), float((err / tol)[none].max())
+    # with it alone: its values, a weight of 1 rounded, the output rounded
+    ref = V[at].repeat_interleave(2, 0).expand(n, H, D)
+    tol = (u_p + 2.0 ** -11 + U[dtype] * (1 + 2.0 ** -6)) * ref.abs() + 2.0 ** -24
+    if code is not None:
+        tol = tol + 2.0 ** -11 * ref.abs() + 2.0 ** -24 * cache.rows(0, "v")[2][at].max()
+    err = (out[:n].double() - ref).abs()
+    assert (err <= tol)[all_].all(), float((err / tol)[all_].max())
 
 
 @pytest.mark.parametrize("dtype", HALF)
