@@ -415,14 +415,15 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         struct Now {
           int t0, e[2], end;
         };
-        // the next item with key tiles, or false
-        auto next = [&](Now& r) {
-          while (true) {
+        // The next item with key tiles, of the next `most` records: 1, or 0 if there is none at all, or
+        // -1 if it is not among them.
+        auto next = [&](Now& r, int most) {
+          for (; most > 0; --most) {
             const int at = nrec % RECORDS;
             if (!mbar_wait(&rec_full[at], static_cast<uint32_t>(nrec / RECORDS) & 1u, a.status,
                            abort_flag)) {
               ok = false;
-              return false;
+              return 0;
             }
             const int tokens = records[at].p.tokens;
             r.t0 = records[at].t0;
@@ -431,33 +432,42 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             r.end = max(r.e[0], r.e[1]);
             mbar_arrive(&rec_empty[at]);
             ++nrec;
-            if (tokens == 0) return false;
-            if (r.end > r.t0) return true;
+            if (tokens == 0) return 0;
+            if (r.end > r.t0) return 1;
           }
+          return -1;
         };
         Now it = {};
-        bool on = next(it);
-        int j = it.t0;
-        if (on) {
-          ok = kv_wait(0, false);
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (it.e[t] <= it.t0) continue;
-            ok = q_wait(t);
+        bool begun = false;  // an item's first scores are on their way
+        int j = 0;
+        while (ok) {
+          if (!begun) {
+            if (next(it, 0x7fffffff) != 1) break;
+            j = it.t0;
+            ok = kv_wait(idx, false);
+            for (int t = 0; t < 2 && ok; ++t) {
+              if (it.e[t] <= it.t0) continue;
+              ok = q_wait(t);
+              if (!ok) break;
+              tc_fence_after();
+              scores(t, idx);
+              if (it.e[t] - it.t0 == 1) tc_commit(&q_empty[t]);
+            }
             if (!ok) break;
-            tc_fence_after();
-            scores(t, 0);
-            if (it.e[t] - it.t0 == 1) tc_commit(&q_empty[t]);
+            tc_commit(&empty[idx % STAGES]);
+            begun = true;
           }
-          if (ok) tc_commit(&empty[0]);
-        }
-        while (ok && on) {
-          // the step after (it, j): the item's next key tile, or another item's first
+          // The step after (it, j): the item's next key tile, or another item's first. Records come no
+          // further than the softmax lets them, which needs this item's products: behind many items
+          // without keys the next one is looked for when these are on their way.
           Now nx = it;
           int nj = j + 1;
           const bool last = nj == it.end;
           bool more = true;
           if (last) {
-            more = next(nx);
+            const int found = next(nx, RECORDS - 1);
+            more = found == 1;
+            begun = found >= 0;
             nj = nx.t0;
             if (!ok) break;
           }
@@ -491,8 +501,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           tc_commit(&empty[uv % STAGES]);
           if (more) tc_commit(&empty[uk % STAGES]);
           idx += 2;
+          if (!begun) continue;
+          if (!more) break;
           it = nx;
-          on = more;
           j = nj;
         }
       }

@@ -96,6 +96,26 @@ def test_items_of_one_and_of_two_tiles(srdit, cuda_device, dtype, code, D):
     _paged(srdit, g, cache, new, 4, dtype, False, q.to(dtype))
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("new,lens,H,Hkv", [
+    ([40, 900, 30], [60, 0, 200], 16, 2), ([300, 1400, 200, 1000, 50], [900, 0, 300, 0, 70], 8, 8),
+    ([132, 9, 25, 391, 850], [3, 18, 277, 151, 2000], 16, 2), ([12000, 100, 9000], [0, 500, 10], 8, 1)])
+def test_many_queries_without_keys(srdit, cuda_device, dtype, code, causal, new, lens, H, Hkv):
+    """Long runs of queries that see no key, before, between and behind others that do."""
+    g = gen(17)
+    cache = Cache(g, lens, Hkv, 64, 32, code or dtype).fill(g, dtype)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q, cu, out = _paged(srdit, g, cache, new, H, dtype, causal, status=status)
+    assert status.item() == 0
+    if code is None:
+        kv = [torch.cat([cache.rows(b, w)[0] for b in range(len(lens))]).to(dtype) for w in "kv"]
+        got = srdit.ops.packed_attn(q, *kv, cu, cu_k=offsets(lens), causal=causal, status=status)
+        check_packed(q, *kv, cu, offsets(lens), got, causal, 64 ** -0.5)
+        assert status.item() == 0
+
+
 @pytest.mark.parametrize("code", CODES)
 def test_a_chunk_of_frames(srdit, cuda_device, code):
     """Two frames of 2304 tokens over four, every token seen; pages of a frame."""
