@@ -18,7 +18,8 @@ struct Offsets {
 
 // The sequence among B that packed row t belongs to, by one warp (B: behind the last one).
 // Rows before the first offset are no sequence's either. With `lens`, len is its entry of it, and
-// begin and end are the sequence's rows: all of them come with one trip to memory.
+// begin and end are the sequence's rows: all of them come with one trip to memory, of up to 32
+// sequences, and another for each 32 times as many.
 SRDIT_DEV int find_sequence(const Offsets& o, int B, int t, Divisor by_each, const int32_t* lens,
                             int& len, int& begin, int& end) {
   if (!o.at) {
@@ -29,21 +30,23 @@ SRDIT_DEV int find_sequence(const Offsets& o, int B, int t, Divisor by_each, con
     return b;
   }
   const int lane = threadIdx.x & 31;
-  for (int base = 0; base < B; base += 32) {  // offsets that are not above t
-    const int n = base + lane;
-    const bool on = n < B;
-    const int to = on ? __ldg(o.at + n + 1) : 0x7fffffff, from = on ? __ldg(o.at + n) : 0;
-    const int l = on && lens ? __ldg(lens + n) : 0;
-    const unsigned below = __ballot_sync(0xffffffffu, to <= t);
-    if (below == 0xffffffffu) continue;
-    const int x = __popc(below);  // (of ascending offsets)
-    const int b = base + x;
-    begin = max(__shfl_sync(0xffffffffu, from, x), 0);
-    end = min(__shfl_sync(0xffffffffu, to, x), o.rows);
-    len = __shfl_sync(0xffffffffu, l, x);
-    return b < B && t >= begin ? b : B;
+  int base = 0, count = B;  // it is among these, or none
+  while (count > 32) {      // offsets that are not above t, one of each 32nd of them
+    const int each = (count + 31) >> 5, n = (lane + 1) * each;
+    const int k = __popc(__ballot_sync(0xffffffffu, n < count && __ldg(o.at + base + n) <= t));
+    base += k * each;
+    count = min(each, count - k * each);
   }
-  return B;
+  const int n = base + lane;
+  const bool on = lane < count;
+  const int to = on ? __ldg(o.at + n + 1) : 0x7fffffff, from = on ? __ldg(o.at + n) : 0;
+  const int l = on && lens ? __ldg(lens + n) : 0;
+  const int x = __popc(__ballot_sync(0xffffffffu, to <= t));  // (of ascending offsets)
+  if (x >= count) return B;
+  begin = max(__shfl_sync(0xffffffffu, from, x), 0);
+  end = min(__shfl_sync(0xffffffffu, to, x), o.rows);
+  len = __shfl_sync(0xffffffffu, l, x);
+  return t >= begin ? base + x : B;
 }
 SRDIT_DEV int find_sequence(const Offsets& o, int B, int t, Divisor by_each) {
   int len, begin, end;

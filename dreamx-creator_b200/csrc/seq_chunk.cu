@@ -1422,49 +1422,49 @@ __global__ void __launch_bounds__(JOIN_COLS / 4 * 32)
   __syncthreads();
   const int cols = (a.D + JOIN_COLS - 1) / JOIN_COLS, tasks = count * (ROWS / 32) * cols;
   for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-  const int which = task / ((ROWS / 32) * cols), rest = task - which * ((ROWS / 32) * cols);
-  const int first = cuts_of[which];  // the CTA that begins the item
-  const Cut cut = all_cuts[first];
-  const int row = rest / cols * 32 + lane;
-  const int d = rest % cols * JOIN_COLS + warp * 4;
-  const int token = row >> a.pack_log, head = cut.h0 + (row & (a.pack - 1));
-  if (token >= cut.tokens || d >= a.D) continue;
-  float m = neg_inf(), l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int p0 = 0; p0 < cut.parts; p0 += 4) {
-    float2 q[4];
-    float v[4][4];
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int p = p0 + y, part = 2 * (first + p) + (p == 0);
-      const bool on = p < cut.parts;
-      const float* ws = a.ws + (static_cast<long long>(part) * DP + d) * ROWS + row;
-      q[y] = on ? __ldg(reinterpret_cast<const float2*>(a.ml) + part * ROWS + row)
-                : make_float2(neg_inf(), 0.f);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) v[y][x] = on ? __ldg(ws + x * ROWS) : 0.f;
+    const int which = task / ((ROWS / 32) * cols), rest = task - which * ((ROWS / 32) * cols);
+    const int first = cuts_of[which];  // the CTA that begins the item
+    const Cut cut = all_cuts[first];
+    const int row = rest / cols * 32 + lane;
+    const int d = rest % cols * JOIN_COLS + warp * 4;
+    const int token = row >> a.pack_log, head = cut.h0 + (row & (a.pack - 1));
+    if (token >= cut.tokens || d >= a.D) continue;
+    float m = neg_inf(), l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < cut.parts; p0 += 4) {
+      float2 q[4];
+      float v[4][4];
+  #pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int p = p0 + y, part = 2 * (first + p) + (p == 0);
+        const bool on = p < cut.parts;
+        const float* ws = a.ws + (static_cast<long long>(part) * DP + d) * ROWS + row;
+        q[y] = on ? __ldg(reinterpret_cast<const float2*>(a.ml) + part * ROWS + row)
+                  : make_float2(neg_inf(), 0.f);
+  #pragma unroll
+        for (int x = 0; x < 4; ++x) v[y][x] = on ? __ldg(ws + x * ROWS) : 0.f;
+      }
+      float mn = m;
+  #pragma unroll
+      for (int y = 0; y < 4; ++y) mn = max2(mn, q[y].x);
+      if (mn == neg_inf()) continue;  // no key seen yet
+      const float f = ex2(m - mn);
+      m = mn;
+      l *= f;
+  #pragma unroll
+      for (int x = 0; x < 4; ++x) acc[x] *= f;
+  #pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        if (q[y].x == neg_inf()) continue;  // it saw no key
+        const float g = ex2(q[y].x - m);
+        l = fmaf(q[y].y, g, l);
+  #pragma unroll
+        for (int x = 0; x < 4; ++x) acc[x] = fmaf(v[y][x], g, acc[x]);
+      }
     }
-    float mn = m;
-#pragma unroll
-    for (int y = 0; y < 4; ++y) mn = max2(mn, q[y].x);
-    if (mn == neg_inf()) continue;  // no key seen yet
-    const float f = ex2(m - mn);
-    m = mn;
-    l *= f;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) acc[x] *= f;
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      if (q[y].x == neg_inf()) continue;  // it saw no key
-      const float g = ex2(q[y].x - m);
-      l = fmaf(q[y].y, g, l);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) acc[x] = fmaf(v[y][x], g, acc[x]);
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (cut.row0 + token) * a.os[0] +
-                            head * a.os[1] + d) =
-      make_uint2(pack2(acc[0] * inv, acc[1] * inv, T{}), pack2(acc[2] * inv, acc[3] * inv, T{}));
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (cut.row0 + token) * a.os[0] +
+                              head * a.os[1] + d) =
+        make_uint2(pack2(acc[0] * inv, acc[1] * inv, T{}), pack2(acc[2] * inv, acc[3] * inv, T{}));
   }
 }
 

@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
     b = blockIdx.y % a.B;
     kvh = blockIdx.y / a.B;
   }
+  // (The body of this loop, to the end of the kernel but for its last lines, is not indented.)
 #pragma unroll 1
   while (s < s1) {
   int blk0, blk1, part = 0, slot_of_part = -1;

@@ -175,3 +175,40 @@ def test_in_a_graph_and_on_another_stream(srdit, cuda_device):
     q, s = quantise(k, torch.float8_e4m3fn)
     want = (q.float() * s[..., None]).to(dt)
     assert torch.equal(ko[16], want[0]) and torch.equal(ko[81], want[1])
+
+
+@pytest.mark.parametrize("code", (torch.int8, None))
+@pytest.mark.parametrize("B", (32, 33, 1050))
+def test_more_sequences_than_lanes(srdit, cuda_device, code, B):
+    """Where a token's sequence is found in steps; many are empty."""
+    g, dt = gen(70 + B), torch.bfloat16
+    new = [(i * 7) % 3 for i in range(B)]
+    lens = [n + i % 2 for i, n in enumerate(new)]
+    cache = Cache(g, lens, 1, 16, 16, code or dt)
+    T, cu = sum(new), offsets(new, 2)
+    kv = randn(g, T + 5, 2, 1, 16).to(dt)
+    for b in range(B):
+        rows = kv[int(cu[b]):int(cu[b + 1])]
+        cache.put(b, lens[b] - new[b], rows[:, 0], rows[:, 1])
+    want = _clone(cache)
+    for x in (cache.k, cache.v):
+        x.view(torch.uint8).zero_()
+    srdit.ops.kv_write(kv[:, 0], kv[:, 1], cache.k, cache.v, cache.table, cache.lens_dev, cu_q=cu,
+                       **cache.scales)
+    got = _clone(cache)
+    at = [cache.places(b, lens[b] - n, lens[b]) for b, n in enumerate(new) if n]
+    pages, rows = (torch.cat(x) for x in zip(*at))
+    for x, y in zip(got, want):
+        if x is not None:
+            assert torch.equal(x[pages, rows], y[pages, rows])
+    cu_k = offsets(new, 1)
+    k, v = (torch.full((T + 4, 1, 16), 5.0, dtype=dt, device="cuda") for _ in range(2))
+    cache.put(0, 0, kv[:lens[0], 0], kv[:lens[0], 1])
+    lo = [lens[b] - n for b, n in enumerate(new)]
+    srdit.ops.kv_read(cache.k, cache.v, cache.table, cu_k, k, v, **cache.scales)
+    for b, n in enumerate(new):
+        if lo[b] == 0 and n:   # the first tokens, that were written
+            first = int(cu_k[b])
+            c = cache.rows(b, "k")[0][:n]
+            assert torch.equal(k[first:first + n].double(), c.to(dt).double())
+    assert (k[:1] == 5).all() and (k[1 + T:] == 5).all() and (v[1 + T:] == 5).all()
