@@ -20,8 +20,8 @@
 //                  keys
 // Either way the running maximum is that of score + log2(unit of the values), so that the weights
 // stay at 2^8 or below, and the sum is of weights in the unit of one. Scales of very different size,
-// those of keys that a row does not see among them, are units of their own. (Scores in base 2 are to
-// be below 2^28: beyond that the rounding of a maximum is more than an exponential takes.)
+// those of keys that a row does not see among them, are units of their own. (Scores in base 2 over
+// codes are to be below 2^26: beyond that the rounding of a maximum is more than an exponential takes.)
 #include <atomic>
 
 #include "seq_attn.cuh"
@@ -35,6 +35,12 @@ constexpr int MIN_SHARE = 4;      // key tiles that a ranged CTA takes at least
 constexpr int RECORDS = 4;
 constexpr int MAX_SEQS = 64;      // sequences that are kept in shared memory
 constexpr int MAX_SORTED = 64;    // pieces that are taken by length
+// A weight is 2^(score c - m), its product not rounded and m the rounded one of the largest score:
+// from |m| = 2^24 on the two are more than one apart, and that score's weight is any number. So
+// where a maximum is FAR or more, products are rounded before m is taken from them. (That branch, not
+// taken, costs 1.5% of a long prompt's time, written so; around the exponentials, or with the scores
+// taken from tensor memory again, 4% to 7%.)
+constexpr float FAR = 4194304.f;
 
 template <int DP, int CODE>
 struct ChunkCfg {
@@ -874,6 +880,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       if (tokens == 0) break;
       const int n_tiles = e - t0;
       float m = neg_inf(), l = 0.f, c = a.c;
+      bool far = false;  // a row's maximum is FAR or more
       // the last key that this row sees, and the least of its warp's
       const int lim = a.causal ? min(len - 1, pos0 + my_token) : len - 1;
       const int lim0 = a.causal ? min(len - 1, pos0 + warp_token) : len - 1;
@@ -886,16 +893,20 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if (FOLD && j == 0) c = q_back[(no & 1) * 256 + t * 128 + row];
         const uint4 gap = gaps[tiles % C::GAPS];
         const bool masked = key0 + TILE - 1 > lim0 || (gap.x | gap.y | gap.z | gap.w) != 0u;
-        // The maximum moves (and O is rescaled) only when a tile's is 8 above it: weights stay below
+        // The maximum moves, whose negative this returns (and O is rescaled) only when a tile's is 8 above it: weights stay below
         // 2^8 and the quotient is the same. (Written so that a NaN raises it too, and stays in l
-        // and O.) Scores of this tile are ready, so the product before it is done.
+        // and O; by the difference, as the sum of a large m and 8 may be m, or far above it.) Scores
+        // of this tile are ready, so the product before it is done.
         auto new_max = [&](float top) {
-          const bool raise = !(top <= m + 8.f) && top != neg_inf();
+          const bool raise = !(top - m <= 8.f) && top != neg_inf();
           const float m_new = raise ? top : m;
           const float alpha = raise ? ex2(m - m_new) : 1.f;
           m = m_new;
           l *= alpha;
-          if (j > 0 && __any_sync(0xffffffffu, raise)) {
+          const float neg_m = m == neg_inf() ? 0.f : -m;
+          if (__any_sync(0xffffffffu, raise)) {
+            if (!CODES) far = __any_sync(0xffffffffu, fabsf(neg_m) >= FAR);
+            if (j > 0) {
 #pragma unroll 1
             for (int w = 0; w < DP / 16; ++w) {
               uint32_t o[16];
@@ -905,7 +916,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
               tmem_st16(o_tmem + w * 16, o);
             }
+            }
           }
+          return neg_m;
         };
         // the first 64 keys' weights, stored by now: their product can begin
         auto publish_half = [&] {
@@ -1042,8 +1055,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             }
             odd = masked && __any_sync(0xffffffffu, not_all);
           }
-          new_max(top);
-          const float neg_m = m == neg_inf() ? 0.f : -m;
+          const float neg_m = new_max(top);
           if (FOLD) l = fmaf(sum_of, ex2(top + neg_m), l);
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
@@ -1121,8 +1133,17 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               mx[w] = max3(mx[w], __uint_as_float(s[w][x]), __uint_as_float(s[w][x + 1]));
             mx[w] = max2(mx[w], __uint_as_float(s[w][31]));
           }
-          new_max(max2(max3(mx[0], mx[1], mx[2]), mx[3]) * c);
-          const float neg_m = m == neg_inf() ? 0.f : -m;
+          float neg_m = new_max(max2(max3(mx[0], mx[1], mx[2]), mx[3]) * c);
+          if (far) {  // scores that times c are what is to be the exponent
+            const float inv = 1.f / c;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                s[w][x] = __float_as_uint(
+                    __fadd_rn(__fmul_rn(__uint_as_float(s[w][x]), c), neg_m) * inv);
+            neg_m = 0.f;
+          }
           const uint64_t c2 = f2_pack(c, c), neg_m2 = f2_pack(neg_m, neg_m);
 #pragma unroll
           for (int w = 0; w < 4; ++w)

@@ -701,7 +701,7 @@ int srdit_kv_read(const srdit_kv_pages* pages, void* k, const long long* k_strid
  * query that sees no key gets 0; rows behind the last sequence are left as they were. What lies
  * behind a sequence's length or is hidden from a query by the causal mask does not matter to it,
  * NaN included. A NaN or an infinity in a value that it does see makes that column of its answer
- * not finite, or all of them NaN. Many rows per key head: |scale q.k| is to stay below 2^27, beyond
+ * not finite, or all of them NaN. Many rows per key head over codes: |scale q.k| is to stay below 2^26, beyond
  * which an answer may be NaN or 0.
  * max_q: no sequence has more queries (0: T; a sequence's further rows may be left as they were);
  * max_kv (pages): about the longest sequence (0: what the table holds), which the work's split goes by and no result.
