@@ -11,9 +11,13 @@
 //
 // Codes are widened to fp16 in registers, which is exact; a key's scale multiplies its scores, a
 // value's scale its weights, both in fp32, so the only rounding is the weights' to fp16. The
-// weights' running maximum is that of score + log2(scale of the value): weight times scale stays at
-// 1 or below, and some are near it, whatever size the scales have, those of keys that are hidden
-// among them; the sum l is of weights in the same unit.
+// weights' running maximum m is that of score + e, where e is the exponent of the value's scale:
+// weight times scale stays below 2, and some are near 1, whatever size the scales have, those of keys
+// that are hidden among them. The sum l is of 2^(score - m + 24): with e from -80 (and scales below it
+// lose digits) to 125 it is in range, and a weight is lost from it when it is 2^-25 of the largest, of
+// scales up to kv_write's 2^121 2^-29. (From weights times 2^-e it would be lost where another's
+// scale is 2^126 times its own.) What takes l from one maximum to the next, 2^(m - m'), may be out of
+// range, and is taken in two halves.
 //
 // The keys are split in one of two ways. Little work: every (sequence, key head) over a cluster of
 // up to 8 CTAs, which join their parts in shared memory. Much: two CTAs on every SM (three over
@@ -32,6 +36,20 @@ constexpr int WARPS = 4;
 constexpr int MAX_SHARED = 1024;  // sequences of a launch by shares
 constexpr int MIN_BLOCKS = 8;     // blocks of a share, at least
 constexpr int SHARE_BLOCKS = 64;  // ... of a CTA, from which shares are taken
+constexpr int LEAST = -80, MOST = 125;  // exponents of values' scales
+constexpr int L_UNIT = 24;        // codes: sums of weights are in the unit of 2^-24
+
+// What takes O and l from one maximum to another that is x larger (x <= 0).
+template <bool CODES>
+struct Fall {
+  float f, half;
+  SRDIT_DEV explicit Fall(float x) : f(0.f), half(ex2(CODES ? x * 0.5f : x)) {
+    f = CODES ? half * half : half;
+  }
+  SRDIT_DEV float add(float l, float sum) const {  // sum + 2^x l
+    return CODES ? fmaf(l * half, half, sum) : fmaf(l, f, sum);
+  }
+};
 
 template <int DP, int NT, int CODE>
 struct StepCfg {
@@ -406,18 +424,16 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
           bad[y][h] = ((g & 1) ? all[2 * h + 1] : all[2 * h]) & (0x11111111u << (g >> 1));
       }
     }
-    // log2 of a value's scale; what a weight in its unit is in the unit of one; the rest of the scale
-    // (1, or what its sign, 0, NaN or infinity is)
-    float lv[NB][2], one[NB][2];
+    // the exponent of a value's scale, less 24, and the scale over it (0, an infinity and a NaN stay)
+    float lv[NB][2];
     if constexpr (CODES) {
 #pragma unroll
       for (int y = 0; y < NB; ++y)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float v = fabsf(vs[y][h]);
-          lv[y][h] = __log2f(fmaxf(v < 3e38f ? v : 0.f, 1e-30f));
-          one[y][h] = ex2(-lv[y][h]);
-          vs[y][h] *= one[y][h];
+          const int e = min(max(static_cast<int>(__float_as_uint(vs[y][h]) >> 23 & 255u), 127 + LEAST), 127 + MOST);
+          vs[y][h] *= exp2_int(127 - e);
+          lv[y][h] = __int_as_float(0x4b000000 | e) - (8388608.f + 127.f + L_UNIT);
         }
     }
     float p[NT][NB][4];
@@ -475,7 +491,7 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float& x = p[n][y][2 * h + e];
-            x = CODES ? __fmaf_rn(x, cq[n][e], lv[y][h]) : __fmul_rn(x, cq[n][e]);
+            x = CODES ? __fmaf_rn(x, cq[n][e], lv[y][h]) : __fmul_rn(x, cq[n][e]);  // (both 24 less)
           }
         float top = max2(p[n][0][e], p[n][0][2 + e]);
         if constexpr (NB == 2) top = max2(top, max2(p[n][1][e], p[n][1][2 + e]));
@@ -483,7 +499,8 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
         for (int x = 4; x < 32; x <<= 1) top = max2(top, __shfl_xor_sync(0xffffffffu, top, x));
         const float mn = max2(m[n][e], top);
         const float neg = mn == neg_inf() ? 0.f : -mn;
-        alpha[n][e] = ex2(m[n][e] + neg);
+        const Fall<CODES> fall(m[n][e] + neg);
+        alpha[n][e] = fall.f;
         moved |= mn != m[n][e];
         m[n][e] = mn;
         float sum = 0.f;
@@ -493,12 +510,17 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
           for (int h = 0; h < 2; ++h) {
             float& x = p[n][y][2 * h + e];
             const bool seen = x != neg_inf();
-            x = ex2(__fadd_rn(x, neg));
-            sum = CODES ? fmaf(x, one[y][h], sum) : sum + x;
-            if constexpr (CODES) x = seen ? x * vs[y][h] : 0.f;
+            const float z = __fadd_rn(x, neg);
+            x = ex2(z);
+            if constexpr (CODES) {
+              sum += ex2(z - lv[y][h]);
+              x = seen ? x * vs[y][h] : 0.f;
+            } else {
+              sum += x;
+            }
             if (bad[y][h] && seen) sum = __int_as_float(0x7fc00000);
           }
-        l[n][e] = fmaf(l[n][e], alpha[n][e], sum);
+        l[n][e] = fall.add(l[n][e], sum);
       }
 #pragma unroll
       for (int y = 0; y < NB; ++y) {
@@ -592,13 +614,14 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         const float2 ml = sml[w][row];
-        const float f = ex2(ml.x - top);
+        const Fall<CODES> fall(ml.x - top);
+        const float f = fall.f;
         const float4 v = *reinterpret_cast<const float4*>(&so[w][row][d]);
         acc.x = fmaf(v.x, f, acc.x);
         acc.y = fmaf(v.y, f, acc.y);
         acc.z = fmaf(v.z, f, acc.z);
         acc.w = fmaf(v.w, f, acc.w);
-        sum = fmaf(ml.y, f, sum);
+        sum = fall.add(ml.y, sum);
       }
     }
     *reinterpret_cast<float4*>(&co[row][d]) = acc;
@@ -644,12 +667,13 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
       if (top != neg_inf()) {
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-          const float f = ex2(pm[y] - top);
+          const Fall<CODES> fall(pm[y] - top);
+          const float f = fall.f;
           acc.x = fmaf(po[y].x, f, acc.x);
           acc.y = fmaf(po[y].y, f, acc.y);
           acc.z = fmaf(po[y].z, f, acc.z);
           acc.w = fmaf(po[y].w, f, acc.w);
-          sum = fmaf(pl[y], f, sum);
+          sum = fall.add(pl[y], sum);
         }
       }
     } else {
@@ -668,7 +692,7 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
     const long long tok = row0 + i;
     const int head = kvh * a.group + row - i * a.group;
     if (wparts == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float inv = sum == 0.f ? 0.f : (CODES ? exp2_int(L_UNIT) : 1.f) / sum;
       *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + tok * a.os[0] + head * a.os[1] + d) =
           make_uint2(pack2(acc.x * inv, acc.y * inv, T{}), pack2(acc.z * inv, acc.w * inv, T{}));
     } else {
@@ -693,7 +717,7 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
 // are in its second slot and the first slots of the CTAs that go on with the same key head. A
 // thread takes four columns of a row and every fourth part, four parts' loads in flight: bounded
 // by their latency.
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool CODES>
 __global__ void __launch_bounds__(512) join_share_kernel(const __grid_constant__ Args a) {
   pdl_begin();
   constexpr int R = 8 * NT;
@@ -712,9 +736,10 @@ __global__ void __launch_bounds__(512) join_share_kernel(const __grid_constant__
     auto add = [&](float2 q, float4 v) {
       if (q.x == neg_inf()) return;  // it saw no key
       const float mn = max2(m, q.x);
-      const float f0 = ex2(m - mn), f1 = ex2(q.x - mn);
+      const Fall<CODES> fall0(m - mn), fall1(q.x - mn);
+      const float f0 = fall0.f, f1 = fall1.f;
       m = mn;
-      l = l * f0 + q.y * f1;
+      l = fall1.add(q.y, fall0.add(l, 0.f));
       acc.x = acc.x * f0 + v.x * f1;
       acc.y = acc.y * f0 + v.y * f1;
       acc.z = acc.z * f0 + v.z * f1;
@@ -744,7 +769,7 @@ __global__ void __launch_bounds__(512) join_share_kernel(const __grid_constant__
     __syncthreads();
     if (way == 0) {
       for (int w = 1; w < min(4, cut.parts); ++w) add(ml_of[w][task], acc_of[w][task]);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : (CODES ? exp2_int(L_UNIT) : 1.f) / l;
       const int i = a.by_group.div(row);
       if (x0 + task < rows * dq)
         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) +
@@ -758,7 +783,7 @@ __global__ void __launch_bounds__(512) join_share_kernel(const __grid_constant__
 
 // One warp per (token, head): joins the parts that went through the workspace, four parts'
 // loads in flight.
-template <typename T>
+template <typename T, bool CODES>
 __global__ void __launch_bounds__(128) join_step_kernel(const __grid_constant__ Args a, int parts) {
   pdl_begin();
   const long long rows = static_cast<long long>(a.T) * a.H;
@@ -789,23 +814,24 @@ __global__ void __launch_bounds__(128) join_step_kernel(const __grid_constant__ 
 #pragma unroll
     for (int x = 0; x < 4; ++x) mn = max2(mn, pm[x].x);
     if (mn == neg_inf()) continue;  // no key seen yet
-    const float f = ex2(m - mn);
+    const Fall<CODES> fall(m - mn);
     m = mn;
-    l *= f;
+    l = fall.add(l, 0.f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= f;
+    for (int e = 0; e < 4; ++e) acc[e] *= fall.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if (pm[x].x == neg_inf()) continue;  // a part that saw no key
-      const float k = ex2(pm[x].x - m);
-      l = fmaf(pm[x].y, k, l);
+      const Fall<CODES> of_part(pm[x].x - m);
+      const float k = of_part.f;
+      l = of_part.add(pm[x].y, l);
       acc[0] = fmaf(v[x].x, k, acc[0]);
       acc[1] = fmaf(v[x].y, k, acc[1]);
       acc[2] = fmaf(v[x].z, k, acc[2]);
       acc[3] = fmaf(v[x].w, k, acc[3]);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : (CODES ? exp2_int(L_UNIT) : 1.f) / l;
   if (on)
     *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + t * a.os[0] + h * a.os[1] + lane * 4) =
         make_uint2(pack2(acc[0] * inv, acc[1] * inv, T{}), pack2(acc[2] * inv, acc[3] * inv, T{}));
@@ -853,12 +879,6 @@ Plan plan_step(const srdit_seq_attn_args& u, int sms) {
   return p;
 }
 
-template <typename T, int DP, int NT>
-static int join_shares(const Args& a, const Plan& p, cudaStream_t stream) {
-  SRDIT_LAUNCH((join_share_kernel<T, DP, NT>), p.ctas, 512, 0, stream, a);
-  return static_cast<int>(cudaGetLastError());
-}
-
 template <typename T, int DP, int NT, int CODE>
 static int launch(const srdit_seq_attn_args& u, const Args& a, const Plan& p, cudaStream_t stream) {
   using C = StepCfg<DP, NT, CODE>;
@@ -876,7 +896,9 @@ static int launch(const srdit_seq_attn_args& u, const Args& a, const Plan& p, cu
                                     static_cast<unsigned>(a.B * a.Hkv));
   rc = launch_clusters(p.cluster, step_kernel<T, DP, NT, CODE>, grid, WARPS * 32, C::SMEM, stream, tk,
                        tv, a, p.cluster);
-  return rc || !p.shared ? rc : join_shares<T, DP, NT>(a, p, stream);
+  if (rc || !p.shared) return rc;
+  SRDIT_LAUNCH((join_share_kernel<T, DP, NT, C::CODES>), p.ctas, 512, 0, stream, a);
+  return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T, int CODE>
@@ -899,8 +921,11 @@ static int run_typed(const srdit_seq_attn_args& u, const Args& a, const Plan& p,
   }
   if (rc || p.parts == 1) return rc;
   const long long rows = static_cast<long long>(u.T) * u.H;
-  SRDIT_LAUNCH((join_step_kernel<T>), static_cast<unsigned>((rows + 3) / 4), 128, 0, stream, a,
-               p.parts);
+  const unsigned blocks = static_cast<unsigned>((rows + 3) / 4);
+  if (u.pages->code == SRDIT_KV_PLAIN)
+    SRDIT_LAUNCH((join_step_kernel<T, false>), blocks, 128, 0, stream, a, p.parts);
+  else
+    SRDIT_LAUNCH((join_step_kernel<T, true>), blocks, 128, 0, stream, a, p.parts);
   return static_cast<int>(cudaGetLastError());
 }
 

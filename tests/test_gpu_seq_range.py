@@ -1,5 +1,5 @@
-"""Attention over pages and of packed prompts where scores are large, against the formula in 64
-bits.
+"""Attention over pages and of packed prompts where numbers are large or far apart: scores of any
+size, and values' scales from 2^-40 to 2^100 side by side, against the formula in 64 bits.
 
 Nothing is added for scores: q and k are such that q.k is exact in 32 bits, and the factor
 c = scale * log2(e) either is a power of two (a scale of ln(2) in fp32, whose product with log2(e)
@@ -25,6 +25,7 @@ from tests.seq_cases import U, Cache, gen, offsets, randn
 pytestmark = pytest.mark.gpu
 
 HALF = (torch.bfloat16, torch.float16)
+CODES = (torch.int8, torch.float8_e4m3fn)
 LN2 = 0.6931471824645996   # ln(2) in fp32
 
 
@@ -122,6 +123,7 @@ def test_large_scores_of_prompts(srdit, cuda_device, dtype, size, sign, causal, 
 WAYS = [([1, 3], [37, 400], 4, 2, 64), ([1], [20000], 2, 1, 128), ([40, 30], [90, 300], 4, 2, 128),
         ([300], [700], 4, 4, 64), ([70], [20000], 8, 2, 128)]
 STEP_SHARES = ([1, 0, 1, 2, 1, 0, 1, 1], [9001, 0, 7, 30000, 12345, 100, 16, 8000], 16, 8, 128)
+FEW = WAYS[:2] + [STEP_SHARES]   # rows per key head
 
 
 @pytest.mark.parametrize("dtype,size", SIZES)
@@ -154,3 +156,80 @@ def test_scores_a_step_apart(srdit, cuda_device, dtype, size, D):
     out = srdit.ops.packed_attn(q, k, v, offsets([n]), causal=False, scale=LN2)
     ref, tol = _answer(q, k.double(), v.double(), 1.0, False)
     _check(out, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("size", (20, 27, 29, 40, 100))
+@pytest.mark.parametrize("sign", (1, -1))
+@pytest.mark.parametrize("new,lens,H,Hkv,D", FEW)
+def test_large_scores_over_codes(srdit, cuda_device, dtype, code, size, sign, new, lens, H, Hkv, D):
+    """Keys of equal scores. Their values' scales are 1 to 2 times a power of two: its exponent and
+    the score are rounded together, so that scores this large with other exponents need not stay
+    equal."""
+    g = gen(83 + size)
+    cache = Cache(g, lens, Hkv, D, 16, code, "heads").fill(g, dtype)
+    cache.vs.copy_(2.0 ** -7 * (1 + torch.rand(cache.vs.shape, generator=g, device="cuda")))
+    q = torch.zeros(sum(new), H, D, dtype=dtype, device="cuda")
+    q[..., 0] = sign * 2.0 ** 12
+    q[..., 17] = 1.0
+    for b, n in enumerate(lens):
+        at = cache.places(b, 0, n)
+        low = torch.rand(n, Hkv, generator=g, device="cuda") < 0.875
+        codes = torch.zeros(n, Hkv, D, device="cuda")
+        codes[..., 0] = torch.where(low, 56.0, 64.0)
+        cache.k.view(torch.uint8)[at] = codes.to(code).view(torch.uint8)
+        cache.ks[at] = 2.0 ** (size - 18)
+    _paged(srdit, cache, q, new, 1.1, True)
+
+
+# ------------------------------------------------------------------ scales far apart
+def _scales(g, cache, lo, hi, zeros=0.1):
+    """Every value's scale 2^lo to 2^hi, evenly over the exponents; a tenth as of rows of zeros."""
+    for b, n in enumerate(cache.lens):
+        at = cache.places(b, 0, n)
+        s = torch.exp2(lo + (hi - lo) * torch.rand(n, cache.Hkv, generator=g, device="cuda"))
+        none = torch.rand(n, cache.Hkv, generator=g, device="cuda") < zeros
+        cache.vs[at] = torch.where(none, 1e-12, s)
+        codes = cache.v.view(torch.uint8)[at]
+        cache.v.view(torch.uint8)[at] = codes.masked_fill(none[..., None], 0)
+
+
+@pytest.mark.parametrize("dtype,lo,hi", [
+    (torch.bfloat16, -40, 100), (torch.bfloat16, 60, 110), (torch.bfloat16, -40, 40),
+    (torch.bfloat16, -80, -40), (torch.float16, -40, 8)])
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("size", (0.0, 0.5, 6.0))
+@pytest.mark.parametrize("new,lens,H,Hkv,D", FEW)
+def test_scales_far_apart(srdit, cuda_device, dtype, lo, hi, code, size, new, lens, H, Hkv, D):
+    """Equal scores, scores of the usual size, and some in which a few keys have all of the weight."""
+    g = gen(84)
+    cache = Cache(g, lens, Hkv, D, 16, code, "heads").fill(g, dtype)
+    _scales(g, cache, lo, hi)
+    q = torch.zeros(sum(new), H, D, dtype=dtype, device="cuda")
+    q[..., 1] = size * torch.randint(-4, 5, (sum(new), H), generator=g, device="cuda").to(dtype)
+    for b, n in enumerate(lens):   # (scores are multiples of 1/8: exact)
+        at = cache.places(b, 0, n)
+        codes = torch.zeros(n, Hkv, D, device="cuda")
+        codes[..., 1] = torch.randint(-8, 9, (n, Hkv), generator=g, device="cuda").float()
+        cache.k.view(torch.uint8)[at] = codes.to(code).view(torch.uint8)
+        cache.ks[at] = 0.25
+    _paged(srdit, cache, q, new, 1.0, True)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("rows", (1, 4))
+@pytest.mark.parametrize("order", (0, 1))
+def test_a_row_of_zeros_beside_one_of_huge_values(srdit, cuda_device, code, rows, order):
+    """Two tokens of equal scores as kv_write leaves them: the answer is half of the huge one."""
+    g, dt, D = gen(85), torch.bfloat16, 64
+    cache = Cache(g, [rows + 1], 1, D, 16, code)
+    k = torch.zeros(rows + 1, 1, D, dtype=dt, device="cuda")
+    v = k.clone()
+    v[order] = (randn(g, 1, D) * 2.0 ** 100).to(dt)
+    cu = torch.tensor([0, rows + 1], dtype=torch.int32, device="cuda")
+    srdit.ops.kv_write(k, v, cache.k, cache.v, cache.table, cache.lens_dev, cu_q=cu, **cache.scales)
+    q = randn(g, rows, 2, D).to(dt)
+    out = _paged(srdit, cache, q, [rows], 1.0, True)
+    want = cache.rows(0, "v")[0][order, 0] / torch.arange(2, rows + 2, device="cuda")[:, None]
+    assert ((out.double() - want[:, None]).abs() <= 2.0 ** -7 * want[:, None].abs() + 2.0 ** 80).all()
