@@ -879,6 +879,12 @@ Plan plan_step(const srdit_seq_attn_args& u, int sms) {
   return p;
 }
 
+template <typename T, int DP, int NT, bool CODES>
+static int join_shares(const Args& a, const Plan& p, cudaStream_t stream) {
+  SRDIT_LAUNCH((join_share_kernel<T, DP, NT, CODES>), p.ctas, 512, 0, stream, a);
+  return static_cast<int>(cudaGetLastError());
+}
+
 template <typename T, int DP, int NT, int CODE>
 static int launch(const srdit_seq_attn_args& u, const Args& a, const Plan& p, cudaStream_t stream) {
   using C = StepCfg<DP, NT, CODE>;
@@ -896,9 +902,7 @@ static int launch(const srdit_seq_attn_args& u, const Args& a, const Plan& p, cu
                                     static_cast<unsigned>(a.B * a.Hkv));
   rc = launch_clusters(p.cluster, step_kernel<T, DP, NT, CODE>, grid, WARPS * 32, C::SMEM, stream, tk,
                        tv, a, p.cluster);
-  if (rc || !p.shared) return rc;
-  SRDIT_LAUNCH((join_share_kernel<T, DP, NT, C::CODES>), p.ctas, 512, 0, stream, a);
-  return static_cast<int>(cudaGetLastError());
+  return rc || !p.shared ? rc : join_shares<T, DP, NT, C::CODES>(a, p, stream);
 }
 
 template <typename T, int CODE>
