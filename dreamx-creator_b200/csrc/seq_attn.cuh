@@ -67,6 +67,22 @@ struct Compute<T, SRDIT_KV_PLAIN> {
   using type = T;
 };
 
+// Over codes parts of rows have sums of weights l in the unit of 2^(m - 24), where m is the maximum of
+// score + exponent of the value's scale: with exponents from -80 to 125 they are in range.
+constexpr int L_UNIT = 24;
+// What takes O and l from one maximum to another that is x larger (x <= 0): a factor for O; l, in which
+// a much smaller factor may count, by two halves of it.
+template <bool CODES>
+struct Fall {
+  float f, half;
+  SRDIT_DEV explicit Fall(float x) : f(0.f), half(ex2(CODES ? x * 0.5f : x)) {
+    f = CODES ? half * half : half;
+  }
+  SRDIT_DEV float add(float l, float sum) const {  // sum + 2^x l
+    return CODES ? fmaf(l * half, half, sum) : fmaf(l, f, sum);
+  }
+};
+
 // 4 codes as fp16 values, exactly: the first two in x, the others in y
 template <int CODE>
 SRDIT_DEV void widen4(uint32_t u, uint32_t& x, uint32_t& y) {

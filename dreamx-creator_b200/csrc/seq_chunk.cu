@@ -18,10 +18,12 @@
 //   bf16 queries   become fp16 times a power of two per row; code times scale is rounded once to
 //                  fp16 (an eighth of the answer's rounding), in units that are a power of two per 32
 //                  keys
-// Either way the running maximum is that of score + log2(unit of the values), so that the weights
-// stay at 2^8 or below, and the sum is of weights in the unit of one. Scales of very different size,
-// those of keys that a row does not see among them, are units of their own. (Scores in base 2 over
-// codes are to be below 2^26: beyond that the rounding of a maximum is more than an exponential takes.)
+// Either way the running maximum is that of score + exponent of the values' unit, so that the weights
+// stay at 2^9 or below, and the sum is of weights in the unit of one. Scales of very different size,
+// those of keys that a row does not see among them, are units of their own; where a sum made from
+// weights and units would lose a weight beside another's large unit, it is kept with a maximum of its
+// own (take_by_key). Scores so large that the rounding of a maximum is more than an exponential takes
+// are rounded, with the unit's exponent, before the maximum is taken from them.
 #include <atomic>
 
 #include "seq_attn.cuh"
@@ -38,9 +40,14 @@ constexpr int MAX_SORTED = 64;    // pieces that are taken by length
 // A weight is 2^(score c - m), its product not rounded and m the rounded one of the largest score:
 // from |m| = 2^24 on the two are more than one apart, and that score's weight is any number. So
 // where a maximum is FAR or more, products are rounded before m is taken from them. (That branch, not
-// taken, costs 1.5% of a long prompt's time, written so; around the exponentials, or with the scores
-// taken from tensor memory again, 4% to 7%.)
+// taken, costs 1.5% of a long prompt's time over keys in 16 bits, written so; around the exponentials, or
+// with the scores taken from tensor memory again, 4% to 7%. Over codes a bound on the scores, or a vote
+// on the largest, sends such tiles to code that units of their own need anyway.)
 constexpr float FAR = 4194304.f;
+// bf16 queries over codes: values' scales that leave every weight that counts in its sum when it is made
+// from products of weight and unit: one is lost that is 2^-62 of the largest. With others the sum of
+// weights has a maximum of its own.
+constexpr float LEAST = 0x1p-44f, MOST = 0x1p20f;
 
 template <int DP, int CODE>
 struct ChunkCfg {
@@ -56,7 +63,9 @@ struct ChunkCfg {
   static constexpr int OFF_SC = OFF_STG + 8 * 2048;
   static constexpr int OFF_UNITS = OFF_SC + (CODES ? SCALES * 1024 : 0);  // ... and units [3][4]
   static constexpr int OFF_OWN = OFF_UNITS + (CODES ? SCALES * 64 : 0);  // ... or keys' own [2][128]
-  static constexpr int OFF_Q = OFF_OWN + (CODES ? SCALES * 256 : 0);  // queries' factors [2][256]
+  static constexpr int OFF_ONE = OFF_OWN + (CODES ? SCALES * 256 : 0);  // units of one: 1, 0, 0
+  static constexpr int OFF_MOST = OFF_ONE + (CODES ? 64 : 0);  // queries' largest factors [2][8 warps]
+  static constexpr int OFF_Q = OFF_MOST + (CODES ? 64 : 0);    // queries' factors [2][256]
   static constexpr int OFF_REC = OFF_Q + (CODES ? 2048 : 0);
   static constexpr int OFF_PIECES = OFF_REC + RECORDS * 64;
   static constexpr int OFF_STEPS = OFF_PIECES + MAX_SLOTS * 32;  // their first key tiles, order
@@ -171,31 +180,62 @@ SRDIT_DEV void each16(uint32_t s_tmem, F f) {
   }
   if (kStore) tmem_st_wait();
 }
-// A row's scores of a tile whose keys and values have units of their own (2^own), as those of weights in
-// base 2, where it sees the key (`seen`); returns the sum of the weights in the unit of one, over
-// 2^(the largest score). (Not inlined: hardly ever run, and beside the softmax it would displace code
-// that is. Only from kernels that leave the warps' registers as they are.)
-__device__ __noinline__ float take_by_key(uint32_t s_tmem, uint4 seen, const int8_t* own, float c) {
+// A row's sum of weights apart from O: it is l 2^(base + over) where O's unit is 2^m.
+struct Sum {
+  float base, over, l;
+};
+// A row's scores of a tile whose keys and values have units of their own (2^own; or null: the tile's, by
+// 32 keys) as those of weights in base 2, rounded, where it sees the key (`seen`); returns the sum of
+// the weights in the unit of one, over 2^(the largest score), or adds it to `to`. (Not inlined: hardly
+// ever run, and beside the softmax it would displace code that is. Only from kernels that leave the
+// warps' registers as they are.)
+__device__ __noinline__ float take_by_key(uint32_t s_tmem, uint4 seen, const int8_t* own,
+                                          const float* units, float c, Sum* to) {
+  auto unit = [&](int x) { return own ? static_cast<float>(own[128 + x]) : units[4 + (x >> 5)]; };
   float top = neg_inf(), sum = 0.f;
   each16<true>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
     const uint32_t vis = (x0 < 32 ? seen.x : x0 < 64 ? seen.y : x0 < 96 ? seen.z : seen.w) >> (x0 & 16);
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      const float f = fmaxf(c * exp2_int(own[x0 + x]), 1.2e-38f);  // (0 times -inf is NaN)
-      const float y = (vis >> x) & 1u
-                          ? fmaf(__uint_as_float(s[x]), f, static_cast<float>(own[128 + x0 + x]))
-                          : neg_inf();
+      const float f = fmaxf(c * (own ? exp2_int(own[x0 + x]) : units[x0 >> 5]), 1.2e-38f);  // (not 0)
+      const float y =
+          (vis >> x) & 1u ? __fmaf_rn(__uint_as_float(s[x]), f, unit(x0 + x)) : neg_inf();
       top = max2(top, y);
       s[x] = __float_as_uint(y);
     }
   });
   const float neg = top == neg_inf() ? 0.f : -top;
+  if (!to) {
+    each16<false>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        sum = fmaf(ex2(__uint_as_float(s[x]) + neg), ex2(-unit(x0 + x)), sum);
+    });
+    return sum;
+  }
+  // Scores in two terms, top and the rest, so that large ones keep the units. (The loops are the whole
+  // warp's: rows that see no key go through them.)
+  float most = neg_inf();
   each16<false>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
 #pragma unroll
     for (int x = 0; x < 16; ++x)
-      sum = fmaf(ex2(__uint_as_float(s[x]) + neg), exp2_int(-own[128 + x0 + x]), sum);
+      most = max2(most, __uint_as_float(s[x]) + neg - unit(x0 + x));
   });
-  return sum;
+  if (most == neg_inf()) most = 0.f;
+  each16<false>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
+#pragma unroll
+    for (int x = 0; x < 16; ++x)
+      sum += ex2(__uint_as_float(s[x]) + neg - unit(x0 + x) - most);
+  });
+  if (top != neg_inf()) {
+    const float fall = to->base == neg_inf() ? neg_inf() : to->base - top + (to->over - most);
+    const bool up = fall <= 0.f;  // (a NaN stays: neither)
+    to->l = up ? fmaf(to->l, ex2(fall), sum) : fmaf(sum, ex2(-fall), to->l);
+    to->base = up ? top : to->base;
+    to->over = up ? most : to->over;
+  }
+  __syncwarp();
+  return 0.f;
 }
 
 template <typename T, int DP, int CODE>
@@ -270,6 +310,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if (FOLD && threadIdx.x < 12)
+    reinterpret_cast<float*>(smem + C::OFF_ONE)[threadIdx.x] = threadIdx.x < 4 ? 1.f : 0.f;
   if (warp >= 4 && static_cast<int>(threadIdx.x) - 128 < min(a.B, MAX_SEQS))
     seqs[threadIdx.x - 128] = Pieces::sequence(a, threadIdx.x - 128);
   tc_fence_before();
@@ -755,6 +797,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         };
         int page[4], page1[4];
         float k[4], v[4];
+        bool apart = false;  // values' scales of the item so far: some beyond LEAST or MOST
         auto fetch = [&](int j) {  // page[]: tile j's
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -794,7 +837,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           if constexpr (FOLD) {
             // 32 keys' scales over 2^e, in [2^6, 2^7) for the largest finite one, so that code times
             // scale, at most 448 x 2^7, is one of fp16. Where one that is not 0 is less than 2^-16 of
-            // the largest and would lose bits, every key of the tile has a unit of its own.
+            // the largest and would lose bits, every key of the tile has a unit of its own, and from
+            // the first value's scale beyond [LEAST, MOST] on every key of the item.
             uint32_t top[8];
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
@@ -802,11 +846,14 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
               top[y] = __reduce_max_sync(0xffffffffu, bits);
               const uint32_t least = __reduce_min_sync(0xffffffffu, bits - 1u) + 1u;
               wide |= __uint_as_float(top[y]) > 65536.f * __uint_as_float(least);
+              apart |= y >= 4 && (__uint_as_float(top[y]) > MOST ||
+                                  (least != 0u && __uint_as_float(least) < LEAST));
             }
+            wide |= apart;
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
               const uint32_t bits = wide ? __float_as_uint(fabsf(x[y])) : top[y];
-              e[y] = max(static_cast<int>(bits >> 23) - 133, -100);
+              e[y] = max(static_cast<int>(bits >> 23) - 133, y < 4 || apart ? -100 : -50);
               x[y] *= exp2_int(-e[y]);
             }
           }
@@ -814,16 +861,16 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           for (int y = 0; y < 8; ++y) scales[place * 256 + y * 32 + lane] = x[y];
           if (lane == 0) gaps[tiles % C::GAPS] = make_uint4(gap[0], gap[1], gap[2], gap[3]);
           if constexpr (FOLD) {
-            // units: 2^e of keys; e of values; what makes a sum of weights one in the unit of one, 0
-            // where keys have their own
+            // units: 2^e of keys; e of values; what makes a sum of weights one in the unit of one; the
+            // largest of the first, infinity where keys have their own; whether sums of weights are
+            // taken apart from O
             float4* un = reinterpret_cast<float4*>(units + place * 16);
             if (lane == 0) {
-              un[0] = wide ? make_float4(1.f, 1.f, 1.f, 1.f)
-                           : make_float4(exp2_int(e[0]), exp2_int(e[1]), exp2_int(e[2]), exp2_int(e[3]));
-              un[1] = wide ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(e[4], e[5], e[6], e[7]);
-              un[2] = wide ? make_float4(0.f, 0.f, 0.f, 0.f)
-                           : make_float4(exp2_int(-e[4]), exp2_int(-e[5]), exp2_int(-e[6]),
-                                         exp2_int(-e[7]));
+              un[0] = make_float4(exp2_int(e[0]), exp2_int(e[1]), exp2_int(e[2]), exp2_int(e[3]));
+              un[1] = make_float4(e[4], e[5], e[6], e[7]);
+              un[2] = make_float4(exp2_int(-e[4]), exp2_int(-e[5]), exp2_int(-e[6]), exp2_int(-e[7]));
+              un[3] = make_float4(wide ? -neg_inf() : exp2_int(max(max(e[0], e[1]), max(e[2], e[3]))),
+                                  apart ? 1.f : 0.f, 0.f, 0.f);
             }
             if (wide) {
 #pragma unroll
@@ -858,8 +905,10 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     const uint32_t s_tmem = tmem_base + t_lane + t * 128u;
     const uint32_t o_tmem = tmem_base + t_lane + 256u + t * 128u;
     uint8_t* stg = smem + C::OFF_STG + (warp - 4) * 2048;
+    Sum* own_sum = reinterpret_cast<Sum*>(stg) + lane;  // (until the item's end)
     const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SC);
     const float* q_back = reinterpret_cast<const float*>(smem + C::OFF_Q);
+    const float* q_most = reinterpret_cast<const float*>(smem + C::OFF_MOST) + warp - 4;
     const int my_token = t * a.rt + (row >> a.pack_log);
     const int warp_token = t * a.rt + (sub * 32 >> a.pack_log);
     int ns = 0, no = 0, idx = 0, tiles = 0;
@@ -880,7 +929,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       if (tokens == 0) break;
       const int n_tiles = e - t0;
       float m = neg_inf(), l = 0.f, c = a.c;
-      bool far = false;  // a row's maximum is FAR or more
+      bool far = false;    // a row's maximum is FAR or more
+      bool apart = false;  // sums of weights are not in l but in own_sum
       // the last key that this row sees, and the least of its warp's
       const int lim = a.causal ? min(len - 1, pos0 + my_token) : len - 1;
       const int lim0 = a.causal ? min(len - 1, pos0 + warp_token) : len - 1;
@@ -893,10 +943,10 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if (FOLD && j == 0) c = q_back[(no & 1) * 256 + t * 128 + row];
         const uint4 gap = gaps[tiles % C::GAPS];
         const bool masked = key0 + TILE - 1 > lim0 || (gap.x | gap.y | gap.z | gap.w) != 0u;
-        // The maximum moves, whose negative this returns (and O is rescaled) only when a tile's is 8 above it: weights stay below
+        // The maximum moves (and O is rescaled) only when a tile's is 8 above it: weights stay below
         // 2^8 and the quotient is the same. (Written so that a NaN raises it too, and stays in l
         // and O; by the difference, as the sum of a large m and 8 may be m, or far above it.) Scores
-        // of this tile are ready, so the product before it is done.
+        // of this tile are ready, so the product before it is done. Returns the maximum's negative.
         auto new_max = [&](float top) {
           const bool raise = !(top - m <= 8.f) && top != neg_inf();
           const float m_new = raise ? top : m;
@@ -942,6 +992,9 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           const float* sc = scales + (tiles % C::SCALES) * 256;
           const float* units =
               reinterpret_cast<const float*>(smem + C::OFF_UNITS) + tiles % C::SCALES * 16;
+          // keys have units of their own, or a score may be 2^25 and more, so that its product with the
+          // factor is to be rounded first: one of fp16 queries and codes times scales is below 2^38
+          const bool by_key = FOLD && !(units[12] * q_most[(no & 1) * 8] < 0x1p-13f);
           // the scores of keys 64 h on, which have been asked for, as they count
           // (fp16 queries: the scales of 64 keys or values are read while the scores are on their way)
           auto read = [&](const float* from, float4 (&f)[16]) {
@@ -983,12 +1036,18 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             tmem_ld32(s_tmem + h * 64, s[0]);
             tmem_ld32(s_tmem + h * 64 + 32, s[1]);
           };
-          const bool wide = FOLD && units[8] == 0.f;  // keys have units of their own
           float sum_of = 0.f;
-          if (wide) {
-            sum_of = take_by_key(
-                s_tmem, make_uint4(seen(0), seen(1), seen(2), seen(3)),
-                reinterpret_cast<const int8_t*>(smem) + C::OFF_OWN + tiles % C::SCALES * 256, c);
+          if (FOLD && by_key) {
+            if (!apart && units[13] != 0.f) {
+              apart = true;
+              *own_sum = {m, 0.f, l};
+              l = 0.f;
+            }
+            const int8_t* own =
+                reinterpret_cast<const int8_t*>(smem) + C::OFF_OWN + tiles % C::SCALES * 256;
+            sum_of = take_by_key(s_tmem, make_uint4(seen(0), seen(1), seen(2), seen(3)),
+                                 units[12] > 3e38f ? own : nullptr, units, c, apart ? own_sum : nullptr);
+            units = reinterpret_cast<const float*>(smem + C::OFF_ONE);
           } else if (FOLD && masked) {
             each16<true>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
               const uint32_t vis = seen(x0 >> 5) >> (x0 & 16);
@@ -997,13 +1056,20 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
                 if (!((vis >> x) & 1u)) s[x] = __float_as_uint(neg_inf());
             });
           }
-          const float cj = wide ? 1.f : c;
+          float cj = FOLD && by_key ? 1.f : c;
           // per 32 keys: the scores' factor, and log2 of the unit that the values are in
           auto factor = [&](int w) {
-            return FOLD ? fmaxf(cj * units[w], 1.2e-38f) : c;  // (0 times -inf is NaN)
+            return FOLD ? fmaxf(cj * units[w], 1.2e-38f) : cj;  // (0 times -inf is NaN)
           };
           float top = neg_inf();
           bool odd = false;  // values of the tile are not finite and hidden from some rows
+          // fp16 queries: the exponent of the unit that weights are in, by keys or of all: that of a
+          // value's scale (of 2^-100 to 2^100)
+          auto exponent = [](float v) {
+            v = fminf(fmaxf(v < 3e38f ? v : 0.f, 1e-30f), 1e30f);
+            return static_cast<float>(static_cast<int>(__float_as_uint(v) >> 23) - 127);
+          };
+          bool taken = false;  // m, from scores
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             uint32_t s[2][32];
@@ -1038,24 +1104,39 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
             }
             most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
             least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
-            auto log2_of = [](float v) { return __log2f(fmaxf(v < 3e38f ? v : 0.f, 1e-30f)); };
-            if (most > 256.f * least) {
-              // Products of weights and scales are to be 2^8 at most, but not all far below it, as
-              // where the largest scale is one that the row does not see: by key.
+            const bool large = fabsf(top) >= FAR && fabsf(top) < -neg_inf();
+            taken = most > 256.f * least || __any_sync(0xffffffffu, large);
+            if (taken) {
+              // Products of weights and scales are to be 2^9 at most, but not all far below it, as
+              // where the largest scale is one that the row does not see: by key. Scores become
+              // exponents, the large ones' products with c rounded before m is taken from them. (Column
+              // by column: the shortest code.)
               top = neg_inf();
-              each16<false>(s_tmem, [&](int x0, uint32_t (&s)[16]) {
-                const uint32_t vis = seen(x0 >> 5) >> (x0 & 16);
-#pragma unroll
-                for (int x = 0; x < 16; ++x)
-                  if ((vis >> x) & 1u)
-                    top = max2(top, fmaf(__uint_as_float(s[x]), c, log2_of(fabsf(sc[128 + x0 + x]))));
+              auto each = [&](bool store, auto f) {
+#pragma unroll 1
+                for (int x = 0; x < TILE; ++x) {
+                  const float s = __uint_as_float(tmem_ld1(s_tmem + x));
+                  tmem_ld_wait();
+                  const float in = exponent(fabsf(sc[128 + x])), y = f(__fmaf_rn(s, c, in), in);
+                  if (store) tmem_st1(s_tmem + x, __float_as_uint(y));
+                }
+              };
+              each(false, [&](float y, float) {
+                top = max2(top, y);
+                return y;
               });
+              const float m_new = !(top - m <= 8.f) && top != neg_inf() ? top : m;
+              const float neg = m_new == neg_inf() ? 0.f : -m_new;
+              each(true, [&](float y, float in) { return __fadd_rn(y, neg) - in; });
+              tmem_st_wait();
+              cj = 1.f;
             } else {
-              top += log2_of(most);
+              top += exponent(most);
             }
             odd = masked && __any_sync(0xffffffffu, not_all);
           }
-          const float neg_m = new_max(top);
+          float neg_m = new_max(top);
+          if (taken) neg_m = 0.f;
           if (FOLD) l = fmaf(sum_of, ex2(top + neg_m), l);
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
@@ -1196,7 +1277,13 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
       if (__any_sync(0xffffffffu, *abort_flag != 0u)) break;
       tc_fence_after();
       idx += 2 * max(steps, 0);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (CODES) l *= exp2_int(L_UNIT);
+      if (FOLD && apart) {  // (l was 0, or NaN where a value seen is not finite)
+        const Sum sum = *own_sum;
+        __syncwarp();
+        l = sum.base == neg_inf() ? 0.f : (l + sum.l) * ex2(sum.base - m + sum.over + L_UNIT);
+      }
+      const float inv = l == 0.f ? 0.f : (CODES ? exp2_int(L_UNIT) : 1.f) / l;
       if (part < 0) {
         // O / l: the warp's 32 rows go through its staging buffer 64 bytes of each at a time
         const int piece = lane & 3;
@@ -1269,6 +1356,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
     const int r8 = lane & 7, y0 = lane >> 3;  // a lane's row of 8, its pieces of 16 bytes
     float* scales = reinterpret_cast<float*>(smem + C::OFF_SC);
     float* q_back = reinterpret_cast<float*>(smem + C::OFF_Q);
+    float* q_most = reinterpret_cast<float*>(smem + C::OFF_MOST);
     int idx = 0, tiles = 0, nq[2] = {0, 0};
     bool ok = true;
     for (int n = 0; ok; ++n) {
@@ -1287,6 +1375,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if (!mbar_wait_warp(&q_loaded[t], static_cast<uint32_t>(nq[t]) & 1u, a.status, abort_flag))
           return false;
         ++nq[t];
+        int least = 120;
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
           const int row = w * 32 + i * 8 + r8;
@@ -1303,6 +1392,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           const int k = fp16_exponent(max(mx & 0xffffu, mx >> 16));
           const float f = exp2_int(k);
+          least = min(least, k);
 #pragma unroll
           for (int x = 0; x < DP / 32; ++x) {
             const int piece = (x & 1) * 4 + y0;
@@ -1314,6 +1404,8 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
           // there before the last scores of the one before, which freed the queries
           if (y0 == 0) q_back[((nq[t] - 1) & 1) * 256 + t * 128 + row] = a.c * exp2_int(-k);
         }
+        least = __reduce_min_sync(0xffffffffu, least);
+        if (lane == 0) q_most[((nq[t] - 1) & 1) * 8 + t * 4 + w] = a.c * exp2_int(-least);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[t]);
@@ -1423,7 +1515,7 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
 constexpr int JOIN_COLS = 32;
 constexpr int JOIN_CTAS = 256;  // of a launch by shares, at most
 
-template <typename T, int DP>
+template <typename T, int DP, bool CODES>
 __global__ void __launch_bounds__(JOIN_COLS / 4 * 32)
     join_chunk_kernel(const __grid_constant__ Args a, int ctas) {
   pdl_begin();
@@ -1470,21 +1562,21 @@ __global__ void __launch_bounds__(JOIN_COLS / 4 * 32)
   #pragma unroll
       for (int y = 0; y < 4; ++y) mn = max2(mn, q[y].x);
       if (mn == neg_inf()) continue;  // no key seen yet
-      const float f = ex2(m - mn);
+      const Fall<CODES> fall(m - mn);
       m = mn;
-      l *= f;
+      l = fall.add(l, 0.f);
   #pragma unroll
-      for (int x = 0; x < 4; ++x) acc[x] *= f;
+      for (int x = 0; x < 4; ++x) acc[x] *= fall.f;
   #pragma unroll
       for (int y = 0; y < 4; ++y) {
         if (q[y].x == neg_inf()) continue;  // it saw no key
-        const float g = ex2(q[y].x - m);
-        l = fmaf(q[y].y, g, l);
+        const Fall<CODES> of_part(q[y].x - m);
+        l = of_part.add(q[y].y, l);
   #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[x] = fmaf(v[y][x], g, acc[x]);
+        for (int x = 0; x < 4; ++x) acc[x] = fmaf(v[y][x], of_part.f, acc[x]);
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : (CODES ? exp2_int(L_UNIT) : 1.f) / l;
     *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (cut.row0 + token) * a.os[0] +
                               head * a.os[1] + d) =
         make_uint2(pack2(acc[0] * inv, acc[1] * inv, T{}), pack2(acc[2] * inv, acc[3] * inv, T{}));
@@ -1556,7 +1648,7 @@ static int launch(const srdit_seq_attn_args& u, const Args& a, const Plan& p, cu
                packed && u.k_stride[1] == 0, packed && u.v_stride[1] == 0);
   rc = static_cast<int>(cudaGetLastError());
   if (rc || !p.ranged) return rc;
-  SRDIT_LAUNCH((join_chunk_kernel<T, DP>), 4 * p.ctas, JOIN_COLS / 4 * 32, 0, stream, a, p.ctas);
+  SRDIT_LAUNCH((join_chunk_kernel<T, DP, C::CODES>), 4 * p.ctas, JOIN_COLS / 4 * 32, 0, stream, a, p.ctas);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -37,19 +37,6 @@ constexpr int MAX_SHARED = 1024;  // sequences of a launch by shares
 constexpr int MIN_BLOCKS = 8;     // blocks of a share, at least
 constexpr int SHARE_BLOCKS = 64;  // ... of a CTA, from which shares are taken
 constexpr int LEAST = -80, MOST = 125;  // exponents of values' scales
-constexpr int L_UNIT = 24;        // codes: sums of weights are in the unit of 2^-24
-
-// What takes O and l from one maximum to another that is x larger (x <= 0).
-template <bool CODES>
-struct Fall {
-  float f, half;
-  SRDIT_DEV explicit Fall(float x) : f(0.f), half(ex2(CODES ? x * 0.5f : x)) {
-    f = CODES ? half * half : half;
-  }
-  SRDIT_DEV float add(float l, float sum) const {  // sum + 2^x l
-    return CODES ? fmaf(l * half, half, sum) : fmaf(l, f, sum);
-  }
-};
 
 template <int DP, int NT, int CODE>
 struct StepCfg {
@@ -431,7 +418,8 @@ __global__ void __launch_bounds__(WARPS * 32, StepCfg<DP, NT, CODE>::PER_SM)
       for (int y = 0; y < NB; ++y)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int e = min(max(static_cast<int>(__float_as_uint(vs[y][h]) >> 23 & 255u), 127 + LEAST), 127 + MOST);
+          const int bits = static_cast<int>(__float_as_uint(vs[y][h]) >> 23 & 255u);
+          const int e = min(max(bits, 127 + LEAST), 127 + MOST);
           vs[y][h] *= exp2_int(127 - e);
           lv[y][h] = __int_as_float(0x4b000000 | e) - (8388608.f + 127.f + L_UNIT);
         }

@@ -123,7 +123,6 @@ def test_large_scores_of_prompts(srdit, cuda_device, dtype, size, sign, causal, 
 WAYS = [([1, 3], [37, 400], 4, 2, 64), ([1], [20000], 2, 1, 128), ([40, 30], [90, 300], 4, 2, 128),
         ([300], [700], 4, 4, 64), ([70], [20000], 8, 2, 128)]
 STEP_SHARES = ([1, 0, 1, 2, 1, 0, 1, 1], [9001, 0, 7, 30000, 12345, 100, 16, 8000], 16, 8, 128)
-FEW = WAYS[:2] + [STEP_SHARES]   # rows per key head
 
 
 @pytest.mark.parametrize("dtype,size", SIZES)
@@ -162,7 +161,7 @@ def test_scores_a_step_apart(srdit, cuda_device, dtype, size, D):
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("size", (20, 27, 29, 40, 100))
 @pytest.mark.parametrize("sign", (1, -1))
-@pytest.mark.parametrize("new,lens,H,Hkv,D", FEW)
+@pytest.mark.parametrize("new,lens,H,Hkv,D", WAYS + [STEP_SHARES])
 def test_large_scores_over_codes(srdit, cuda_device, dtype, code, size, sign, new, lens, H, Hkv, D):
     """Keys of equal scores. Their values' scales are 1 to 2 times a power of two: its exponent and
     the score are rounded together, so that scores this large with other exponents need not stay
@@ -200,7 +199,7 @@ def _scales(g, cache, lo, hi, zeros=0.1):
     (torch.bfloat16, -80, -40), (torch.float16, -40, 8)])
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("size", (0.0, 0.5, 6.0))
-@pytest.mark.parametrize("new,lens,H,Hkv,D", FEW)
+@pytest.mark.parametrize("new,lens,H,Hkv,D", WAYS + [STEP_SHARES])
 def test_scales_far_apart(srdit, cuda_device, dtype, lo, hi, code, size, new, lens, H, Hkv, D):
     """Equal scores, scores of the usual size, and some in which a few keys have all of the weight."""
     g = gen(84)
@@ -218,7 +217,7 @@ def test_scales_far_apart(srdit, cuda_device, dtype, lo, hi, code, size, new, le
 
 
 @pytest.mark.parametrize("code", CODES)
-@pytest.mark.parametrize("rows", (1, 4))
+@pytest.mark.parametrize("rows", (1, 40))
 @pytest.mark.parametrize("order", (0, 1))
 def test_a_row_of_zeros_beside_one_of_huge_values(srdit, cuda_device, code, rows, order):
     """Two tokens of equal scores as kv_write leaves them: the answer is half of the huge one."""
