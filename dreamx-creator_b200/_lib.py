@@ -11,6 +11,9 @@ import ctypes
 import pathlib
 import struct
 import threading
+import warnings
+
+from . import build
 
 PKG = pathlib.Path(__file__).resolve().parent
 LIB_PATH = PKG / "lib" / "libsrdit_b200.so"
@@ -235,16 +238,23 @@ def lib() -> ctypes.CDLL:
 
 def calls():
     """The extension that calls some entry points with torch tensors (csrc/torch_calls.cpp), or
-    None where it is not built: the wrappers then make their checks in Python."""
-    path = LIB_PATH.parent / "_srdit_calls.so"
+    None where it is not built for the running torch, or does not load: the wrappers then make
+    their checks in Python."""
+    import importlib.util
+    path = build.calls_path()
     if not path.exists():
         return None
-    import importlib.util
-    spec = importlib.util.spec_from_file_location("_srdit_calls", path)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
     names = ("srdit_kv_write", "srdit_kv_read", "srdit_seq_attn", "srdit_seq_attn_workspace")
-    module.init(*(ctypes.cast(getattr(lib(), n), c_vp).value for n in names))
+    entries = [ctypes.cast(getattr(lib(), n), c_vp).value for n in names]
+    try:
+        spec = importlib.util.spec_from_file_location("_srdit_calls", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.init(*entries)
+    except (ImportError, OSError) as e:
+        warnings.warn(f"{path} does not load, so the wrappers make all of their checks in Python: "
+                      f"{e}", RuntimeWarning, stacklevel=2)
+        return None
     return module
 
 
