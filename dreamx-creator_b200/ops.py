@@ -7,6 +7,7 @@ there is no fallback when the library or a GPU is missing.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -400,6 +401,14 @@ def _short(name, entry, *args):
     return True
 
 
+def _fill(layout, into, *fields):
+    """Put a call's numbers into its C structure; those that its fields do not hold are refused."""
+    try:
+        layout.pack_into(into, 0, *fields)
+    except (struct.error, OverflowError) as e:
+        raise _lib.SrditError(f"sizes or numbers that the call's arguments do not hold: {e}") from None
+
+
 def _int32(t, n, what):
     if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise _lib.SrditError(f"{what} must be contiguous int32 [{n}]")
@@ -440,9 +449,8 @@ def _pages(k_pages, v_pages, table, k_scale, v_scale, dtype):
         ss = k_scale.stride() + v_scale.stride()
     p = _lib.KvPages()
     B = entries[0]
-    _lib.KV_PAGES_LAYOUT.pack_into(
-        p, 0, k_pages.data_ptr(), v_pages.data_ptr(), *scales, code, dt, n, size, Hkv, D,
-        *ks[:3], *vs[:3], *ss, table.data_ptr(), ts[0], entries[1], B)
+    _fill(_lib.KV_PAGES_LAYOUT, p, k_pages.data_ptr(), v_pages.data_ptr(), *scales, code, dt, n, size,
+          Hkv, D, *ks[:3], *vs[:3], *ss, table.data_ptr(), ts[0], entries[1], B)
     return p, B, Hkv, D
 
 
@@ -455,6 +463,8 @@ def _kv_rows(k, v, Hkv, D):
                               f"[tokens, {Hkv}, {D}] of one type each")
     if ks[2] != 1 or vs[2] != 1:
         raise _lib.SrditError(f"k, v need unit stride over D, have {ks}, {vs}")
+    if shape[0] > 0x7fffffff:   # (a C int)
+        raise _lib.SrditError(f"{shape[0]} tokens")
     st = _lib.KvStrides(ks[0], ks[1], vs[0], vs[1])
     return shape[0], st, ctypes.addressof(st)
 
@@ -523,17 +533,16 @@ def _seq_attn(kind, q, out, Hkv, width, B, pages, k, v, Tk, kv_strides, cu_q, cu
     if qs[2] != 1 or os[2] != 1:
         raise _lib.SrditError(f"q, out need unit stride over D, have {qs}, {os}")
     a = _lib.SeqAttnArgs()
-    fill = _lib.SEQ_ATTN_LAYOUT.pack_into
     fields = (pages, q.data_ptr(), k, v, out.data_ptr(), dt, T, Tk, B, H, Hkv, D, qs[0], qs[1],
               *kv_strides, os[0], os[1], cu_q, cu_k, kv_lens, max_q, max_kv, bool(causal),
               D ** -0.5 if scale is None else scale)
     st = 0 if status is None else status.data_ptr()
-    fill(a, 0, *fields, 0, 0, st)
+    _fill(_lib.SEQ_ATTN_LAYOUT, a, *fields, 0, 0, st)
     ref = ctypes.byref(a)
     kib = _lib.count("srdit_seq_attn_workspace", ref)
     if kib:
         ws = torch.empty(kib << 10, dtype=torch.uint8, device=q.device)
-        fill(a, 0, *fields, ws.data_ptr(), kib << 10, st)
+        _fill(_lib.SEQ_ATTN_LAYOUT, a, *fields, ws.data_ptr(), kib << 10, st)
     _launch("srdit_seq_attn", ref, stream, kind=kind, work=4 * T * H * D * (max_kv or Tk))
     if kib:
         Stats.launches += 1   # a second kernel joins the parts
@@ -564,8 +573,7 @@ def paged_attn(q, k_pages, v_pages, page_table, kv_lens, out=None, *, cu_q=None,
     return _seq_attn("paged_attn", q, out, Hkv, D, B, ctypes.addressof(p), 0, 0, 0, (0, 0, 0, 0),
                      0 if cu_q is None else _int32(cu_q, B + 1, "cu_q"), 0,
                      _int32(kv_lens, B, "kv_lens"), max_q,
-                     p.table_width * p.page_size if max_kv is None else max_kv, causal, scale,
-                     status, stream)
+                     0 if max_kv is None else max_kv, causal, scale, status, stream)
 
 
 def packed_attn(q, k, v, cu_q, out=None, *, cu_k=None, causal=True, scale=None, status=None):
