@@ -25,7 +25,9 @@ class Stats:
     events recorded on the launching stream around the launch and ``work`` its
     algorithmic FLOPs (GEMM, attention) or bytes (row kernels), so a profiling
     pass can attribute time per kernel kind. Leave it None in timed regions:
-    the event records themselves cost time.
+    the event records themselves cost time, and the lengths of packed sequences
+    are read from the device, behind the launch (not while a graph is captured:
+    ``work`` is 0 then).
     """
     launches = 0
     events = None
@@ -41,7 +43,7 @@ def _launch(name, *args, kind=None, work=0):
     Stats.launches += 1
     if ev is not None:
         e1.record()
-        ev.append((kind or name, e0, e1, int(work)))
+        ev.append((kind or name, e0, e1, int(work() if callable(work) else work)))
 
 
 def _ptr(t):
@@ -469,6 +471,42 @@ def _kv_rows(k, v, Hkv, D):
     return shape[0], st, ctypes.addressof(st)
 
 
+def _row_ends(cu, T, B):
+    """The rows of B packed sequences as the kernels take them: (first, behind the last) of each."""
+    if cu is None:
+        return [(b * (T // B), (b + 1) * (T // B)) for b in range(B)]
+    at = [min(max(x, 0), T) for x in cu.tolist()]
+    return [(x, max(x, y)) for x, y in zip(at, at[1:])]
+
+
+def _kv_bytes(T, B, cu, Hkv, D, rows, pages):
+    """Bytes that kv_write and kv_read move: every sequence's rows, here and in the cache."""
+    def work():
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        held = D * pages.itemsize + (0 if pages == rows else 4)   # a scale with codes
+        return 2 * Hkv * (D * rows.itemsize + held) * sum(y - x for x, y in _row_ends(cu, T, B))
+    return work
+
+
+def _attn_flops(shape, B, cu_q, keys, causal):
+    """FLOPs of attention of packed sequences: 4 D for each query, head and key that it sees.
+    ``keys()``: the sequences' lengths."""
+    def work():
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        (T, H, D), seen = shape, 0
+        for (x, y), L in zip(_row_ends(cu_q, T, B), keys()):
+            n = y - x
+            if causal:   # the last of n sees L keys, each before it one less
+                rows = min(n, L)
+                seen += rows * L - rows * (rows - 1) // 2
+            else:
+                seen += n * L
+        return 4 * H * D * seen
+    return work
+
+
 def kv_write(k, v, k_pages, v_pages, page_table, kv_lens, *, cu_q=None, k_scale=None,
              v_scale=None):
     """Write new tokens' k, v [T, Hkv, D] (bf16 or fp16) into a cache's pages.
@@ -488,7 +526,7 @@ def kv_write(k, v, k_pages, v_pages, page_table, kv_lens, *, cu_q=None, k_scale=
     T, st, at = _kv_rows(k, v, Hkv, D)
     _launch("srdit_kv_write", ctypes.byref(p), k.data_ptr(), at, v.data_ptr(), at + 16, T,
             None if cu_q is None else _int32(cu_q, B + 1, "cu_q"), _int32(kv_lens, B, "kv_lens"),
-            stream, kind="kv_write", work=6 * T * Hkv * D)
+            stream, kind="kv_write", work=_kv_bytes(T, B, cu_q, Hkv, D, k.dtype, k_pages.dtype))
 
 
 def kv_read(k_pages, v_pages, page_table, cu_k, k=None, v=None, *, total=None, dtype=None,
@@ -513,12 +551,13 @@ def kv_read(k_pages, v_pages, page_table, cu_k, k=None, v=None, *, total=None, d
     p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, k.dtype)
     T, st, at = _kv_rows(k, v, Hkv, D)
     _launch("srdit_kv_read", ctypes.byref(p), k.data_ptr(), at, v.data_ptr(), at + 16, T,
-            _int32(cu_k, B + 1, "cu_k"), stream, kind="kv_read", work=6 * T * Hkv * D)
+            _int32(cu_k, B + 1, "cu_k"), stream, kind="kv_read",
+            work=_kv_bytes(T, B, cu_k, Hkv, D, k.dtype, k_pages.dtype))
     return k, v
 
 
 def _seq_attn(kind, q, out, Hkv, width, B, pages, k, v, Tk, kv_strides, cu_q, cu_k, kv_lens, max_q,
-              max_kv, causal, scale, status, stream):
+              max_kv, causal, scale, status, stream, work):
     shape, dtype, qs = q.shape, q.dtype, q.stride()
     if len(shape) != 3 or shape[2] != width or Hkv == 0 or shape[1] % Hkv:
         raise _lib.SrditError(f"q {tuple(shape)} [tokens, heads, D] does not go with {Hkv} key heads "
@@ -543,7 +582,7 @@ def _seq_attn(kind, q, out, Hkv, width, B, pages, k, v, Tk, kv_strides, cu_q, cu
     if kib:
         ws = torch.empty(kib << 10, dtype=torch.uint8, device=q.device)
         _fill(_lib.SEQ_ATTN_LAYOUT, a, *fields, ws.data_ptr(), kib << 10, st)
-    _launch("srdit_seq_attn", ref, stream, kind=kind, work=4 * T * H * D * (max_kv or Tk))
+    _launch("srdit_seq_attn", ref, stream, kind=kind, work=work)
     if kib:
         Stats.launches += 1   # a second kernel joins the parts
     return out
@@ -570,10 +609,13 @@ def paged_attn(q, k_pages, v_pages, page_table, kv_lens, out=None, *, cu_q=None,
     p, B, Hkv, D = _pages(k_pages, v_pages, page_table, k_scale, v_scale, q.dtype)
     if max_q is None:
         max_q = q.shape[0] if cu_q is not None or B == 0 else q.shape[0] // B
+    held = p.table_width * p.page_size
+    work = _attn_flops(q.shape, B, cu_q, lambda: [min(max(x, 0), held) for x in kv_lens.tolist()],
+                       causal)
     return _seq_attn("paged_attn", q, out, Hkv, D, B, ctypes.addressof(p), 0, 0, 0, (0, 0, 0, 0),
                      0 if cu_q is None else _int32(cu_q, B + 1, "cu_q"), 0,
                      _int32(kv_lens, B, "kv_lens"), max_q,
-                     0 if max_kv is None else max_kv, causal, scale, status, stream)
+                     0 if max_kv is None else max_kv, causal, scale, status, stream, work)
 
 
 def packed_attn(q, k, v, cu_q, out=None, *, cu_k=None, causal=True, scale=None, status=None):
@@ -598,10 +640,13 @@ def packed_attn(q, k, v, cu_q, out=None, *, cu_k=None, causal=True, scale=None, 
     B = cu_q.numel() - 1
     if B < 0 or (cu_k is None and shape[0] != q.shape[0]):
         raise _lib.SrditError(f"{B} sequences; without cu_k k and v have q's {q.shape[0]} rows")
+    ends = cu_q if cu_k is None else cu_k
+    work = _attn_flops(q.shape, B, cu_q, lambda: [y - x for x, y in _row_ends(ends, shape[0], B)],
+                       causal)
     return _seq_attn("packed_attn", q, out, shape[1], shape[2], B, 0, k.data_ptr(), v.data_ptr(),
                      shape[0], (ks[0], ks[1], vs[0], vs[1]), _int32(cu_q, B + 1, "cu_q"),
                      0 if cu_k is None else _int32(cu_k, B + 1, "cu_k"), 0, 0, 0, causal, scale,
-                     status, stream)
+                     status, stream, work)
 
 
 def row_reduce(x, op, out=None):
