@@ -55,7 +55,8 @@ static int check(const srdit_seq_attn_args& a) {
     return SRDIT_EINVAL;
   }
   if (a.B == 0 || a.T == 0 || a.H == 0) return 1;
-  if (!a.q || !a.out || !(a.scale > 0.f) || a.scale > 3.4028234e38f) return SRDIT_EINVAL;
+  // (scores are taken in base 2: its factor has to be a number too)
+  if (!a.q || !a.out || !(a.scale > 0.f) || !(a.scale * kLog2e <= 3.4028234e38f)) return SRDIT_EINVAL;
   if (a.H > 1 && a.q_stride[1] == 0) return SRDIT_EINVAL;  // (of the inputs, key heads may be repeated)
   if (!a.cu_q && a.T % a.B) return SRDIT_EINVAL;
   if (paged ? !a.kv_lens : (a.Tk > 0 && (!a.k || !a.v)) || (!a.cu_k && !a.cu_q && a.Tk % a.B))

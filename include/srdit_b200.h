@@ -707,7 +707,8 @@ int srdit_kv_read(const srdit_kv_pages* pages, void* k, const long long* k_strid
  * (srdit_kv_write's are 2^-40 to 2^121), side by side in any order.
  * max_q: no sequence has more queries (0: T; a sequence's further rows may be left as they were);
  * max_kv (pages): about the longest sequence (0: what the table holds), which the work's split goes by and no result.
- * Views as in srdit_cross_attn (bases 16-byte aligned, strides multiples of 8). scale > 0.
+ * Views as in srdit_cross_attn (bases 16-byte aligned, strides multiples of 8). scale > 0,
+ * scale log2(e) finite.
  * workspace: where srdit_seq_attn_workspace (which reads the arguments, not the tensors) returns
  * n > 0, n KiB, 16-byte aligned. T * H at most 2^26, B * Hkv at most 65535, Tk at most 2^31 - 256.
  * Replaces: flash_attention over packed sequences (attention.py:61-168), with a cache in pages.

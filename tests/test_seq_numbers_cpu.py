@@ -30,6 +30,14 @@ def test_numbers(srdit, ops, kw):
         ops.paged_attn(torch.zeros(1, 1, 16, dtype=DT), k, v, table, lens, **kw)
 
 
+@pytest.mark.parametrize("scale", (2.4e38, 3.4e38))
+def test_a_scale_without_a_factor_in_base_2(srdit, ops, scale):
+    """scale log2(e) beyond fp32: rows whose scores are 0 would be NaN."""
+    x, cu = torch.zeros(1, 1, 16, dtype=DT), torch.tensor([0, 1], dtype=torch.int32)
+    with pytest.raises(srdit._lib.SrditError, match="-1"):
+        ops.packed_attn(x, x, x, cu, scale=scale)
+
+
 @pytest.mark.parametrize("max_kv", (None, 0, 7))
 def test_a_table_of_more_than_the_kernels_count(srdit, ops, max_kv):
     k, v, table, lens = _cache(size=1 << 24, width=256, pages=0)   # 2^32 tokens
