@@ -1,7 +1,8 @@
 // seq_chunk.cu -- attention of many query rows per key head: whole prompts, and chunks of new
 // tokens over the pages of a cache. Bounded by the chain of a query tile, scores, softmax, product:
-// 6912 queries on 13824 keys of 24 heads of 128, 16 bits, 918 us, 1280 TFLOP/s; 2 x 512 on 16384 e4m3
-// keys, 32 heads over 8, 360 us, 750 TFLOP/s.
+// 6912 queries on 13824 keys of 24 heads of 128, 16 bits, 970 us at full clocks and 1050 to 1080 in a row,
+// where the card's power holds them at 1.6 of 1.97 GHz, 1090 to 1210 TFLOP/s; 2 x 512 on 16384 e4m3 keys,
+// 32 heads over 8, 388 us, 700 TFLOP/s.
 //
 // A work item is up to 2 rt tokens of one sequence with `pack` heads of one group side by side,
 // as two query tiles of 128 rows that share every key tile; while one is in its softmax the other
@@ -986,9 +987,10 @@ __global__ void __launch_bounds__(ChunkCfg<DP, CODE>::THREADS, 1)
         if constexpr (CODES) {
           // Two passes over the scores, 64 of them at a time, so that the code is short: with all 128
           // in registers at once, as below, it does not fit the instruction caches beside that of the
-          // warps that widen codes. (2 x 512 queries on 16384 e4m3 keys, 32 heads over 8 of 128: 421
-          // us so, 406 in passes of 32, 361 in passes of 64; the same keys in 16 bits 258. Masks, which few
-          // tiles need, go over the scores once before, in a short loop: 366 -> 354.)
+          // warps that widen codes. (2 x 512 queries on 16384 e4m3 keys, 32 heads over 8 of 128, when this
+          // was chosen: 421 us so, 406 in passes of 32, 361 in passes of 64; masks, which few tiles need, as
+          // a short loop over the scores before took 3% off. With what large scores and scales far apart
+          // need 388; the same keys in 16 bits 264 to 297, by the clocks.)
           const float* sc = scales + (tiles % C::SCALES) * 256;
           const float* units =
               reinterpret_cast<const float*>(smem + C::OFF_UNITS) + tiles % C::SCALES * 16;
@@ -1607,7 +1609,10 @@ Plan plan_chunk(const srdit_seq_attn_args& u, int sms) {
       (u.B == 1 ? (u.T + 2 * p.rt - 1) / (2 * p.rt) : p.slots - u.B / 2) * static_cast<long long>(p.nhp);
   if (p.slots <= MAX_SLOTS && items * (held / TILE + 1) < (1ll << 30)) {
     // CTAs of shares go through keys at different places and miss what others have fetched: a step
-    // takes a quarter more
+    // takes a quarter more. (us whole and shared out, 32 heads over 8 of 128: 64 queries on 512 keys
+    // 16.5 and 18.4, on 1024 24.2 and 20.3, on 32768 511 and 53; 512 on 16384 264 and 148, two of them 299 and
+    // 329; a prompt of 1024 24 and 34. The last round of 6912 on 13824, 24 heads: 1148 and 1082, all of it
+    // in shares 1323; of 2304 on 6912 223 and 202.)
     const long long rounds = (some + sms - 1) / sms, steps = some * tiles;
     const long long whole = rounds * tiles, shared = steps / sms * 5 / 4 + 7;
     if (some < sms || u.causal) {

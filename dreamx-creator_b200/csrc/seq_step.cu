@@ -22,9 +22,9 @@
 // The keys are split in one of two ways. Little work: every (sequence, key head) over a cluster of
 // up to 8 CTAs, which join their parts in shared memory. Much: two CTAs on every SM (three over
 // codes) take equal shares of all blocks, whatever the sequences' lengths, and join_share_kernel
-// joins what the shares cut. 32 sequences of up to 4096 keys, 32 heads over 8 of 128, bf16: 51 us,
-// 5.3 TB/s; 8 of 32768 in e4m3: 109 us, 5.0 TB/s, where widening the codes takes 46% of the issue
-// slots.
+// joins what the shares cut. 32 sequences of up to 4096 keys, 32 heads over 8 of 128, bf16: 52 us,
+// 5.2 TB/s; 8 of 32768 169 us, 6.4 TB/s, in e4m3 107, 5.2 TB/s, in int8 107 to 116, where widening the
+// codes takes 46% of the issue slots.
 #include <atomic>
 
 #include "seq_attn.cuh"
@@ -838,9 +838,12 @@ Plan plan_step(const srdit_seq_attn_args& u, int sms) {
   const long long blocks = (keys + size - 1) / size;
   p.cluster = p.parts = p.splits = 1;
   // By shares from SHARE_BLOCKS blocks a CTA, two CTAs an SM, three of codes (which take more
-  // instructions a byte). 32 sequences, 32 heads over 8, one token, up to 4096 keys each: 51 us, by
-  // clusters 63, e4m3 44 and 61; all with 2048: 50 and 44; 16 with 2048: 30 and 26 (30 blocks a
-  // CTA); 64 with up to 512 e4m3: 27 and 18 (9). (blocks x sequences in 32 bits)
+  // instructions a byte). The lengths are not known here: shares gain where they differ, and cost where
+  // they are equal. us by shares and by clusters, one token, 32 heads over 8 of 128: 32 sequences of up to
+  // 4096 keys 52 and 64, e4m3 43 and 61; 8 of up to 32768 105 and 124, e4m3 69 and 110; 128 of up to 1024 56
+  // and 52. All of one length: 32 of 4096 90 and 83, e4m3 60 and 63; 32 of 2048 50 and 45; 8 of 32768 167 and
+  // 157, e4m3 107 and 118; 16 of 4096 with four tokens 63 and 52. Fewer blocks: 32 of up to 1024 24 and
+  // 20.5 (55 blocks a CTA), 8 of 2048 21 and 17 (28). (blocks x sequences in 32 bits)
   const long long ctas = (size == 16 ? 2ll : per_sm) * sms;
   if (u.B <= MAX_SHARED && pairs * blocks >= SHARE_BLOCKS * ctas && u.Hkv <= ctas &&
       u.B * (held / size + 1) < (1ll << 31)) {

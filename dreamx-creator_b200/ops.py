@@ -598,7 +598,9 @@ def paged_attn(q, k_pages, v_pages, page_table, kv_lens, out=None, *, cu_q=None,
     own, else all kv_lens[b] of them. One that sees none gets zeros; rows of out behind the last
     sequence are left as they were. ``max_q``: no sequence has more new tokens (default: T / B
     without ``cu_q``, else T; steps of one token each say 1); ``max_kv``: about the longest
-    sequence (default: what the table holds), by which work is split. ``scale``: D ** -0.5."""
+    sequence (default: what the table holds), by which work is split. ``scale``: D ** -0.5.
+    T * H at most 2^26, B * kv_heads at most 65535. Scales of values 0, or 2^-80 to 2^121 (fp16 q:
+    2^100)."""
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if _short("paged_attn", "srdit_seq_attn", q, k_pages, v_pages, page_table, kv_lens, out, cu_q,

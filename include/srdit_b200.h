@@ -703,8 +703,9 @@ int srdit_kv_read(const srdit_kv_pages* pages, void* k, const long long* k_strid
  * NaN included. A NaN or an infinity in a value that it does see makes that column of its answer
  * not finite, or all of them NaN.
  * Scores may have any size that fp32 holds, q.k and scale log2(e) q.k; over codes one is rounded to
- * fp32 together with the exponent of its value's scale. Values' scales: 0, or 2^-80 to 2^121
- * (srdit_kv_write's are 2^-40 to 2^121), side by side in any order.
+ * fp32 together with the exponent of its value's scale. Values' scales: 0, or 2^-80 to 2^121 (for fp16,
+ * whose answers end at 2^16, to 2^100; srdit_kv_write's are 2^-40 to 2^121, of fp16 to 2^10), side by
+ * side in any order.
  * max_q: no sequence has more queries (0: T; a sequence's further rows may be left as they were);
  * max_kv (pages): about the longest sequence (0: what the table holds), which the work's split goes by and no result.
  * Views as in srdit_cross_attn (bases 16-byte aligned, strides multiples of 8). scale > 0,
