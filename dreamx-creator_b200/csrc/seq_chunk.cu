@@ -1,7 +1,7 @@
 // seq_chunk.cu -- attention of many query rows per key head: whole prompts, and chunks of new
 // tokens over the pages of a cache. Bounded by the chain of a query tile, scores, softmax, product:
-// 6912 queries on 13824 keys of 24 heads of 128, 16 bits, 970 us at full clocks and 1050 to 1080 in a row,
-// where the card's power holds them at 1.6 of 1.97 GHz, 1090 to 1210 TFLOP/s; 2 x 512 on 16384 e4m3 keys,
+// 6912 queries on 13824 keys of 24 heads of 128, 16 bits, 970 us at full clocks and 1050 to 1100 in a row,
+// where the card's power holds them at 1.6 of 1.97 GHz, 1070 to 1210 TFLOP/s; 2 x 512 on 16384 e4m3 keys,
 // 32 heads over 8, 388 us, 700 TFLOP/s.
 //
 // A work item is up to 2 rt tokens of one sequence with `pack` heads of one group side by side,
